@@ -52,6 +52,7 @@ EXPORTED = [
     "hyp_rope", "hyp_sample_greedy", "hyp_sample_greedy_topk", "hyp_sample_stochastic",
     "hyp_kv_cache_create", "hyp_kv_cache_free", "hyp_kv_cache_buffers", "hyp_kv_cache_write", "hyp_attention",
     "hyp_attention_prepare", "hyp_residual_rms_norm",
+    "hyp_batch_plan", "hyp_batch_prepare",
     "hyp_model_create", "hyp_model_free", "hyp_model_load", "hyp_kvstate_create", "hyp_kvstate_free",
     "hyp_prefill_chunk", "hyp_decode_block", "hyp_prefill_chunk_sampled", "hyp_decode_block_sampled",
     "hyp_step_result_create", "hyp_step_result_free", "hyp_step_result_fields", "hyp_model_forward_hidden",
@@ -192,6 +193,28 @@ class SamplingConfig(ctypes.Structure):
                 ("min_p", ctypes.c_float), ("seed", ctypes.c_uint64)]
 
 
+class BatchFields(ctypes.Structure):
+    """HypBatch: a step of batched serving."""
+    _fields_ = [
+        ("requests", ctypes.c_uint32),
+        ("block_size", ctypes.c_uint32),
+        ("num_blocks", ctypes.c_uint32),
+        ("max_blocks", ctypes.c_uint32),
+        ("max_rows", ctypes.c_uint32),
+        ("prefix_len", ctypes.c_uint32),
+        ("prefix_table", ctypes.c_void_p),
+        ("tables", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("row_start", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+    ]
+
+
+SLOT_NONE = 0xFFFFFFFF      # HYP_SLOT_NONE
+REQUEST_DONE = 0xFFFFFFFF   # HYP_REQUEST_DONE
+
+
 class StepResultFields(ctypes.Structure):
     """HypStepResultFields (hyperion_mlx.h:157-176)."""
     _fields_ = [
@@ -287,6 +310,8 @@ def load_library(path: str) -> ctypes.CDLL:
         "hyp_attention_prepare": [_P, _P, _P, _U32, _U32, _P, _P, _P, ctypes.c_float, _U32, ctypes.c_float, _U32,
                                   _P],
         "hyp_residual_rms_norm": [_P, _P, _P, _P, _P, _P, _U32, _U32, ctypes.c_float, _P],
+        "hyp_batch_plan": [_P, _P, _P, _P, _P, _P, _P, _P],
+        "hyp_batch_prepare": [_P, _P, _P, _P, _U32, _P, _P, _P, ctypes.c_float, _U32, ctypes.c_float, _P, _P],
         "hyp_model_create": [_PP],
         "hyp_model_free": [_PP],
         "hyp_model_load": [_P, ctypes.POINTER(GeometryParams), ctypes.c_char_p],
@@ -477,6 +502,26 @@ class DeviceArray:
             self.close()
         except Exception:
             pass
+
+
+class DeviceView(DeviceArray):
+    """Device memory that something else owns, as the calls here take it: an object with
+    data_ptr(), shape and nbytes (a torch tensor), which the view keeps alive."""
+
+    def __init__(self, owner):
+        self.owner = owner
+        self.shape = tuple(int(n) for n in owner.shape)
+        self.nbytes = int(owner.nbytes)
+        self._p = ctypes.c_void_p(owner.data_ptr())
+
+    def to_host(self, stream: Stream) -> np.ndarray:
+        raise TypeError("a DeviceView is read through its owner")
+
+    def upload(self, a: np.ndarray, stream: Stream) -> None:
+        raise TypeError("a DeviceView is written through its owner")
+
+    def close(self) -> None:
+        pass
 
 
 class QWeight:
@@ -715,6 +760,41 @@ def attention_prepare(q: "DeviceArray", k_raw: "DeviceArray", v_raw: Optional["D
     offset.. <- rope(k_norm(k_raw)) and v_norm(v_raw) (v_raw None: of k_raw)."""
     call("hyp_attention_prepare", q.ptr, k_raw.ptr, None if v_raw is None else v_raw.ptr, L, n_heads, cache.handle,
          q_norm.ptr, k_norm.ptr, eps, rotated, base, offset, stream.handle)
+
+
+class Batch:
+    """HypBatch: requests decoded together over one paged cache per layer, behind a shared
+    prefix. tables [requests, max_blocks], lens [requests], row_start [requests + 1], slots and
+    positions [max_rows], prefix_table: device arrays of uint32, which the batch keeps alive."""
+
+    def __init__(self, block_size: int, num_blocks: int, tables: "DeviceArray", lens: "DeviceArray",
+                 row_start: "DeviceArray", slots: "DeviceArray", positions: "DeviceArray", prefix_len: int = 0,
+                 prefix_table: Optional["DeviceArray"] = None):
+        requests, max_blocks = tables.shape
+        if lens.shape != (requests,) or row_start.shape != (requests + 1,) or slots.shape != positions.shape:
+            raise ValueError("batch: lens [requests], row_start [requests + 1], slots and positions [max_rows]")
+        if prefix_table is not None and prefix_table.shape[0] * block_size < prefix_len:
+            raise ValueError("batch: the prefix table is shorter than the prefix")
+        self.arrays = (tables, lens, row_start, slots, positions, prefix_table)
+        self.fields = BatchFields(requests, block_size, num_blocks, max_blocks, slots.shape[0], prefix_len,
+                                  None if prefix_table is None else prefix_table.ptr, tables.ptr, lens.ptr,
+                                  row_start.ptr, slots.ptr, positions.ptr)
+        self._ref = ctypes.byref(self.fields)
+
+    def plan(self, lens: "DeviceArray", new_tokens: "DeviceArray", free_blocks: "DeviceArray", taken: "DeviceArray",
+             taken_out: "DeviceArray", served: "DeviceArray", stream: "Stream") -> None:
+        """hyp_batch_plan: the step's tables, lengths, row starts, slots and positions from the
+        requests' lengths and new tokens (REQUEST_DONE: its blocks go back)."""
+        call("hyp_batch_plan", self._ref, lens.ptr, new_tokens.ptr, free_blocks.ptr, taken.ptr, taken_out.ptr,
+             served.ptr, stream.handle)
+
+    def prepare(self, q: "DeviceArray", k_raw: "DeviceArray", v_raw: Optional["DeviceArray"], n_heads: int,
+                cache: KvCache, q_norm: "DeviceArray", k_norm: "DeviceArray", eps: float, rotated: int, base: float,
+                q_out: "DeviceArray", stream: "Stream") -> None:
+        """hyp_batch_prepare: q_out <- rope(q_norm(q)) at each row's position; the cache's slots
+        of the rows <- rope(k_norm(k_raw)) and v_norm(v_raw) (v_raw None: of k_raw)."""
+        call("hyp_batch_prepare", self._ref, q.ptr, k_raw.ptr, None if v_raw is None else v_raw.ptr, n_heads,
+             cache.handle, q_norm.ptr, k_norm.ptr, eps, rotated, base, q_out.ptr, stream.handle)
 
 
 def residual_rms_norm(branch: "DeviceArray", residual: "DeviceArray", post_w: "DeviceArray",

@@ -12,6 +12,7 @@
 #include <new>
 #include <string>
 
+#include "batch.h"
 #include "hyperion_hip.h"
 #include "kernels.h"
 #include "decoder.h"
@@ -884,6 +885,97 @@ HypStatus hyp_attention_prepare(void* q, const void* k_raw, const void* v_raw, u
         a.base = rope_base;
         a.eps = eps;
         hyperion::hip::launch_attn_prepare(a, s);
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+// The checks that every batch call makes, and the batch as the kernels take it.
+hyperion::hip::BatchView batch_ref(const HypBatch* b) {
+    REQUIRE_ARG(b != nullptr, "batch is null");
+    REQUIRE_ARG(b->requests <= hyperion::hip::kMaxRequests, "a batch has at most 4096 requests");
+    REQUIRE_ARG(b->block_size > 0 && b->block_size <= 65536u && (b->block_size & (b->block_size - 1u)) == 0u,
+                "block_size must be a power of two, at most 65536");
+    REQUIRE_ARG(static_cast<uint64_t>(b->num_blocks) * b->block_size < (1ull << 30),
+                "num_blocks * block_size must be below 2^30");
+    REQUIRE_ARG(b->num_blocks > 0, "num_blocks must be positive");
+    REQUIRE_ARG(b->max_rows <= hyperion::hip::kMaxBatchRows, "a step has at most 2^20 rows");
+    REQUIRE_ARG(b->prefix_len <= hyperion::hip::kMaxPositions, "prefix_len must be at most 2^24");
+    REQUIRE_ARG(b->prefix_len == 0 || b->prefix_table != nullptr, "a prefix needs its prefix_table");
+    REQUIRE_ARG(b->requests == 0 || b->max_blocks == 0 || b->tables != nullptr, "tables must be a non-null device pointer");
+    REQUIRE_ARG(b->requests == 0 || b->lens != nullptr, "lens must be a non-null device pointer");
+    REQUIRE_ARG(b->row_start != nullptr, "row_start must be a non-null device pointer");
+    uint32_t shift = 0;
+    while ((1u << shift) < b->block_size) ++shift;
+    return {b->requests, shift,     b->num_blocks, b->max_blocks, b->max_rows, b->prefix_len, b->prefix_table,
+            b->tables,   b->lens,   b->row_start,  b->slots,      b->positions};
+}
+
+HypKvCacheOpaque& batch_cache(const HypBatch& b, HypKvCache cache, uint32_t n_heads) {
+    HypKvCacheOpaque& c = kv_ref(cache);
+    REQUIRE_ARG(static_cast<uint64_t>(b.num_blocks) * b.block_size <= c.capacity,
+                "the cache must hold num_blocks * block_size tokens");
+    REQUIRE_ARG(n_heads > 0 && n_heads % c.num_kv_heads == 0, "n_heads must be a multiple of the cache's num_kv_heads");
+    REQUIRE_ARG(static_cast<uint64_t>(b.max_rows) * n_heads * c.head_dim < (1ull << 31), "q too large");
+    return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+HypStatus hyp_batch_plan(const HypBatch* batch, const uint32_t* lens, const uint32_t* new_tokens,
+                         uint32_t* free_blocks, const uint32_t* taken, uint32_t* taken_out, uint32_t* served,
+                         HypStream stream) {
+    return abi_call("hyp_batch_plan", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        REQUIRE_ARG(b.requests == 0 || (lens != nullptr && new_tokens != nullptr),
+                    "lens and new_tokens must be non-null device pointers");
+        REQUIRE_ARG(free_blocks != nullptr && taken != nullptr && taken_out != nullptr && served != nullptr,
+                    "free_blocks, taken, taken_out and served must be non-null device pointers");
+        REQUIRE_ARG(b.max_rows == 0 || (b.slots != nullptr && b.positions != nullptr),
+                    "slots and positions must be non-null device pointers");
+        hyperion::hip::launch_batch_plan(b, lens, new_tokens, free_blocks, taken, taken_out, served, s);
+    });
+}
+
+HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_raw, const void* v_raw,
+                            uint32_t n_heads, HypKvCache cache, const void* q_norm, const void* k_norm, float eps,
+                            uint32_t rotated_dims, float rope_base, void* q_out, HypStream stream) {
+    return abi_call("hyp_batch_prepare", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
+        if (b.max_rows == 0) return;
+        REQUIRE_ARG(b.slots != nullptr && b.positions != nullptr, "slots and positions must be non-null device pointers");
+        REQUIRE_ARG(q != nullptr && k_raw != nullptr && q_norm != nullptr && k_norm != nullptr && q_out != nullptr,
+                    "q, k_raw, q_norm, k_norm and q_out must be non-null device pointers");
+        REQUIRE_ARG(aligned16(q) && aligned16(k_raw) && aligned16(v_raw) && aligned16(q_norm) && aligned16(k_norm) &&
+                        aligned16(q_out),
+                    "q, k_raw, v_raw, q_norm, k_norm and q_out must be 16-byte aligned");
+        REQUIRE_ARG(std::isfinite(eps) && eps >= 0.0f, "eps must be finite and >= 0");
+        REQUIRE_ARG(rotated_dims <= c.head_dim && rotated_dims % 2u == 0u, "rotated_dims must be even and <= head_dim");
+        REQUIRE_ARG(std::isfinite(rope_base) && rope_base > 0.0f, "rope_base must be finite and positive");
+        hyperion::hip::BatchPrepareArgs a{};
+        a.q = static_cast<const uint16_t*>(q);
+        a.k_raw = static_cast<const uint16_t*>(k_raw);
+        a.v_raw = static_cast<const uint16_t*>(v_raw);
+        a.q_norm = static_cast<const uint16_t*>(q_norm);
+        a.k_norm = static_cast<const uint16_t*>(k_norm);
+        a.q_out = static_cast<uint16_t*>(q_out);
+        a.cache_k = static_cast<uint16_t*>(c.k.data());
+        a.cache_v = static_cast<uint16_t*>(c.v.data());
+        a.n_heads = n_heads;
+        a.n_kv_heads = c.num_kv_heads;
+        a.head_dim = c.head_dim;
+        a.rotated = rotated_dims;
+        a.capacity = c.capacity;
+        a.base = rope_base;
+        a.eps = eps;
+        hyperion::hip::launch_batch_prepare(b, a, s);
     });
 }
 

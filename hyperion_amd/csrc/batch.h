@@ -1,0 +1,45 @@
+// A step of batched serving as the kernels see it (HypBatch, hyperion_hip.h): requests whose
+// tokens lie in blocks of one paged cache per layer, behind a prefix that all of them share.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "hyperion_hip.h"
+
+namespace hyperion::hip {
+
+constexpr uint32_t kMaxRequests = 4096;            // their running sums fit one workgroup's LDS
+constexpr uint32_t kMaxBatchRows = 1u << 20;
+constexpr uint32_t kMaxPositions = 1u << 24;       // positions are exact in fp32 below
+
+struct BatchView {
+    uint32_t requests, shift, num_blocks, max_blocks, max_rows, prefix;   // block size 1 << shift
+    const uint32_t* prefix_table;
+    uint32_t* tables;      // [requests][max_blocks]
+    uint32_t* lens;        // [requests]
+    uint32_t* row_start;   // [requests + 1]
+    uint32_t* slots;       // [max_rows]
+    uint32_t* positions;   // [max_rows]
+};
+
+void launch_batch_plan(const BatchView& b, const uint32_t* lens, const uint32_t* new_tokens, uint32_t* free_blocks,
+                       const uint32_t* taken, uint32_t* taken_out, uint32_t* served, hipStream_t stream);
+
+struct BatchPrepareArgs {
+    const uint16_t* q;       // [max_rows][n_heads][head_dim]
+    const uint16_t* k_raw;   // [max_rows][n_kv_heads][head_dim]
+    const uint16_t* v_raw;   // the same, or null: V = norm(k_raw)
+    const uint16_t* q_norm;
+    const uint16_t* k_norm;
+    uint16_t* q_out;
+    uint16_t* cache_k;       // [capacity][n_kv_heads][head_dim]
+    uint16_t* cache_v;
+    uint32_t n_heads, n_kv_heads, head_dim, rotated, capacity;
+    float base, eps;
+};
+void launch_batch_prepare(const BatchView& b, const BatchPrepareArgs& a, hipStream_t stream);
+
+}  // namespace hyperion::hip

@@ -384,6 +384,79 @@ HypStatus hyp_residual_rms_norm(const void* branch, void* residual, const void* 
                                 const void* next_weight, void* next, uint32_t m, uint32_t hidden, float eps,
                                 HypStream stream);
 
+/* ---- batches: requests decoded together over one paged cache per layer ------------------
+ * What serving several sequences at once needs next to the calls above, whose caches hold
+ * one sequence each; the reference has no counterpart (it decodes one sequence). A step is
+ * hyp_batch_plan once, then per layer hyp_batch_prepare and hyp_batch_attention between the
+ * projections (which take the step's rows as m), and hyp_batch_sample on the logits. No call
+ * allocates or synchronises, so a step can be recorded into a graph; everything that changes
+ * from step to step (lengths, blocks, rows) is device memory that the calls read there.
+ *
+ * Token blocks: a HypKvCache of at least num_blocks * block_size slots is the pool, block i
+ * being its slots [i * block_size, (i + 1) * block_size). Request r's own token j lies in
+ * block tables[r][j / block_size] at j % block_size, and stands at position prefix_len + j
+ * behind a prefix that all requests share, whose token j lies in block
+ * prefix_table[j / block_size]. One batch serves the caches of all layers.
+ *
+ * The arrays are device memory, borrowed for the call; the struct itself is host memory.
+ * Their contents are not visible to the host without a copy: calls never read or write
+ * outside the cache or the arrays whatever they hold, and a block id >= num_blocks is a block
+ * without tokens (nothing is stored there, its keys are not seen). */
+typedef struct HypBatch {
+    uint32_t requests;              /* request slots, at most 4096 */
+    uint32_t block_size;            /* tokens of a block: a power of two, at most 65536 */
+    uint32_t num_blocks;            /* blocks of the pool */
+    uint32_t max_blocks;            /* entries of a request's row of tables */
+    uint32_t max_rows;              /* rows of the step's arrays, at most 2^20 */
+    uint32_t prefix_len;            /* tokens of the shared prefix (0: none), at most 2^24 */
+    const uint32_t* prefix_table;   /* [ceil(prefix_len / block_size)], NULL without a prefix */
+    uint32_t* tables;               /* [requests][max_blocks] */
+    uint32_t* lens;                 /* [requests]: own tokens, this step's among them */
+    uint32_t* row_start;            /* [requests + 1]: request r's rows are row_start[r] .. row_start[r + 1] - 1 */
+    uint32_t* slots;                /* [max_rows]: a row's cache slot, or HYP_SLOT_NONE */
+    uint32_t* positions;            /* [max_rows] */
+} HypBatch;
+
+#define HYP_SLOT_NONE 0xFFFFFFFFu
+#define HYP_REQUEST_DONE 0xFFFFFFFFu
+
+/* One step's tables, slot map and positions from the requests' lengths. lens [requests] holds
+ * the tokens each request has (may be batch->lens itself), new_tokens [requests] those it gets
+ * now (0: none; HYP_REQUEST_DONE: it has ended). free_blocks [num_blocks] is a stack of block
+ * ids whose entries free_blocks[taken .. num_blocks - 1] are free; taken and taken_out are one
+ * uint32 each (may be the same).
+ *  - Requests that are done: their blocks go back to the stack, in the order of requests and
+ *    of their tables, as entries [taken - returned, taken); batch->lens becomes 0 and their
+ *    slot can take a new request in the next step. Their row of tables is left as it is.
+ *  - The others are served in order: request r gets the blocks its new tokens need from the
+ *    stack's entry taken - returned upwards (returned ones first), written to its row of
+ *    tables behind those it has; its rows follow the previous request's.
+ *  - served (one uint32) is the first request that does not fit (more than max_rows rows, more
+ *    blocks than are free, more than max_blocks entries, a position past 2^24), or requests
+ *    when all do. It and all behind it get no rows and no blocks in this step.
+ *  - batch->lens: the lengths with the new tokens. batch->row_start, slots and positions: the
+ *    step's rows; rows behind the last have slot HYP_SLOT_NONE and position 0.
+ * All outputs are deterministic. Nothing that is read is changed where taken_out and
+ * batch->lens are arrays of their own, but the entries of the stack below taken. */
+HypStatus hyp_batch_plan(const HypBatch* batch, const uint32_t* lens, const uint32_t* new_tokens,
+                         uint32_t* free_blocks, const uint32_t* taken, uint32_t* taken_out, uint32_t* served,
+                         HypStream stream);
+
+/* hyp_attention_prepare for a batch's rows: row t of the step (t < row_start[requests]) at
+ * positions[t], its K and V stored to slots[t] of the cache (HYP_SLOT_NONE or a slot outside the
+ * cache: not stored),
+ *   q_out[t][h]  <- rope(rms_norm(q[t][h], q_norm))            every head h (q_out may be q);
+ *   K[slot]      <- rope(rms_norm(k_raw[t][j], k_norm))        every kv head j;
+ *   V[slot]      <- rms_norm(v_raw[t][j]) without a weight     (v_raw NULL reads k_raw).
+ * q, q_out [max_rows][n_heads][head_dim], k_raw / v_raw [max_rows][num_kv_heads][head_dim],
+ * q_norm / k_norm bf16 [head_dim], all device memory, 16-byte aligned; the angles as hyp_rope
+ * forms them (positions below 2^24). Values stay fp32 from the input to one rounding of each
+ * output, where hyp_attention_prepare rounds after every step. Rows of one step have different
+ * slots (as a plan gives them); rows behind the last are left as they are. */
+HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_raw, const void* v_raw,
+                            uint32_t n_heads, HypKvCache cache, const void* q_norm, const void* k_norm, float eps,
+                            uint32_t rotated_dims, float rope_base, void* q_out, HypStream stream);
+
 /* ---- the model, its KV state and the step ABI (hyperion_mlx.h:50-248) -------------------
  * The reference's model-level entry points over this library's kernels: hyp_model_load
  * makes the projections, norm vectors and layer scalars resident; hyp_prefill_chunk and

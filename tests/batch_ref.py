@@ -1,0 +1,67 @@
+"""Batched serving in numpy, in 64 bits: the references of test_batch_cpu.py and
+test_gpu_batch.py, written from the entry points' definitions."""
+import numpy as np
+
+NONE = 0xFFFFFFFF
+DONE = 0xFFFFFFFF
+
+
+def blocks(tokens, size):
+    return -(-tokens // size)
+
+
+def plan(lens, new, tables, free, taken, block, max_rows, prefix):
+    """hyp_batch_plan one request and one block at a time, as a list is walked. Returns tables,
+    free, taken, served, lens, row_start, slots, positions; entries of free below the returned
+    taken are not defined."""
+    tables, free = tables.copy(), free.copy()
+    num, max_blocks = free.size, tables.shape[1]
+    back = [int(b) for r, (n, m) in enumerate(zip(lens, new)) if m == DONE
+            for b in tables[r, :min(blocks(int(n), block), max_blocks)]][:int(taken)]
+    top = int(taken) - len(back)
+    free[top:int(taken)] = back
+    out, start, slots, positions, served = [], [0], [], [], None
+    for r, (n, m) in enumerate(zip(lens.tolist(), new.tolist())):
+        if m == DONE:
+            out.append(0)
+            start.append(len(slots))
+            continue
+        have, need = blocks(n, block), blocks(n + m, block)
+        if served is None and (len(slots) + m > max_rows or top + need - have > num or need > max_blocks or
+                               prefix + n + m > 2**24):
+            served = r
+        if served is not None:
+            out.append(n)
+            start.append(len(slots))
+            continue
+        tables[r, have:need] = free[top:top + need - have]
+        top += need - have
+        for j in range(n, n + m):
+            b = int(tables[r, j // block])
+            slots.append(b * block + j % block if b < num else NONE)
+            positions.append(prefix + j)
+        out.append(n + m)
+        start.append(len(slots))
+    rest = max_rows - len(slots)
+    return (tables, free, top, len(lens) if served is None else served, np.array(out, np.uint32),
+            np.array(start, np.uint32), np.array(slots + [NONE] * rest, np.uint32),
+            np.array(positions + [0] * rest, np.uint32))
+
+
+def rms(x, weight=None, eps=1e-6):
+    x = x.astype(np.float64)
+    y = x / np.sqrt(np.mean(x * x, -1, keepdims=True) + eps)
+    return y if weight is None else y * weight.astype(np.float64)
+
+
+def rope(x, positions, rotated, base):
+    """x [rows, heads, d] float64; angles are float32 products, as hyp_rope defines them."""
+    d = x.shape[-1]
+    i = np.arange(rotated // 2)
+    inv = (float(np.float32(base)) ** (-2.0 * i / d)).astype(np.float32)
+    theta = (positions.astype(np.float32)[:, None] * inv).astype(np.float64)[:, None]
+    y = x.copy()
+    a, b = x[..., :rotated // 2], x[..., d // 2:d // 2 + rotated // 2]
+    y[..., :rotated // 2] = a * np.cos(theta) - b * np.sin(theta)
+    y[..., d // 2:d // 2 + rotated // 2] = a * np.sin(theta) + b * np.cos(theta)
+    return y
