@@ -52,7 +52,7 @@ EXPORTED = [
     "hyp_rope", "hyp_sample_greedy", "hyp_sample_greedy_topk", "hyp_sample_stochastic",
     "hyp_kv_cache_create", "hyp_kv_cache_free", "hyp_kv_cache_buffers", "hyp_kv_cache_write", "hyp_attention",
     "hyp_attention_prepare", "hyp_residual_rms_norm",
-    "hyp_batch_plan", "hyp_batch_prepare",
+    "hyp_batch_plan", "hyp_batch_prepare", "hyp_batch_attention", "hyp_batch_attention_workspace",
     "hyp_model_create", "hyp_model_free", "hyp_model_load", "hyp_kvstate_create", "hyp_kvstate_free",
     "hyp_prefill_chunk", "hyp_decode_block", "hyp_prefill_chunk_sampled", "hyp_decode_block_sampled",
     "hyp_step_result_create", "hyp_step_result_free", "hyp_step_result_fields", "hyp_model_forward_hidden",
@@ -312,6 +312,8 @@ def load_library(path: str) -> ctypes.CDLL:
         "hyp_residual_rms_norm": [_P, _P, _P, _P, _P, _P, _U32, _U32, ctypes.c_float, _P],
         "hyp_batch_plan": [_P, _P, _P, _P, _P, _P, _P, _P],
         "hyp_batch_prepare": [_P, _P, _P, _P, _U32, _P, _P, _P, ctypes.c_float, _U32, ctypes.c_float, _P, _P],
+        "hyp_batch_attention": [_P, _P, _U32, _P, _U32, ctypes.c_float, _P, _P, _SZ, _P],
+        "hyp_batch_attention_workspace": [_P, _U32, _P, ctypes.POINTER(_SZ)],
         "hyp_model_create": [_PP],
         "hyp_model_free": [_PP],
         "hyp_model_load": [_P, ctypes.POINTER(GeometryParams), ctypes.c_char_p],
@@ -795,6 +797,19 @@ class Batch:
         of the rows <- rope(k_norm(k_raw)) and v_norm(v_raw) (v_raw None: of k_raw)."""
         call("hyp_batch_prepare", self._ref, q.ptr, k_raw.ptr, None if v_raw is None else v_raw.ptr, n_heads,
              cache.handle, q_norm.ptr, k_norm.ptr, eps, rotated, base, q_out.ptr, stream.handle)
+
+
+    def attention_workspace_bytes(self, n_heads: int, cache: KvCache) -> int:
+        """Bytes of a workspace for attention() with this batch's sizes."""
+        out = _SZ()
+        call("hyp_batch_attention_workspace", self._ref, n_heads, cache.handle, ctypes.byref(out))
+        return int(out.value)
+
+    def attention(self, q: "DeviceArray", n_heads: int, cache: KvCache, window: int, scale: float, out: "DeviceArray",
+                  workspace: "DeviceArray", stream: "Stream") -> None:
+        """hyp_batch_attention: the step's rows over the shared prefix and their own tokens."""
+        call("hyp_batch_attention", self._ref, q.ptr, n_heads, cache.handle, window, scale, out.ptr, workspace.ptr,
+             workspace.nbytes, stream.handle)
 
 
 def residual_rms_norm(branch: "DeviceArray", residual: "DeviceArray", post_w: "DeviceArray",

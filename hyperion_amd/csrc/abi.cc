@@ -979,6 +979,43 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
     });
 }
 
+HypStatus hyp_batch_attention(const HypBatch* batch, const void* q, uint32_t n_heads, HypKvCache cache,
+                              uint32_t window, float scale, void* out, void* workspace, size_t workspace_bytes,
+                              HypStream stream) {
+    return abi_call("hyp_batch_attention", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
+        REQUIRE_ARG(std::isfinite(scale), "scale must be finite");
+        if (b.max_rows == 0 || b.requests == 0) return;
+        REQUIRE_ARG(q != nullptr && out != nullptr, "q and out must be non-null device pointers");
+        REQUIRE_ARG(workspace != nullptr, "workspace must be a non-null device pointer");
+        REQUIRE_ARG(aligned16(q) && aligned16(out) && aligned16(workspace), "q, out and workspace must be 16-byte aligned");
+        hyperion::hip::BatchAttentionArgs a{};
+        a.q = static_cast<const uint16_t*>(q);
+        a.cache_k = static_cast<const uint16_t*>(c.k.data());
+        a.cache_v = static_cast<const uint16_t*>(c.v.data());
+        a.out = static_cast<uint16_t*>(out);
+        a.workspace = workspace;
+        a.workspace_bytes = workspace_bytes;
+        a.n_heads = n_heads;
+        a.n_kv_heads = c.num_kv_heads;
+        a.head_dim = c.head_dim;
+        a.window = window;
+        a.scale = scale;
+        hyperion::hip::launch_batch_attention(b, a, s);
+    });
+}
+
+HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads, HypKvCache cache, size_t* out_bytes) {
+    return abi_call("hyp_batch_attention_workspace", [&] {
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
+        REQUIRE_ARG(out_bytes != nullptr, "out_bytes must be non-null");
+        *out_bytes = hyperion::hip::batch_attention_workspace_bytes(b, n_heads, c.num_kv_heads, c.head_dim);
+    });
+}
+
 HypStatus hyp_residual_rms_norm(const void* branch, void* residual, const void* post_weight, const void* scalar,
                                 const void* next_weight, void* next, uint32_t m, uint32_t hidden, float eps,
                                 HypStream stream) {

@@ -42,4 +42,17 @@ struct BatchPrepareArgs {
 };
 void launch_batch_prepare(const BatchView& b, const BatchPrepareArgs& a, hipStream_t stream);
 
+struct BatchAttentionArgs {
+    const uint16_t* q;         // [max_rows][n_heads][head_dim]
+    const uint16_t* cache_k;   // [capacity][n_kv_heads][head_dim]
+    const uint16_t* cache_v;
+    uint16_t* out;
+    void* workspace;
+    size_t workspace_bytes;
+    uint32_t n_heads, n_kv_heads, head_dim, window;
+    float scale;
+};
+size_t batch_attention_workspace_bytes(const BatchView& b, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+void launch_batch_attention(const BatchView& b, const BatchAttentionArgs& a, hipStream_t stream);
+
 }  // namespace hyperion::hip

@@ -457,6 +457,26 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
                             uint32_t n_heads, HypKvCache cache, const void* q_norm, const void* k_norm, float eps,
                             uint32_t rotated_dims, float rope_base, void* q_out, HypStream stream);
 
+/* Attention of the step's rows over the shared prefix and each request's own tokens: row t of
+ * request r (t = row_start[r] + i, of n rows) stands at position prefix_len + lens[r] - n + i and
+ * sees the key positions p <= its own (with window > 0: p > its own - window) that are tokens of
+ * the prefix or of the request. Grouped-query heads and layouts as hyp_attention: q, out
+ * [max_rows][n_heads][head_dim], device bf16, 16-byte aligned; the scores are scale * q.k (scale
+ * finite). The rows' own K and V are read from the cache: call hyp_batch_prepare first. The
+ * prefix's keys are read for all rows of the batch at once.
+ * fp32 scores and softmax, probabilities in two bf16 terms, output rounded to bf16. A row that
+ * sees no key above -inf gives zeros; a NaN or +inf score that it sees gives NaN; keys that it does not see
+ * change nothing, whatever they hold. Rows behind row_start[requests] are left as they are.
+ * workspace: device memory of hyp_batch_attention_workspace's bytes, 16-byte aligned, whose
+ * contents need not be kept between calls; calls that overlap need one each, and so do graphs
+ * whose replays overlap. Row starts must not decrease. */
+HypStatus hyp_batch_attention(const HypBatch* batch, const void* q, uint32_t n_heads, HypKvCache cache,
+                              uint32_t window, float scale, void* out, void* workspace, size_t workspace_bytes,
+                              HypStream stream);
+/* The workspace of hyp_batch_attention for batches of this size (requests, max_rows and whether there is a
+ * prefix; host only). */
+HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads, HypKvCache cache, size_t* out_bytes);
+
 /* ---- the model, its KV state and the step ABI (hyperion_mlx.h:50-248) -------------------
  * The reference's model-level entry points over this library's kernels: hyp_model_load
  * makes the projections, norm vectors and layer scalars resident; hyp_prefill_chunk and

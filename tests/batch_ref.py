@@ -65,3 +65,42 @@ def rope(x, positions, rotated, base):
     y[..., :rotated // 2] = a * np.cos(theta) - b * np.sin(theta)
     y[..., d // 2:d // 2 + rotated // 2] = a * np.sin(theta) + b * np.cos(theta)
     return y
+
+
+def attention(q, ck, cv, tables, lens, row_start, block, num_blocks, prefix, prefix_table, window, scale):
+    """hyp_batch_attention in float64, a row at a time: q [rows, H, D], ck / cv [slots, KVH, D] float64.
+    Returns the output and, for each row, an upper bound of sum |q||k| over its keys (for the error
+    of its scores). NaN of keys that a row does not see is never touched."""
+    rows, H, D = q.shape
+    KVH = ck.shape[1]
+    G = H // KVH
+    out, size = np.zeros(q.shape), np.zeros((rows, H))
+    shared = [(j, int(prefix_table[j // block]) * block + j % block) for j in range(prefix)
+              if prefix_table[j // block] < num_blocks]
+    for r, n in enumerate(lens):
+        t0, t1 = int(row_start[r]), int(row_start[r + 1])
+        if t0 == t1:
+            continue
+        n = min(int(n), tables.shape[1] * block)
+        own = [(prefix + j, int(tables[r, j // block]) * block + j % block) for j in range(n)
+               if tables[r, j // block] < num_blocks]
+        keys = np.array(shared + own, np.int64).reshape(-1, 2)
+        for t in range(t0, t1):
+            pos = prefix + n - (t1 - t0) + (t - t0)
+            seen = keys[:, 0] <= pos
+            if window:
+                seen &= keys[:, 0] > pos - window
+            at = keys[seen, 1]
+            if at.size == 0:
+                continue
+            k, v = ck[at], cv[at]
+            for h in range(H):
+                s = scale * (k[:, h // G] @ q[t, h])
+                size[t, h] = np.max(np.abs(k[:, h // G]) @ np.abs(q[t, h]), initial=0.0)
+                m = np.max(s)
+                if m == -np.inf:
+                    continue
+                w = np.exp(s - m)
+                live = w != 0
+                out[t, h] = (w[live] @ v[live, h // G]) / w.sum()
+    return out, size

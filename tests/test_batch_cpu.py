@@ -66,11 +66,20 @@ def prepare_args(b, **over):
             a["base"], a["out"], a["stream"])
 
 
+def attention_args(b, **over):
+    a = dict(q=P, heads=4, cache=CACHE, window=0, scale=1.0, out=P, work=P, bytes=1 << 40, stream=STREAM)
+    a.update(over)
+    return (ctypes.byref(b), a["q"], a["heads"], a["cache"], a["window"], a["scale"], a["out"], a["work"], a["bytes"],
+            a["stream"])
+
+
 @pytest.mark.parametrize("over,says", BAD_BATCHES)
 def test_bad_batches_are_refused_by_every_call(over, says):
     b = fields(**over)
     refused("hyp_batch_plan", *plan_args(b), says=says)
     refused("hyp_batch_prepare", *prepare_args(b), says=says)
+    refused("hyp_batch_attention", *attention_args(b), says=says)
+    refused("hyp_batch_attention_workspace", ctypes.byref(b), 4, CACHE, ctypes.byref(ctypes.c_size_t()), says=says)
 
 
 @pytest.mark.parametrize("over", [dict(lens=None), dict(new=None), dict(free=None), dict(taken=None),
@@ -92,8 +101,38 @@ def test_prepare_refusals(over, says):
     refused("hyp_batch_prepare", *prepare_args(fields(), **over), says=says)
 
 
+@pytest.mark.parametrize("over,says", [
+    (dict(q=None), "non-null"), (dict(out=None), "non-null"), (dict(work=None), "non-null"),
+    (dict(q=ctypes.c_void_p(0x1002)), "aligned"), (dict(out=ctypes.c_void_p(0x1008)), "aligned"),
+    (dict(work=ctypes.c_void_p(0x1004)), "aligned"), (dict(heads=0), "multiple"), (dict(heads=3), "multiple"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(bytes=1000), "workspace too small"),
+    (dict(cache=None), "null"), (dict(stream=None), "null")])
+def test_attention_refusals(over, says):
+    refused("hyp_batch_attention", *attention_args(fields(), **over), says=says)
+
+
+def workspace(b, heads=4):
+    out = ctypes.c_size_t()
+    assert hy.lib().hyp_batch_attention_workspace(ctypes.byref(b), heads, CACHE, ctypes.byref(out)) == 0, hy.last_error()
+    return out.value
+
+
+def test_attention_workspace_is_what_the_call_asks_for():
+    b = fields()
+    need = workspace(b)
+    refused("hyp_batch_attention", *attention_args(b, bytes=need - 1), says="too small")
+    assert workspace(fields(max_rows=64)) > need > workspace(fields(prefix_len=0))
+    refused("hyp_batch_attention_workspace", ctypes.byref(b), 4, CACHE, None, says="out_bytes")
+
+
+def test_attention_refuses_what_its_counters_do_not_hold():
+    b = fields(num_blocks=16, block_size=64, max_blocks=1 << 24, max_rows=1 << 20)
+    refused("hyp_batch_attention", *attention_args(b, bytes=1 << 60), says="too many rows")
+
+
 def test_a_pool_beyond_the_cache_is_refused():
     refused("hyp_batch_prepare", *prepare_args(fields(num_blocks=65)), says="must hold")
+    refused("hyp_batch_attention", *attention_args(fields(num_blocks=65)), says="must hold")
     refused("hyp_batch_prepare", *prepare_args(fields(max_rows=1 << 20), heads=32), says="too large")
 
 

@@ -296,3 +296,254 @@ def test_prepare_turns_as_rope_does(stream):
     hy.rope(xd, rows, H, D, D, 1e4, offset, ref, stream)
     assert np.array_equal(got.to_host(stream), ref.to_host(stream))
     assert np.array_equal(read_cache(cache, (64, H, D), stream)[0][:rows], ref.to_host(stream))
+
+
+# ---- attention --------------------------------------------------------------------------------
+
+def f64(bits):
+    return syn.bf16_to_f32(bits).astype(np.float64)
+
+
+class Scene:
+    """A batch's cache, tables and rows for attention, on the host and the device."""
+
+    def __init__(self, seed, stream, lens, rows, H, KVH, D, block=16, prefix=0, window=0, scale=None, extra_rows=0,
+                 spread=2.0):
+        rng = np.random.default_rng(seed)
+        self.stream, self.H, self.KVH, self.D = stream, H, KVH, D
+        self.block, self.prefix, self.window = block, prefix, window
+        self.scale = D ** -0.5 if scale is None else scale
+        counts = [R.blocks(prefix, block)] + [R.blocks(n, block) for n in lens]
+        self.num = sum(counts) + 2
+        order = rng.permutation(self.num).astype(np.uint32)
+        self.prefix_table = order[:counts[0]]
+        self.tables = np.full((len(lens), max(counts[1:]) + 1), R.NONE, np.uint32)
+        at = counts[0]
+        for r, c in enumerate(counts[1:]):
+            self.tables[r, :c] = order[at:at + c]
+            at += c
+        self.lens = np.array(lens, np.uint32)
+        self.row_start = np.concatenate(([0], np.cumsum(rows))).astype(np.uint32)
+        self.rows = int(self.row_start[-1])
+        bits = lambda size, *shape: syn.bf16_bits((size * rng.standard_normal(shape)).astype(np.float32))  # noqa: E731
+        size = 1.0 if scale is None else D ** -0.25
+        self.q = bits(spread * size, self.rows + extra_rows, H, D)
+        self.ck, self.cv = bits(size, self.num * block, KVH, D), bits(1.0, self.num * block, KVH, D)
+
+    def live_slots(self):
+        """Slots that hold tokens."""
+        at = [int(self.prefix_table[j // self.block]) * self.block + j % self.block for j in range(self.prefix)]
+        for r, n in enumerate(self.lens):
+            at += [int(self.tables[r, j // self.block]) * self.block + j % self.block for j in range(int(n))]
+        at = np.array(at, np.int64)
+        return at[at < self.num * self.block]
+
+    def place(self):
+        s = self.stream
+        self.cache = hy.KvCache(self.num * self.block, self.KVH, self.D)
+        fill_cache(self.cache, self.ck, self.cv, s)
+        n = max(1, self.q.shape[0])
+        self.d_lens, self.d_start = dev(self.lens, s), dev(self.row_start, s)
+        self.d_tables = dev(self.tables, s)
+        self.batch = hy.Batch(self.block, self.num, self.d_tables, self.d_lens, self.d_start,
+                              dev(np.zeros(n, np.uint32), s), dev(np.zeros(n, np.uint32), s), self.prefix,
+                              dev(self.prefix_table, s) if self.prefix else None)
+        self.d_q, self.d_out = dev(self.q, s), dev(np.full(self.q.shape, 0x7FC0, np.uint16), s)
+        need = self.batch.attention_workspace_bytes(self.H, self.cache)
+        self.work = dev(np.full(need + 256, 0xFF, np.uint8), s)   # (parts are NaN until they are written)
+        self.work.nbytes = need
+        return self
+
+    def run(self, stream=None):
+        self.batch.attention(self.d_q, self.H, self.cache, self.window, self.scale, self.d_out, self.work,
+                             stream or self.stream)
+
+    def result(self):
+        out = self.d_out.to_host(self.stream)
+        self.work.nbytes += 256
+        assert np.all(self.work.to_host(self.stream)[-256:] == 0xFF)   # nothing behind the workspace
+        self.work.nbytes -= 256
+        return out
+
+    def check(self, what=""):
+        out = self.result()
+        assert np.all(out[self.rows:] == 0x7FC0)   # rows behind the last are left as they were
+        self.compare(out, what)
+        return out
+
+    def compare(self, out, what=""):
+        """One rounding, 2^-8. Below it: a score is off by the fp32 sums of its product (one rounding a step
+        of 32 dims, and a few for its scaling), which moves every weight by as much, and a
+        probability in two bf16 terms by 2^-16."""
+        ck, cv = f64(self.ck), f64(self.cv)
+        ref, size = R.attention(f64(self.q[:self.rows]), ck, cv, self.tables, self.lens, self.row_start, self.block,
+                                self.num, self.prefix, self.prefix_table, self.window, self.scale)
+        got = f64(out[:self.rows])
+        score = (self.D / 32 + 8) * 2.0**-24 * abs(self.scale) * size[..., None]
+        vmax = np.max(np.abs(cv[self.live_slots()]), initial=0.0, where=np.isfinite(cv[self.live_slots()]))
+        bound = 2.0**-8 * np.abs(ref) + vmax * (2.0**-15 + 2 * score)
+        err = np.abs(got - ref)
+        say(f"  attention {what}: worst {np.max(err / bound, initial=0.0):.3f} of the bound")
+        assert np.all(err <= bound), what
+
+
+SCENES = [
+    # lens, rows, H, KVH, D, block, prefix, window, scale
+    ([1], [1], 4, 2, 64, 16, 0, 0, None),                              # one token sees itself
+    ([5, 1, 0, 33], [1, 1, 0, 1], 16, 8, 256, 16, 0, 0, 1.0),          # an idle request
+    ([40, 7, 65, 64], [1, 1, 1, 1], 16, 8, 256, 16, 100, 0, 1.0),      # a prefix that ends inside a block
+    ([40, 7, 165, 64], [1, 1, 1, 1], 16, 8, 256, 16, 90, 128, 1.0),    # a window across prefix and own tokens
+    ([300, 20], [1, 1], 16, 8, 256, 32, 200, 64, 1.0),                 # a window past the prefix for one of them
+    ([10, 3, 129], [1, 1, 1], 16, 1, 512, 16, 333, 0, 1.0),
+    ([900, 2, 31], [1, 1, 1], 16, 1, 512, 64, 0, 0, 1.0),
+    ([17, 50, 100], [1, 1, 1], 32, 8, 128, 8, 63, 0, None),
+    ([17, 50, 100], [1, 1, 1], 12, 12, 64, 1, 5, 0, None),             # a block a token
+    ([17, 50], [1, 1], 7, 1, 64, 16, 1000, 0, None),                   # odd heads
+    ([30, 9, 64, 33], [5, 9, 1, 4], 16, 8, 256, 16, 50, 0, 1.0),       # drafts
+    ([30, 90, 64, 33], [5, 70, 1, 33], 16, 8, 256, 16, 50, 40, 1.0),   # prompts' ends, window
+    ([40, 33, 130], [40, 33, 64], 16, 1, 512, 16, 70, 0, 1.0),         # whole questions
+    ([260, 1], [257, 1], 6, 2, 128, 128, 0, 0, None),
+    ([30, 200, 1], [30, 99, 1], 8, 8, 64, 16, 45, 50, None),
+    ([70] * 70, [1] * 70, 4, 2, 64, 16, 20, 0, None),                  # more requests than a wave has lanes
+    ([3, 200] * 65, [1, 2] * 65, 4, 1, 128, 16, 64, 100, None),
+    ([9000], [1], 8, 1, 128, 16, 0, 0, None),                          # one long request over many workers
+    ([1], [1], 4, 1, 64, 32, 20000, 0, None),
+]
+
+
+@pytest.mark.parametrize("lens,rows,H,KVH,D,block,prefix,window,scale", SCENES)
+def test_attention(stream, lens, rows, H, KVH, D, block, prefix, window, scale):
+    say(f"attention {len(lens)} requests H={H} KVH={KVH} D={D} block={block} prefix={prefix} window={window}")
+    s = Scene(sum(lens) + D, stream, lens, rows, H, KVH, D, block, prefix, window, scale, extra_rows=3).place()
+    s.run()
+    first = s.check()
+    s.run()
+    assert np.array_equal(first, s.result())   # the same bits again
+
+
+@pytest.mark.parametrize("D,KVH", [(64, 4), (256, 2), (512, 1)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_attention_ignores_what_it_does_not_see(stream, D, KVH, bad):
+    """Every slot without a token, the tokens that a draft row does not see yet, and those before a
+    window hold what is not finite; so does a block outside the pool's place in the cache."""
+    s = Scene(D, stream, [20, 37, 50], [3, 1, 18], 4 * KVH, KVH, D, 16, 45, 30)
+    poison = syn.bf16_bits(np.array([bad], np.float32))[0]
+    rest = np.setdiff1d(np.arange(s.num * s.block), s.live_slots())
+    s.ck[rest], s.cv[rest] = poison, poison
+    s.cv[int(s.tables[0, 1]) * 16 + 3] = poison         # request 0's token 19: seen by its last row alone
+    s.ck[int(s.prefix_table[0]) * 16 + 2] = poison      # before every window
+    s.cv[int(s.prefix_table[0]) * 16 + 2] = poison
+    s.place()
+    s.run()
+    out = s.result()
+    seen = out[2].copy()
+    assert np.all(~np.isfinite(f64(seen)))              # that row takes it
+    out[2] = 0
+    s.cv[int(s.tables[0, 1]) * 16 + 3] = 0
+    ck, cv = f64(s.ck), f64(s.cv)
+    want, _ = R.attention(f64(s.q), ck, cv, s.tables, s.lens, s.row_start, 16, s.num, s.prefix, s.prefix_table, s.window,
+                          s.scale)
+    got = f64(out)
+    keep = np.arange(s.rows) != 2
+    vmax = np.max(np.abs(cv), where=np.isfinite(cv), initial=0.0)
+    assert np.all(np.abs(got - want)[keep] <= 2.0**-8 * np.abs(want[keep]) + vmax * 2.0**-12)
+
+
+def test_attention_scores_that_are_not_finite(stream):
+    """Rows whose every score is -inf give zeros; a NaN score gives NaN; -inf scores beside finite ones
+    weigh nothing; the lowest finite value is a value."""
+    D = 64
+    s = Scene(1, stream, [20, 20, 20, 20], [1, 1, 1, 1], 2, 2, D, 16, 0, 0, scale=1.0)
+    at = [s.tables[r, :2].astype(np.int64) for r in range(4)]
+    for r in range(4):
+        s.q[r] = syn.bf16_bits(np.ones((2, D), np.float32))
+    inf, nan, low = (syn.bf16_bits(np.array([v], np.float32))[0] for v in (-np.inf, np.nan, -3e38))
+    for b in at[0]:
+        s.ck[b * 16:(b + 1) * 16] = inf
+    s.ck[at[1][0] * 16 + 5, :, 3] = nan
+    s.ck[at[2][0] * 16 + 5, :, 3] = inf
+    s.ck[at[3][0] * 16 + 7, :, 0] = low
+    s.place()
+    s.run()
+    out = f64(s.result())
+    assert np.all(out[0] == 0.0) and np.all(np.isnan(out[1]))
+    ref, _ = R.attention(f64(s.q[2:]), f64(s.ck), f64(s.cv), s.tables[2:], s.lens[2:], u32(0, 1, 2), 16, s.num, 0, u32(), 0,
+                         1.0)
+    assert np.all(np.abs(out[2:] - ref) <= 2.0**-8 * np.abs(ref) + 2.0**-12)
+
+
+def test_attention_blocks_outside_the_pool_hold_no_tokens(stream):
+    s = Scene(2, stream, [40, 40, 20], [1, 1, 2], 8, 2, 128, 8, 30, 0)
+    s.tables[0, 1] = s.num                   # a block in the middle
+    s.tables[1, :] = 0xFFFFFF00              # every own block
+    s.prefix_table[2] = 4000000000
+    s.place()
+    s.run()
+    s.check("with missing blocks")
+
+
+def test_attention_lengths_at_odds_with_rows(stream):
+    """More rows than tokens: the first rows stand before the own tokens, or before everything. Lengths
+    past the tables end at the tables."""
+    s = Scene(3, stream, [2, 0, 30, 1], [6, 4, 2, 9], 4, 2, 64, 16, 5, 0)
+    s.lens[2] = 4000000000
+    s.tables = s.tables[:, :2]
+    s.place()
+    s.run()
+    out = f64(s.result())
+    s.lens[2] = 32
+    ref, _ = R.attention(f64(s.q), f64(s.ck), f64(s.cv), s.tables, s.lens, s.row_start, 16, s.num, 5, s.prefix_table, 0,
+                         s.scale)
+    assert np.any(np.all(ref == 0, axis=(1, 2)))     # rows that see nothing are among them
+    assert np.all(np.abs(out - ref) <= 2.0**-8 * np.abs(ref) + 2.0**-12 * 6)
+
+
+@pytest.mark.parametrize("starts", [(0, 9, 3, 20, 5), (7, 3, 2, 1, 0), (0, 4000000000, 2, 9, 12), (0, 2, 4, 6, 99), (5, 6, 7, 8, 9),
+                                    (0, 12, 0, 12, 12)])
+def test_attention_holds_its_bounds_on_damaged_row_starts(stream, starts):
+    s = Scene(4, stream, [30, 20, 9, 40], [3, 3, 3, 3], 4, 2, 64, 16, 20, 0)
+    s.row_start = np.array(starts, np.uint32)
+    s.rows = 0
+    s.place()
+    s.run()
+    s.result()                               # (the workspace's end is untouched; the outputs are not defined)
+
+
+def test_attention_recorded_and_replayed_with_new_lengths(stream):
+    """A graph reads the lengths on the device; two recorded calls with a workspace each replay beside
+    one another."""
+    other = hy.Stream()
+    scenes = [Scene(7 + i, stream, [30, 200, 64], [1, 1, 1], 16, 8, 256, 16, 70, 0, 1.0).place() for i in range(2)]
+    graphs = []
+    for s, st in zip(scenes, (stream, other)):
+        with hy.Graph.capture(st) as g:
+            s.run(st)
+        graphs.append(g)
+    for cut in (0, 29, 5, 17):
+        for s in scenes:
+            s.lens = np.array([30 - cut, 200 - 6 * cut, 64], np.uint32)
+            s.d_lens.upload(s.lens, stream)
+            s.d_out.upload(np.full(s.q.shape, 0x7FC0, np.uint16), stream)
+        for g, st in zip(graphs, (stream, other)):
+            g.launch(st)
+        other.synchronize()
+        for s in scenes:
+            s.check(f"replayed, {cut} fewer")
+    for g in graphs:
+        g.close()
+    other.close()
+
+
+def test_attention_of_one_request_agrees_with_hyp_attention(stream):
+    """Blocks in order and no prefix: the batch's attention is hyp_attention's over a linear cache, up
+    to the latter's probabilities in one bf16 term."""
+    H, KVH, D, n = 16, 8, 256, 700
+    s = Scene(11, stream, [n], [1], H, KVH, D, 16, 0, 0, 1.0)
+    s.tables[0, :R.blocks(n, 16)] = np.arange(R.blocks(n, 16))
+    s.place()
+    s.run()
+    got = f64(s.check("in order"))
+    out = hy.DeviceArray(s.q.shape, np.uint16)
+    hy.call("hyp_attention", s.d_q.ptr, None, None, 1, H, s.cache.handle, n - 1, n - 1, 0, out.ptr, stream.handle)
+    ref = f64(out.to_host(stream))
+    assert np.all(np.abs(got - ref) <= 2.0**-7 * np.abs(ref) + 2.0**-9 * np.max(np.abs(f64(s.cv))))
