@@ -53,6 +53,7 @@ EXPORTED = [
     "hyp_kv_cache_create", "hyp_kv_cache_free", "hyp_kv_cache_buffers", "hyp_kv_cache_write", "hyp_attention",
     "hyp_attention_prepare", "hyp_residual_rms_norm",
     "hyp_batch_plan", "hyp_batch_prepare", "hyp_batch_attention", "hyp_batch_attention_workspace",
+    "hyp_sample_batch", "hyp_sample_batch_workspace",
     "hyp_model_create", "hyp_model_free", "hyp_model_load", "hyp_kvstate_create", "hyp_kvstate_free",
     "hyp_prefill_chunk", "hyp_decode_block", "hyp_prefill_chunk_sampled", "hyp_decode_block_sampled",
     "hyp_step_result_create", "hyp_step_result_free", "hyp_step_result_fields", "hyp_model_forward_hidden",
@@ -314,6 +315,8 @@ def load_library(path: str) -> ctypes.CDLL:
         "hyp_batch_prepare": [_P, _P, _P, _P, _U32, _P, _P, _P, ctypes.c_float, _U32, ctypes.c_float, _P, _P],
         "hyp_batch_attention": [_P, _P, _U32, _P, _U32, ctypes.c_float, _P, _P, _SZ, _P],
         "hyp_batch_attention_workspace": [_P, _U32, _P, ctypes.POINTER(_SZ)],
+        "hyp_sample_batch": [_P, _U32, _U32, _P, _P, _P, _P, _P, _SZ, _P],
+        "hyp_sample_batch_workspace": [_U32, _U32, ctypes.POINTER(_SZ)],
         "hyp_model_create": [_PP],
         "hyp_model_free": [_PP],
         "hyp_model_load": [_P, ctypes.POINTER(GeometryParams), ctypes.c_char_p],
@@ -994,6 +997,23 @@ def sample_stochastic(logits: DeviceArray, vocab: int, sampling: Optional[Sampli
     ptr = ctypes.c_void_p((logits.ptr.value or 0) + 2 * row_offset * vocab) if row_offset else logits.ptr
     call("hyp_sample_stochastic", ptr, vocab, _sampling(sampling), rng_state & 0xFFFFFFFFFFFFFFFF, out.ptr,
          stream.handle)
+
+
+def sample_batch_workspace_bytes(rows: int, vocab: int) -> int:
+    """Bytes of a workspace for sample_batch() of this many rows."""
+    out = _SZ()
+    call("hyp_sample_batch_workspace", rows, vocab, ctypes.byref(out))
+    return int(out.value)
+
+
+def sample_batch(logits: DeviceArray, rows: int, vocab: int, configs: DeviceArray, uniforms: DeviceArray,
+                 tokens: DeviceArray, logprobs: Optional[DeviceArray], workspace: Optional[DeviceArray],
+                 stream: Stream) -> None:
+    """hyp_sample_batch: tokens[r] of each row of logits, drawn with configs[r] (device array of
+    SamplingConfig) and uniforms[r]; logprobs[r] too unless None."""
+    call("hyp_sample_batch", logits.ptr, rows, vocab, configs.ptr, uniforms.ptr, tokens.ptr,
+         None if logprobs is None else logprobs.ptr, None if workspace is None else workspace.ptr,
+         0 if workspace is None else workspace.nbytes, stream.handle)
 
 
 def topk_samples(out: DeviceArray, rows: int, stream: Stream):

@@ -17,6 +17,7 @@
 #include "kernels.h"
 #include "decoder.h"
 #include "qlinear.h"
+#include "sample_batch.h"
 #include "sampling.h"
 #include "step_program_host.h"
 
@@ -1013,6 +1014,35 @@ HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads,
         HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
         REQUIRE_ARG(out_bytes != nullptr, "out_bytes must be non-null");
         *out_bytes = hyperion::hip::batch_attention_workspace_bytes(b, n_heads, c.num_kv_heads, c.head_dim);
+    });
+}
+
+HypStatus hyp_sample_batch(const void* logits, uint32_t rows, uint32_t vocab, const HypSamplingConfig* configs,
+                           const float* uniforms, uint32_t* tokens, float* logprobs, void* workspace,
+                           size_t workspace_bytes, HypStream stream) {
+    return abi_call("hyp_sample_batch", [&] {
+        hipStream_t s = stream_of(stream);
+        if (rows == 0) return;
+        REQUIRE_ARG(vocab <= hyperion::hip::sample_batch_max_vocab(), "vocab must be at most 2^23");
+        REQUIRE_ARG(rows <= hyperion::hip::kMaxBatchRows, "a call has at most 2^20 rows");
+        REQUIRE_ARG(vocab == 0 || logits != nullptr, "logits must be a non-null device pointer");
+        REQUIRE_ARG(configs != nullptr && uniforms != nullptr && tokens != nullptr,
+                    "configs, uniforms and tokens must be non-null device pointers");
+        REQUIRE_ARG((reinterpret_cast<uintptr_t>(configs) & 7u) == 0u, "configs must be 8-byte aligned");
+        const size_t need = hyperion::hip::sample_batch_workspace_bytes(rows, vocab);
+        REQUIRE_ARG(workspace_bytes >= need && (need == 0 || workspace != nullptr), "batch sampling: workspace too small");
+        REQUIRE_ARG(aligned16(workspace), "workspace must be 16-byte aligned");
+        hyperion::hip::launch_sample_batch(static_cast<const uint16_t*>(logits), rows, vocab, configs, uniforms, tokens,
+                                           logprobs, workspace, workspace_bytes, s);
+    });
+}
+
+HypStatus hyp_sample_batch_workspace(uint32_t rows, uint32_t vocab, size_t* out_bytes) {
+    return abi_call("hyp_sample_batch_workspace", [&] {
+        REQUIRE_ARG(out_bytes != nullptr, "out_bytes must be non-null");
+        REQUIRE_ARG(vocab <= hyperion::hip::sample_batch_max_vocab(), "vocab must be at most 2^23");
+        REQUIRE_ARG(rows <= hyperion::hip::kMaxBatchRows, "a call has at most 2^20 rows");
+        *out_bytes = hyperion::hip::sample_batch_workspace_bytes(rows, vocab);
     });
 }
 

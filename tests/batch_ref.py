@@ -104,3 +104,26 @@ def attention(q, ck, cv, tables, lens, row_start, block, num_blocks, prefix, pre
                 live = w != 0
                 out[t, h] = (w[live] @ v[live, h // G]) / w.sum()
     return out, size
+
+
+def sample(logits, temperature, top_k, top_p, min_p, u):
+    """hyp_sample_batch of one row of float values, in float64: (token, logprob)."""
+    x = logits.astype(np.float64) + 0.0
+    live = np.flatnonzero(~np.isnan(x) & (x > -np.inf))
+    if live.size == 0:
+        return 0, -np.inf
+    order = live[np.argsort(-x[live], kind="stable")]
+    v = x[order]
+    greedy = not temperature > 0
+    t = 1.0 if greedy else float(temperature)
+    w = (v == np.inf).astype(np.float64) if v[0] == np.inf else np.exp((v - v[0]) / t)
+    mass = np.cumsum(w)
+    keep = v.size if top_k <= 0 else min(v.size, top_k)
+    if 0 < top_p < 1:
+        keep = min(keep, int(np.count_nonzero(mass - w < float(top_p) * mass[-1])))
+    if min_p > 0:
+        keep = min(keep, int(np.count_nonzero(w >= float(min_p))))
+    keep = 1 if greedy else max(1, keep)
+    goal = (min(float(u), 1.0 - 2.0**-24) if u > 0 else 0.0) * mass[keep - 1]
+    j = min(int(np.count_nonzero(mass[:keep] <= goal)), keep - 1)
+    return int(order[j]), float(np.log(w[j] / mass[-1])) if w[j] > 0 else -np.inf

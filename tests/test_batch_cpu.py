@@ -169,3 +169,41 @@ def test_rope_reference_turns_pairs():
     theta = float(np.float32(3) * np.float32(100.0 ** -0.25))
     assert np.allclose(y[0, 0, [1, 5]], [np.cos(theta), np.sin(theta)], atol=1e-15)
     assert np.array_equal(R.rope(x, np.array([3]), 2, 100.0), x)   # pair 1 lies past the rotated dims
+
+
+def sample_args(**over):
+    a = dict(logits=P, rows=3, vocab=1000, configs=P, uniforms=P, tokens=P, logprobs=P, work=P, bytes=1 << 40, stream=STREAM)
+    a.update(over)
+    return tuple(a.values())
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(logits=None), "logits"), (dict(configs=None), "configs"), (dict(uniforms=None), "uniforms"),
+    (dict(tokens=None), "tokens"), (dict(vocab=(1 << 23) + 1), "2^23"), (dict(rows=(1 << 20) + 1), "2^20"),
+    (dict(configs=ctypes.c_void_p(0x1004)), "aligned"), (dict(work=ctypes.c_void_p(0x1008)), "aligned"),
+    (dict(stream=None), "null"), (dict(stream=CACHE), "magic")])
+def test_sample_refusals(over, says):
+    refused("hyp_sample_batch", *sample_args(**over), says=says)
+
+
+def test_sample_workspace_is_what_the_call_asks_for():
+    for rows, vocab in ((1, 262144), (64, 262144), (300, 262144), (2, 100)):
+        need = hy.sample_batch_workspace_bytes(rows, vocab)
+        if need:
+            refused("hyp_sample_batch", *sample_args(rows=rows, vocab=vocab, bytes=need - 1), says="too small")
+            refused("hyp_sample_batch", *sample_args(rows=rows, vocab=vocab, work=None), says="too small")
+    refused("hyp_sample_batch_workspace", 1, 10, None, says="out_bytes")
+    refused("hyp_sample_batch_workspace", 1, (1 << 23) + 1, ctypes.byref(ctypes.c_size_t()), says="2^23")
+    assert hy.lib().hyp_sample_batch(None, 0, 0, None, None, None, None, None, 0, STREAM) == 0   # no rows: nothing to do
+
+
+def test_sample_reference_closed_forms():
+    x = np.log(np.array([0.1, 0.4, 0.1, 0.4]))
+    for u, token in ((0.0, 1), (0.39, 1), (0.41, 3), (0.79, 3), (0.81, 0), (0.91, 2), (0.999, 2), (1.0, 2)):
+        assert R.sample(x, 1.0, 0, 0.0, 0.0, u)[0] == token       # value descending, then index ascending
+    assert R.sample(x, 0.0, 0, 0.0, 0.0, 0.9) == (1, pytest.approx(np.log(0.4)))
+    assert R.sample(x, 1.0, 3, 0.0, 0.0, 0.95)[0] == 0            # 0.4, 0.4, 0.1 kept
+    assert R.sample(x, 1.0, 0, 0.79, 0.0, 0.99)[0] == 3           # the nucleus ends with the token that reaches it
+    assert R.sample(x, 1.0, 0, 0.0, 0.3, 0.99)[0] == 3
+    assert R.sample(np.array([-np.inf, np.nan]), 1.0, 0, 0.0, 0.0, 0.5) == (0, -np.inf)
+    assert R.sample(np.array([3.0, np.inf, np.inf]), 1.0, 0, 0.0, 0.0, 0.7) == (2, pytest.approx(np.log(0.5)))

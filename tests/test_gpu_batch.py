@@ -547,3 +547,186 @@ def test_attention_of_one_request_agrees_with_hyp_attention(stream):
     hy.call("hyp_attention", s.d_q.ptr, None, None, 1, H, s.cache.handle, n - 1, n - 1, 0, out.ptr, stream.handle)
     ref = f64(out.to_host(stream))
     assert np.all(np.abs(got - ref) <= 2.0**-7 * np.abs(ref) + 2.0**-9 * np.max(np.abs(f64(s.cv))))
+
+
+# ---- sampling ---------------------------------------------------------------------------------
+
+CONFIG = np.dtype([("temperature", "<f4"), ("top_k", "<i4"), ("top_p", "<f4"), ("min_p", "<f4"), ("seed", "<u8")])
+
+
+def draw(stream, bits, configs, uniforms, logprobs=True, unaligned=False):
+    """Tokens and logprobs of rows of logits; `unaligned` puts the rows 2 bytes past an aligned place."""
+    rows, vocab = bits.shape
+    flat = np.concatenate((np.zeros(1, np.uint16), bits.ravel())) if unaligned else bits
+    d = dev(flat, stream)
+    if unaligned:
+        class Behind:
+            ptr = ctypes.c_void_p(d.ptr.value + 2)
+        at = Behind()
+    else:
+        at = d
+    need = hy.sample_batch_workspace_bytes(rows, vocab)
+    work = dev(np.full(need + 64, 0xA5, np.uint8), stream)
+    work.nbytes = need
+    tok = dev(np.full(rows + 1, 0xDEAD, np.uint32), stream)
+    lp = dev(np.full(rows + 1, 7.0, np.float32), stream) if logprobs else None
+    hy.sample_batch(at, rows, vocab, dev(configs, stream), dev(np.asarray(uniforms, np.float32), stream), tok, lp, work,
+                    stream)
+    tokens = tok.to_host(stream)
+    assert tokens[rows] == 0xDEAD
+    work.nbytes = need + 64
+    assert np.all(work.to_host(stream)[need:] == 0xA5)
+    if not logprobs:
+        return tokens[:rows], None
+    values = lp.to_host(stream)
+    assert values[rows] == 7.0
+    return tokens[:rows], values[:rows]
+
+
+def check_draw(stream, bits, configs, uniforms, what, **kw):
+    tokens, logprobs = draw(stream, bits, configs, uniforms, **kw)
+    values = syn.bf16_to_f32(bits).reshape(bits.shape)
+    for r in range(bits.shape[0]):
+        c = configs[r]
+        token, lp = R.sample(values[r], float(c["temperature"]), int(c["top_k"]), float(c["top_p"]), float(c["min_p"]),
+                             float(np.float32(uniforms[r])))
+        assert tokens[r] == token, (what, r, c, uniforms[r], int(tokens[r]), token)
+        if logprobs is not None:
+            # one rounding to fp32 of a value with an fp64 error far below it
+            assert logprobs[r] == lp or abs(logprobs[r] - lp) <= 2.0**-24 * abs(lp) + 1e-12, (what, r, logprobs[r], lp)
+
+
+def mixed(rng, rows, vocab):
+    c = np.zeros(rows, CONFIG)
+    c["temperature"] = np.where(rng.random(rows) < 0.15, 0.0, rng.uniform(0.2, 2.0, rows))
+    c["top_k"] = np.where(rng.random(rows) < 0.4, 0, rng.integers(1, vocab + 3, rows))
+    c["top_p"] = np.where(rng.random(rows) < 0.3, rng.integers(0, 2, rows), rng.uniform(0.05, 1.0, rows))
+    c["min_p"] = np.where(rng.random(rows) < 0.5, 0.0, rng.uniform(0.0, 0.4, rows))
+    c["seed"] = rng.integers(0, 2**63, rows)
+    return c
+
+
+@pytest.mark.parametrize("rows,vocab,spread", [(1, 1, 3.0), (1, 2, 3.0), (3, 7, 3.0), (5, 63, 8.0), (2, 513, 1.0),
+                                               (40, 1000, 3.0), (300, 300, 2.0), (9, 8193, 0.05), (6, 50001, 3.0),
+                                               (1, 262144, 3.0), (4, 262144, 9.0), (33, 20000, 3.0), (2, 1000003, 2.0)])
+def test_sample(stream, rows, vocab, spread):
+    say(f"sample rows={rows} vocab={vocab} spread={spread}")
+    rng = np.random.default_rng(rows * 7 + vocab)
+    bits = syn.bf16_bits(np.clip(spread * rng.standard_normal((rows, vocab)), -30, 30).astype(np.float32))
+    configs, uniforms = mixed(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    check_draw(stream, bits, configs, uniforms, "mixed")
+    check_draw(stream, bits, configs, uniforms, "unaligned rows", unaligned=True, logprobs=False)
+    configs[:] = (1.0, 0, 0.0, 0.0, 0)
+    check_draw(stream, bits, configs, np.linspace(0, 1, rows, dtype=np.float32), "temperature alone")
+
+
+def shaped(kind, rng, vocab):
+    x = 3.0 * rng.standard_normal(vocab)
+    if kind == "equal":
+        x[:] = 1.5
+    elif kind == "two values":
+        x = np.where(rng.random(vocab) < 0.5, 2.0, 2.25)
+    elif kind == "zeros":
+        x = np.where(rng.random(vocab) < 0.5, 0.0, -0.0)
+    elif kind == "next to zero":
+        x = 1e-9 * rng.standard_normal(vocab)
+    elif kind == "some next to zero":
+        x[::3] = 1e-9 * rng.standard_normal(x[::3].size)
+    elif kind == "large":
+        x = 90.0 * x
+    elif kind == "largest":
+        x = np.where(rng.random(vocab) < 0.01, 3.3e38, x)
+    elif kind == "lowest masked":
+        x = np.where(rng.random(vocab) < 0.9, -3.3895e38, x)   # bf16's lowest
+    elif kind == "masked":
+        x = np.where(rng.random(vocab) < 0.9, -np.inf, x)
+    elif kind == "one left":
+        x[:] = -np.inf
+        x[vocab // 2] = -4.0
+    elif kind == "nan":
+        x = np.where(rng.random(vocab) < 0.1, np.nan, x)
+    elif kind == "infinite":
+        x = np.where(rng.random(vocab) < 0.02, np.inf, x)
+    elif kind == "nothing":
+        x = np.where(rng.random(vocab) < 0.5, np.nan, -np.inf)
+    elif kind == "below":
+        x = -200.0 - np.abs(40.0 * x)
+    elif kind == "denormal":
+        x = 1e-39 * rng.standard_normal(vocab)
+    elif kind == "descending":
+        x = np.linspace(20, -20, vocab)
+    return syn.bf16_bits(x.astype(np.float32))
+
+
+@pytest.mark.parametrize("vocab", [999, 70000])
+@pytest.mark.parametrize("kind", ["equal", "two values", "zeros", "next to zero", "some next to zero", "large", "largest",
+                                  "lowest masked", "masked", "one left", "nan", "infinite", "nothing", "below", "denormal",
+                                  "descending"])
+def test_sample_rows_of_every_kind(stream, kind, vocab):
+    say(f"sample {kind} vocab={vocab}")
+    rng = np.random.default_rng(vocab)
+    rows = 8
+    bits = np.stack([shaped(kind, rng, vocab) for _ in range(rows)])
+    configs = mixed(rng, rows, vocab)
+    configs["temperature"][:3] = (1.0, 0.0, 50.0)
+    configs[4] = (1.0, 0, 0.5, 0.0, 0)
+    configs[5] = (0.7, 0, 0.0, 0.0, 0)
+    configs[6] = (30.0, 100, 0.0, 0.0, 0)
+    check_draw(stream, bits, configs, rng.random(rows).astype(np.float32), kind)
+
+
+def test_sample_configurations_at_their_ends(stream):
+    """What a configuration may hold beyond its ranges: temperatures below 0, NaN, tiny, infinite;
+    top_k below 0 and past the vocabulary; top_p of 0, 1, NaN; min_p of 1 and more; uniforms of
+    0, next to 1, 1, NaN, negative."""
+    rng = np.random.default_rng(8)
+    vocab = 3000
+    rows = [(t, k, p, m, 0) for t in (1.0, -1.0, np.nan, 1e-30, np.inf) for k in (0, -5, 1, vocab + 9)
+            for p in (0.0, 1.0, np.nan, 1e-9, 0.3) for m in (0.0, 1.0, 2.0, np.nan, -1.0)]
+    configs = np.array(rows, CONFIG)
+    bits = syn.bf16_bits((2.0 * rng.standard_normal((len(rows), vocab))).astype(np.float32))
+    uniforms = np.resize(np.array([0.0, 0.5, 1.0 - 2.0**-24, 1.0, np.nan, -3.0, 2.0**-40], np.float32), len(rows))
+    check_draw(stream, bits, configs, uniforms, "ends")
+
+
+def test_sample_rows_do_not_depend_on_their_batch(stream):
+    """A row gives the same token and the same bits of its logprob alone and in batches of any size."""
+    rng = np.random.default_rng(9)
+    rows, vocab = 270, 40000
+    bits = syn.bf16_bits((3.0 * rng.standard_normal((rows, vocab))).astype(np.float32))
+    configs, uniforms = mixed(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    tokens, logprobs = draw(stream, bits, configs, uniforms)
+    for n in (1, 2, 9, 64, 150):
+        at = slice(7, 7 + n)
+        some, values = draw(stream, bits[at], configs[at], uniforms[at])
+        assert np.array_equal(some, tokens[at]) and np.array_equal(values.view(np.uint32), logprobs[at].view(np.uint32)), n
+
+
+def test_sample_an_empty_vocabulary(stream):
+    tokens, logprobs = draw(stream, np.zeros((2, 0), np.uint16), mixed(np.random.default_rng(0), 2, 1), [0.5, 0.5])
+    assert tokens.tolist() == [0, 0] and np.all(logprobs == -np.inf)
+
+
+def test_sample_in_a_graph(stream):
+    """Recorded once, replayed with other logits, configurations and uniforms."""
+    rng = np.random.default_rng(10)
+    rows, vocab = 5, 30000
+    d, c, u = hy.DeviceArray((rows, vocab), np.uint16), hy.DeviceArray((rows,), CONFIG), hy.DeviceArray((rows,), np.float32)
+    tok, lp = hy.DeviceArray((rows,), np.uint32), hy.DeviceArray((rows,), np.float32)
+    need = hy.sample_batch_workspace_bytes(rows, vocab)
+    work = hy.DeviceArray((need,), np.uint8)
+    with hy.Graph.capture(stream) as g:
+        hy.sample_batch(d, rows, vocab, c, u, tok, lp, work, stream)
+    for _ in range(4):
+        bits = syn.bf16_bits((3.0 * rng.standard_normal((rows, vocab))).astype(np.float32))
+        configs, uniforms = mixed(rng, rows, vocab), rng.random(rows).astype(np.float32)
+        for a, host in ((d, bits), (c, configs), (u, uniforms)):
+            a.upload(host, stream)
+        g.launch(stream)
+        tokens = tok.to_host(stream)
+        same, _ = draw(stream, bits, configs, uniforms)
+        assert np.array_equal(tokens, same)
+        want = [R.sample(syn.bf16_to_f32(bits[r]), *(float(configs[r]["temperature"]), int(configs[r]["top_k"]),
+                         float(configs[r]["top_p"]), float(configs[r]["min_p"]), float(uniforms[r])))[0] for r in range(rows)]
+        assert tokens.tolist() == want
+    g.close()
