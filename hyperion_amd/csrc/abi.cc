@@ -904,7 +904,6 @@ hyperion::hip::BatchView batch_ref(const HypBatch* b) {
     REQUIRE_ARG(b->num_blocks > 0, "num_blocks must be positive");
     REQUIRE_ARG(b->max_rows <= hyperion::hip::kMaxBatchRows, "a step has at most 2^20 rows");
     REQUIRE_ARG(b->prefix_len <= hyperion::hip::kMaxPositions, "prefix_len must be at most 2^24");
-    REQUIRE_ARG(b->prefix_len == 0 || b->prefix_table != nullptr, "a prefix needs its prefix_table");
     REQUIRE_ARG(b->requests == 0 || b->max_blocks == 0 || b->tables != nullptr, "tables must be a non-null device pointer");
     REQUIRE_ARG(b->requests == 0 || b->lens != nullptr, "lens must be a non-null device pointer");
     REQUIRE_ARG(b->row_start != nullptr, "row_start must be a non-null device pointer");
@@ -987,6 +986,7 @@ HypStatus hyp_batch_attention(const HypBatch* batch, const void* q, uint32_t n_h
         hipStream_t s = stream_of(stream);
         const hyperion::hip::BatchView b = batch_ref(batch);
         HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
+        REQUIRE_ARG(b.prefix == 0 || b.prefix_table != nullptr, "a prefix needs its prefix_table");
         REQUIRE_ARG(std::isfinite(scale), "scale must be finite");
         if (b.max_rows == 0 || b.requests == 0) return;
         REQUIRE_ARG(q != nullptr && out != nullptr, "q and out must be non-null device pointers");

@@ -409,7 +409,7 @@ typedef struct HypBatch {
     uint32_t max_blocks;            /* entries of a request's row of tables */
     uint32_t max_rows;              /* rows of the step's arrays, at most 2^20 */
     uint32_t prefix_len;            /* tokens of the shared prefix (0: none), at most 2^24 */
-    const uint32_t* prefix_table;   /* [ceil(prefix_len / block_size)], NULL without a prefix */
+    const uint32_t* prefix_table;   /* [ceil(prefix_len / block_size)]; only hyp_batch_attention reads it */
     uint32_t* tables;               /* [requests][max_blocks] */
     uint32_t* lens;                 /* [requests]: own tokens, this step's among them */
     uint32_t* row_start;            /* [requests + 1]: request r's rows are row_start[r] .. row_start[r + 1] - 1 */

@@ -46,7 +46,6 @@ BAD_BATCHES = [
     (dict(num_blocks=1 << 26), "below 2^30"),
     (dict(max_rows=(1 << 20) + 1), "2^20 rows"),
     (dict(prefix_len=(1 << 24) + 1), "2^24"),
-    (dict(prefix_table=None), "prefix_table"),
     (dict(tables=None), "tables"),
     (dict(lens=None), "lens"),
     (dict(row_start=None), "row_start"),
@@ -133,6 +132,7 @@ def test_attention_refuses_what_its_counters_do_not_hold():
 def test_a_pool_beyond_the_cache_is_refused():
     refused("hyp_batch_prepare", *prepare_args(fields(num_blocks=65)), says="must hold")
     refused("hyp_batch_attention", *attention_args(fields(num_blocks=65)), says="must hold")
+    refused("hyp_batch_attention", *attention_args(fields(prefix_table=None)), says="prefix_table")
     refused("hyp_batch_prepare", *prepare_args(fields(max_rows=1 << 20), heads=32), says="too large")
 
 
