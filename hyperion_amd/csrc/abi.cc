@@ -1013,7 +1013,7 @@ HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads,
         const hyperion::hip::BatchView b = batch_ref(batch);
         HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
         REQUIRE_ARG(out_bytes != nullptr, "out_bytes must be non-null");
-        *out_bytes = hyperion::hip::batch_attention_workspace_bytes(b, n_heads, c.num_kv_heads, c.head_dim);
+        *out_bytes = hyperion::hip::batch_attention_workspace_bytes(b, n_heads, c.head_dim);
     });
 }
 

@@ -52,7 +52,7 @@ struct BatchAttentionArgs {
     uint32_t n_heads, n_kv_heads, head_dim, window;
     float scale;
 };
-size_t batch_attention_workspace_bytes(const BatchView& b, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+size_t batch_attention_workspace_bytes(const BatchView& b, uint32_t n_heads, uint32_t head_dim);
 void launch_batch_attention(const BatchView& b, const BatchAttentionArgs& a, hipStream_t stream);
 
 }  // namespace hyperion::hip

@@ -69,12 +69,13 @@ def rope(x, positions, rotated, base):
 
 def attention(q, ck, cv, tables, lens, row_start, block, num_blocks, prefix, prefix_table, window, scale):
     """hyp_batch_attention in float64, a row at a time: q [rows, H, D], ck / cv [slots, KVH, D] float64.
-    Returns the output and, for each row, an upper bound of sum |q||k| over its keys (for the error
-    of its scores). NaN of keys that a row does not see is never touched."""
+    Returns the output, for each row the largest sum |q||k| over its keys (for the error of its scores),
+    and the weighted mean distance of its values from the output (for the error of its weights). NaN of
+    keys that a row does not see is never touched."""
     rows, H, D = q.shape
     KVH = ck.shape[1]
     G = H // KVH
-    out, size = np.zeros(q.shape), np.zeros((rows, H))
+    out, size, apart = np.zeros(q.shape), np.zeros((rows, H)), np.zeros(q.shape)
     shared = [(j, int(prefix_table[j // block]) * block + j % block) for j in range(prefix)
               if prefix_table[j // block] < num_blocks]
     for r, n in enumerate(lens):
@@ -103,7 +104,8 @@ def attention(q, ck, cv, tables, lens, row_start, block, num_blocks, prefix, pre
                 w = np.exp(s - m)
                 live = w != 0
                 out[t, h] = (w[live] @ v[live, h // G]) / w.sum()
-    return out, size
+                apart[t, h] = (w[live] @ np.abs(v[live, h // G] - out[t, h])) / w.sum()
+    return out, size, apart
 
 
 def sample(logits, temperature, top_k, top_p, min_p, u):

@@ -371,17 +371,28 @@ class Scene:
         self.compare(out, what)
         return out
 
+    def one_term(self):
+        """Whether some rows go through wide tiles, whose probabilities are one bf16 term."""
+        G = self.H // self.KVH
+        n = np.diff(self.row_start.astype(np.int64)) * G
+        tiles = lambda r: -(-r // 128)  # noqa: E731
+        return n.sum() > 16 and bool(self.prefix or np.any(n > 16) or 4 * tiles(n).sum() <= 5 * tiles(n.sum()))
+
     def compare(self, out, what=""):
         """One rounding, 2^-8. Below it: a score is off by the fp32 sums of its product (one rounding a step
         of 32 dims, and a few for its scaling), which moves every weight by as much, and a
-        probability in two bf16 terms by 2^-16."""
+        probability in two bf16 terms by 2^-16. One term moves a weight by up to 2^-8 of itself; the output
+        is the mean by the moved weights, so off by at most 2^-8 / (1 - 2^-8) of its values' mean
+        distance from it."""
         ck, cv = f64(self.ck), f64(self.cv)
-        ref, size = R.attention(f64(self.q[:self.rows]), ck, cv, self.tables, self.lens, self.row_start, self.block,
+        ref, size, apart = R.attention(f64(self.q[:self.rows]), ck, cv, self.tables, self.lens, self.row_start, self.block,
                                 self.num, self.prefix, self.prefix_table, self.window, self.scale)
         got = f64(out[:self.rows])
         score = (self.D / 32 + 8) * 2.0**-24 * abs(self.scale) * size[..., None]
         vmax = np.max(np.abs(cv[self.live_slots()]), initial=0.0, where=np.isfinite(cv[self.live_slots()]))
         bound = 2.0**-8 * np.abs(ref) + vmax * (2.0**-15 + 2 * score)
+        if self.one_term():
+            bound += 2.0**-8 * (1 + 2.0**-7) * apart
         err = np.abs(got - ref)
         say(f"  attention {what}: worst {np.max(err / bound, initial=0.0):.3f} of the bound")
         assert np.all(err <= bound), what
@@ -441,12 +452,12 @@ def test_attention_ignores_what_it_does_not_see(stream, D, KVH, bad):
     out[2] = 0
     s.cv[int(s.tables[0, 1]) * 16 + 3] = 0
     ck, cv = f64(s.ck), f64(s.cv)
-    want, _ = R.attention(f64(s.q), ck, cv, s.tables, s.lens, s.row_start, 16, s.num, s.prefix, s.prefix_table, s.window,
+    want, _, far = R.attention(f64(s.q), ck, cv, s.tables, s.lens, s.row_start, 16, s.num, s.prefix, s.prefix_table, s.window,
                           s.scale)
     got = f64(out)
     keep = np.arange(s.rows) != 2
     vmax = np.max(np.abs(cv), where=np.isfinite(cv), initial=0.0)
-    assert np.all(np.abs(got - want)[keep] <= 2.0**-8 * np.abs(want[keep]) + vmax * 2.0**-12)
+    assert np.all(np.abs(got - want)[keep] <= 2.0**-8 * np.abs(want[keep]) + vmax * 2.0**-12 + 2.0**-8 * 1.01 * far[keep])
 
 
 def test_attention_scores_that_are_not_finite(stream):
@@ -467,9 +478,9 @@ def test_attention_scores_that_are_not_finite(stream):
     s.run()
     out = f64(s.result())
     assert np.all(out[0] == 0.0) and np.all(np.isnan(out[1]))
-    ref, _ = R.attention(f64(s.q[2:]), f64(s.ck), f64(s.cv), s.tables[2:], s.lens[2:], u32(0, 1, 2), 16, s.num, 0, u32(), 0,
+    ref, _, far = R.attention(f64(s.q[2:]), f64(s.ck), f64(s.cv), s.tables[2:], s.lens[2:], u32(0, 1, 2), 16, s.num, 0, u32(), 0,
                          1.0)
-    assert np.all(np.abs(out[2:] - ref) <= 2.0**-8 * np.abs(ref) + 2.0**-12)
+    assert np.all(np.abs(out[2:] - ref) <= 2.0**-8 * np.abs(ref) + 2.0**-12 + 2.0**-8 * 1.01 * far)
 
 
 def test_attention_blocks_outside_the_pool_hold_no_tokens(stream):
@@ -492,10 +503,10 @@ def test_attention_lengths_at_odds_with_rows(stream):
     s.run()
     out = f64(s.result())
     s.lens[2] = 32
-    ref, _ = R.attention(f64(s.q), f64(s.ck), f64(s.cv), s.tables, s.lens, s.row_start, 16, s.num, 5, s.prefix_table, 0,
+    ref, _, far = R.attention(f64(s.q), f64(s.ck), f64(s.cv), s.tables, s.lens, s.row_start, 16, s.num, 5, s.prefix_table, 0,
                          s.scale)
     assert np.any(np.all(ref == 0, axis=(1, 2)))     # rows that see nothing are among them
-    assert np.all(np.abs(out - ref) <= 2.0**-8 * np.abs(ref) + 2.0**-12 * 6)
+    assert np.all(np.abs(out - ref) <= 2.0**-8 * np.abs(ref) + 2.0**-12 * 6 + 2.0**-8 * 1.01 * far)
 
 
 @pytest.mark.parametrize("starts", [(0, 9, 3, 20, 5), (7, 3, 2, 1, 0), (0, 4000000000, 2, 9, 12), (0, 2, 4, 6, 99), (5, 6, 7, 8, 9),
