@@ -918,6 +918,7 @@ HypKvCacheOpaque& batch_cache(const HypBatch& b, HypKvCache cache, uint32_t n_he
     REQUIRE_ARG(static_cast<uint64_t>(b.num_blocks) * b.block_size <= c.capacity,
                 "the cache must hold num_blocks * block_size tokens");
     REQUIRE_ARG(n_heads > 0 && n_heads % c.num_kv_heads == 0, "n_heads must be a multiple of the cache's num_kv_heads");
+    REQUIRE_ARG(n_heads <= 1024u, "n_heads must be at most 1024");
     REQUIRE_ARG(static_cast<uint64_t>(b.max_rows) * n_heads * c.head_dim < (1ull << 31), "q too large");
     return c;
 }

@@ -17,8 +17,9 @@
 // 16x16x32 products, transposed: S^T = K Q^T with the keys' rows straight from memory as the A
 // operand, so a lane holds 8 of a block's keys for one query row and its probabilities are the B
 // operand of O^T = V^T P^T as they stand. V rows go to the wave's own LDS (16-byte loads with the
-// LDS as destination, chunks XOR-swizzled) and come back by transposing reads. The next block's K
-// rows are requested before this one's softmax, its table entries a block earlier.
+// LDS as destination) and come back by transposing reads. The next block's K rows are requested
+// before this one's softmax, its V rows behind its products, its table entries a block earlier; a compute
+// unit's other waves keep the memory busy in between.
 // Probabilities enter as two bf16 terms (p and what its rounding left): the products wait for
 // memory here, and one term alone would add the error of a second rounding to the output's.
 //
@@ -26,6 +27,7 @@
 #include <algorithm>
 
 #include "attention.h"
+#include "attention_batch_walk.h"
 #include "attention_tile.h"
 #include "batch.h"
 #include "common.h"
@@ -36,274 +38,21 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kTileRows = 16;
-constexpr uint32_t kComputeUnits = 256;
-constexpr uint32_t kMaxParts = 256;     // of one group: what a merge reads for a row
 constexpr uint32_t kMergeThreads = 256;
-constexpr uint32_t kScribeRequests = 64;
+constexpr uint32_t kMergeRows = 64;        // (row, head) pairs of a workgroup, at most
+constexpr uint32_t kMergeGroups = 2048;    // workgroups before one takes several
 
-// What the first launch's scribes leave for the others.
-struct Header {
-    uint32_t per, blocks, tiles;         // few rows: units a worker; the prefix's blocks and tiles
-    uint32_t wide_per, wide_units;       // wide tiles: units a worker, of all
-    uint32_t wide_lo, wide_blocks, wide_tiles;   // the prefix's first block, blocks and tiles there
-    uint32_t apart;                      // every request's tiles take the prefix's keys too
-    uint32_t rows;                       // of all requests
-    uint32_t unused[6];
-};
-struct Record {
-    uint32_t unit0, tiles, blocks;                 // few rows
-    uint32_t wide_unit0, wide_tiles, wide_head;    // wide tiles; units of one kv head
-    uint32_t unused[2];
-};
-struct RowRecord {
-    uint32_t request, row;   // its request, its row there
-    int32_t pos;             // its position
-    uint32_t unused;
-};
-
-struct BatchParams {
-    BatchView b;
-    const uint16_t* q;
-    const uint16_t* ck;
-    const uint16_t* cv;
-    uint16_t* out;
-    Header* header;
-    Record* request;
-    RowRecord* row;
-    // Unnormalised rows with their (m, l). Tiles that one worker walked whole, by output row: [0] of
-    // the prefix, [1] of the own tokens. Otherwise the worker's piece 2 w (its first) or 2 w + 1.
-    float2* whole_ml[2];   // [max_rows][H]
-    float* whole_o[2];     // [max_rows][H][D]
-    float2* part_ml;       // [piece][kTileRows]
-    float* part_o;         // [piece][kTileRows][D]
-    float2* wide_ml;       // [piece][kChunkRows]
-    float* wide_o;         // [piece][kChunkRows][D]
-    uint32_t H, KVH, G, window, workers, wide_workers;
-    float scale;        // with log2(e)
-};
-
-// One wave in a workgroup: its LDS holds V rows of a block of 32 keys.
+// A block of 32 keys in LDS: 1 KB units of 8 keys by 64 dims, the unit of keys 8 o and dims 64 g at
+// o D/64 + g, in it each key's 128 bytes as eight 16-byte pieces. One load fills a unit from 8 whole cache
+// lines: lane l brings piece l % 8 of key l / 8. (A load whose neighbouring lanes take 16 bytes of
+// different rows each runs at half the rate.) Which piece of the row stands where is exchanged by key
+// (swizzles below), so that the pieces one operand read takes lie on different banks.
 template <uint32_t D>
-struct RowsLds {
-    static constexpr uint32_t kRow = D * 2u;
-    static constexpr uint32_t kChunks = D / 8u;
-    static constexpr uint32_t kBytes = kKeyBlock * kRow;
-    static constexpr uint32_t kWaves = D >= 512u ? 4u : (D == 256u ? 8u : (D == 128u ? 12u : 16u));   // of a compute unit
-    // A transposing read takes 16 rows (4 kb + 0..3) at one pair of chunks: rows 8 apart share banks.
-    static constexpr uint32_t swz(uint32_t row) { return D == 64u ? ((row >> 1) & 3u) << 1 : (row & 7u) << 1; }
+struct BlockLds {
+    static constexpr uint32_t kGroups = D / 64u;
+    static constexpr uint32_t kOctet = kGroups * 1024u;       // 8 keys
+    static constexpr uint32_t kBytes = 4u * kOctet;
 };
-
-template <uint32_t D>
-constexpr uint32_t kWorkers = kComputeUnits * RowsLds<D>::kWaves;
-
-// A request's (or the prefix's) part of the work for few rows.
-struct Source {
-    uint32_t row0, rows;   // query rows (tokens)
-    uint32_t lo, hi;       // keys [lo, hi) that some row sees
-    int32_t pos;           // the first row's position, counted from the source's key 0
-    uint32_t tiles, blocks;
-    __device__ uint32_t units(uint32_t KVH) const { return KVH * tiles * blocks; }
-};
-
-__device__ __forceinline__ uint32_t tiles_of(uint32_t rows, uint32_t G) { return (rows * G + kTileRows - 1u) / kTileRows; }
-__device__ __forceinline__ uint32_t wide_tiles_of(uint32_t rows, uint32_t G) { return (rows * G + kChunkRows - 1u) / kChunkRows; }
-
-// sum over i < n of floor((a i + b) / m): the whole parts of a and b over m, then the same sum with m
-// and a exchanged.
-__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
-    uint64_t sum = 0u;
-    while (n != 0u) {
-        sum += n * (n - 1u) / 2u * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const uint64_t top = a * n + b;
-        if (top < m) break;
-        n = top / m;
-        b = top % m;
-        const uint64_t t = m;
-        m = a;
-        a = t;
-    }
-    return sum;
-}
-
-// The key blocks of a request's wide tiles. Tile k's rows end at position pos0 + (128 k + 127) / G, so
-// its blocks end at end(k) = floor((128 k + 127 + G (pos0 + 32)) / 32 G), at most all of them, and with
-// a window no more than `most` of them are seen.
-struct WideSpan {
-    uint32_t G, all, most;
-    uint64_t c;
-    __device__ WideSpan(uint32_t G_, uint32_t keys, int32_t pos0, uint32_t window) : G(G_) {
-        all = (keys + kKeyBlock - 1u) / kKeyBlock;
-        const uint64_t seen = (static_cast<uint64_t>(window) + 127u / G + 63u) / kKeyBlock;
-        // (Rows before position 0 are counted from there: their tiles start as much earlier.)
-        const uint64_t early = pos0 < 0 ? (31u - static_cast<int64_t>(pos0)) / kKeyBlock : 0u;
-        most = window != 0u && seen + early < all ? static_cast<uint32_t>(seen + early) : all;
-        c = 127u + static_cast<uint64_t>(G) * (static_cast<uint32_t>(max(pos0, 0)) + 32u);
-    }
-    __device__ uint32_t end(uint32_t k) const {
-        const uint64_t e = (128ull * k + c) / (32ull * G);
-        return e < all ? static_cast<uint32_t>(e) : all;
-    }
-    __device__ uint32_t units(uint32_t k) const { return min(end(k), most); }
-    // Units of the tiles before k: those whose end is below `most`, then `most` each.
-    __device__ uint32_t before(uint32_t k) const {
-        const uint64_t full = 32ull * G * most;
-        const uint64_t rising = full > c ? min(static_cast<uint64_t>(k), (full - c + 127u) / 128u) : 0u;
-        return static_cast<uint32_t>(floor_sum(rising, 32ull * G, 128u, c) + (k - rising) * most);
-    }
-};
-
-__device__ __forceinline__ Source request_source(const BatchParams& p, uint32_t r) {
-    Source s{0u, 0u, 0u, 0u, 0, 0u, 0u};
-    if (r >= p.b.requests) return s;
-    s.row0 = min(p.b.row_start[r], p.b.max_rows);
-    s.rows = max(min(p.b.row_start[r + 1u], p.b.max_rows), s.row0) - s.row0;
-    const uint64_t held = min(static_cast<uint64_t>(p.b.max_blocks) << p.b.shift, static_cast<uint64_t>(1u << 30));
-    s.hi = min(p.b.lens[r], static_cast<uint32_t>(held));
-    s.pos = static_cast<int32_t>(s.hi) - static_cast<int32_t>(s.rows);
-    if (p.window != 0u && static_cast<int64_t>(s.pos) + 1 > p.window) s.lo = s.pos + 1u - p.window;
-    s.tiles = tiles_of(s.rows, p.G);
-    s.blocks = s.rows != 0u && s.hi > s.lo ? (s.hi - s.lo + kKeyBlock - 1u) / kKeyBlock : 0u;
-    return s;
-}
-
-__device__ __forceinline__ uint32_t wave_incl(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const uint32_t y = __shfl_up(v, d, 64);
-        if (lane >= d) v += y;
-    }
-    return v;
-}
-
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
-    return v;
-}
-
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(v, m, 64)));
-    return v;
-}
-
-__device__ __forceinline__ int32_t wave_min(int32_t v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = min(v, static_cast<int32_t>(__shfl_xor(v, m, 64)));
-    return v;
-}
-
-// Which rows go where. Rows of one request that fill wide tiles by themselves read the prefix there, at
-// one pass over all their keys, where that takes at most a quarter more tiles than the rows of all
-// requests together would (apart). Otherwise the prefix is taken for all rows together, in wide tiles
-// from 17 rows on, and a request's own tokens in wide tiles where its rows pass 16.
-struct Walk {
-    Source mine;                // this lane's request of the chunk
-    uint32_t chunk = 0;         // first request of the chunk
-    uint32_t units0;            // before the chunk
-    uint32_t units1;            // inclusive sums over the chunk's lanes
-    Source prefix;              // of few rows
-    uint32_t total;             // units of all
-    uint32_t rows_all;
-    int32_t first_pos;          // the least position of all rows
-    bool apart;
-
-    __device__ bool wide(const BatchParams& p, uint32_t rows) const { return apart || rows * p.G > kTileRows; }
-    // A request as the workers for few rows see it.
-    __device__ Source few(const BatchParams& p, uint32_t r) const {
-        Source s = request_source(p, r);
-        if (wide(p, s.rows)) s.blocks = 0u;
-        return s;
-    }
-    __device__ void load(const BatchParams& p, uint32_t lane) {
-        mine = few(p, chunk + lane);
-        units1 = wave_incl(mine.units(p.KVH), lane);
-    }
-    // Totals of the batch and the prefix's part; then the first chunk. Returns units a worker; 0
-    // where the row starts are no rows of the batch (they would pass the workspace).
-    __device__ uint32_t open(const BatchParams& p, uint32_t lane) {
-        uint32_t rows = 0u, sum = 0u, tiles = 0u;
-        int32_t first = 0x7fffffff;
-        for (uint32_t r = lane; r < p.b.requests; r += 64u) {
-            const Source s = request_source(p, r);
-            sum = min(sum + s.rows, 1u << 25);
-            rows = max(rows, s.row0 + s.rows);
-            tiles += wide_tiles_of(s.rows, p.G);
-            if (s.rows != 0u) first = min(first, s.pos);
-        }
-        if (static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(wave_sum(sum))) > p.b.max_rows) return 0u;
-        rows_all = __builtin_amdgcn_readfirstlane(wave_max(rows));
-        tiles = __builtin_amdgcn_readfirstlane(wave_sum(tiles));
-        first_pos = static_cast<int32_t>(p.b.prefix) + __builtin_amdgcn_readfirstlane(wave_min(first));
-        apart = rows_all * p.G > kTileRows && 4u * tiles <= 5u * wide_tiles_of(rows_all, p.G);
-        uint32_t units = 0u, most = 0u;
-        for (uint32_t r = lane; r < p.b.requests; r += 64u) {
-            const Source s = few(p, r);
-            units += s.units(p.KVH);
-            most = max(most, s.blocks);
-        }
-        units = __builtin_amdgcn_readfirstlane(wave_sum(units));
-        most = __builtin_amdgcn_readfirstlane(wave_max(most));
-        prefix = Source{0u, rows_all, 0u, p.b.prefix, 0, 0u, 0u};
-        if (rows_all != 0u) {
-            prefix.pos = first_pos;
-            if (p.window != 0u && static_cast<int64_t>(first_pos) + 1 > p.window) prefix.lo = first_pos + 1u - p.window;
-            prefix.tiles = tiles_of(rows_all, p.G);
-            if (!wide(p, rows_all) && prefix.hi > prefix.lo)
-                prefix.blocks = (prefix.hi - prefix.lo + kKeyBlock - 1u) / kKeyBlock;
-        }
-        most = max(most, prefix.blocks);
-        total = units + prefix.units(p.KVH);
-        units0 = prefix.units(p.KVH);
-        load(p, lane);
-        return max(max((total + p.workers - 1u) / p.workers, (most + kMaxParts - 2u) / (kMaxParts - 1u)), 1u);
-    }
-    // On to the chunk that holds unit u (u >= units0).
-    __device__ void seek(const BatchParams& p, uint32_t u, uint32_t lane) {
-        while (chunk + 64u < p.b.requests && u >= units0 + __builtin_amdgcn_readlane(units1, 63)) next(p, lane);
-    }
-    __device__ void next(const BatchParams& p, uint32_t lane) {
-        units0 += __builtin_amdgcn_readlane(units1, 63);
-        chunk += 64u;
-        load(p, lane);
-    }
-    // Whether some rows see keys of the prefix outside their request's tiles.
-    __device__ bool has_prefix(const BatchParams& p) const {
-        return prefix.blocks != 0u || (!apart && wide(p, rows_all) && prefix.hi > prefix.lo);
-    }
-    // The keys that a request's wide tiles walk: the prefix's before its own where apart.
-    __device__ WideSpan span(const BatchParams& p, const Source& s) const {
-        const uint32_t pre = apart ? p.b.prefix : 0u;
-        return WideSpan(p.G, s.rows != 0u ? pre + s.hi : 0u, static_cast<int32_t>(pre) + s.pos, p.window);
-    }
-    __device__ uint32_t wide_head(const BatchParams& p, const Source& s) const {
-        return wide(p, s.rows) && s.rows != 0u ? span(p, s).before(wide_tiles_of(s.rows, p.G)) : 0u;
-    }
-};
-
-__device__ __forceinline__ Source shfl_source(const Source& s, uint32_t from) {
-    return Source{static_cast<uint32_t>(__builtin_amdgcn_readlane(s.row0, from)),
-                  static_cast<uint32_t>(__builtin_amdgcn_readlane(s.rows, from)),
-                  static_cast<uint32_t>(__builtin_amdgcn_readlane(s.lo, from)),
-                  static_cast<uint32_t>(__builtin_amdgcn_readlane(s.hi, from)),
-                  __builtin_amdgcn_readlane(s.pos, from),
-                  static_cast<uint32_t>(__builtin_amdgcn_readlane(s.tiles, from)),
-                  static_cast<uint32_t>(__builtin_amdgcn_readlane(s.blocks, from))};
-}
-
-// Position of token row t, whatever its request (counted from the prefix's key 0).
-__device__ __forceinline__ int32_t row_position(const BatchParams& p, uint32_t t) {
-    uint32_t lo = 0u, hi = p.b.requests;
-    while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) / 2u;
-        if (p.b.row_start[mid] <= t) lo = mid; else hi = mid;
-    }
-    const Source s = request_source(p, lo);
-    return static_cast<int32_t>(p.b.prefix) + s.pos + static_cast<int32_t>(t - s.row0);
-}
 
 // One query row again over its visible keys [j0, j1) of a segment alone, against the same
 // reference ref: the matrix products take masked keys with a probability of 0, which a value of V
@@ -365,17 +114,15 @@ template <uint32_t D>
 __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source& s, const uint32_t* table, bool is_prefix,
                                              uint32_t hk, uint32_t tile, uint32_t b0, uint32_t b1, uint32_t to,
                                              uint32_t piece, uint32_t lds, uint32_t lane) {
-    using Lds = RowsLds<D>;
     constexpr uint32_t kSteps = D / 32u;
     constexpr uint32_t kDTiles = D / 16u;
-    constexpr uint32_t kUnitRows = 512u / D;                // V rows of one 1 KB load
-    constexpr uint32_t kUnits = kKeyBlock / kUnitRows;
+    constexpr uint32_t kGroups = BlockLds<D>::kGroups;
     const uint32_t j16 = lane & 15u;
     const uint32_t kb = lane >> 4;
     const uint32_t rows = s.rows * p.G;
     const uint32_t r = tile * kTileRows + j16;
     const bool live = r < rows;
-    const uint32_t token = (live ? r : tile * kTileRows) / p.G;
+    const uint32_t token = p.by_G.of(live ? r : tile * kTileRows);
     const uint32_t head = hk * p.G + (live ? r : tile * kTileRows) - token * p.G;
     const uint16_t* q_row = p.q + (static_cast<size_t>(s.row0 + token) * p.H + head) * D;
 
@@ -401,27 +148,40 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
     };
 
     const size_t head_at = static_cast<size_t>(hk) * D;
-    const size_t stride = static_cast<size_t>(p.KVH) * D;
+    const uint32_t stride = p.KVH * D;
     bf16x8_t kf[2][kSteps];
-    const auto load_k = [&](const uint32_t (&slot)[2]) {
+    // Rows of the block that is loaded next: K of keys 16 c + j16 (the operand's), V of keys 8 o + lane / 8.
+    const uint16_t* const ck = p.ck + head_at + kb * 8u;
+    const uint16_t* const cv = p.cv + head_at + (((lane & 7u) ^ (((lane >> 4) & 3u) << 1)) * 8u);
+    uint32_t slot = 0u;   // of key lane % 32
+    const auto row_of = [&](uint32_t key) {
+        return static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(slot), static_cast<int>(key), 64))) * stride;
+    };
+    const auto load_k = [&] {
 #pragma unroll
         for (uint32_t c = 0; c < 2u; ++c) {
-            const uint16_t* row = p.ck + static_cast<size_t>(slot[c]) * stride + head_at + kb * 8u;
+            const uint16_t* row = ck + row_of(16u * c + j16);
 #pragma unroll
             for (uint32_t st = 0; st < kSteps; ++st) kf[c][st] = *reinterpret_cast<const bf16x8_t*>(row + st * 32u);
         }
     };
-    // Slots of keys jb + 16 c + j16 from their table entries; a block outside the pool gives slot 0
-    // and its bit in the mask of keys that are there (bit 16 c + j16).
-    uint32_t there = 0xFFFFFFFFu;
-    const auto slots_from = [&](const uint32_t (&entry)[2], uint32_t jb, uint32_t (&slot)[2]) {
-        bool ok[2];
+    const auto load_v = [&] {
 #pragma unroll
-        for (uint32_t c = 0; c < 2u; ++c) {
-            ok[c] = entry[c] < p.b.num_blocks;
-            slot[c] = ok[c] ? slot_at(entry[c], jb + 16u * c + j16) : 0u;
+        for (uint32_t oc = 0; oc < 4u; ++oc) {
+            const uint16_t* row = cv + row_of(8u * oc + (lane >> 3));
+#pragma unroll
+            for (uint32_t g = 0; g < kGroups; ++g)
+                __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(row + g * 64u),
+                                                 reinterpret_cast<HYP_LDS void*>(lds + (oc * kGroups + g) * 1024u), 16, 0, 0);
         }
-        there = (static_cast<uint32_t>(__ballot(ok[0])) & 0xFFFFu) | (static_cast<uint32_t>(__ballot(ok[1])) << 16);
+    };
+    // From the keys' table entries; a block outside the pool gives slot 0 and a 0 in the mask of keys
+    // that are there.
+    uint32_t there = 0xFFFFFFFFu;
+    const auto slot_from = [&](uint32_t entry, uint32_t j) {
+        const bool ok = entry < p.b.num_blocks;
+        there = static_cast<uint32_t>(__ballot(ok));
+        return ok ? slot_at(entry, j) : 0u;
     };
 
     f32x4_t o[kDTiles];
@@ -430,36 +190,24 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
     float m = -__builtin_huge_valf();
     float l = 0.0f;
 
-    uint32_t entry[2], slot[2];
+    const uint32_t n32 = lane & 31u;
     const uint32_t j_first = s.lo + b0 * kKeyBlock;
-#pragma unroll
-    for (uint32_t c = 0; c < 2u; ++c) entry[c] = entry_of(j_first + 16u * c + j16);
-    slots_from(entry, j_first, slot);
-    load_k(slot);
-#pragma unroll
-    for (uint32_t c = 0; c < 2u; ++c) entry[c] = entry_of(j_first + kKeyBlock + 16u * c + j16);
+    slot = slot_from(entry_of(j_first + n32), j_first + n32);
+    load_k();
+    load_v();
+    uint32_t entry = entry_of(j_first + kKeyBlock + n32);
 
-    // V operand of dim tile t: group kb reads key rows 4 kb + 0..3 (then + 16), dims 16 t + 0..15.
-    const uint32_t vrow = 4u * kb + (j16 >> 2);
-    const uint32_t v_at = lds + vrow * Lds::kRow + ((((j16 >> 1) & 1u) ^ Lds::swz(vrow)) << 4) + (j16 & 1u) * 8u;
+    // V operand of dim tile t: group kb reads keys 4 kb + 0..3 (then + 16) at pieces 2 (t % 4) + 0..1 of unit
+    // t / 4; pair t % 4 of key k stands at (t % 4) ^ (k / 2 % 4).
+    const uint32_t vkey = 4u * kb + (j16 >> 2);
+    const uint32_t v_at = lds + (vkey >> 3) * BlockLds<D>::kOctet + (vkey & 7u) * 128u + (((vkey >> 1) & 3u) << 5) +
+                          ((j16 >> 1) & 1u) * 16u + (j16 & 1u) * 8u;
     for (uint32_t b = b0; b < b1; ++b) {
         const uint32_t jb = s.lo + b * kKeyBlock;
         const bool more = b + 1u < b1;
         const uint32_t now_there = there;
-        // V of this block (the last block's reads of the LDS are done: their products are).
-        uint32_t ln = lane;
-        asm volatile("" : "+v"(ln));   // per-lane offsets formed here, not kept in registers over the walk
-#pragma unroll
-        for (uint32_t u = 0; u < kUnits; ++u) {
-            const uint32_t vr = u * kUnitRows + ln / Lds::kChunks;
-            const int own = static_cast<int>(slot[u * kUnitRows / 16u]);   // lane j16 holds row 16 c + j16's
-            const uint32_t at = static_cast<uint32_t>(kUnitRows == 1u ? __builtin_amdgcn_readlane(own, u & 15u)
-                                                                      : __shfl(own, static_cast<int>(vr & 15u), 64));
-            const uint16_t* src = p.cv + static_cast<size_t>(at) * stride + head_at +
-                                  (((ln % Lds::kChunks) ^ Lds::swz(vr)) * 8u);
-            __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)src,
-                                             reinterpret_cast<HYP_LDS void*>(lds + u * 1024u), 16, 0, 0);
-        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // K and V of this block have landed
+        __builtin_amdgcn_sched_barrier(0);
         f32x4_t sc[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (uint32_t st = 0; st < kSteps; ++st)
@@ -468,10 +216,9 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
                 sc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c][st], q[st], sc[c], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (more) {
-            slots_from(entry, jb + kKeyBlock, slot);
-            load_k(slot);
-#pragma unroll
-            for (uint32_t c = 0; c < 2u; ++c) entry[c] = entry_of(jb + 2u * kKeyBlock + 16u * c + j16);
+            slot = slot_from(entry, jb + kKeyBlock + n32);
+            load_k();
+            entry = entry_of(jb + 2u * kKeyBlock + n32);
         }
         __builtin_amdgcn_sched_barrier(0);
 
@@ -508,21 +255,15 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
         const bf16x8_t pl = round_p(pr);
 #pragma unroll
         for (uint32_t t = 0; t < kDTiles; ++t) o[t] *= alpha;
-        // V has landed: of the loads behind it (the next block's 2 kSteps of K, its successor's
-        // entries) no more than the K rows' number is outstanding.
-        if (more) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2u * kSteps) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (uint32_t t = 0; t < kDTiles; ++t) {
-            const uint32_t c = 2u * t;
-            const bf16x8_t v = lds_read_tr((v_at ^ ((c & 15u) << 4)) + (c & ~15u) * 16u, 16u * Lds::kRow);
+            const bf16x8_t v = lds_read_tr((v_at ^ ((t % 4u) << 5)) + (t / 4u) * 1024u, 2u * BlockLds<D>::kOctet);
             o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph, o[t], 0, 0, 0);
             o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl, o[t], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // (The products are issued, so their reads of the LDS are done.)
+        if (more) load_v();
         __builtin_amdgcn_sched_barrier(0);
     }
     l = add_lane_xor32(add_lane_xor16(l));
@@ -557,7 +298,7 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
     for (; odd_rows != 0u; odd_rows &= odd_rows - 1u) {
         const uint32_t i = __builtin_ctz(odd_rows);
         const uint32_t rr = tile * kTileRows + i;
-        const uint32_t tok = rr / p.G;
+        const uint32_t tok = p.by_G.of(rr);
         const uint16_t* src = p.q + (static_cast<size_t>(s.row0 + tok) * p.H + hk * p.G + (rr - tok * p.G)) * D;
         const int32_t j0 = max(__shfl(first, static_cast<int>(i)), static_cast<int32_t>(j_first));
         const int32_t j1 = min(__shfl(last, static_cast<int>(i)), static_cast<int32_t>(s.lo + b1 * kKeyBlock) - 1) + 1;
@@ -582,98 +323,6 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
     }
 }
 
-// What the other launches need of the walk: the chunk's requests and their rows.
-__device__ __forceinline__ void scribe(const BatchParams& p, Walk& w, uint32_t per, uint32_t chunk, uint32_t lane) {
-    if (per == 0u) {
-        if (chunk == 0u && lane == 0u) *p.header = Header{};
-        return;
-    }
-    // The prefix's wide tiles (for all rows together) come first.
-    uint32_t tiles = 0u, blocks = 0u, lo = 0u;
-    if (!w.apart && w.wide(p, w.rows_all) && w.prefix.hi > w.prefix.lo) {
-        tiles = wide_tiles_of(w.rows_all, p.G);
-        lo = w.prefix.lo / kKeyBlock;
-        blocks = (w.prefix.hi + kKeyBlock - 1u) / kKeyBlock - lo;
-    }
-    const uint32_t first_unit = p.KVH * tiles * blocks;
-    uint32_t unit0 = first_unit;
-    const auto head_of = [&](const Source& s) { return w.wide_head(p, s); };
-    const auto tiles_here = [&](const Source& s) { return w.wide(p, s.rows) ? wide_tiles_of(s.rows, p.G) : 0u; };
-    while (w.chunk < chunk) {
-        unit0 += wave_sum(p.KVH * head_of(w.mine));
-        w.next(p, lane);
-    }
-    const Source s = w.mine;
-    const uint32_t r = chunk + lane;
-    const uint32_t head = head_of(s);
-    const uint32_t wt = tiles_here(s);
-    const uint32_t units1 = wave_incl(p.KVH * head, lane);
-    if (r < p.b.requests) {
-        p.request[r] = Record{w.units0 + w.units1 - s.units(p.KVH), s.tiles, s.blocks, unit0 + units1 - p.KVH * head, wt, head,
-                              {}};
-    }
-    for (uint32_t i = 0; i < 64u; ++i) {
-        const uint32_t row0 = __builtin_amdgcn_readlane(s.row0, i);
-        const uint32_t rows = __builtin_amdgcn_readlane(s.rows, i);
-        const int32_t pos = static_cast<int32_t>(p.b.prefix) + __builtin_amdgcn_readlane(s.pos, i);
-        for (uint32_t t = lane; t < rows; t += 64u)
-            p.row[row0 + t] = RowRecord{chunk + i, t, pos + static_cast<int32_t>(t), 0u};
-    }
-    if (chunk + 64u < p.b.requests) return;
-    // The last chunk knows all units.
-    const uint32_t all = unit0 + __builtin_amdgcn_readlane(units1, 63);
-    uint32_t most = max(blocks, wave_max(w.apart ? (p.b.prefix + s.hi) / kKeyBlock + 1u : s.hi / kKeyBlock + 1u));
-    for (uint32_t c = lane; c < chunk; c += 64u) most = max(most, request_source(p, c).hi / kKeyBlock + 1u + (w.apart ? p.b.prefix / kKeyBlock + 1u : 0u));
-    most = wave_max(most);
-    if (lane == 0u) {
-        const uint32_t wide_per = max(max((all + p.wide_workers - 1u) / p.wide_workers,
-                                          (most + kMaxParts - 2u) / (kMaxParts - 1u)), 1u);
-        *p.header = Header{per, w.prefix.blocks, w.prefix.tiles, wide_per, all, lo, blocks, tiles, w.apart ? 1u : 0u, w.rows_all, {}};
-    }
-}
-
-template <uint32_t D>
-__global__ __launch_bounds__(64, RowsLds<D>::kWaves / 4u) void attn_batch_rows_kernel(BatchParams p) {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[];
-    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((HYP_LDS uint8_t*)lds_mem));
-    const uint32_t lane = threadIdx.x;
-    Walk w;
-    const uint32_t per = w.open(p, lane);
-    if (blockIdx.x >= p.workers) {
-        scribe(p, w, per, (blockIdx.x - p.workers) * kScribeRequests, lane);
-        return;
-    }
-    const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * per;
-    if (per == 0u || begin >= w.total) return;
-    uint32_t u = static_cast<uint32_t>(begin);
-    const uint32_t end = min(u + per, w.total);
-    while (u < end) {
-        Source s = w.prefix;
-        const uint32_t* table = p.b.prefix_table;
-        uint32_t unit0 = 0u;
-        bool is_prefix = true;
-        if (u >= w.prefix.units(p.KVH)) {
-            w.seek(p, u, lane);
-            const uint64_t behind = __ballot(u < w.units0 + w.units1);
-            if (behind == 0u) return;   // (not with u below the total)
-            const uint32_t at = __builtin_ctzll(behind);
-            s = shfl_source(w.mine, at);
-            table = p.b.tables + static_cast<size_t>(w.chunk + at) * p.b.max_blocks;
-            unit0 = w.units0 + __builtin_amdgcn_readlane(w.units1, at) - s.units(p.KVH);
-            is_prefix = false;
-        }
-        const uint32_t g = (u - unit0) / s.blocks;
-        const uint32_t b0 = u - unit0 - g * s.blocks;
-        const uint32_t b1 = min(s.blocks, b0 + (end - u));
-        const uint32_t hk = g / s.tiles;
-        const uint32_t to = b1 - b0 < s.blocks ? kToPiece : (!is_prefix && !w.has_prefix(p) ? kToOutput : kToRows);
-        rows_segment<D>(p, s, table, is_prefix, __builtin_amdgcn_readfirstlane(hk),
-                        __builtin_amdgcn_readfirstlane(g - hk * s.tiles), __builtin_amdgcn_readfirstlane(b0),
-                        __builtin_amdgcn_readfirstlane(b1), to, 2u * blockIdx.x + (u == begin ? 0u : 1u), lds, lane);
-        u += b1 - b0;
-    }
-}
-
 // Wide tiles (attn_batch_tiles_kernel): the arithmetic of attention_chunk.hip's kernel - 128 query rows
 // of one kv head, 32 a wave on 32x32x16 products, S^T = K Q^T and O^T = V^T P^T, K and V rows by loads
 // straight to two LDS stages - over paged keys. A lane looks up the slot of key lane % 32 of the block
@@ -685,25 +334,24 @@ __global__ __launch_bounds__(64, RowsLds<D>::kWaves / 4u) void attn_batch_rows_k
 // output's own rounding.)
 template <uint32_t D>
 struct TilesLds {
-    static constexpr uint32_t kRow = D * 2u;
-    static constexpr uint32_t kChunks = D / 8u;
-    static constexpr uint32_t kV = kKeyBlock * kRow;
-    static constexpr uint32_t kStage = 2u * kKeyBlock * kRow;
+    static constexpr uint32_t kV = BlockLds<D>::kBytes;
+    static constexpr uint32_t kStage = 2u * BlockLds<D>::kBytes;
     static constexpr uint32_t kOutRow = D * 2u + 16u;
+    static constexpr uint32_t kOutChunks = D / 8u;
     static constexpr uint32_t kOut = kChunkRows * kOutRow;
     static constexpr uint32_t kBytes = 2u * kStage > kOut ? 2u * kStage : kOut;
-    static constexpr uint32_t k_swz(uint32_t row) { return (row & 15u) & (kChunks - 1u); }
-    static constexpr uint32_t v_swz(uint32_t row) { return (((row & 3u) << 2) | ((row >> 1) & 2u)) & (kChunks - 1u); }
 };
 
-constexpr uint32_t kTileThreads = 256;
-constexpr uint32_t kTileWaves = kTileThreads / 64u;
 constexpr uint32_t kWaveRows = 32;
 constexpr float kRescaleLog2 = 8.0f;
 
-// Workers: as many workgroups as the device holds at once.
-template <uint32_t D>
-constexpr uint32_t kWideWorkers = kComputeUnits * (D >= 512u ? 1u : 2u);
+// Workgroups: as many as the device holds at once.
+constexpr uint32_t groups_of(uint32_t D) { return kComputeUnits * (D >= 512u ? 1u : 2u); }
+
+struct TileShared {
+    int32_t range[kGroupWaves][2];   // the waves' first and last keys
+    int32_t pos[kChunkRows];         // positions of a prefix tile's tokens
+};
 
 // The keys that a tile walks, positions 0 .. keys - 1: `pre` of the prefix's tokens, then own ones.
 struct Sequence {
@@ -711,13 +359,13 @@ struct Sequence {
     uint32_t pre, keys;
     uint32_t row0, rows;   // query rows (tokens)
     int32_t pos;           // the first one's position among the keys
-    bool by_record;        // rows of many requests: their positions from the records
+    bool by_request;       // rows of all requests: pos is their least position
 };
 
 template <uint32_t D>
 __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequence& s, uint32_t hk, uint32_t tile,
                                              uint32_t b0, uint32_t b1, uint32_t to, uint32_t piece, uint32_t lds,
-                                             int32_t (*range)[2]) {
+                                             TileShared& shared) {
     using Lds = TilesLds<D>;
     const uint32_t tid = threadIdx.x;
     const uint32_t lane = tid & 63u;
@@ -727,34 +375,48 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
     const uint32_t rows = s.rows * p.G;
     const uint32_t wrow0 = tile * kChunkRows + wave * kWaveRows;
     const uint32_t qrow = min(wrow0 + n, rows - 1u);   // rows past the end repeat the last (not stored)
-    const uint32_t qt = qrow / p.G;
-    const size_t out_row = static_cast<size_t>(s.row0 + qt) * p.H + hk * p.G + (qrow - qt * p.G);
-
+    const uint32_t qt = p.by_G.of(qrow);
     constexpr uint32_t kSteps = D / 16u;
     constexpr uint32_t kDTiles = D / 32u;
     bf16x8_t q[kSteps];
     {
-        const uint16_t* src = p.q + out_row * D + h * 8u;
+        const uint16_t* src = p.q + (static_cast<size_t>(s.row0 + qt) * p.H + hk * p.G + (qrow - qt * p.G)) * D + h * 8u;
 #pragma unroll
         for (uint32_t st = 0; st < kSteps; ++st) q[st] = *reinterpret_cast<const bf16x8_t*>(src + st * 16u);
     }
     // The keys [first, last] that this lane's row sees, and the blocks that some row of the tile sees.
-    const int32_t pos = s.by_record ? p.row[s.row0 + qt].pos : s.pos + static_cast<int32_t>(qt);
+    int32_t pos = s.pos + static_cast<int32_t>(qt);
+    if (s.by_request) {
+        pos = 0x3fffffff;   // past the prefix
+        if (p.window != 0u || s.pos < static_cast<int32_t>(s.keys) - 1) {
+            const uint32_t t0 = p.by_G.of(tile * kChunkRows);
+            const uint32_t t1 = p.by_G.of(min((tile + 1u) * kChunkRows, rows) - 1u);
+            if (tid < kChunkRows) shared.pos[tid] = -1;   // (a row of no request)
+            __syncthreads();
+            for (uint32_t r = tid; r < p.b.requests; r += kGroupThreads) {
+                const Source src = request_source(p, r);
+                for (uint32_t t = max(t0, src.row0); t < src.row0 + src.rows && t <= t1; ++t)
+                    shared.pos[t - t0] = static_cast<int32_t>(p.b.prefix) + src.pos + static_cast<int32_t>(t - src.row0);
+            }
+            __syncthreads();
+            pos = shared.pos[qt - t0];
+        }
+    }
     const int32_t last = min(static_cast<int32_t>(s.keys) - 1, pos);
     const int32_t first = p.window != 0u ? max(0, static_cast<int32_t>(max(static_cast<int64_t>(pos) + 1 - p.window, int64_t{0}))) : 0;
     {
         const int32_t lo = wave_min(first), hi = -wave_min(-last);
         if (lane == 0u) {
-            range[wave][0] = lo;
-            range[wave][1] = hi;
+            shared.range[wave][0] = lo;
+            shared.range[wave][1] = hi;
         }
     }
     __syncthreads();
-    int32_t lo = range[0][0], hi = range[0][1];
+    int32_t lo = shared.range[0][0], hi = shared.range[0][1];
 #pragma unroll
-    for (uint32_t w = 1; w < kTileWaves; ++w) {
-        lo = min(lo, range[w][0]);
-        hi = max(hi, range[w][1]);
+    for (uint32_t w = 1; w < kGroupWaves; ++w) {
+        lo = min(lo, shared.range[w][0]);
+        hi = max(hi, shared.range[w][1]);
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
@@ -785,25 +447,33 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
         return ok ? slot_at(entry, j) : 0u;
     };
 
-    constexpr uint32_t kUnitRows = 512u / D;
-    constexpr uint32_t kUnits = kKeyBlock / kUnitRows / kTileWaves;   // of a wave
-    const size_t stride = static_cast<size_t>(p.KVH) * D;
-    const uint16_t* const ck = p.ck + static_cast<size_t>(hk) * D;
-    const uint16_t* const cv = p.cv + static_cast<size_t>(hk) * D;
-    // Unit i of the wave (1 KB of K rows and of V rows) of the block whose slots are given, into stage st.
-    const auto load_unit = [&](uint32_t slots, uint32_t st, uint32_t i) {
-        uint32_t ln = lane;
-        asm volatile("" : "+v"(ln));   // per-lane addresses formed here, not kept in registers over the walk
-        const uint32_t unit = wave + kTileWaves * i;
-        const uint32_t r = unit * kUnitRows + ln / Lds::kChunks;
-        const uint32_t phys = ln % Lds::kChunks;
-        const uint32_t slot = static_cast<uint32_t>(kUnitRows == 1u ? __builtin_amdgcn_readlane(static_cast<int>(slots), unit)
-                                                                    : __shfl(static_cast<int>(slots), static_cast<int>(r), 64));
-        const size_t at = static_cast<size_t>(slot) * stride;
-        HYP_LDS void* kd = reinterpret_cast<HYP_LDS void*>(lds + st * Lds::kStage + unit * 1024u);
-        HYP_LDS void* vd = reinterpret_cast<HYP_LDS void*>(lds + st * Lds::kStage + Lds::kV + unit * 1024u);
-        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(ck + at + (phys ^ Lds::k_swz(r)) * 8u), kd, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(cv + at + (phys ^ Lds::v_swz(r)) * 8u), vd, 16, 0, 0);
+    // Wave w loads keys 8 w .. 8 w + 7 of a block, K and V. Piece c of K of key k stands at c ^ k_swz(k), of V
+    // at c ^ v_swz(k): an operand read takes one piece of 32 keys of K, four pieces of 8 keys of V.
+    constexpr uint32_t kGroups = BlockLds<D>::kGroups;
+    const uint32_t stride = p.KVH * D;
+    const uint16_t* const ck = p.ck + hk * D;
+    const uint16_t* const cv = p.cv + hk * D;
+    // Registers are short at head_dim 256 and 512: what follows from the lane alone is formed where it is
+    // used, from the lane's number counted anew.
+    const auto lane_again = [] {
+        uint32_t ln;
+        asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(ln));
+        return ln;
+    };
+    size_t at = 0u;   // the row of this lane's key, of the block that is loaded next
+    const auto load_unit = [&](uint32_t st, uint32_t g) {
+        const uint32_t ln = lane_again();
+        const uint32_t k_piece = (ln & 7u) ^ (((ln >> 4) & 3u) | ((wave & 1u) << 2));
+        const uint32_t v_piece = (ln & 7u) ^ (((ln >> 4) & 1u) << 2);
+        const uint32_t to_lds = lds + st * Lds::kStage + (wave * kGroups + g) * 1024u;
+        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(ck + at + k_piece * 8u + g * 64u),
+                                         reinterpret_cast<HYP_LDS void*>(to_lds), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(cv + at + v_piece * 8u + g * 64u),
+                                         reinterpret_cast<HYP_LDS void*>(to_lds + Lds::kV), 16, 0, 0);
+    };
+    const auto row_of = [&](uint32_t slot) {
+        const uint32_t key = 8u * wave + (lane_again() >> 3);
+        return static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(slot), static_cast<int>(key), 64))) * stride;
     };
 
     f32x16_t o[kDTiles];
@@ -814,25 +484,34 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
     float m = -__builtin_huge_valf();   // the softmax reference (log2 domain) of row n
     float l = 0.0f;                     // the sum over this lane's keys
 
-    const uint32_t k_at = lds + n * Lds::kRow + ((h ^ Lds::k_swz(n)) << 4);
-    constexpr uint32_t kSpan = Lds::kChunks < 16u ? Lds::kChunks : 16u;   // chunks a swizzle permutes
-    constexpr uint32_t kAhead = 4u;
-    const uint32_t j16 = lane & 15u;
-    const uint32_t vrow = 4u * h + (j16 >> 2);
-    const uint32_t vchunk = 2u * ((lane >> 4) & 1u) + ((j16 >> 1) & 1u);
-    const uint32_t v_at = lds + Lds::kV + vrow * Lds::kRow + ((vchunk ^ Lds::v_swz(vrow)) << 4) + (j16 & 1u) * 8u;
+    // K operand of step st: key n, piece 2 (st % 4) + h of unit st / 4.
+    constexpr uint32_t kAhead = D == 256u ? 3u : 4u;
+    const auto k_address = [&] {
+        const uint32_t ln = lane_again();
+        const uint32_t key = ln & 31u;
+        const uint32_t swz = ((key >> 1) & 3u) | (((key >> 3) & 1u) << 2);
+        return lds + (key >> 3) * BlockLds<D>::kOctet + (key & 7u) * 128u + (((ln >> 5) ^ swz) << 4);
+    };
+    // V operand of dim tile dt, step t: 16-lane group g reads keys 16 t + 4 h + 0..3 (then + 8) at pieces
+    // 4 (dt % 2) + 2 (g % 2) + 0..1 of unit dt / 2.
+    const auto v_address = [&] {
+        const uint32_t ln = lane_again();
+        const uint32_t key = 4u * (ln >> 5) + ((ln >> 2) & 3u);
+        return lds + Lds::kV + key * 128u + (((key >> 1) & 1u) << 6) + ((ln >> 4) & 1u) * 32u + ((ln >> 1) & 1u) * 16u +
+               (ln & 1u) * 8u;
+    };
 
-    uint32_t slots = 0u, entry = 0u;   // of the block whose rows are requested next
+    uint32_t entry = 0u;
     if (b0 < b1) {
-        slots = slot_from(entry_of(b0 * kKeyBlock + n), b0 * kKeyBlock + n);
+        at = row_of(slot_from(entry_of(b0 * kKeyBlock + n), b0 * kKeyBlock + n));
         entry = entry_of((b0 + 1u) * kKeyBlock + n);
 #pragma unroll
-        for (uint32_t i = 0; i < kUnits; ++i) load_unit(slots, 0u, i);
+        for (uint32_t g = 0; g < kGroups; ++g) load_unit(0u, g);
     }
-    const auto v_read = [&](uint32_t stage, uint32_t u) {
-        const uint32_t c = 4u * (u / 2u);
-        const uint32_t at = ((v_at + stage) ^ ((c % kSpan) << 4)) + (c / kSpan) * kSpan * 16u;
-        return lds_read_tr(at + 16u * (u % 2u) * Lds::kRow, 8u * Lds::kRow);
+    const auto v_read = [&](uint32_t v_at, uint32_t v_odd, uint32_t u) {   // v_at, v_odd: of even and odd dim tiles
+        const uint32_t dt = u / 2u;
+        return lds_read_tr((dt % 2u == 0u ? v_at : v_odd) + (dt / 2u) * 1024u + (u % 2u) * 2u * BlockLds<D>::kOctet,
+                           BlockLds<D>::kOctet);
     };
     constexpr uint32_t kProducts = 2u * kDTiles;
     constexpr bool kLazy = D >= 512u;
@@ -851,15 +530,12 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 __syncthreads();   // block b has landed, and every wave has left the other stage
                 now_there = there;
                 // (The last block loads what it loaded before once more: the same bytes.)
-                if (b + 1u < b1) slots = slot_from(entry, jb + kKeyBlock + n);
-                entry = entry_of(jb + 2u * kKeyBlock + n);
+                if (b + 1u < b1) at = row_of(slot_from(entry, jb + kKeyBlock + (lane_again() & 31u)));
             }
             again = false;
             const uint32_t stage_n = (b + 1u - b0) & 1u;
-            const auto k_read = [&](uint32_t st) {
-                const uint32_t c = 2u * st;
-                return lds_read16(((k_at + stage) ^ ((c % kSpan) << 4)) + (c / kSpan) * kSpan * 16u);
-            };
+            const uint32_t k_at = k_address() + stage;
+            const auto k_read = [&](uint32_t st) { return lds_read16((k_at ^ ((st % 4u) << 5)) + (st / 4u) * 1024u); };
             f32x16_t sc;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
@@ -872,13 +548,16 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 __builtin_amdgcn_sched_barrier(0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[st % kAhead], q[st], sc, 0, 0, 0);
                 if (st + kAhead < kSteps) kf[st % kAhead] = k_read(st + kAhead);
-                if (st % (kSteps / kUnits) == 0u) load_unit(slots, stage_n, st / (kSteps / kUnits));
+                if (st % 4u == 1u) load_unit(stage_n, st / 4u);
             }
             __builtin_amdgcn_sched_barrier(0);
+            const uint32_t entry_next = entry_of(jb + 2u * kKeyBlock + (lane_again() & 31u));
             bf16x8_t vf[kAhead];
+            const uint32_t v_at = v_address() + stage;
+            const uint32_t v_odd = v_at ^ 64u;
             if constexpr (D != 256u) {   // (at 256 their registers are short)
 #pragma unroll
-                for (uint32_t u = 0; u < kAhead; ++u) vf[u] = v_read(stage, u);
+                for (uint32_t u = 0; u < kAhead; ++u) vf[u] = v_read(v_at, v_odd, u);
                 __builtin_amdgcn_sched_barrier(0);
             }
 
@@ -911,6 +590,7 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 m = m_new;
                 l *= alpha;
             }
+            entry = entry_next;
             const float ref = m > -__builtin_huge_valf() ? m : 0.0f;
             float pr[16];
 #pragma unroll
@@ -929,13 +609,13 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
             if constexpr (D == 256u) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (uint32_t u = 0; u < kAhead; ++u) vf[u] = v_read(stage, u);
+                for (uint32_t u = 0; u < kAhead; ++u) vf[u] = v_read(v_at, v_odd, u);
             }
 #pragma unroll
             for (uint32_t u = 0; u < kProducts; ++u) {
                 __builtin_amdgcn_sched_barrier(0);
                 o[u / 2u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u % kAhead], pb[u % 2u], o[u / 2u], 0, 0, 0);
-                if (u + kAhead < kProducts) vf[u % kAhead] = v_read(stage, u + kAhead);
+                if (u + kAhead < kProducts) vf[u % kAhead] = v_read(v_at, v_odd, u + kAhead);
                 if (!kLazy && u / 2u + 1u < kDTiles) {   // the next tile, half of it in each product's shadow
 #pragma unroll
                     for (uint32_t i = 0; i < 8u; ++i) o[u / 2u + 1u][8u * (u % 2u) + i] *= alpha;
@@ -956,28 +636,33 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last loads: none writes LDS past here
     l = half_sum(l);
 
+    const uint32_t ln = lane_again();
+    const uint32_t on = ln & 31u, oh = ln >> 5;   // this lane's row and half again
+    const bool live = wrow0 + on < rows;
+    const uint32_t ot = p.by_G.of(wrow0 + on);
+    const size_t out_row = static_cast<size_t>(s.row0 + ot) * p.H + hk * p.G + (wrow0 + on - ot * p.G);
     float zero = 0.0f;
 #pragma unroll
     for (uint32_t dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) zero = fmaf(o[dt][i], 0.0f, zero);
-    const uint64_t odd_lanes = __ballot(zero != 0.0f && wrow0 + n < rows);
+    const uint64_t odd_lanes = __ballot(zero != 0.0f && live);
     const uint32_t odd_rows = static_cast<uint32_t>(odd_lanes) | static_cast<uint32_t>(odd_lanes >> 32);
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    const size_t prow = to == kToRows ? out_row : static_cast<size_t>(piece) * kChunkRows + wave * kWaveRows + n;
-    float* const po = to == kToRows ? p.whole_o[s.by_record ? 0 : 1] : p.wide_o;
+    const size_t prow = to == kToRows ? out_row : static_cast<size_t>(piece) * kChunkRows + wave * kWaveRows + on;
+    float* const po = to == kToRows ? p.whole_o[s.by_request ? 0 : 1] : p.wide_o;
 
     // o[dt][i] is dim 32 dt + 8 (i / 4) + 4 h + i % 4 of row n.
     __syncthreads();   // every wave has left the stages
     if (to != kToOutput) {
-        if (wrow0 + n < rows) {
+        if (live) {
 #pragma unroll
             for (uint32_t dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
                 for (uint32_t u = 0; u < 4u; ++u)
-                    *reinterpret_cast<float4*>(po + prow * D + 32u * dt + 8u * u + 4u * h) =
+                    *reinterpret_cast<float4*>(po + prow * D + 32u * dt + 8u * u + 4u * oh) =
                         make_float4(o[dt][4 * u], o[dt][4 * u + 1], o[dt][4 * u + 2], o[dt][4 * u + 3]);
-            if (h == 0u) (to == kToRows ? p.whole_ml[s.by_record ? 0 : 1] : p.wide_ml)[prow] = make_float2(m, l);
+            if (oh == 0u) (to == kToRows ? p.whole_ml[s.by_request ? 0 : 1] : p.wide_ml)[prow] = make_float2(m, l);
         }
     } else {
         // The wave's rows through LDS (its own part of the stages), then out as 16-byte pieces of whole rows.
@@ -989,17 +674,17 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 u32x2_t w;
                 w.x = cvt_pk_bf16(o[dt][4 * u] * inv, o[dt][4 * u + 1] * inv);
                 w.y = cvt_pk_bf16(o[dt][4 * u + 2] * inv, o[dt][4 * u + 3] * inv);
-                *reinterpret_cast<HYP_LDS u32x2_t*>(out_lds + n * Lds::kOutRow + (32u * dt + 8u * u + 4u * h) * 2u) = w;
+                *reinterpret_cast<HYP_LDS u32x2_t*>(out_lds + on * Lds::kOutRow + (32u * dt + 8u * u + 4u * oh) * 2u) = w;
             }
         __syncthreads();
-        for (uint32_t c = lane; c < kWaveRows * Lds::kChunks; c += 64u) {
-            const uint32_t r = c / Lds::kChunks;
+        for (uint32_t c = ln; c < kWaveRows * Lds::kOutChunks; c += 64u) {
+            const uint32_t r = c / Lds::kOutChunks;
             const uint32_t gr = wrow0 + r;
             if (gr >= rows) break;
-            const uint32_t t = gr / p.G;
-            const size_t dst = (static_cast<size_t>(s.row0 + t) * p.H + hk * p.G + (gr - t * p.G)) * D + (c % Lds::kChunks) * 8u;
+            const uint32_t t = p.by_G.of(gr);
+            const size_t dst = (static_cast<size_t>(s.row0 + t) * p.H + hk * p.G + (gr - t * p.G)) * D + (c % Lds::kOutChunks) * 8u;
             *reinterpret_cast<u32x4_t*>(p.out + dst) =
-                *reinterpret_cast<const HYP_LDS u32x4_t*>(out_lds + r * Lds::kOutRow + (c % Lds::kChunks) * 16u);
+                *reinterpret_cast<const HYP_LDS u32x4_t*>(out_lds + r * Lds::kOutRow + (c % Lds::kOutChunks) * 16u);
         }
         __syncthreads();   // the next segment's loads go to the same place
     }
@@ -1008,7 +693,7 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's own stores of these rows are done
     for (uint32_t todo = odd_rows; todo != 0u; todo &= todo - 1u) {
         const uint32_t i = __builtin_ctz(todo);
-        const uint32_t tok = (wrow0 + i) / p.G;
+        const uint32_t tok = p.by_G.of(wrow0 + i);
         const size_t to_row = static_cast<size_t>(s.row0 + tok) * p.H + hk * p.G + (wrow0 + i - tok * p.G);
         const int32_t j0 = max(__shfl(first, static_cast<int>(i)), static_cast<int32_t>(b0 * kKeyBlock));
         const int32_t j1 = min(__shfl(last, static_cast<int>(i)), static_cast<int32_t>(b1 * kKeyBlock) - 1) + 1;
@@ -1032,52 +717,44 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
     }
 }
 
+// A workgroup's units of wide tiles.
 template <uint32_t D>
-__global__ __launch_bounds__(kTileThreads, D >= 512u ? 1 : 2) void attn_batch_tiles_kernel(BatchParams p) {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[];
-    __shared__ int32_t range[kTileWaves][2];
-    __shared__ uint32_t found;
-    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((HYP_LDS uint8_t*)lds_mem));
-    const Header head = *p.header;
-    const uint64_t from = static_cast<uint64_t>(blockIdx.x) * head.wide_per;
-    if (head.wide_per == 0u || from >= head.wide_units) return;
-    const uint32_t begin = static_cast<uint32_t>(from);
-    const uint32_t end = min(begin + head.wide_per, head.wide_units);
+__device__ __forceinline__ void wide_units(const BatchParams& p, uint32_t worker, uint32_t begin, uint32_t end, uint32_t lds,
+                                           TileShared& shared) {
+    const uint32_t lane = threadIdx.x & 63u;
     uint32_t u = begin;
     while (u < end) {
-        Sequence s{nullptr, p.b.prefix, p.b.prefix, 0u, head.rows, 0, true};
+        // (Formed again for each tile rather than kept in registers beside the tile's.)
+        Walk w;
+        if (!w.open(p, lane)) return;
+        Sequence s{nullptr, p.b.prefix, p.b.prefix, 0u, w.rows, w.first_pos, true};
         uint32_t hk, tile, off, blocks, block0;
-        if (u < p.KVH * head.wide_tiles * head.wide_blocks) {
-            const uint32_t g = u / head.wide_blocks;
-            blocks = head.wide_blocks;
-            block0 = head.wide_lo;
+        if (u < p.KVH * w.wide_tiles * w.wide_blocks) {
+            const uint32_t g = u / w.wide_blocks;
+            blocks = w.wide_blocks;
+            block0 = w.wide_lo;
             off = u - g * blocks;
-            hk = g / head.wide_tiles;
-            tile = g - hk * head.wide_tiles;
+            hk = g / w.wide_tiles;
+            tile = g - hk * w.wide_tiles;
         } else {
-            __syncthreads();   // the last round's `found` has been read
-            if (threadIdx.x == 0u) found = p.b.requests;
-            __syncthreads();
-            for (uint32_t r = threadIdx.x; r < p.b.requests; r += kTileThreads) {
-                const Record rec = p.request[r];
-                if (u >= rec.wide_unit0 && u - rec.wide_unit0 < p.KVH * rec.wide_head) found = r;
-            }
-            __syncthreads();
-            const uint32_t r = __builtin_amdgcn_readfirstlane(found);
-            if (r >= p.b.requests) return;   // (not with u below the total)
-            const Record rec = p.request[r];
-            const Source src = request_source(p, r);
-            s.own = p.b.tables + static_cast<size_t>(r) * p.b.max_blocks;
-            s.pre = head.apart != 0u ? p.b.prefix : 0u;
+            Chunk c;
+            c.open(p, w, lane, true);
+            const uint32_t at = c.seek(p, w, u, lane);
+            if (at == 64u) return;   // (not with u below the total)
+            const Source src = source_of_lane(c.mine, at);
+            const uint32_t head = from_lane(c.head, at);
+            const uint32_t rel = u - (c.before + from_lane(c.incl, at) - p.KVH * head);
+            s.own = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
+            s.pre = w.apart ? p.b.prefix : 0u;
             s.keys = s.pre + src.hi;
             s.row0 = src.row0;
             s.rows = src.rows;
             s.pos = static_cast<int32_t>(s.pre) + src.pos;
-            s.by_record = false;
-            const WideSpan span(p.G, s.keys, s.pos, p.window);
-            hk = (u - rec.wide_unit0) / rec.wide_head;
-            const uint32_t x = u - rec.wide_unit0 - hk * rec.wide_head;
-            uint32_t t0 = 0u, t1 = rec.wide_tiles;   // the last tile with before() <= x
+            s.by_request = false;
+            const WideSpan span = w.span(p, src);
+            hk = rel / head;
+            const uint32_t x = rel - hk * head;
+            uint32_t t0 = 0u, t1 = wide_tiles_of(src.rows, p.G);   // the last tile with before() <= x
             while (t1 - t0 > 1u) {
                 const uint32_t mid = (t0 + t1) / 2u;
                 if (span.before(mid) <= x) t0 = mid; else t1 = mid;
@@ -1088,104 +765,198 @@ __global__ __launch_bounds__(kTileThreads, D >= 512u ? 1 : 2) void attn_batch_ti
             block0 = span.end(tile) - blocks;
         }
         const uint32_t take = min(blocks - off, end - u);
-        const bool complete = !s.by_record && (head.apart != 0u || (head.blocks == 0u && head.wide_blocks == 0u));
+        const bool complete = !s.by_request && !w.has_prefix();
         const uint32_t to = take < blocks ? kToPiece : (complete ? kToOutput : kToRows);
-        tile_segment<D>(p, s, __builtin_amdgcn_readfirstlane(hk), __builtin_amdgcn_readfirstlane(tile),
-                        __builtin_amdgcn_readfirstlane(block0 + off), __builtin_amdgcn_readfirstlane(block0 + off + take), to,
-                        2u * blockIdx.x + (u == begin ? 0u : 1u), lds, range);
-        u += take;
+        tile_segment<D>(p, s, scalar(hk), scalar(tile), scalar(block0 + off), scalar(block0 + off + take), to,
+                        2u * worker + (u == begin ? 0u : 1u), lds, shared);
+        u = scalar(u + take);
     }
 }
 
-// Joins a row's pieces of the prefix and of its own tokens: one workgroup per row and head, D/4
-// lanes across the dims and as many pieces side by side as fit, then across those in LDS. Rows that
-// one tile's walk finished are left alone.
+// A wave's units of tiles of few rows.
 template <uint32_t D>
-__global__ __launch_bounds__(kMergeThreads) void attn_batch_merge_kernel(BatchParams p) {
+__device__ __forceinline__ void few_units(const BatchParams& p, const Walk& w, uint32_t worker, uint32_t begin, uint32_t end,
+                                          uint32_t lds, uint32_t lane) {
+    Chunk c;
+    c.open(p, w, lane, false);
+    uint32_t u = begin;
+    while (u < end) {
+        Source s = w.prefix;
+        const uint32_t* table = p.b.prefix_table;
+        uint32_t unit0 = 0u;
+        const bool is_prefix = u < w.prefix.units(p.KVH);
+        if (!is_prefix) {
+            const uint32_t at = c.seek(p, w, u, lane);
+            if (at == 64u) return;   // (not with u below the total)
+            s = source_of_lane(c.mine, at);
+            table = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
+            unit0 = c.before + from_lane(c.incl, at) - s.units(p.KVH);
+        }
+        const uint32_t g = floor_div(u - unit0, s.blocks);
+        const uint32_t b0 = u - unit0 - g * s.blocks;
+        const uint32_t b1 = min(s.blocks, b0 + (end - u));
+        const uint32_t hk = floor_div(g, s.tiles);
+        const uint32_t to = b1 - b0 < s.blocks ? kToPiece : (!is_prefix && !w.has_prefix() ? kToOutput : kToRows);
+        rows_segment<D>(p, s, table, is_prefix, scalar(hk), scalar(g - hk * s.tiles), scalar(b0), scalar(b1), to,
+                        2u * worker + (u == begin ? 0u : 1u), lds, lane);
+        u += b1 - b0;
+    }
+}
+
+template <uint32_t D>
+__global__ __launch_bounds__(kGroupThreads, D >= 512u ? 1 : 2) void attn_batch_kernel(BatchParams p) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[];
+    __shared__ TileShared shared;
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((HYP_LDS uint8_t*)lds_mem));
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = scalar(threadIdx.x >> 6);
+    if (blockIdx.x >= p.groups) {
+        scribe(p, ((blockIdx.x - p.groups) * kGroupWaves + wave) * 64u, lane);
+        return;
+    }
+    Walk w;
+    if (!w.open(p, lane)) return;
+    if (blockIdx.x < w.wide_groups) {
+        const uint32_t begin = blockIdx.x * w.wide_per;
+        wide_units<D>(p, blockIdx.x, begin, min(begin + w.wide_per, w.wide_units), lds, shared);
+    } else {
+        const uint32_t worker = (blockIdx.x - w.wide_groups) * kGroupWaves + wave;
+        const uint64_t begin = static_cast<uint64_t>(worker) * w.few_per;
+        if (begin >= w.units) return;   // (no barrier follows)
+        few_units<D>(p, w, worker, static_cast<uint32_t>(begin), min(static_cast<uint32_t>(begin) + w.few_per, w.units),
+                     lds + wave * BlockLds<D>::kBytes, lane);
+    }
+}
+
+// Where a row's pieces lie: of the prefix [0] and of its own tokens [1].
+struct Pieces {
+    uint32_t count;    // 0: no keys there
+    uint32_t place;    // the first worker's piece, then 2 (first + 1), 2 (first + 2), ...
+    uint32_t next;     // 2 (first + 1)
+    uint32_t at;       // the row's place in its tile
+    bool wide;
+
+    __device__ void set(uint32_t unit0, uint32_t blocks, uint32_t per, uint32_t row, bool wide_) {
+        const uint32_t tile_rows = wide_ ? kChunkRows : kTileRows;
+        at = row % tile_rows;
+        wide = wide_;
+        count = 0u;
+        if (blocks == 0u) return;
+        const uint32_t first = floor_div(unit0, per);
+        count = floor_div(unit0 + blocks - 1u, per) - first + 1u;
+        place = 2u * first + (first * per < unit0 ? 1u : 0u);
+        next = 2u * first + 2u;
+    }
+};
+
+// Joins the pieces of rows that one tile's walk did not finish. A workgroup takes `each` consecutive
+// (row, head) pairs: its first threads find their pieces, one pair a thread, then all of it joins the
+// pairs that have any left: D/4 lanes across the dims and as many pieces side by side as fit, then across
+// those in LDS.
+template <uint32_t D>
+__global__ __launch_bounds__(kMergeThreads) void attn_batch_merge_kernel(BatchParams p, Divisor by_H, uint32_t each) {
     constexpr uint32_t kLanes = D / 4u;
     constexpr uint32_t kSide = kMergeThreads / kLanes;
     __shared__ float4 acc[kSide][kLanes];
     __shared__ float2 ml[kSide];
-    const uint32_t t = blockIdx.x;
-    if (t >= min(p.b.row_start[p.b.requests], p.b.max_rows)) return;
-    const uint32_t h = blockIdx.y;
+    __shared__ Pieces found[kMergeRows][2];
+    __shared__ uint64_t todo_of;
+    const uint32_t first_pair = blockIdx.x * each;
+    if (threadIdx.x < 64u) {
+        const uint32_t pair = first_pair + threadIdx.x;
+        const uint32_t t = by_H.of(pair);
+        const uint32_t h = pair - t * p.H;
+        bool todo = threadIdx.x < each && t < min(p.b.row_start[p.b.requests], p.b.max_rows);
+        if (todo) {
+            const Header head = *p.header;
+            const RowRecord row = p.row[t];
+            // (Row starts that skip a row leave its record unwritten.)
+            todo = head.few_per != 0u && row.request < p.b.requests && p.b.row_start[row.request] + row.row == t &&
+                   t < p.b.row_start[row.request + 1u];
+            if (todo) {
+                const Record own = p.request[row.request];
+                const uint32_t hk = p.by_G.of(h);
+                const uint32_t pr = t * p.G + (h - hk * p.G);           // its row among all rows of the kv head
+                const uint32_t orow = row.row * p.G + (h - hk * p.G);   // and among its request's
+                Pieces a, b;
+                if (head.wide_blocks != 0u) {
+                    a.set((hk * head.wide_tiles + pr / kChunkRows) * head.wide_blocks, head.wide_blocks, head.wide_per, pr, true);
+                } else {
+                    a.set((hk * head.tiles + pr / kTileRows) * head.blocks, head.blocks, head.few_per, pr, false);
+                }
+                if (own.wide_head != 0u) {
+                    const Source src = request_source(p, row.request);
+                    const uint32_t pre = head.apart != 0u ? p.b.prefix : 0u;
+                    const WideSpan span(p.G, pre + src.hi, static_cast<int32_t>(pre) + src.pos, p.window);
+                    const uint32_t tile = orow / kChunkRows;
+                    b.set(own.wide_unit0 + hk * own.wide_head + span.before(tile), span.units(tile), head.wide_per, orow, true);
+                } else {
+                    b.set(own.unit0 + (hk * own.tiles + orow / kTileRows) * own.blocks, own.blocks, head.few_per, orow, false);
+                }
+                todo = b.count != 1u || (head.apart == 0u && (head.blocks != 0u || head.wide_blocks != 0u));
+                found[threadIdx.x][0] = a;
+                found[threadIdx.x][1] = b;
+            }
+        }
+        const uint64_t left = __ballot(todo);
+        if (threadIdx.x == 0u) todo_of = left;
+    }
+    __syncthreads();
     const uint32_t side = threadIdx.x / kLanes;
     const uint32_t c = threadIdx.x % kLanes;
-    const Header head = *p.header;
-    const RowRecord row = p.row[t];
-    // (Row starts that skip a row leave its record unwritten.)
-    if (head.per == 0u || row.request >= p.b.requests || p.b.row_start[row.request] + row.row != t ||
-        t >= p.b.row_start[row.request + 1u]) return;
-    const Record own = p.request[row.request];
-    const uint32_t hk = h / p.G;
-    const size_t out_row = static_cast<size_t>(t) * p.H + h;
-    // The pieces of the prefix [0] and of the own tokens [1]: none, the whole rows, or those of workers
-    // first .. first + count - 1.
-    struct Pieces {
-        uint32_t count, first, at, tile_rows;
-        bool whole, later;   // later: the first worker's piece is not its first
-    };
-    const auto pieces = [&](uint32_t unit0, uint32_t blocks, uint32_t per, uint32_t at, uint32_t tile_rows) {
-        Pieces x{0u, 0u, at, tile_rows, false, false};
-        if (blocks == 0u) return x;
-        x.first = unit0 / per;
-        x.count = (unit0 + blocks - 1u) / per - x.first + 1u;
-        x.whole = x.count == 1u;
-        x.later = x.first * per < unit0;
-        return x;
-    };
-    const uint32_t pr = t * p.G + (h - hk * p.G);         // its row among all rows of the kv head
-    const uint32_t orow = row.row * p.G + (h - hk * p.G);   // and among its request's
-    Pieces part[2];
-    part[0] = head.wide_blocks != 0u ? pieces((hk * head.wide_tiles + pr / kChunkRows) * head.wide_blocks, head.wide_blocks,
-                                              head.wide_per, pr % kChunkRows, kChunkRows)
-                                     : pieces((hk * head.tiles + pr / kTileRows) * head.blocks, head.blocks, head.per,
-                                              pr % kTileRows, kTileRows);
-    if (own.wide_head != 0u) {
-        const Source src = request_source(p, row.request);
-        const uint32_t pre = head.apart != 0u ? p.b.prefix : 0u;
-        const WideSpan span(p.G, pre + src.hi, static_cast<int32_t>(pre) + src.pos, p.window);
-        const uint32_t tile = orow / kChunkRows;
-        part[1] = pieces(own.wide_unit0 + hk * own.wide_head + span.before(tile), span.units(tile), head.wide_per,
-                         orow % kChunkRows, kChunkRows);
-    } else {
-        part[1] = pieces(own.unit0 + (hk * own.tiles + orow / kTileRows) * own.blocks, own.blocks, head.per, orow % kTileRows,
-                         kTileRows);
+    for (uint64_t todo = todo_of; todo != 0u; todo &= todo - 1u) {
+        const uint32_t i = static_cast<uint32_t>(__builtin_ctzll(todo));
+        const size_t out_row = first_pair + i;
+        const Pieces a = found[i][0], b = found[i][1];
+        float m = -__builtin_huge_valf();
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const auto join = [&](const float2& x, const float4& v) {
+            if (x.y == 0.0f) return;   // nothing seen there
+            const float m_new = fmaxf(m, x.x);
+            const float ref = m_new > -__builtin_huge_valf() ? m_new : 0.0f;
+            const float f = __builtin_amdgcn_exp2f(m - ref);
+            const float g = __builtin_amdgcn_exp2f(x.x - ref);
+            m = m_new;
+            l = l * f + x.y * g;
+            o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
+        };
+        const uint32_t all = a.count + b.count;
+        const auto load = [&](uint32_t k, float2& x, float4& v) {
+            const bool own = k >= a.count;
+            const uint32_t w = own ? k - a.count : k;
+            const bool whole = (own ? b.count : a.count) == 1u;
+            const bool wide = own ? b.wide : a.wide;
+            const uint32_t place = w == 0u ? (own ? b.place : a.place) : (own ? b.next : a.next) + 2u * (w - 1u);
+            const size_t r = whole ? out_row : static_cast<size_t>(place) * (wide ? kChunkRows : kTileRows) + (own ? b.at : a.at);
+            const float2* pml = whole ? p.whole_ml[own ? 1 : 0] : (wide ? p.wide_ml : p.part_ml);
+            const float* po = whole ? p.whole_o[own ? 1 : 0] : (wide ? p.wide_o : p.part_o);
+            x = pml[r];
+            v = *reinterpret_cast<const float4*>(po + r * D + 4u * c);
+        };
+        // Four pieces in flight.
+        for (uint32_t k = side; k < all; k += 4u * kSide) {
+            float2 x[4];
+            float4 v[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u) {
+                x[u] = make_float2(0.0f, 0.0f);
+                if (k + u * kSide < all) load(k + u * kSide, x[u], v[u]);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u) join(x[u], v[u]);
+        }
+        acc[side][c] = o;
+        if (c == 0u) ml[side] = make_float2(m, l);
+        __syncthreads();
+        if (side == 0u) {
+            for (uint32_t k = 1; k < kSide; ++k) join(ml[k], acc[k][c]);
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            *reinterpret_cast<uint2*>(p.out + out_row * D + 4u * c) =
+                make_uint2(cvt_pk_bf16(o.x * inv, o.y * inv), cvt_pk_bf16(o.z * inv, o.w * inv));
+        }
+        __syncthreads();
     }
-    if (part[1].whole && (head.apart != 0u || (head.blocks == 0u && head.wide_blocks == 0u))) return;
-    float m = -__builtin_huge_valf();
-    float l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const auto join = [&](const float2& x, const float4& v) {
-        if (x.y == 0.0f) return;   // nothing seen there
-        const float m_new = fmaxf(m, x.x);
-        const float ref = m_new > -__builtin_huge_valf() ? m_new : 0.0f;
-        const float a = __builtin_amdgcn_exp2f(m - ref);
-        const float b = __builtin_amdgcn_exp2f(x.x - ref);
-        m = m_new;
-        l = l * a + x.y * b;
-        o = make_float4(o.x * a + v.x * b, o.y * a + v.y * b, o.z * a + v.z * b, o.w * a + v.w * b);
-    };
-    const uint32_t all = part[0].count + part[1].count;
-    for (uint32_t i = side; i < all; i += kSide) {
-        const uint32_t k = i < part[0].count ? 0u : 1u;
-        const Pieces& x = part[k];
-        const uint32_t w = k == 0u ? i : i - part[0].count;
-        const uint32_t piece = 2u * (x.first + w) + (w == 0u && x.later ? 1u : 0u);
-        const bool wide = x.tile_rows == kChunkRows;
-        const size_t r = x.whole ? out_row : static_cast<size_t>(piece) * x.tile_rows + x.at;
-        const float2* pml = x.whole ? p.whole_ml[k] : (wide ? p.wide_ml : p.part_ml);
-        const float* po = x.whole ? p.whole_o[k] : (wide ? p.wide_o : p.part_o);
-        join(pml[r], *reinterpret_cast<const float4*>(po + r * D + 4u * c));
-    }
-    acc[side][c] = o;
-    if (c == 0u) ml[side] = make_float2(m, l);
-    __syncthreads();
-    if (side != 0u) return;
-    for (uint32_t i = 1; i < kSide; ++i) join(ml[i], acc[i][c]);
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    *reinterpret_cast<uint2*>(p.out + out_row * D + 4u * c) =
-        make_uint2(cvt_pk_bf16(o.x * inv, o.y * inv), cvt_pk_bf16(o.z * inv, o.w * inv));
 }
 
 constexpr size_t align256(size_t n) { return (n + 255u) & ~size_t{255u}; }
@@ -1194,16 +965,6 @@ constexpr size_t align256(size_t n) { return (n + 255u) & ~size_t{255u}; }
 struct Layout {
     size_t request, row, whole_ml[2], whole_o[2], ml, o, wide_ml, wide_o, bytes;
 };
-
-uint32_t workers_of(uint32_t D) {
-    switch (D) {
-        case 64: return kWorkers<64>;
-        case 128: return kWorkers<128>;
-        case 256: return kWorkers<256>;
-        default: return kWorkers<512>;
-    }
-}
-uint32_t wide_workers_of(uint32_t D) { return D >= 512u ? kWideWorkers<512> : kWideWorkers<256>; }
 
 Layout layout_of(const BatchView& b, uint32_t H, uint32_t D) {
     const size_t rows = static_cast<size_t>(b.max_rows) * H;
@@ -1220,7 +981,7 @@ Layout layout_of(const BatchView& b, uint32_t H, uint32_t D) {
         l.whole_ml[k] = take(rows * sizeof(float2));
         l.whole_o[k] = take(rows * D * sizeof(float));
     }
-    const size_t pieces = 2u * workers_of(D) * kTileRows, wide = 2u * wide_workers_of(D) * kChunkRows;
+    const size_t pieces = 2u * groups_of(D) * kGroupWaves * kTileRows, wide = 2u * groups_of(D) * kChunkRows;
     l.ml = take(pieces * sizeof(float2));
     l.o = take(pieces * D * sizeof(float));
     l.wide_ml = take(wide * sizeof(float2));
@@ -1231,28 +992,27 @@ Layout layout_of(const BatchView& b, uint32_t H, uint32_t D) {
 
 template <uint32_t D>
 void launch_d(BatchParams p, hipStream_t stream) {
-    static_assert(RowsLds<D>::kBytes <= 65536u && sizeof(Header) <= 256u, "batch attention");
-    constexpr size_t lds = TilesLds<D>::kBytes;
-    if (lds > 65536u) {
+    constexpr size_t lds = TilesLds<D>::kBytes > kGroupWaves * BlockLds<D>::kBytes ? TilesLds<D>::kBytes
+                                                                                 : kGroupWaves * BlockLds<D>::kBytes;
+    static_assert(lds + sizeof(TileShared) <= 160u * 1024u && sizeof(Header) <= 256u, "batch attention");
+    if (lds + sizeof(TileShared) > 65536u) {
         static thread_local int configured_device = -1;
         int dev = 0;
         HYP_HIP_CHECK(hipGetDevice(&dev));
         if (configured_device != dev) {
-            HYP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_batch_tiles_kernel<D>),
+            HYP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_batch_kernel<D>),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
             configured_device = dev;
         }
     }
-    p.workers = kWorkers<D>;
-    p.wide_workers = kWideWorkers<D>;
-    const uint32_t scribes = (p.b.requests + kScribeRequests - 1u) / kScribeRequests;
-    hipLaunchKernelGGL(attn_batch_rows_kernel<D>, dim3(p.workers + scribes), dim3(64), RowsLds<D>::kBytes, stream, p);
+    p.groups = groups_of(D);
+    const uint32_t scribes = (p.b.requests + 64u * kGroupWaves - 1u) / (64u * kGroupWaves);
+    hipLaunchKernelGGL(attn_batch_kernel<D>, dim3(p.groups + scribes), dim3(kGroupThreads), lds, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
-    if (static_cast<uint64_t>(p.b.max_rows) * p.G > kTileRows) {   // (fewer rows make no wide tile)
-        hipLaunchKernelGGL(attn_batch_tiles_kernel<D>, dim3(p.wide_workers), dim3(kTileThreads), lds, stream, p);
-        HYP_HIP_CHECK(hipGetLastError());
-    }
-    hipLaunchKernelGGL(attn_batch_merge_kernel<D>, dim3(p.b.max_rows, p.H), dim3(kMergeThreads), 0, stream, p);
+    const uint64_t pairs = static_cast<uint64_t>(p.b.max_rows) * p.H;
+    const uint32_t each = static_cast<uint32_t>(std::min<uint64_t>((pairs + kMergeGroups - 1u) / kMergeGroups, kMergeRows));
+    hipLaunchKernelGGL(attn_batch_merge_kernel<D>, dim3(static_cast<uint32_t>((pairs + each - 1u) / each)),
+                       dim3(kMergeThreads), 0, stream, p, Divisor(p.H), each);
     HYP_HIP_CHECK(hipGetLastError());
 }
 
@@ -1292,6 +1052,7 @@ void launch_batch_attention(const BatchView& b, const BatchAttentionArgs& a, hip
     p.H = a.n_heads;
     p.KVH = a.n_kv_heads;
     p.G = static_cast<uint32_t>(G);
+    p.by_G = Divisor(p.G);
     p.window = a.window;
     p.scale = a.scale * kLog2e;
     switch (a.head_dim) {

@@ -1,0 +1,379 @@
+// How hyp_batch_attention's work is cut (see attention_batch.hip).
+//
+// A unit is a block of 32 keys for a tile of query rows of one kv head. Tiles are of two kinds: of few
+// rows (16, a wave each) and wide (128, a workgroup each), and units of a kind are numbered tile by tile: the
+// prefix's tiles by kv head, then each request's by kv head. Every workgroup finds its units itself from
+// the lengths in device memory, 64 requests at a time across a wave's lanes; the launch has a fixed number of
+// workgroups whatever the lengths, each with the same number of consecutive units of one kind.
+#pragma once
+
+#include "attention.h"
+#include "batch.h"
+#include "common.h"
+
+namespace hyperion::hip {
+
+constexpr uint32_t kTileRows = 16;
+constexpr uint32_t kComputeUnits = 256;
+constexpr uint32_t kMaxParts = 256;     // of one tile: what the merge reads for a row
+// A workgroup's time for a unit of a wide tile by that for one of few rows: a tile has one block of keys in
+// flight at a time, four waves have one each.
+constexpr uint32_t kWideCost = 4;
+constexpr uint32_t kGroupThreads = 256;
+constexpr uint32_t kGroupWaves = kGroupThreads / 64u;
+
+// n / d for a divisor that the host knows: n times 2^36 / d rounded up, exact while n d < 2^36 (rows times
+// heads are below 2^25, heads at most 2^10). (A division is some 30 instructions, and a wave that takes a block
+// or two forms several.)
+struct Divisor {
+    uint64_t inverse;   // 2^36 / d, rounded up
+    uint32_t d;
+    Divisor() = default;
+    explicit Divisor(uint32_t d_) : inverse(((1ull << 36) + d_ - 1u) / d_), d(d_) {}
+    __device__ uint32_t of(uint32_t n) const { return static_cast<uint32_t>((n * inverse) >> 36); }
+};
+
+// ceil(n / d): from fp32, then put right.
+__device__ __forceinline__ uint32_t ceil_div(uint32_t n, uint32_t d) {
+    uint32_t q = static_cast<uint32_t>(static_cast<float>(n) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+    while (static_cast<uint64_t>(q) * d > n) --q;   // q <= n / d
+    while (static_cast<uint64_t>(q) * d < n) ++q;
+    return q;
+}
+// floor(n / d), the same way.
+__device__ __forceinline__ uint32_t floor_div(uint32_t n, uint32_t d) {
+    const uint32_t q = ceil_div(n, d);
+    return static_cast<uint64_t>(q) * d > n ? q - 1u : q;
+}
+
+// What the attention launch's scribes leave for the merge.
+struct Header {
+    uint32_t few_per, wide_per;            // units of a wave, of a workgroup; few_per 0: no batch
+    uint32_t blocks, tiles;                // the prefix in tiles of few rows
+    uint32_t wide_blocks, wide_tiles;      // the prefix in wide tiles
+    uint32_t apart;                        // every request's tiles take the prefix's keys too
+    uint32_t unused[9];
+};
+struct Record {
+    uint32_t unit0, tiles, blocks;                 // few rows
+    uint32_t wide_unit0, wide_tiles, wide_head;    // wide tiles; units of one kv head
+    uint32_t unused[2];
+};
+struct RowRecord {
+    uint32_t request, row;   // its request, its row there
+};
+
+struct BatchParams {
+    BatchView b;
+    const uint16_t* q;
+    const uint16_t* ck;
+    const uint16_t* cv;
+    uint16_t* out;
+    Header* header;
+    Record* request;
+    RowRecord* row;
+    // Unnormalised rows with their (m, l). Tiles that one worker walked whole, by output row: [0] of
+    // the prefix, [1] of the own tokens. Otherwise worker w's piece 2 w (its first) or 2 w + 1.
+    float2* whole_ml[2];   // [max_rows][H]
+    float* whole_o[2];     // [max_rows][H][D]
+    float2* part_ml;       // [piece][kTileRows]
+    float* part_o;         // [piece][kTileRows][D]
+    float2* wide_ml;       // [piece][kChunkRows]
+    float* wide_o;         // [piece][kChunkRows][D]
+    uint32_t H, KVH, G, window, groups;   // groups: workgroups of the launch
+    Divisor by_G;
+    float scale;           // with log2(e)
+};
+
+// A request's (or the prefix's) part of the work for few rows.
+struct Source {
+    uint32_t row0, rows;   // query rows (tokens)
+    uint32_t lo, hi;       // keys [lo, hi) that some row sees
+    int32_t pos;           // the first row's position, counted from the source's key 0
+    uint32_t tiles, blocks;
+    __device__ uint32_t units(uint32_t KVH) const { return KVH * tiles * blocks; }
+};
+
+__device__ __forceinline__ uint32_t tiles_of(uint32_t rows, uint32_t G) { return (rows * G + kTileRows - 1u) / kTileRows; }
+__device__ __forceinline__ uint32_t wide_tiles_of(uint32_t rows, uint32_t G) { return (rows * G + kChunkRows - 1u) / kChunkRows; }
+
+// sum over i < n of floor((a i + b) / m): the whole parts of a and b over m, then the same sum with m
+// and a exchanged. (a n + b below 2^32, the sum too.)
+__device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    uint32_t sum = 0u;
+    while (n != 0u) {
+        const uint32_t qa = a / m, qb = b / m;
+        sum += static_cast<uint32_t>(static_cast<uint64_t>(n) * (n - 1u) / 2u * qa) + n * qb;
+        a -= qa * m;
+        b -= qb * m;
+        const uint32_t top = a * n + b;
+        if (top < m) break;
+        n = top / m;
+        b = top - n * m;
+        const uint32_t t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+
+// The key blocks of a request's wide tiles. Tile k's rows end at position pos0 + (128 k + 127) / G, so its
+// blocks end at floor((pos0 + (128 k + 127) / G + 32) / 32), which with pos0 + 32 = 32 q + r is
+// end(k) = q + floor((128 k + G r + 127) / 32 G); at most all blocks, and with a window no more than `most`
+// of them are seen.
+struct WideSpan {
+    uint32_t G, all, most, q, c;
+    __device__ WideSpan(uint32_t G_, uint32_t keys, int32_t pos0, uint32_t window) : G(G_) {
+        all = (keys + kKeyBlock - 1u) / kKeyBlock;
+        most = all;
+        if (window != 0u) {
+            const uint64_t seen = (static_cast<uint64_t>(window) + 127u / G + 63u) / kKeyBlock;
+            // (Rows before position 0 are counted from there: their tiles start as much earlier.)
+            const uint64_t early = pos0 < 0 ? (31u - static_cast<int64_t>(pos0)) / kKeyBlock : 0u;
+            if (seen + early < all) most = static_cast<uint32_t>(seen + early);
+        }
+        const uint32_t x = static_cast<uint32_t>(max(pos0, 0)) + kKeyBlock;
+        q = x / kKeyBlock;
+        c = G * (x % kKeyBlock) + 127u;
+    }
+    __device__ uint32_t end(uint32_t k) const { return min(q + (128u * k + c) / (32u * G), all); }
+    __device__ uint32_t units(uint32_t k) const { return min(end(k), most); }
+    // Units of the tiles before k: those whose end is below `most`, then `most` each.
+    __device__ uint32_t before(uint32_t k) const {
+        uint32_t rising = 0u;
+        if (most > q) {
+            const uint64_t full = 32ull * G * (most - q);
+            if (full > c) rising = static_cast<uint32_t>(min(static_cast<uint64_t>(k), (full - c + 127u) >> 7));
+        }
+        return rising * q + floor_sum(rising, 32u * G, 128u, c) + (k - rising) * most;
+    }
+};
+
+__device__ __forceinline__ Source request_source(const BatchParams& p, uint32_t r) {
+    Source s{0u, 0u, 0u, 0u, 0, 0u, 0u};
+    if (r >= p.b.requests) return s;
+    s.row0 = min(p.b.row_start[r], p.b.max_rows);
+    s.rows = max(min(p.b.row_start[r + 1u], p.b.max_rows), s.row0) - s.row0;
+    const uint64_t held = min(static_cast<uint64_t>(p.b.max_blocks) << p.b.shift, static_cast<uint64_t>(1u << 30));
+    s.hi = min(p.b.lens[r], static_cast<uint32_t>(held));
+    s.pos = static_cast<int32_t>(s.hi) - static_cast<int32_t>(s.rows);
+    if (p.window != 0u && static_cast<int64_t>(s.pos) + 1 > p.window) s.lo = s.pos + 1u - p.window;
+    s.tiles = tiles_of(s.rows, p.G);
+    s.blocks = s.rows != 0u && s.hi > s.lo ? (s.hi - s.lo + kKeyBlock - 1u) / kKeyBlock : 0u;
+    return s;
+}
+
+// The same value in every lane, as a scalar.
+__device__ __forceinline__ uint32_t scalar(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
+__device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+
+// Inclusive scan over the wave by register moves between lanes: 1, 2, 4 and 8 lanes on within rows of
+// 16, then the last lane of row 0 and 2 to the next row, of row 1 to the upper half. `none` is the operation's
+// neutral value. (Through LDS permutes a reduction takes six times their latency, and a call forms ten.)
+template <typename Op>
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t none, Op&& op) {
+    const int n = static_cast<int>(none);
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x111, 0xF, 0xF, false)));
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x112, 0xF, 0xF, false)));
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x114, 0xF, 0xF, false)));
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x118, 0xF, 0xF, false)));
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x142, 0xA, 0xF, false)));
+    return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x143, 0xC, 0xF, false)));
+}
+__device__ __forceinline__ uint32_t wave_incl(uint32_t v) {
+    return wave_scan(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) { return from_lane(wave_incl(v), 63u); }
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    return from_lane(wave_scan(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); }), 63u);
+}
+__device__ __forceinline__ int32_t wave_min(int32_t v) {
+    return static_cast<int32_t>(from_lane(wave_scan(static_cast<uint32_t>(v), 0x7FFFFFFFu, [](uint32_t a, uint32_t b) {
+        return static_cast<uint32_t>(min(static_cast<int32_t>(a), static_cast<int32_t>(b)));
+    }), 63u));
+}
+
+// The batch as one wave sees it. Which rows go where: rows of one request that fill wide tiles by
+// themselves read the prefix there, at one pass over all their keys, where that takes at most a quarter
+// more tiles than the rows of all requests together would (apart). Otherwise the prefix is taken for all
+// rows together, in wide tiles from 17 rows on, and a request's own tokens in wide tiles where its rows
+// pass 16.
+struct Walk {
+    uint32_t rows;              // of all requests
+    int32_t first_pos;          // their least position
+    bool apart;
+    Source prefix;              // the prefix in tiles of few rows (its keys [lo, hi) in either kind)
+    uint32_t wide_tiles, wide_lo, wide_blocks;   // and in wide ones
+    uint32_t units, wide_units;                  // of all
+    uint32_t wide_groups, wide_per, few_per;     // workgroups 0 .. wide_groups - 1 take wide tiles
+
+    __device__ bool wide(const BatchParams& p, uint32_t n) const { return apart || n * p.G > kTileRows; }
+    __device__ uint32_t few_units(const BatchParams& p, const Source& s) const { return wide(p, s.rows) ? 0u : s.units(p.KVH); }
+    // The keys that a request's wide tiles walk: the prefix's before its own where apart.
+    __device__ WideSpan span(const BatchParams& p, const Source& s) const {
+        const uint32_t pre = apart ? p.b.prefix : 0u;
+        return WideSpan(p.G, pre + s.hi, static_cast<int32_t>(pre) + s.pos, p.window);
+    }
+    // Units of a request's wide tiles of one kv head.
+    __device__ uint32_t wide_head(const BatchParams& p, const Source& s) const {
+        return s.rows != 0u && wide(p, s.rows) ? span(p, s).before(wide_tiles_of(s.rows, p.G)) : 0u;
+    }
+    __device__ bool has_prefix() const { return prefix.blocks != 0u || wide_blocks != 0u; }
+
+    // False where the row starts are no rows of the batch (they would pass the workspace).
+    __device__ bool open(const BatchParams& p, uint32_t lane) {
+        const Source mine = request_source(p, lane);
+        uint32_t sum = 0u, top = 0u, tiles = 0u;
+        int32_t first = 0x7fffffff;
+        for (uint32_t r = lane; r < p.b.requests; r += 64u) {
+            const Source s = r == lane ? mine : request_source(p, r);
+            sum = min(sum + s.rows, 1u << 25);
+            top = max(top, s.row0 + s.rows);
+            tiles += wide_tiles_of(s.rows, p.G);
+            if (s.rows != 0u) first = min(first, s.pos);
+        }
+        if (wave_sum(sum) > p.b.max_rows) return false;
+        rows = wave_max(top);
+        first_pos = wave_min(first);
+        apart = rows * p.G > kTileRows && 4u * wave_sum(tiles) <= 5u * wide_tiles_of(rows, p.G);
+        uint32_t n = 0u, most = 0u, wide_n = 0u, wide_most = 0u;
+        for (uint32_t r = lane; r < p.b.requests; r += 64u) {
+            const Source s = r == lane ? mine : request_source(p, r);
+            if (s.rows == 0u) continue;
+            if (wide(p, s.rows)) {
+                wide_n += p.KVH * wide_head(p, s);
+                wide_most = max(wide_most, ((apart ? p.b.prefix : 0u) + s.hi) / kKeyBlock + 1u);
+            } else {
+                n += s.units(p.KVH);
+                most = max(most, s.blocks);
+            }
+        }
+        prefix = Source{0u, rows, 0u, p.b.prefix, 0, tiles_of(rows, p.G), 0u};
+        wide_tiles = wide_lo = wide_blocks = 0u;
+        if (rows != 0u && !apart) {
+            first_pos += static_cast<int32_t>(p.b.prefix);
+            prefix.pos = first_pos;
+            if (p.window != 0u && static_cast<int64_t>(first_pos) + 1 > p.window) prefix.lo = first_pos + 1u - p.window;
+            if (prefix.hi > prefix.lo) {
+                if (wide(p, rows)) {
+                    wide_tiles = wide_tiles_of(rows, p.G);
+                    wide_lo = prefix.lo / kKeyBlock;
+                    wide_blocks = (prefix.hi + kKeyBlock - 1u) / kKeyBlock - wide_lo;
+                } else {
+                    prefix.blocks = (prefix.hi - prefix.lo + kKeyBlock - 1u) / kKeyBlock;
+                }
+            }
+        }
+        most = max(wave_max(most), prefix.blocks);
+        units = wave_sum(n) + prefix.units(p.KVH);
+        wide_units = p.KVH * wide_tiles * wide_blocks;
+        if (rows * p.G > kTileRows) {
+            wide_units += wave_sum(wide_n);
+            wide_most = max(wave_max(wide_most), wide_blocks);
+        }
+        wide_groups = 0u;
+        wide_per = 1u;
+        if (wide_units != 0u) {
+            wide_groups = p.groups;
+            if (units != 0u) {
+                const float cost = static_cast<float>(wide_units) * kWideCost;
+                const float share = cost * __builtin_amdgcn_rcpf(cost + static_cast<float>(units));
+                wide_groups = min(max(static_cast<uint32_t>(static_cast<float>(p.groups) * share), 1u), p.groups - 1u);
+            }
+            wide_per = max(ceil_div(wide_units, wide_groups), (wide_most + kMaxParts - 2u) / (kMaxParts - 1u));
+            wide_groups = ceil_div(wide_units, wide_per);
+        }
+        const uint32_t waves = max((p.groups - wide_groups) * kGroupWaves, 1u);
+        few_per = max(max(ceil_div(units, waves), (most + kMaxParts - 2u) / (kMaxParts - 1u)), 1u);
+        return true;
+    }
+};
+
+// Requests 64 at a time, with running sums of their units of one kind.
+struct Chunk {
+    Source mine;       // this lane's request
+    uint32_t base;     // the first request
+    uint32_t before;   // units before it
+    uint32_t incl;     // with this lane's request
+    uint32_t head;     // wide tiles: this lane's units of one kv head
+    bool wide;
+
+    __device__ void load(const BatchParams& p, const Walk& w, uint32_t lane) {
+        mine = request_source(p, base + lane);
+        head = wide ? w.wide_head(p, mine) : 0u;
+        incl = wave_incl(wide ? p.KVH * head : w.few_units(p, mine));
+    }
+    __device__ void open(const BatchParams& p, const Walk& w, uint32_t lane, bool wide_) {
+        wide = wide_;
+        base = 0u;
+        before = wide ? p.KVH * w.wide_tiles * w.wide_blocks : w.prefix.units(p.KVH);
+        load(p, w, lane);
+    }
+    __device__ uint32_t own_units(const BatchParams& p, const Walk& w) const { return wide ? p.KVH * head : w.few_units(p, mine); }
+    __device__ void next(const BatchParams& p, const Walk& w, uint32_t lane) {
+        before += from_lane(incl, 63u);
+        base += 64u;
+        load(p, w, lane);
+    }
+    // The lane whose request holds unit u (u >= before); 64 where none does.
+    __device__ uint32_t seek(const BatchParams& p, const Walk& w, uint32_t u, uint32_t lane) {
+        while (base + 64u < p.b.requests && u >= before + from_lane(incl, 63u))
+            next(p, w, lane);
+        const uint64_t behind = __ballot(u < before + incl);
+        return behind == 0u ? 64u : static_cast<uint32_t>(__builtin_ctzll(behind));
+    }
+};
+
+__device__ __forceinline__ Source source_of_lane(const Source& s, uint32_t from) {
+    return Source{from_lane(s.row0, from), from_lane(s.rows, from),  from_lane(s.lo, from),    from_lane(s.hi, from),
+                  __builtin_amdgcn_readlane(s.pos, from), from_lane(s.tiles, from), from_lane(s.blocks, from)};
+}
+
+// Position of token row t, whatever its request (counted from the prefix's key 0).
+__device__ __forceinline__ int32_t row_position(const BatchParams& p, uint32_t t) {
+    uint32_t lo = 0u, hi = p.b.requests;
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (p.b.row_start[mid] <= t) lo = mid; else hi = mid;
+    }
+    const Source s = request_source(p, lo);
+    return static_cast<int32_t>(p.b.prefix) + s.pos + static_cast<int32_t>(t - s.row0);
+}
+
+// What the merge needs: a wave writes 64 requests and their rows.
+__device__ __forceinline__ void scribe(const BatchParams& p, uint32_t chunk, uint32_t lane) {
+    Walk w;
+    if (!w.open(p, lane)) {
+        if (chunk == 0u && lane == 0u) *p.header = Header{};
+        return;
+    }
+    if (chunk == 0u && lane == 0u) {
+        *p.header = Header{w.few_per, w.wide_per, w.prefix.blocks, w.prefix.tiles, w.wide_blocks, w.wide_tiles, w.apart ? 1u : 0u, {}};
+    }
+    if (chunk >= p.b.requests) return;
+    Chunk few, wide;
+    few.open(p, w, lane, false);
+    wide.open(p, w, lane, true);
+    while (few.base < chunk) {
+        few.next(p, w, lane);
+        wide.next(p, w, lane);
+    }
+    const Source s = few.mine;
+    const bool is_wide = w.wide(p, s.rows);
+    if (chunk + lane < p.b.requests) {
+        p.request[chunk + lane] = Record{few.before + few.incl - few.own_units(p, w), s.tiles, is_wide ? 0u : s.blocks,
+                                         wide.before + wide.incl - wide.own_units(p, w),
+                                         is_wide ? wide_tiles_of(s.rows, p.G) : 0u, wide.head, {}};
+    }
+    for (uint32_t i = 0; i < 64u; ++i) {
+        const uint32_t row0 = from_lane(s.row0, i);
+        const uint32_t n = from_lane(s.rows, i);
+        for (uint32_t t = lane; t < n; t += 64u) p.row[row0 + t] = RowRecord{chunk + i, t};
+    }
+}
+
+}  // namespace hyperion::hip
