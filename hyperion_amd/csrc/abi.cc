@@ -988,7 +988,7 @@ HypStatus hyp_batch_attention(const HypBatch* batch, const void* q, uint32_t n_h
         const hyperion::hip::BatchView b = batch_ref(batch);
         HypKvCacheOpaque& c = batch_cache(*batch, cache, n_heads);
         REQUIRE_ARG(b.prefix == 0 || b.prefix_table != nullptr, "a prefix needs its prefix_table");
-        REQUIRE_ARG(std::isfinite(scale), "scale must be finite");
+        REQUIRE_ARG(std::isfinite(scale) && scale > 0.0f, "scale must be finite and positive");
         if (b.max_rows == 0 || b.requests == 0) return;
         REQUIRE_ARG(q != nullptr && out != nullptr, "q and out must be non-null device pointers");
         REQUIRE_ARG(workspace != nullptr, "workspace must be a non-null device pointer");

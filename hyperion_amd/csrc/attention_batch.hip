@@ -37,6 +37,7 @@ namespace hyperion::hip {
 namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kMergeThreads = 256;
 constexpr uint32_t kMergeRows = 64;        // (row, head) pairs of a workgroup, at most
@@ -461,14 +462,20 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
         return ln;
     };
     size_t at = 0u;   // the row of this lane's key, of the block that is loaded next
-    const auto load_unit = [&](uint32_t st, uint32_t g) {
+    struct Pieces2 {
+        const uint16_t *k, *v;
+    };
+    const auto pieces_at = [&] {
         const uint32_t ln = lane_again();
         const uint32_t k_piece = (ln & 7u) ^ (((ln >> 4) & 3u) | ((wave & 1u) << 2));
         const uint32_t v_piece = (ln & 7u) ^ (((ln >> 4) & 1u) << 2);
+        return Pieces2{ck + at + k_piece * 8u, cv + at + v_piece * 8u};
+    };
+    const auto load_unit = [&](const Pieces2& from, uint32_t st, uint32_t g) {
         const uint32_t to_lds = lds + st * Lds::kStage + (wave * kGroups + g) * 1024u;
-        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(ck + at + k_piece * 8u + g * 64u),
-                                         reinterpret_cast<HYP_LDS void*>(to_lds), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(cv + at + v_piece * 8u + g * 64u),
+        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(from.k + g * 64u), reinterpret_cast<HYP_LDS void*>(to_lds), 16,
+                                         0, 0);
+        __builtin_amdgcn_global_load_lds((const HYP_GLOBAL void*)(from.v + g * 64u),
                                          reinterpret_cast<HYP_LDS void*>(to_lds + Lds::kV), 16, 0, 0);
     };
     const auto row_of = [&](uint32_t slot) {
@@ -506,7 +513,7 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
         at = row_of(slot_from(entry_of(b0 * kKeyBlock + n), b0 * kKeyBlock + n));
         entry = entry_of((b0 + 1u) * kKeyBlock + n);
 #pragma unroll
-        for (uint32_t g = 0; g < kGroups; ++g) load_unit(0u, g);
+        for (uint32_t g = 0; g < kGroups; ++g) load_unit(pieces_at(), 0u, g);
     }
     const auto v_read = [&](uint32_t v_at, uint32_t v_odd, uint32_t u) {   // v_at, v_odd: of even and odd dim tiles
         const uint32_t dt = u / 2u;
@@ -514,9 +521,9 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                            BlockLds<D>::kOctet);
     };
     constexpr uint32_t kProducts = 2u * kDTiles;
-    constexpr bool kLazy = D >= 512u;
     float mx = 0.0f;
-    // kLazy as in attention_chunk.hip: a block that outgrows the reference ends the inner loop before it
+    // As attention_chunk.hip at head_dim 512: O is rescaled only when a row's maximum has grown by more than
+    // 2^kRescaleLog2 since the last time. A block that outgrows the reference ends the inner loop before it
     // touches O, the outer loop rescales, and the inner loop takes the same block again.
     uint32_t b = b0;
     uint32_t now_there = there;
@@ -540,6 +547,7 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
             bf16x8_t kf[kAhead];
+            const Pieces2 from = pieces_at();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (uint32_t st = 0; st < kAhead; ++st) kf[st] = k_read(st);
@@ -548,7 +556,7 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 __builtin_amdgcn_sched_barrier(0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[st % kAhead], q[st], sc, 0, 0, 0);
                 if (st + kAhead < kSteps) kf[st % kAhead] = k_read(st + kAhead);
-                if (st % 4u == 1u) load_unit(stage_n, st / 4u);
+                if (st % 4u == 1u) load_unit(from, stage_n, st / 4u);
             }
             __builtin_amdgcn_sched_barrier(0);
             const uint32_t entry_next = entry_of(jb + 2u * kKeyBlock + (lane_again() & 31u));
@@ -567,45 +575,34 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 for (uint32_t i = 0; i < 16u; ++i) {
                     const uint32_t k = 8u * (i / 4u) + 4u * h + (i & 3u);
                     const int32_t j = static_cast<int32_t>(jb + k);
-                    sc[i] = j <= last && j >= first && ((now_there >> k) & 1u) != 0u ? sc[i] * p.scale : -__builtin_huge_valf();
+                    sc[i] = j <= last && j >= first && ((now_there >> k) & 1u) != 0u ? sc[i] : -__builtin_huge_valf();
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[i] *= p.scale;
             }
             mx = sc[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-            mx = half_max(mx);
-            if constexpr (kLazy) m = m == -__builtin_huge_valf() ? mx : m;   // O is still zero: nothing to rescale
-            float alpha = 1.0f;
-            if constexpr (kLazy) {
-                if (__any(mx > m + kRescaleLog2)) {
-                    again = true;
-                    break;
-                }
-            } else {
-                const float m_new = fmaxf(m, mx);
-                alpha = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
-                m = m_new;
-                l *= alpha;
+            mx = half_max(mx) * p.scale;
+            m = m == -__builtin_huge_valf() ? mx : m;   // O is still zero: nothing to rescale
+            if (__any(mx > m + kRescaleLog2)) {
+                again = true;
+                break;
             }
             entry = entry_next;
             const float ref = m > -__builtin_huge_valf() ? m : 0.0f;
             float pr[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(sc[i] - ref);
+            for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale, -ref));
+            // The sum takes them as rounded, two at a time.
+            uint32_t two[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                two[i] = cvt_pk_bf16(pr[2 * i], pr[2 * i + 1]);
+                l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two[i]), bf16x2_t{1.0f, 1.0f}, l, false);
+            }
             bf16x8_t pb[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) pb[t] = round_p(pr + 8 * t);
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum += bf16_bits_to_f32(__builtin_bit_cast(u16x8_t, pb[i / 8])[i % 8]);
-            l += sum;
-            if constexpr (!kLazy) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[0][i] *= alpha;
-            }
+            for (int t = 0; t < 2; ++t)
+                pb[t] = __builtin_bit_cast(bf16x8_t, make_uint4(two[4 * t], two[4 * t + 1], two[4 * t + 2], two[4 * t + 3]));
             if constexpr (D == 256u) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -616,10 +613,6 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
                 __builtin_amdgcn_sched_barrier(0);
                 o[u / 2u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u % kAhead], pb[u % 2u], o[u / 2u], 0, 0, 0);
                 if (u + kAhead < kProducts) vf[u % kAhead] = v_read(v_at, v_odd, u + kAhead);
-                if (!kLazy && u / 2u + 1u < kDTiles) {   // the next tile, half of it in each product's shadow
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) o[u / 2u + 1u][8u * (u % 2u) + i] *= alpha;
-                }
             }
         }
         if (again) {

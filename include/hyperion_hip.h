@@ -461,8 +461,8 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
  * request r (t = row_start[r] + i, of n rows) stands at position prefix_len + lens[r] - n + i and
  * sees the key positions p <= its own (with window > 0: p > its own - window) that are tokens of
  * the prefix or of the request. Grouped-query heads and layouts as hyp_attention: q, out
- * [max_rows][n_heads][head_dim], device bf16, 16-byte aligned; the scores are scale * q.k (scale
- * finite). The rows' own K and V are read from the cache: call hyp_batch_prepare first. The
+ * [max_rows][n_heads][head_dim], n_heads at most 1024, device bf16, 16-byte aligned; the scores are
+ * scale * q.k (scale finite and positive). The rows' own K and V are read from the cache: call hyp_batch_prepare first. The
  * prefix's keys are read for all rows of the batch at once.
  * fp32 scores and softmax, probabilities in two bf16 terms, output rounded to bf16. A row that
  * sees no key above -inf gives zeros; a NaN or +inf score that it sees gives NaN; keys that it does not see

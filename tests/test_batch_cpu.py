@@ -104,7 +104,8 @@ def test_prepare_refusals(over, says):
     (dict(q=None), "non-null"), (dict(out=None), "non-null"), (dict(work=None), "non-null"),
     (dict(q=ctypes.c_void_p(0x1002)), "aligned"), (dict(out=ctypes.c_void_p(0x1008)), "aligned"),
     (dict(work=ctypes.c_void_p(0x1004)), "aligned"), (dict(heads=0), "multiple"), (dict(heads=3), "multiple"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(bytes=1000), "workspace too small"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(heads=1026), "1024"), (dict(bytes=1000), "workspace too small"),
     (dict(cache=None), "null"), (dict(stream=None), "null")])
 def test_attention_refusals(over, says):
     refused("hyp_batch_attention", *attention_args(fields(), **over), says=says)
