@@ -346,9 +346,6 @@ struct TilesLds {
 constexpr uint32_t kWaveRows = 32;
 constexpr float kRescaleLog2 = 8.0f;
 
-// Workgroups: as many as the device holds at once.
-constexpr uint32_t groups_of(uint32_t D) { return kComputeUnits * (D >= 512u ? 1u : 2u); }
-
 struct TileShared {
     int32_t range[kGroupWaves][2];   // the waves' first and last keys
     int32_t pos[kChunkRows];         // positions of a prefix tile's tokens
@@ -718,25 +715,24 @@ __device__ __forceinline__ void wide_units(const BatchParams& p, uint32_t worker
     uint32_t u = begin;
     while (u < end) {
         // (Formed again for each tile rather than kept in registers beside the tile's.)
-        Walk w;
+        Walk<true> w;
         if (!w.open(p, lane)) return;
         Sequence s{nullptr, p.b.prefix, p.b.prefix, 0u, w.rows, w.first_pos, true};
-        uint32_t hk, tile, off, blocks, block0;
-        if (u < p.KVH * w.wide_tiles * w.wide_blocks) {
-            const uint32_t g = u / w.wide_blocks;
+        const uint32_t hk = floor_div(u, w.wide_head_units);
+        const uint32_t in_head = u - hk * w.wide_head_units;
+        uint32_t tile, off, blocks, block0;   // off: units before u, with kTileCost before the blocks
+        if (in_head < w.prefix_units()) {
             blocks = w.wide_blocks;
             block0 = w.wide_lo;
-            off = u - g * blocks;
-            hk = g / w.wide_tiles;
-            tile = g - hk * w.wide_tiles;
+            tile = floor_div(in_head, blocks + kTileCost);
+            off = in_head - tile * (blocks + kTileCost);
         } else {
-            Chunk c;
+            Chunk<Walk<true>> c;
             c.open(p, w, lane, true);
-            const uint32_t at = c.seek(p, w, u, lane);
+            const uint32_t at = c.seek(p, w, in_head, lane);
             if (at == 64u) return;   // (not with u below the total)
             const Source src = source_of_lane(c.mine, at);
-            const uint32_t head = from_lane(c.head, at);
-            const uint32_t rel = u - (c.before + from_lane(c.incl, at) - p.KVH * head);
+            const uint32_t x = in_head - (c.before + from_lane(c.incl, at) - from_lane(c.own, at));
             s.own = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
             s.pre = w.apart ? p.b.prefix : 0u;
             s.keys = s.pre + src.hi;
@@ -745,8 +741,6 @@ __device__ __forceinline__ void wide_units(const BatchParams& p, uint32_t worker
             s.pos = static_cast<int32_t>(s.pre) + src.pos;
             s.by_request = false;
             const WideSpan span = w.span(p, src);
-            hk = rel / head;
-            const uint32_t x = rel - hk * head;
             uint32_t t0 = 0u, t1 = wide_tiles_of(src.rows, p.G);   // the last tile with before() <= x
             while (t1 - t0 > 1u) {
                 const uint32_t mid = (t0 + t1) / 2u;
@@ -757,20 +751,26 @@ __device__ __forceinline__ void wide_units(const BatchParams& p, uint32_t worker
             blocks = span.units(tile);
             block0 = span.end(tile) - blocks;
         }
-        const uint32_t take = min(blocks - off, end - u);
+        const uint32_t take = min(blocks + kTileCost - off, end - u);
         const bool complete = !s.by_request && !w.has_prefix();
-        const uint32_t to = take < blocks ? kToPiece : (complete ? kToOutput : kToRows);
-        tile_segment<D>(p, s, scalar(hk), scalar(tile), scalar(block0 + off), scalar(block0 + off + take), to,
-                        2u * worker + (u == begin ? 0u : 1u), lds, shared);
+        const uint32_t to = take < blocks + kTileCost ? kToPiece : (complete ? kToOutput : kToRows);
+        const uint32_t piece = 2u * worker + (u == begin ? 0u : 1u);
+        const uint32_t b0 = max(off, kTileCost) - kTileCost;
+        const uint32_t b1 = max(off + take, kTileCost) - kTileCost;
+        if (b0 < b1) {
+            tile_segment<D>(p, s, scalar(hk), scalar(tile), scalar(block0 + b0), scalar(block0 + b1), to, piece, lds, shared);
+        } else if (threadIdx.x < kChunkRows) {   // a piece without blocks
+            p.wide_ml[static_cast<size_t>(piece) * kChunkRows + threadIdx.x] = make_float2(-__builtin_huge_valf(), 0.0f);
+        }
         u = scalar(u + take);
     }
 }
 
 // A wave's units of tiles of few rows.
-template <uint32_t D>
-__device__ __forceinline__ void few_units(const BatchParams& p, const Walk& w, uint32_t worker, uint32_t begin, uint32_t end,
+template <uint32_t D, typename W>
+__device__ __forceinline__ void few_units(const BatchParams& p, const W& w, uint32_t worker, uint32_t begin, uint32_t end,
                                           uint32_t lds, uint32_t lane) {
-    Chunk c;
+    Chunk<W> c;
     c.open(p, w, lane, false);
     uint32_t u = begin;
     while (u < end) {
@@ -796,22 +796,32 @@ __device__ __forceinline__ void few_units(const BatchParams& p, const Walk& w, u
     }
 }
 
-template <uint32_t D>
-__global__ __launch_bounds__(kGroupThreads, D >= 512u ? 1 : 2) void attn_batch_kernel(BatchParams p) {
+// Workgroups: as many as the device holds at once.
+constexpr uint32_t groups_of(uint32_t D, bool wide) {
+    return kComputeUnits * (D >= 512u ? 1u : (wide || D == 256u ? 2u : (D == 128u ? 3u : 4u)));
+}
+
+// Without kWide every tile is of few rows (Walk). Both kinds go in one launch: two launches, one after the
+// other, took 124 us for one's 107 (64 rows behind 2000 tokens at head_dim 256, window 1024), 173 for 133 (96
+// rows behind 777 at 128) and 115 for 111 (50 rows behind 16001 at 512).
+template <uint32_t D, bool kWide>
+__global__ __launch_bounds__(kGroupThreads, groups_of(D, kWide) / kComputeUnits) void attn_batch_kernel(BatchParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[];
-    __shared__ TileShared shared;
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((HYP_LDS uint8_t*)lds_mem));
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = scalar(threadIdx.x >> 6);
-    if (blockIdx.x >= p.groups) {
-        scribe(p, ((blockIdx.x - p.groups) * kGroupWaves + wave) * 64u, lane);
+    constexpr uint32_t kGroups = groups_of(D, kWide);
+    if (blockIdx.x >= kGroups) {
+        scribe<kWide>(p, ((blockIdx.x - kGroups) * kGroupWaves + wave) * 64u, lane);
         return;
     }
-    Walk w;
+    Walk<kWide> w;
     if (!w.open(p, lane)) return;
-    if (blockIdx.x < w.wide_groups) {
-        const uint32_t begin = blockIdx.x * w.wide_per;
-        wide_units<D>(p, blockIdx.x, begin, min(begin + w.wide_per, w.wide_units), lds, shared);
+    if (kWide && blockIdx.x < w.wide_groups) {
+        __shared__ TileShared shared;
+        const uint32_t worker = scalar(w.worker(blockIdx.x));
+        const uint32_t begin = worker * w.wide_per;
+        wide_units<D>(p, worker, begin, min(begin + w.wide_per, w.wide_units), lds, shared);
     } else {
         const uint32_t worker = (blockIdx.x - w.wide_groups) * kGroupWaves + wave;
         const uint64_t begin = static_cast<uint64_t>(worker) * w.few_per;
@@ -873,16 +883,17 @@ __global__ __launch_bounds__(kMergeThreads) void attn_batch_merge_kernel(BatchPa
                 const uint32_t orow = row.row * p.G + (h - hk * p.G);   // and among its request's
                 Pieces a, b;
                 if (head.wide_blocks != 0u) {
-                    a.set((hk * head.wide_tiles + pr / kChunkRows) * head.wide_blocks, head.wide_blocks, head.wide_per, pr, true);
+                    const uint32_t cost = head.wide_blocks + kTileCost;
+                    a.set(hk * head.wide_head + pr / kChunkRows * cost, cost, head.wide_per, pr, true);
                 } else {
                     a.set((hk * head.tiles + pr / kTileRows) * head.blocks, head.blocks, head.few_per, pr, false);
                 }
-                if (own.wide_head != 0u) {
+                if (own.wide_units != 0u) {
                     const Source src = request_source(p, row.request);
                     const uint32_t pre = head.apart != 0u ? p.b.prefix : 0u;
                     const WideSpan span(p.G, pre + src.hi, static_cast<int32_t>(pre) + src.pos, p.window);
                     const uint32_t tile = orow / kChunkRows;
-                    b.set(own.wide_unit0 + hk * own.wide_head + span.before(tile), span.units(tile), head.wide_per, orow, true);
+                    b.set(hk * head.wide_head + own.wide_unit0 + span.before(tile), span.cost(tile), head.wide_per, orow, true);
                 } else {
                     b.set(own.unit0 + (hk * own.tiles + orow / kTileRows) * own.blocks, own.blocks, head.few_per, orow, false);
                 }
@@ -974,7 +985,7 @@ Layout layout_of(const BatchView& b, uint32_t H, uint32_t D) {
         l.whole_ml[k] = take(rows * sizeof(float2));
         l.whole_o[k] = take(rows * D * sizeof(float));
     }
-    const size_t pieces = 2u * groups_of(D) * kGroupWaves * kTileRows, wide = 2u * groups_of(D) * kChunkRows;
+    const size_t pieces = 2u * groups_of(D, false) * kGroupWaves * kTileRows, wide = 2u * groups_of(D, true) * kChunkRows;
     l.ml = take(pieces * sizeof(float2));
     l.o = take(pieces * D * sizeof(float));
     l.wide_ml = take(wide * sizeof(float2));
@@ -983,25 +994,43 @@ Layout layout_of(const BatchView& b, uint32_t H, uint32_t D) {
     return l;
 }
 
-template <uint32_t D>
-void launch_d(BatchParams p, hipStream_t stream) {
-    constexpr size_t lds = TilesLds<D>::kBytes > kGroupWaves * BlockLds<D>::kBytes ? TilesLds<D>::kBytes
-                                                                                 : kGroupWaves * BlockLds<D>::kBytes;
+template <uint32_t D, bool kWide>
+void launch_walk(BatchParams p, hipStream_t stream) {
+    constexpr size_t few = kGroupWaves * BlockLds<D>::kBytes;
+    constexpr size_t lds = kWide && TilesLds<D>::kBytes > few ? TilesLds<D>::kBytes : few;
     static_assert(lds + sizeof(TileShared) <= 160u * 1024u && sizeof(Header) <= 256u, "batch attention");
     if (lds + sizeof(TileShared) > 65536u) {
         static thread_local int configured_device = -1;
         int dev = 0;
         HYP_HIP_CHECK(hipGetDevice(&dev));
         if (configured_device != dev) {
-            HYP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_batch_kernel<D>),
+            HYP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_batch_kernel<D, kWide>),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
             configured_device = dev;
         }
     }
-    p.groups = groups_of(D);
+    p.groups = groups_of(D, kWide);
+    // Of two kinds of tile each gets a share of the workgroups. Measured with 1 to 12: 50 rows behind 16001 tokens at
+    // head_dim 512 took 83 us with 1.5, 95 with 2.5 and 112 with 4; 64 behind 2000 at 256 took 100 with 5.5, 106 with 4
+    // and 102 with 10; at 128 what was tried made a hundredth's difference.
+    p.wide_cost = D >= 512u ? 1.5f : (D == 256u ? 5.5f : 4.0f);
     const uint32_t scribes = (p.b.requests + 64u * kGroupWaves - 1u) / (64u * kGroupWaves);
-    hipLaunchKernelGGL(attn_batch_kernel<D>, dim3(p.groups + scribes), dim3(kGroupThreads), lds, stream, p);
+    hipLaunchKernelGGL((attn_batch_kernel<D, kWide>), dim3(p.groups + scribes), dim3(kGroupThreads), lds, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
+}
+
+template <uint32_t D>
+void launch_d(const BatchParams& p, hipStream_t stream) {
+    // Tiles of few rows alone where no more than 16 rows of a kv head can be, and without a prefix where
+    // there are no more rows than requests (a decode step; should one request hold many of them, its keys are
+    // read for every 16). Without the wide tiles' registers 64 decode rows took 77 us, not 84 (head_dim 256,
+    // no prefix), 4 rows behind 100 tokens 12.5, not 13.8.
+    if (static_cast<uint64_t>(p.b.max_rows) * p.G <= kTileRows ||
+        (p.b.prefix == 0u && p.b.max_rows <= p.b.requests && p.G <= kTileRows)) {
+        launch_walk<D, false>(p, stream);
+    } else {
+        launch_walk<D, true>(p, stream);
+    }
     const uint64_t pairs = static_cast<uint64_t>(p.b.max_rows) * p.H;
     const uint32_t each = static_cast<uint32_t>(std::min<uint64_t>((pairs + kMergeGroups - 1u) / kMergeGroups, kMergeRows));
     hipLaunchKernelGGL(attn_batch_merge_kernel<D>, dim3(static_cast<uint32_t>((pairs + each - 1u) / each)),
@@ -1022,7 +1051,7 @@ void launch_batch_attention(const BatchView& b, const BatchAttentionArgs& a, hip
     const uint64_t G = a.n_heads / a.n_kv_heads;
     const uint64_t tiles = (static_cast<uint64_t>(b.max_rows) * G / kTileRows + std::min(b.requests, b.max_rows) + 1u) * 2u;
     const uint64_t keys = b.prefix + std::min<uint64_t>(static_cast<uint64_t>(b.max_blocks) << b.shift, 1u << 30);
-    HYP_REQUIRE(keys < (1ull << 30) && tiles * a.n_kv_heads * (keys / kKeyBlock + 1u) < (1ull << 31),
+    HYP_REQUIRE(keys < (1ull << 30) && tiles * a.n_kv_heads * (keys / kKeyBlock + 1u + kTileCost) < (1ull << 31),
                 HYP_STATUS_INVALID_ARGUMENT, "batch attention: too many rows for tables this long");
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     BatchParams p{};

@@ -1,10 +1,12 @@
 // How hyp_batch_attention's work is cut (see attention_batch.hip).
 //
-// A unit is a block of 32 keys for a tile of query rows of one kv head. Tiles are of two kinds: of few
-// rows (16, a wave each) and wide (128, a workgroup each), and units of a kind are numbered tile by tile: the
-// prefix's tiles by kv head, then each request's by kv head. Every workgroup finds its units itself from
-// the lengths in device memory, 64 requests at a time across a wave's lanes; the launch has a fixed number of
-// workgroups whatever the lengths, each with the same number of consecutive units of one kind.
+// A unit is a block of 32 keys for a tile of query rows of one kv head. Tiles are of two kinds: of few rows
+// (16, a wave each) and wide (128, a workgroup each; kTileCost units come before a wide tile's blocks, for what it
+// costs to begin one). Units of a kind are numbered tile by tile: of few rows the prefix's tiles by kv head, then each
+// request's by kv head; wide ones kv head by kv head, in each the prefix's, then request by request. Every
+// workgroup finds its units itself from the lengths in device memory, 64 requests at a time across a wave's lanes; the
+// launch has a fixed number of workgroups whatever the lengths, each with the same number of consecutive units of
+// one kind.
 #pragma once
 
 #include "attention.h"
@@ -16,9 +18,8 @@ namespace hyperion::hip {
 constexpr uint32_t kTileRows = 16;
 constexpr uint32_t kComputeUnits = 256;
 constexpr uint32_t kMaxParts = 256;     // of one tile: what the merge reads for a row
-// A workgroup's time for a unit of a wide tile by that for one of few rows: a tile has one block of keys in
-// flight at a time, four waves have one each.
-constexpr uint32_t kWideCost = 4;
+constexpr uint32_t kTileCost = 4;
+constexpr uint32_t kXcds = 8;
 constexpr uint32_t kGroupThreads = 256;
 constexpr uint32_t kGroupWaves = kGroupThreads / 64u;
 
@@ -51,13 +52,14 @@ struct Header {
     uint32_t few_per, wide_per;            // units of a wave, of a workgroup; few_per 0: no batch
     uint32_t blocks, tiles;                // the prefix in tiles of few rows
     uint32_t wide_blocks, wide_tiles;      // the prefix in wide tiles
+    uint32_t wide_head;                    // units of the wide tiles of one kv head
     uint32_t apart;                        // every request's tiles take the prefix's keys too
-    uint32_t unused[9];
+    uint32_t unused[8];
 };
 struct Record {
     uint32_t unit0, tiles, blocks;                 // few rows
-    uint32_t wide_unit0, wide_tiles, wide_head;    // wide tiles; units of one kv head
-    uint32_t unused[2];
+    uint32_t wide_unit0, wide_units;               // wide tiles, within a kv head
+    uint32_t unused[3];
 };
 struct RowRecord {
     uint32_t request, row;   // its request, its row there
@@ -83,6 +85,7 @@ struct BatchParams {
     uint32_t H, KVH, G, window, groups;   // groups: workgroups of the launch
     Divisor by_G;
     float scale;           // with log2(e)
+    float wide_cost;       // a workgroup's time for a unit of a wide tile, by that of its waves for one of few rows
 };
 
 // A request's (or the prefix's) part of the work for few rows.
@@ -138,14 +141,15 @@ struct WideSpan {
     }
     __device__ uint32_t end(uint32_t k) const { return min(q + (128u * k + c) / (32u * G), all); }
     __device__ uint32_t units(uint32_t k) const { return min(end(k), most); }
-    // Units of the tiles before k: those whose end is below `most`, then `most` each.
+    __device__ uint32_t cost(uint32_t k) const { return units(k) + kTileCost; }
+    // Units of the tiles before k, with what they cost: those whose end is below `most`, then `most` each.
     __device__ uint32_t before(uint32_t k) const {
         uint32_t rising = 0u;
         if (most > q) {
             const uint64_t full = 32ull * G * (most - q);
             if (full > c) rising = static_cast<uint32_t>(min(static_cast<uint64_t>(k), (full - c + 127u) >> 7));
         }
-        return rising * q + floor_sum(rising, 32u * G, 128u, c) + (k - rising) * most;
+        return rising * q + floor_sum(rising, 32u * G, 128u, c) + (k - rising) * most + k * kTileCost;
     }
 };
 
@@ -201,7 +205,8 @@ __device__ __forceinline__ int32_t wave_min(int32_t v) {
 // themselves read the prefix there, at one pass over all their keys, where that takes at most a quarter
 // more tiles than the rows of all requests together would (apart). Otherwise the prefix is taken for all
 // rows together, in wide tiles from 17 rows on, and a request's own tokens in wide tiles where its rows
-// pass 16.
+// pass 16. Without kWide there are no wide tiles.
+template <bool kWide>
 struct Walk {
     uint32_t rows;              // of all requests
     int32_t first_pos;          // their least position
@@ -209,9 +214,10 @@ struct Walk {
     Source prefix;              // the prefix in tiles of few rows (its keys [lo, hi) in either kind)
     uint32_t wide_tiles, wide_lo, wide_blocks;   // and in wide ones
     uint32_t units, wide_units;                  // of all
+    uint32_t wide_head_units;                    // of one kv head's wide tiles
     uint32_t wide_groups, wide_per, few_per;     // workgroups 0 .. wide_groups - 1 take wide tiles
 
-    __device__ bool wide(const BatchParams& p, uint32_t n) const { return apart || n * p.G > kTileRows; }
+    __device__ bool wide(const BatchParams& p, uint32_t n) const { return kWide && (apart || n * p.G > kTileRows); }
     __device__ uint32_t few_units(const BatchParams& p, const Source& s) const { return wide(p, s.rows) ? 0u : s.units(p.KVH); }
     // The keys that a request's wide tiles walk: the prefix's before its own where apart.
     __device__ WideSpan span(const BatchParams& p, const Source& s) const {
@@ -220,9 +226,21 @@ struct Walk {
     }
     // Units of a request's wide tiles of one kv head.
     __device__ uint32_t wide_head(const BatchParams& p, const Source& s) const {
-        return s.rows != 0u && wide(p, s.rows) ? span(p, s).before(wide_tiles_of(s.rows, p.G)) : 0u;
+        return kWide && s.rows != 0u && wide(p, s.rows) ? span(p, s).before(wide_tiles_of(s.rows, p.G)) : 0u;
     }
     __device__ bool has_prefix() const { return prefix.blocks != 0u || wide_blocks != 0u; }
+    // Units of the prefix's wide tiles of one kv head.
+    __device__ uint32_t prefix_units() const { return wide_blocks != 0u ? wide_tiles * (wide_blocks + kTileCost) : 0u; }
+    // The worker for workgroup i. Workgroups go to the XCDs in turn, and each of those has a cache of its own:
+    // an XCD takes consecutive workers, whose tiles share keys. Not where the prefix's tiles are most of the work: then
+    // consecutive workers take a tile's keys in turn (200 rows behind 900 tokens at head_dim 256: 151 us so, 159 in
+    // that order; 24 prompts of 9 to 250 rows behind 6000 at 512: 625 us so, 591 in that order).
+    __device__ uint32_t worker(uint32_t i) const {
+        if (2u * prefix_units() >= wide_head_units) return i;
+        const uint32_t n = wide_groups / kXcds, more = wide_groups % kXcds;
+        const uint32_t x = i % kXcds;
+        return x * n + min(x, more) + i / kXcds;
+    }
 
     // False where the row starts are no rows of the batch (they would pass the workspace).
     __device__ bool open(const BatchParams& p, uint32_t lane) {
@@ -233,19 +251,19 @@ struct Walk {
             const Source s = r == lane ? mine : request_source(p, r);
             sum = min(sum + s.rows, 1u << 25);
             top = max(top, s.row0 + s.rows);
-            tiles += wide_tiles_of(s.rows, p.G);
+            if (kWide) tiles += wide_tiles_of(s.rows, p.G);
             if (s.rows != 0u) first = min(first, s.pos);
         }
         if (wave_sum(sum) > p.b.max_rows) return false;
         rows = wave_max(top);
         first_pos = wave_min(first);
-        apart = rows * p.G > kTileRows && 4u * wave_sum(tiles) <= 5u * wide_tiles_of(rows, p.G);
+        apart = kWide && rows * p.G > kTileRows && 4u * wave_sum(tiles) <= 5u * wide_tiles_of(rows, p.G);
         uint32_t n = 0u, most = 0u, wide_n = 0u, wide_most = 0u;
         for (uint32_t r = lane; r < p.b.requests; r += 64u) {
             const Source s = r == lane ? mine : request_source(p, r);
             if (s.rows == 0u) continue;
             if (wide(p, s.rows)) {
-                wide_n += p.KVH * wide_head(p, s);
+                wide_n += wide_head(p, s);
                 wide_most = max(wide_most, ((apart ? p.b.prefix : 0u) + s.hi) / kKeyBlock + 1u);
             } else {
                 n += s.units(p.KVH);
@@ -270,21 +288,22 @@ struct Walk {
         }
         most = max(wave_max(most), prefix.blocks);
         units = wave_sum(n) + prefix.units(p.KVH);
-        wide_units = p.KVH * wide_tiles * wide_blocks;
-        if (rows * p.G > kTileRows) {
-            wide_units += wave_sum(wide_n);
+        wide_head_units = kWide ? prefix_units() : 0u;
+        if (kWide && rows * p.G > kTileRows) {
+            wide_head_units += wave_sum(wide_n);
             wide_most = max(wave_max(wide_most), wide_blocks);
         }
+        wide_units = p.KVH * wide_head_units;
         wide_groups = 0u;
         wide_per = 1u;
-        if (wide_units != 0u) {
+        if (kWide && wide_units != 0u) {
             wide_groups = p.groups;
             if (units != 0u) {
-                const float cost = static_cast<float>(wide_units) * kWideCost;
+                const float cost = static_cast<float>(wide_units) * p.wide_cost;
                 const float share = cost * __builtin_amdgcn_rcpf(cost + static_cast<float>(units));
                 wide_groups = min(max(static_cast<uint32_t>(static_cast<float>(p.groups) * share), 1u), p.groups - 1u);
             }
-            wide_per = max(ceil_div(wide_units, wide_groups), (wide_most + kMaxParts - 2u) / (kMaxParts - 1u));
+            wide_per = max(ceil_div(wide_units, wide_groups), (wide_most + kTileCost + kMaxParts - 2u) / (kMaxParts - 1u));
             wide_groups = ceil_div(wide_units, wide_per);
         }
         const uint32_t waves = max((p.groups - wide_groups) * kGroupWaves, 1u);
@@ -294,33 +313,33 @@ struct Walk {
 };
 
 // Requests 64 at a time, with running sums of their units of one kind.
+template <typename W>
 struct Chunk {
     Source mine;       // this lane's request
     uint32_t base;     // the first request
     uint32_t before;   // units before it
     uint32_t incl;     // with this lane's request
-    uint32_t head;     // wide tiles: this lane's units of one kv head
+    uint32_t own;      // this lane's units (of wide tiles: in one kv head)
     bool wide;
 
-    __device__ void load(const BatchParams& p, const Walk& w, uint32_t lane) {
+    __device__ void load(const BatchParams& p, const W& w, uint32_t lane) {
         mine = request_source(p, base + lane);
-        head = wide ? w.wide_head(p, mine) : 0u;
-        incl = wave_incl(wide ? p.KVH * head : w.few_units(p, mine));
+        own = wide ? w.wide_head(p, mine) : w.few_units(p, mine);
+        incl = wave_incl(own);
     }
-    __device__ void open(const BatchParams& p, const Walk& w, uint32_t lane, bool wide_) {
+    __device__ void open(const BatchParams& p, const W& w, uint32_t lane, bool wide_) {
         wide = wide_;
         base = 0u;
-        before = wide ? p.KVH * w.wide_tiles * w.wide_blocks : w.prefix.units(p.KVH);
+        before = wide ? w.prefix_units() : w.prefix.units(p.KVH);
         load(p, w, lane);
     }
-    __device__ uint32_t own_units(const BatchParams& p, const Walk& w) const { return wide ? p.KVH * head : w.few_units(p, mine); }
-    __device__ void next(const BatchParams& p, const Walk& w, uint32_t lane) {
+    __device__ void next(const BatchParams& p, const W& w, uint32_t lane) {
         before += from_lane(incl, 63u);
         base += 64u;
         load(p, w, lane);
     }
     // The lane whose request holds unit u (u >= before); 64 where none does.
-    __device__ uint32_t seek(const BatchParams& p, const Walk& w, uint32_t u, uint32_t lane) {
+    __device__ uint32_t seek(const BatchParams& p, const W& w, uint32_t u, uint32_t lane) {
         while (base + 64u < p.b.requests && u >= before + from_lane(incl, 63u))
             next(p, w, lane);
         const uint64_t behind = __ballot(u < before + incl);
@@ -345,17 +364,18 @@ __device__ __forceinline__ int32_t row_position(const BatchParams& p, uint32_t t
 }
 
 // What the merge needs: a wave writes 64 requests and their rows.
+template <bool kWide>
 __device__ __forceinline__ void scribe(const BatchParams& p, uint32_t chunk, uint32_t lane) {
-    Walk w;
+    Walk<kWide> w;
     if (!w.open(p, lane)) {
         if (chunk == 0u && lane == 0u) *p.header = Header{};
         return;
     }
     if (chunk == 0u && lane == 0u) {
-        *p.header = Header{w.few_per, w.wide_per, w.prefix.blocks, w.prefix.tiles, w.wide_blocks, w.wide_tiles, w.apart ? 1u : 0u, {}};
+        *p.header = Header{w.few_per, w.wide_per, w.prefix.blocks, w.prefix.tiles, w.wide_blocks, w.wide_tiles, w.wide_head_units, w.apart ? 1u : 0u, {}};
     }
     if (chunk >= p.b.requests) return;
-    Chunk few, wide;
+    Chunk<Walk<kWide>> few, wide;
     few.open(p, w, lane, false);
     wide.open(p, w, lane, true);
     while (few.base < chunk) {
@@ -365,9 +385,8 @@ __device__ __forceinline__ void scribe(const BatchParams& p, uint32_t chunk, uin
     const Source s = few.mine;
     const bool is_wide = w.wide(p, s.rows);
     if (chunk + lane < p.b.requests) {
-        p.request[chunk + lane] = Record{few.before + few.incl - few.own_units(p, w), s.tiles, is_wide ? 0u : s.blocks,
-                                         wide.before + wide.incl - wide.own_units(p, w),
-                                         is_wide ? wide_tiles_of(s.rows, p.G) : 0u, wide.head, {}};
+        p.request[chunk + lane] = Record{few.before + few.incl - few.own, s.tiles, is_wide ? 0u : s.blocks,
+                                         wide.before + wide.incl - wide.own, wide.own, {}};
     }
     for (uint32_t i = 0; i < 64u; ++i) {
         const uint32_t row0 = from_lane(s.row0, i);
