@@ -10,12 +10,12 @@
 // leaves the result independent of how the counting went, and right next to a border up to fp64
 // rounding.
 //
-// One workgroup takes a row:
-//  1. counts by value in LDS. A bin for each bf16 value of magnitude 2^-25 .. 2^7 (8192), one for
+// Steps, with one workgroup for 2 and 3 and, unless there are rows enough, several for 1:
+//  1. counts by value in LDS, each workgroup's for its chunk of the row; a second launch adds a row's chunks. A bin for each bf16 value of magnitude 2^-25 .. 2^7 (8192), one for
 //     what is nearer to 0, one for what is above and one for what is below;
 //  2. every thread takes 9 neighbouring bins, their weights, and scans of count and mass over the
 //     workgroup; then the kept count, the kept mass, the drawn rank, its bin and its number j there;
-//  3. the j-th token of that value, by counting along the row.
+//  3. the j-th token of that value: the chunk that holds it by the chunks' counts, then by counting along it.
 // Rows whose other three bins matter to the result (a value above 2^7; several values nearer to 0 than
 // 2^-25; values below -2^7 that are not negligible at this temperature) take the same steps over
 // windows of 8192 values of the whole order, counting the row again for each.
@@ -167,29 +167,20 @@ __device__ __forceinline__ Before block_scan(double mass, uint32_t count, Block&
     return b;
 }
 
-struct RowLds {
+struct alignas(16) RowLds {
     uint32_t count[kThreads * kPer];
     Block block;
     uint32_t infinite;             // +inf tokens
     uint32_t centre_lo, centre_hi; // least and largest place of the values next to 0
     uint32_t drawn, number;        // the drawn value's bits, the token's number among those
+    uint32_t bin;                  // and its bin, kBins where that is none of the first way
     double kept;
     uint32_t rank;
 };
 
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* __restrict__ logits, uint32_t vocab,
-                                                               const HypSamplingConfig* __restrict__ configs,
-                                                               const float* __restrict__ uniforms,
-                                                               uint32_t* __restrict__ tokens, float* __restrict__ logprobs) {
-    __shared__ RowLds s;
+// s.count, s.infinite, s.centre_lo and s.centre_hi of the tokens [begin, end) of a row. (A call has a barrier at its end.)
+__device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin, uint32_t end, RowLds& s) {
     const uint32_t tid = threadIdx.x;
-    const uint32_t lane = tid & 63u;
-    const uint32_t wave = tid >> 6;
-    const uint32_t row_at = blockIdx.x;
-    const uint16_t* row = logits + static_cast<size_t>(row_at) * vocab;
-    const RowParams prm = row_params(configs, uniforms, row_at);
-
-    // 1. Counts by value.
     for (uint32_t i = tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
     if (tid == 0u) {
         s.infinite = 0u;
@@ -197,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         s.centre_hi = 0u;
     }
     __syncthreads();
-    for_tokens(row, 0u, vocab, tid, kThreads, [&](uint32_t, uint32_t b) {
+    for_tokens(row, begin, end, tid, kThreads, [&](uint32_t, uint32_t b) {
         const uint32_t f = (b & 0x7FFFu) - kLow;
         uint32_t bin = (b & 0x8000u) != 0u ? kCentre + 1u + f : kFine - f;
         if (f >= kFine) {
@@ -215,11 +206,105 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         atomicAdd(&s.count[bin], 1u);
     });
     __syncthreads();
+}
+
+// A chunk's counts between the two launches (a chunk has at most kMaxChunk tokens: 16 bits do).
+constexpr uint32_t kStoredBins = (kBins + 7u) & ~7u;
+constexpr uint32_t kMaxChunk = 32768;
+struct alignas(16) ChunkCounts {
+    uint16_t count[kStoredBins];
+    uint32_t infinite, centre_lo, centre_hi, unused;
+};
+static_assert(kStoredBins <= kThreads * kPer && kMaxChunk < 65536u, "a chunk's counts");
+
+struct Chunks {
+    uint32_t n, tokens;   // chunks of a row, tokens of a chunk (the last one's may be fewer)
+};
+
+__global__ __launch_bounds__(kThreads) void sample_count_kernel(const uint16_t* __restrict__ logits, uint32_t vocab,
+                                                                Chunks chunks, ChunkCounts* __restrict__ counts) {
+    __shared__ RowLds s;
+    const uint32_t row = blockIdx.x / chunks.n;
+    const uint32_t begin = min(vocab, (blockIdx.x - row * chunks.n) * chunks.tokens);
+    count_values(logits + static_cast<size_t>(row) * vocab, begin, min(vocab, begin + chunks.tokens), s);
+    ChunkCounts& c = counts[blockIdx.x];
+    uint2* const out = reinterpret_cast<uint2*>(c.count);
+    for (uint32_t i = threadIdx.x; i < kStoredBins / 4u; i += kThreads) {
+        const uint4 n = *reinterpret_cast<const uint4*>(&s.count[4u * i]);
+        out[i] = make_uint2(n.x | n.y << 16, n.z | n.w << 16);
+    }
+    if (threadIdx.x == 0u) {
+        c.infinite = s.infinite;
+        c.centre_lo = s.centre_lo;
+        c.centre_hi = s.centre_hi;
+    }
+}
+
+// The same for a whole row, from its chunks.
+__device__ __forceinline__ void sum_counts(const ChunkCounts* counts, uint32_t n, RowLds& s) {
+    const uint32_t tid = threadIdx.x;
+    for (uint32_t i = kStoredBins + tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
+    for (uint32_t i = tid; i < kStoredBins / 4u; i += kThreads) {
+        uint4 sum = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 8
+        for (uint32_t c = 0; c < n; ++c) {
+            const uint2 v = reinterpret_cast<const uint2*>(counts[c].count)[i];
+            sum.x += v.x & 0xFFFFu;
+            sum.y += v.x >> 16;
+            sum.z += v.y & 0xFFFFu;
+            sum.w += v.y >> 16;
+        }
+        *reinterpret_cast<uint4*>(&s.count[4u * i]) = sum;
+    }
+    if (tid < 64u) {
+        uint32_t infinite = 0u, lo = 0xFFFFFFFFu, hi = 0u;
+        for (uint32_t c = tid; c < n; c += 64u) {
+            infinite += counts[c].infinite;
+            lo = min(lo, counts[c].centre_lo);
+            hi = max(hi, counts[c].centre_hi);
+        }
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) {
+            infinite += __shfl_xor(infinite, m, 64);
+            lo = min(lo, static_cast<uint32_t>(__shfl_xor(lo, m, 64)));
+            hi = max(hi, static_cast<uint32_t>(__shfl_xor(hi, m, 64)));
+        }
+        if (tid == 0u) {
+            s.infinite = infinite;
+            s.centre_lo = lo;
+            s.centre_hi = hi;
+        }
+    }
+    __syncthreads();
+}
+
+template <bool kSplit>
+__global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* __restrict__ logits, uint32_t vocab,
+                                                               const HypSamplingConfig* __restrict__ configs,
+                                                               const float* __restrict__ uniforms, Chunks chunks,
+                                                               const ChunkCounts* __restrict__ counts,
+                                                               uint32_t* __restrict__ tokens, float* __restrict__ logprobs) {
+    __shared__ RowLds s;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t lane = tid & 63u;
+    const uint32_t wave = tid >> 6;
+    const uint32_t row_at = blockIdx.x;
+    const uint16_t* row = logits + static_cast<size_t>(row_at) * vocab;
+    const RowParams prm = row_params(configs, uniforms, row_at);
+
+    // 1. Counts by value.
+    if constexpr (kSplit) {
+        counts += static_cast<size_t>(row_at) * chunks.n;
+        sum_counts(counts, chunks.n, s);
+    } else {
+        count_values(row, 0u, vocab, s);
+    }
 
     // 2. The drawn value and the token's number among those of that value.
     const uint32_t first = kPer * tid;
     uint32_t infinite = s.infinite;
     double logprob;
+    if (tid == 0u) s.bin = kBins;
     if (infinite != 0u) {
         // Weight 1 for each, 0 for everything else.
         uint32_t kept = infinite;
@@ -375,6 +460,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
                 if (rank - count < n) {
                     s.drawn = bits_of(bin);
                     s.number = rank - count;
+                    if (!slow) s.bin = bin;
                 }
             });
         });
@@ -382,12 +468,37 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         logprob = (value_of(s.drawn) - top) / prm.t - log(total);
     }
 
-    // 3. The token: each wave counts a stretch of the row, the one that holds it looks again.
+    // 3. The token: each wave counts a stretch of the row (or of the chunk that holds it), the one that
+    // holds it looks again.
     const uint32_t drawn = s.drawn;
     uint32_t number = s.number;
-    const uint32_t stretch = ((vocab + kWaves - 1u) / kWaves + 511u) & ~511u;
-    const uint32_t begin = min(vocab, wave * stretch);
-    const uint32_t end = min(vocab, begin + stretch);
+    uint32_t from_token = 0u, to_token = vocab;
+    if (kSplit && s.bin != kBins) {
+        const uint32_t bin = s.bin;
+        uint32_t chunk = 0u;
+        for (uint32_t base = 0; base < chunks.n; base += 64u) {   // (every wave for itself)
+            const uint32_t n = base + lane < chunks.n ? counts[base + lane].count[bin] : 0u;
+            uint32_t incl = n;
+#pragma unroll
+            for (uint32_t d = 1; d < 64u; d <<= 1) {
+                const uint32_t y = __shfl_up(incl, d, 64);
+                if (lane >= d) incl += y;
+            }
+            const uint64_t past = __ballot(incl > number);
+            if (past != 0u) {
+                const int at = __builtin_ctzll(past);
+                chunk = base + static_cast<uint32_t>(at);
+                number -= __shfl(incl - n, at, 64);
+                break;
+            }
+            number -= __shfl(incl, 63, 64);
+        }
+        from_token = min(vocab, chunk * chunks.tokens);
+        to_token = min(vocab, from_token + chunks.tokens);
+    }
+    const uint32_t stretch = ((to_token - from_token + kWaves - 1u) / kWaves + 511u) & ~511u;
+    const uint32_t begin = min(to_token, from_token + wave * stretch);
+    const uint32_t end = min(to_token, begin + stretch);
     uint32_t mine = 0u;
     for_tokens(row, begin, end, lane, 64u, [&](uint32_t, uint32_t b) { mine += plain_bits(b) == drawn ? 1u : 0u; });
 #pragma unroll
@@ -425,17 +536,44 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
     }
 }
 
+// A row's chunks: enough workgroups for the device (two are on a compute unit), but no more than the second launch
+// reads in little time. Measured with 256 .. 1024 workgroups, chunks of 4096 .. 16384 and 16 .. 64 of them:
+// 400 rows of 128000 took 83 us with 512 workgroups and more, 114 with 256; one row of 262144 took 27.5 us with 16
+// chunks, 29 with 32 and 37 with 64; what else was tried differed by a tenth at most.
+constexpr uint32_t kFill = 512;
+constexpr uint32_t kMinChunk = 8192;
+constexpr uint32_t kMostChunks = 16;
+Chunks chunks_of(uint32_t rows, uint32_t vocab) {
+    uint32_t n = rows == 0u ? 1u : std::min((kFill + rows - 1u) / rows, std::min(vocab / kMinChunk + 1u, kMostChunks));
+    if (n <= 1u) return {1u, vocab};
+    n = std::max(n, (vocab + kMaxChunk - 1u) / kMaxChunk);
+    const uint32_t tokens = std::min(((vocab + n - 1u) / n + 511u) & ~511u, kMaxChunk);
+    return {(vocab + tokens - 1u) / tokens, tokens};
+}
+
 }  // namespace
 
 uint32_t sample_batch_max_vocab() { return kMaxVocab; }
 
-size_t sample_batch_workspace_bytes(uint32_t, uint32_t) { return 0u; }
+size_t sample_batch_workspace_bytes(uint32_t rows, uint32_t vocab) {
+    const Chunks c = chunks_of(rows, vocab);
+    return c.n > 1u ? static_cast<size_t>(rows) * c.n * sizeof(ChunkCounts) : 0u;
+}
 
 void launch_sample_batch(const uint16_t* logits, uint32_t rows, uint32_t vocab, const HypSamplingConfig* configs,
-                         const float* uniforms, uint32_t* tokens, float* logprobs, void*, size_t,
-                         hipStream_t stream) {
-    hipLaunchKernelGGL(sample_rows_kernel, dim3(rows), dim3(kThreads), 0, stream, logits, vocab, configs, uniforms, tokens,
-                       logprobs);
+                         const float* uniforms, uint32_t* tokens, float* logprobs, void* workspace,
+                         size_t, hipStream_t stream) {
+    const Chunks c = chunks_of(rows, vocab);
+    if (c.n > 1u) {
+        ChunkCounts* const counts = static_cast<ChunkCounts*>(workspace);
+        hipLaunchKernelGGL(sample_count_kernel, dim3(rows * c.n), dim3(kThreads), 0, stream, logits, vocab, c, counts);
+        HYP_HIP_CHECK(hipGetLastError());
+        hipLaunchKernelGGL(sample_rows_kernel<true>, dim3(rows), dim3(kThreads), 0, stream, logits, vocab, configs, uniforms,
+                           c, counts, tokens, logprobs);
+    } else {
+        hipLaunchKernelGGL(sample_rows_kernel<false>, dim3(rows), dim3(kThreads), 0, stream, logits, vocab, configs,
+                           uniforms, c, nullptr, tokens, logprobs);
+    }
     HYP_HIP_CHECK(hipGetLastError());
 }
 
