@@ -12,6 +12,7 @@
 #include "attention.h"
 #include "batch.h"
 #include "common.h"
+#include "wave.h"
 
 namespace hyperion::hip {
 
@@ -170,36 +171,6 @@ __device__ __forceinline__ Source request_source(const BatchParams& p, uint32_t 
 // The same value in every lane, as a scalar.
 __device__ __forceinline__ uint32_t scalar(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
 __device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-
-__device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) {
-    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
-}
-
-// Inclusive scan over the wave by register moves between lanes: 1, 2, 4 and 8 lanes on within rows of
-// 16, then the last lane of row 0 and 2 to the next row, of row 1 to the upper half. `none` is the operation's
-// neutral value. (Through LDS permutes a reduction takes six times their latency, and a call forms ten.)
-template <typename Op>
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t none, Op&& op) {
-    const int n = static_cast<int>(none);
-    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x111, 0xF, 0xF, false)));
-    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x112, 0xF, 0xF, false)));
-    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x114, 0xF, 0xF, false)));
-    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x118, 0xF, 0xF, false)));
-    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x142, 0xA, 0xF, false)));
-    return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(n, static_cast<int>(v), 0x143, 0xC, 0xF, false)));
-}
-__device__ __forceinline__ uint32_t wave_incl(uint32_t v) {
-    return wave_scan(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
-}
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) { return from_lane(wave_incl(v), 63u); }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    return from_lane(wave_scan(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); }), 63u);
-}
-__device__ __forceinline__ int32_t wave_min(int32_t v) {
-    return static_cast<int32_t>(from_lane(wave_scan(static_cast<uint32_t>(v), 0x7FFFFFFFu, [](uint32_t a, uint32_t b) {
-        return static_cast<uint32_t>(min(static_cast<int32_t>(a), static_cast<int32_t>(b)));
-    }), 63u));
-}
 
 // The batch as one wave sees it. Which rows go where: rows of one request that fill wide tiles by
 // themselves read the prefix there, at one pass over all their keys, where that takes at most a quarter

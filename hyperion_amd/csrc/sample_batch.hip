@@ -25,6 +25,7 @@
 #include "common.h"
 #include "kernels.h"
 #include "sample_batch.h"
+#include "wave.h"
 
 namespace hyperion::hip {
 namespace {
@@ -46,7 +47,7 @@ constexpr uint32_t kMaxVocab = 1u << 23;
 static_assert(kBins <= kThreads * kPer, "a thread's bins");
 
 struct RowParams {
-    double t;        // the weights' temperature (1 for a greedy row)
+    double by_t;     // 1 / the weights' temperature (1 for a greedy row)
     double top_p, min_p, u;
     uint32_t top_k;  // 0: off
     bool greedy;
@@ -56,7 +57,7 @@ __device__ __forceinline__ RowParams row_params(const HypSamplingConfig* configs
     const HypSamplingConfig c = configs[row];
     RowParams r;
     r.greedy = !(c.temperature > 0.0f);
-    r.t = r.greedy ? 1.0 : static_cast<double>(c.temperature);
+    r.by_t = r.greedy ? 1.0 : 1.0 / static_cast<double>(c.temperature);
     r.top_p = c.top_p > 0.0f && c.top_p < 1.0f ? static_cast<double>(c.top_p) : 0.0;
     r.min_p = c.min_p > 0.0f ? static_cast<double>(c.min_p) : 0.0;
     r.top_k = c.top_k > 0 ? static_cast<uint32_t>(c.top_k) : 0u;
@@ -95,55 +96,33 @@ __device__ __forceinline__ void for_tokens(const uint16_t* row, uint32_t begin, 
     for (uint32_t k = i; k < end && k < i + 8u; ++k) f(k, static_cast<uint32_t>(row[k]));
 }
 
-// Sums over the workgroup, each value in the same order for every thread.
 struct Block {
     double d[kWaves];
-    uint64_t u[kWaves];
+    uint32_t u[kWaves];
 };
 
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, Block& s) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0u) s.u[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t r = 0u;
-    for (uint32_t w = 0; w < kWaves; ++w) r += s.u[w];
-    return r;
-}
-
 __device__ __forceinline__ uint32_t block_min(uint32_t v, Block& s) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = min(v, static_cast<uint32_t>(__shfl_xor(v, m, 64)));
+    v = from_lane(wave_scan(v, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0u) s.u[threadIdx.x >> 6] = v;
     __syncthreads();
     uint32_t r = 0xFFFFFFFFu;
-    for (uint32_t w = 0; w < kWaves; ++w) r = min(r, static_cast<uint32_t>(s.u[w]));
+    for (uint32_t w = 0; w < kWaves; ++w) r = min(r, s.u[w]);
     return r;
 }
 
-// Mass and count before this thread's bins, and the totals.
+// Mass and count before this thread's bins, and the totals: added in the same order for every thread.
 struct Before {
     double mass, mass_all;
     uint32_t count, count_all;
 };
 
+// (Every wave has left the block's words.)
 __device__ __forceinline__ Before block_scan(double mass, uint32_t count, Block& s) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = threadIdx.x >> 6;
-    double m = mass;
-    uint32_t c = count;
-#pragma unroll
-    for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const double y = __shfl_up(m, d, 64);
-        const uint32_t z = __shfl_up(c, d, 64);
-        if (lane >= d) {
-            m += y;
-            c += z;
-        }
-    }
-    __syncthreads();
+    const double m = wave_incl(mass);
+    const uint32_t c = wave_incl(count);
     if (lane == 63u) {
         s.d[wave] = m;
         s.u[wave] = c;
@@ -156,15 +135,27 @@ __device__ __forceinline__ Before block_scan(double mass, uint32_t count, Block&
             b.count = b.count_all;
         }
         b.mass_all += s.d[w];
-        b.count_all += static_cast<uint32_t>(s.u[w]);
+        b.count_all += s.u[w];
     }
     const double mx = __shfl_up(m, 1u, 64);
-    const uint32_t cx = __shfl_up(c, 1u, 64);
-    if (lane != 0u) {
-        b.mass += mx;
-        b.count += cx;
-    }
+    if (lane != 0u) b.mass += mx;
+    b.count += c - count;
     return b;
+}
+
+// e^x of an x <= 0: 2^n e^r with r = x - n ln 2 in [-ln 2 / 2, ln 2 / 2], the series to r^13 (the rest is below 2^-57).
+// Without the library's branches nine of them run side by side.
+__device__ __forceinline__ double exp_below(double x) {
+    x = fmin(fmax(x, -1100.0), 0.0);
+    const double n = __builtin_rint(x * 0x1.71547652b82fep+0);
+    const double r = __builtin_fma(n, -0x1.abc9e3b39803fp-56, __builtin_fma(n, -0x1.62e42fefa39efp-1, x));
+    double y = 1.0 / 6227020800.0;
+    constexpr double kSeries[] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0,
+                                  1.0 / 5040.0,      1.0 / 720.0,      1.0 / 120.0,     1.0 / 24.0,     1.0 / 6.0,
+                                  0.5,               1.0,              1.0};
+#pragma unroll
+    for (const double c : kSeries) y = __builtin_fma(y, r, c);
+    return __builtin_amdgcn_ldexp(y, static_cast<int>(n));
 }
 
 struct alignas(16) RowLds {
@@ -174,8 +165,9 @@ struct alignas(16) RowLds {
     uint32_t centre_lo, centre_hi; // least and largest place of the values next to 0
     uint32_t drawn, number;        // the drawn value's bits, the token's number among those
     uint32_t bin;                  // and its bin, kBins where that is none of the first way
-    double kept;
-    uint32_t rank;
+    double kept;                   // the kept tokens' mass
+    uint32_t keep, rank;           // how many tokens the filters keep, the drawn one's rank
+    uint32_t lead[kWaves];         // a wave's first bin with a token
 };
 
 // s.count, s.infinite, s.centre_lo and s.centre_hi of the tokens [begin, end) of a row. (A call has a barrier at its end.)
@@ -240,41 +232,57 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(const uint16_t* 
     }
 }
 
-// The same for a whole row, from its chunks.
+// The same for a whole row, from its chunks: eight bins to a thread, the last ones to the first lanes, a chunk each.
 __device__ __forceinline__ void sum_counts(const ChunkCounts* counts, uint32_t n, RowLds& s) {
     const uint32_t tid = threadIdx.x;
-    for (uint32_t i = kStoredBins + tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
-    for (uint32_t i = tid; i < kStoredBins / 4u; i += kThreads) {
-        uint4 sum = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 8
-        for (uint32_t c = 0; c < n; ++c) {
-            const uint2 v = reinterpret_cast<const uint2*>(counts[c].count)[i];
-            sum.x += v.x & 0xFFFFu;
-            sum.y += v.x >> 16;
-            sum.z += v.y & 0xFFFFu;
-            sum.w += v.y >> 16;
+    static_assert(kStoredBins == 8u * kThreads + 8u && kBins <= 8u * kThreads + 4u, "a thread's bins");
+    uint32_t sum[8] = {};
+    const auto add = [&](uint4 v) HYP_INLINE {
+        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            sum[2u * k] += word[k] & 0xFFFFu;
+            sum[2u * k + 1u] += word[k] >> 16;
         }
-        *reinterpret_cast<uint4*>(&s.count[4u * i]) = sum;
-    }
+    };
     if (tid < 64u) {
-        uint32_t infinite = 0u, lo = 0xFFFFFFFFu, hi = 0u;
+        uint32_t infinite = 0u, lo = 0xFFFFFFFFu, hi = 0u, last[4] = {};
         for (uint32_t c = tid; c < n; c += 64u) {
+            const uint2 v = *reinterpret_cast<const uint2*>(counts[c].count + 8u * kThreads);
             infinite += counts[c].infinite;
             lo = min(lo, counts[c].centre_lo);
             hi = max(hi, counts[c].centre_hi);
+            last[0] += v.x & 0xFFFFu;
+            last[1] += v.x >> 16;
+            last[2] += v.y & 0xFFFFu;
+            last[3] += v.y >> 16;
         }
+        infinite = wave_sum(infinite);
+        lo = from_lane(wave_scan(lo, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);
+        hi = wave_max(hi);
 #pragma unroll
-        for (int m = 32; m > 0; m >>= 1) {
-            infinite += __shfl_xor(infinite, m, 64);
-            lo = min(lo, static_cast<uint32_t>(__shfl_xor(lo, m, 64)));
-            hi = max(hi, static_cast<uint32_t>(__shfl_xor(hi, m, 64)));
-        }
+        for (uint32_t k = 0; k < 4u; ++k) last[k] = wave_sum(last[k]);
         if (tid == 0u) {
             s.infinite = infinite;
             s.centre_lo = lo;
             s.centre_hi = hi;
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) s.count[8u * kThreads + k] = last[k];
         }
     }
+    uint32_t c = 0;
+    for (; c + 8u <= n; c += 8u) {
+        uint4 v[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) v[k] = reinterpret_cast<const uint4*>(counts[c + k].count)[tid];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) add(v[k]);
+    }
+#pragma unroll 4
+    for (; c < n; ++c) add(reinterpret_cast<const uint4*>(counts[c].count)[tid]);
+    *reinterpret_cast<uint4*>(&s.count[8u * tid]) = make_uint4(sum[0], sum[1], sum[2], sum[3]);
+    *reinterpret_cast<uint4*>(&s.count[8u * tid + 4u]) = make_uint4(sum[4], sum[5], sum[6], sum[7]);
+    for (uint32_t i = 8u * kThreads + 4u + tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
     __syncthreads();
 }
 
@@ -302,9 +310,25 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
 
     // 2. The drawn value and the token's number among those of that value.
     const uint32_t first = kPer * tid;
-    uint32_t infinite = s.infinite;
+    const uint32_t infinite = s.infinite;
+    uint32_t num[kPer];   // this thread's bins: tokens,
+    double weight[kPer];  // weights
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) num[i] = s.count[first + i];
+    {
+        uint32_t lead = 0xFFFFFFFFu;
+#pragma unroll
+        for (uint32_t i = kPer; i-- > 0u;) lead = num[i] != 0u ? first + i : lead;
+        const uint64_t has = __ballot(lead != 0xFFFFFFFFu);
+        lead = from_lane(lead, has != 0u ? static_cast<uint32_t>(__builtin_ctzll(has)) : 0u);
+        if (lane == 0u) s.lead[wave] = lead;
+    }
+    if (tid == 0u) {
+        s.bin = kBins;
+        s.keep = s.rank = 0xFFFFFFFFu;
+    }
+    __syncthreads();
     double logprob;
-    if (tid == 0u) s.bin = kBins;
     if (infinite != 0u) {
         // Weight 1 for each, 0 for everything else.
         uint32_t kept = infinite;
@@ -319,9 +343,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         __syncthreads();
     } else {
         uint32_t lead = 0xFFFFFFFFu;
-        for (uint32_t i = 0; i < kPer; ++i)
-            if (lead == 0xFFFFFFFFu && s.count[first + i] != 0u) lead = first + i;
-        lead = block_min(lead, s.block);
+        for (uint32_t w = 0; w < kWaves; ++w) lead = min(lead, s.lead[w]);
         if (lead == 0xFFFFFFFFu) {   // nothing above -inf
             if (tid == 0u) {
                 tokens[row_at] = 0u;
@@ -333,9 +355,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
             return bin <= kFine ? kLow + (kFine - bin) : (bin == kCentre ? bits_at(s.centre_lo) : 0x8000u | (kLow + (bin - kCentre - 1u)));
         };
         // The long way's windows that hold values, and its largest value.
-        const uint32_t below = s.count[kBelow];
         bool slow = lead == kAbove || lead == kBelow || (s.count[kCentre] != 0u && s.centre_lo != s.centre_hi);
-        if (!slow && below != 0u) slow = !((value_of(fine_bits(lead)) + 128.0) / prm.t > 80.0);   // (2^23 times e^-80)
+        if (!slow && s.count[kBelow] != 0u)   // (2^23 times e^-80)
+            slow = !((value_of(fine_bits(lead)) + 128.0) * prm.by_t > 80.0);
         double top = 0.0;
         uint32_t windows = 1u;
         if (slow) {
@@ -357,27 +379,32 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         }
         uint32_t window = 0u;   // the first place of the window in hand
         const auto bits_of = [&](uint32_t bin) HYP_INLINE { return slow ? bits_at(window + bin) : fine_bits(bin); };
-        double weight[kPer];
         Before at{};
+        uint32_t here = 0u;     // this thread's tokens
         const auto weigh = [&]() HYP_INLINE {
-            double mass = 0.0;
-            uint32_t count = 0u;
+            here = 0u;
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) {
-                const uint32_t n = s.count[first + i];
-                const uint32_t bin = first + i;
+                here += num[i];
                 weight[i] = 0.0;
-                if (n != 0u && (slow || bin != kBelow)) weight[i] = exp((value_of(bits_of(bin)) - top) / prm.t);
-                mass += n * weight[i];
-                count += n;
             }
-            at = block_scan(mass, count, s.block);
+            double mass = 0.0;
+            if (here != 0u) {
+#pragma unroll
+                for (uint32_t i = 0; i < kPer; ++i) {
+                    const uint32_t bin = first + i;
+                    const double w = exp_below((value_of(bits_of(bin)) - top) * prm.by_t);
+                    if (num[i] != 0u && (slow || bin != kBelow)) weight[i] = w;
+                    mass += num[i] * weight[i];
+                }
+            }
+            at = block_scan(mass, here, s.block);
         };
         if (!slow) weigh();
-        // f() with each window's counts and weights in hand, and what lies before the window.
+        // f() with each window's counts and weights in hand, and what lies before this thread's bins.
         const auto over_windows = [&](auto&& f) HYP_INLINE {
             if (!slow) {
-                f(0.0, 0u);
+                f(at.mass, at.count);
                 return;
             }
             double mass = 0.0;
@@ -394,82 +421,115 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
                     if (finite_bits(b) && d < kWindow) atomicAdd(&s.count[d], 1u);
                 });
                 __syncthreads();
+#pragma unroll
+                for (uint32_t i = 0; i < kPer; ++i) num[i] = s.count[first + i];
                 weigh();
-                f(mass, count);
+                f(mass + at.mass, count + at.count);
                 mass += at.mass_all;
                 count += at.count_all;
             }
         };
-        // Runs over this thread's bins: f(bin index, tokens, weight, mass before, tokens before).
-        const auto over_bins = [&](double mass, uint32_t count, auto&& f) HYP_INLINE {
-            mass += at.mass;
-            count += at.count;
+        // The mass up to and with this thread's bins.
+        const auto mass_with = [&](double mass) HYP_INLINE {
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) {
-                const uint32_t n = s.count[first + i];
-                f(first + i, n, weight[i], mass, count);
-                mass += n * weight[i];
-                count += n;
-            }
+            for (uint32_t i = 0; i < kPer; ++i) mass += num[i] * weight[i];
+            return mass;
         };
         double total = 0.0;
         uint32_t all = 0u;
-        over_windows([&](double mass, uint32_t count) HYP_INLINE {
-            total = mass + at.mass_all;
-            all = count + at.count_all;
-        });
+        if (slow) {
+            over_windows([&](double, uint32_t) HYP_INLINE {
+                total += at.mass_all;
+                all += at.count_all;
+            });
+        } else {
+            total = at.mass_all;
+            all = at.count_all;
+        }
         uint32_t kept = all;
         if (prm.top_k != 0u) kept = min(kept, prm.top_k);
         if (prm.top_p != 0.0 || prm.min_p != 0.0) {
-            uint64_t both = 0u;   // tokens that top-p keeps, and min-p
-            over_windows([&](double m0, uint32_t c0) HYP_INLINE {
-                over_bins(m0, c0, [&](uint32_t, uint32_t n, double w, double mass, uint32_t) HYP_INLINE {
-                    if (n == 0u) return;
-                    uint32_t c = n;
-                    if (prm.top_p != 0.0) {
-                        const double room = prm.top_p * total - mass;
-                        c = room <= 0.0 ? 0u : (room >= n * w ? n : min(n, static_cast<uint32_t>(ceil(room / w))));
+            // A wave's first lane whose bins a filter does not keep whole goes through them.
+            const double enough = prm.top_p * total;
+            over_windows([&](double mass, uint32_t count) HYP_INLINE {
+                uint32_t keep = 0xFFFFFFFFu;
+                if (prm.top_p != 0.0) {
+                    const uint64_t past = __ballot(mass_with(mass) > enough);
+                    if (past != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(past))) {
+                        keep = count;
+                        double m = mass;
+#pragma unroll
+                        for (uint32_t i = 0; i < kPer; ++i) {
+                            const double room = enough - m;
+                            const double some = num[i] * weight[i];
+                            if (num[i] != 0u && room > 0.0)
+                                keep += room >= some ? num[i] : min(num[i], static_cast<uint32_t>(ceil(room / weight[i])));
+                            m += some;
+                        }
                     }
-                    both += c;
-                    if (w >= prm.min_p) both += static_cast<uint64_t>(n) << 32;
-                });
+                }
+                uint32_t light = 0u;   // before the first token that min-p drops
+                bool dropped = false;
+#pragma unroll
+                for (uint32_t i = 0; i < kPer; ++i) {
+                    dropped = dropped || (num[i] != 0u && weight[i] < prm.min_p);
+                    light += dropped ? 0u : num[i];
+                }
+                const uint64_t drops = __ballot(dropped);
+                if (drops != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(drops))) keep = min(keep, count + light);
+                if (keep != 0xFFFFFFFFu) atomicMin(&s.keep, keep);
             });
-            both = block_sum(both, s.block);
-            kept = min(kept, min(static_cast<uint32_t>(both), static_cast<uint32_t>(both >> 32)));
+            __syncthreads();
+            kept = min(kept, s.keep);
         }
         kept = prm.greedy ? 1u : max(kept, 1u);
         // The kept tokens' mass, the rank of the draw, its value.
-        over_windows([&](double m0, uint32_t c0) HYP_INLINE {
-            over_bins(m0, c0, [&](uint32_t, uint32_t n, double w, double mass, uint32_t count) HYP_INLINE {
-                if (kept - 1u - count < n) s.kept = mass + (kept - count) * w;
-            });
+        over_windows([&](double mass, uint32_t count) HYP_INLINE {
+            if (kept - 1u - count >= here) return;
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) {
+                if (kept - 1u - count < num[i]) s.kept = mass + (kept - count) * weight[i];
+                mass += num[i] * weight[i];
+                count += num[i];
+            }
         });
         __syncthreads();
         const double goal = prm.u * s.kept;
-        uint32_t rank = 0xFFFFFFFFu;
-        over_windows([&](double m0, uint32_t c0) HYP_INLINE {
-            over_bins(m0, c0, [&](uint32_t, uint32_t n, double w, double mass, uint32_t count) HYP_INLINE {
-                if (rank != 0xFFFFFFFFu || n == 0u || !(mass + n * w > goal)) return;
-                const double j = (goal - mass) / w;
-                rank = count + (j > 0.0 ? min(static_cast<uint32_t>(fmin(j, 4.0e9)), n - 1u) : 0u);
-            });
-        });
-        rank = min(block_min(rank, s.block), kept - 1u);
-        over_windows([&](double m0, uint32_t c0) HYP_INLINE {
-            over_bins(m0, c0, [&](uint32_t bin, uint32_t n, double, double, uint32_t count) HYP_INLINE {
-                if (rank - count < n) {
-                    s.drawn = bits_of(bin);
-                    s.number = rank - count;
-                    if (!slow) s.bin = bin;
+        over_windows([&](double mass, uint32_t count) HYP_INLINE {
+            const uint64_t past = __ballot(mass_with(mass) > goal);
+            if (past == 0u || lane != static_cast<uint32_t>(__builtin_ctzll(past))) return;
+            uint32_t rank = 0xFFFFFFFFu;
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) {
+                if (rank == 0xFFFFFFFFu && num[i] != 0u && mass + num[i] * weight[i] > goal) {
+                    const double j = (goal - mass) / weight[i];
+                    rank = count + (j > 0.0 ? min(static_cast<uint32_t>(fmin(j, 4.0e9)), num[i] - 1u) : 0u);
                 }
-            });
+                mass += num[i] * weight[i];
+                count += num[i];
+            }
+            atomicMin(&s.rank, rank);
         });
         __syncthreads();
-        logprob = (value_of(s.drawn) - top) / prm.t - log(total);
+        const uint32_t rank = min(s.rank, kept - 1u);
+        over_windows([&](double, uint32_t count) HYP_INLINE {
+            if (rank - count >= here) return;
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) {
+                if (rank - count < num[i]) {
+                    s.drawn = bits_of(first + i);
+                    s.number = rank - count;
+                    if (!slow) s.bin = first + i;
+                }
+                count += num[i];
+            }
+        });
+        __syncthreads();
+        logprob = (value_of(s.drawn) - top) * prm.by_t - log(total);
     }
 
-    // 3. The token: each wave counts a stretch of the row (or of the chunk that holds it), the one that
-    // holds it looks again.
+    // 3. The token, in the row or in the chunk that holds it: each wave marks the value's places in its stretch, 512
+    // tokens a step.
     const uint32_t drawn = s.drawn;
     uint32_t number = s.number;
     uint32_t from_token = 0u, to_token = vocab;
@@ -478,61 +538,73 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         uint32_t chunk = 0u;
         for (uint32_t base = 0; base < chunks.n; base += 64u) {   // (every wave for itself)
             const uint32_t n = base + lane < chunks.n ? counts[base + lane].count[bin] : 0u;
-            uint32_t incl = n;
-#pragma unroll
-            for (uint32_t d = 1; d < 64u; d <<= 1) {
-                const uint32_t y = __shfl_up(incl, d, 64);
-                if (lane >= d) incl += y;
-            }
+            const uint32_t incl = wave_incl(n);
             const uint64_t past = __ballot(incl > number);
             if (past != 0u) {
-                const int at = __builtin_ctzll(past);
-                chunk = base + static_cast<uint32_t>(at);
-                number -= __shfl(incl - n, at, 64);
+                const uint32_t holder = static_cast<uint32_t>(__builtin_ctzll(past));
+                chunk = base + holder;
+                number -= from_lane(incl - n, holder);
                 break;
             }
-            number -= __shfl(incl, 63, 64);
+            number -= from_lane(incl, 63u);
         }
         from_token = min(vocab, chunk * chunks.tokens);
         to_token = min(vocab, from_token + chunks.tokens);
     }
-    const uint32_t stretch = ((to_token - from_token + kWaves - 1u) / kWaves + 511u) & ~511u;
-    const uint32_t begin = min(to_token, from_token + wave * stretch);
-    const uint32_t end = min(to_token, begin + stretch);
-    uint32_t mine = 0u;
-    for_tokens(row, begin, end, lane, 64u, [&](uint32_t, uint32_t b) { mine += plain_bits(b) == drawn ? 1u : 0u; });
+    constexpr uint32_t kStep = 512u, kSteps = 8u;
+    for (uint32_t base = from_token; base < to_token; base += kWaves * kSteps * kStep) {
+        const uint32_t end = min(to_token, base + kWaves * kSteps * kStep);
+        const uint32_t steps = (end - base + kWaves * kStep - 1u) / (kWaves * kStep);
+        const uint32_t begin = base + wave * steps * kStep + 8u * lane;   // the lane's, of the first step
+        Eight e[kSteps];
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) mine += __shfl_xor(mine, m, 64);
-    __syncthreads();
-    if (lane == 0u) s.block.u[wave] = mine;
-    __syncthreads();
-    for (uint32_t w = 0; w < wave; ++w) number -= static_cast<uint32_t>(s.block.u[w]);   // (wraps past the holder)
-    if (number >= mine) return;
-    for (uint32_t at = begin; at < end; at += 512u) {
-        uint32_t n = 0u;
-        const uint32_t from = at + 8u * lane;
-        for (uint32_t k = from; k < min(end, from + 8u); ++k) n += plain_bits(row[k]) == drawn ? 1u : 0u;
-        uint32_t incl = n;
+        for (uint32_t k = 0; k < kSteps; ++k)
+            if (k < steps && begin + k * kStep + 8u <= end) __builtin_memcpy(&e[k], row + begin + k * kStep, 16);
+        uint64_t hits = 0u;   // a byte a step
 #pragma unroll
-        for (uint32_t d = 1; d < 64u; d <<= 1) {
-            const uint32_t y = __shfl_up(incl, d, 64);
-            if (lane >= d) incl += y;
+        for (uint32_t k = 0; k < kSteps; ++k) {
+            const uint32_t from = begin + k * kStep;
+            if (k >= steps || from >= end) continue;
+            uint32_t bits = 0u;
+            if (from + 8u <= end) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) bits |= plain_bits(e[k].v[i]) == drawn ? 1u << i : 0u;
+            } else {
+                for (uint32_t i = 0; from + i < end; ++i) bits |= plain_bits(row[from + i]) == drawn ? 1u << i : 0u;
+            }
+            hits |= static_cast<uint64_t>(bits) << (8u * k);
         }
-        const uint32_t before = incl - n;
-        if (number - before < n) {
-            uint32_t left = number - before;
-            for (uint32_t k = from; k < min(end, from + 8u); ++k) {
-                if (plain_bits(row[k]) != drawn) continue;
-                if (left == 0u) {
-                    tokens[row_at] = k;
+        const uint32_t mine = wave_sum(static_cast<uint32_t>(__popcll(hits)));
+        __syncthreads();
+        if (lane == 0u) s.block.u[wave] = mine;
+        __syncthreads();
+        uint32_t before = 0u, all = 0u;
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            if (w == wave) before = all;
+            all += s.block.u[w];
+        }
+        if (number >= all) {
+            number -= all;
+            continue;
+        }
+        uint32_t left = number - before;   // (wraps past the holder)
+        if (left >= mine) return;
+        for (uint32_t k = 0; k < steps; ++k) {
+            uint32_t bits = static_cast<uint32_t>(hits >> (8u * k)) & 0xFFu;
+            const uint32_t n = static_cast<uint32_t>(__popc(bits));
+            const uint32_t incl = wave_incl(n);
+            const uint32_t step = from_lane(incl, 63u);
+            if (left < step) {
+                if (left - (incl - n) < n) {
+                    for (uint32_t i = left - (incl - n); i != 0u; --i) bits &= bits - 1u;
+                    tokens[row_at] = begin + k * kStep + static_cast<uint32_t>(__builtin_ctz(bits));
                     if (logprobs != nullptr) logprobs[row_at] = static_cast<float>(logprob);
                 }
-                --left;
+                return;
             }
+            left -= step;
         }
-        const uint32_t here = __shfl(incl, 63, 64);
-        if (number < here) return;
-        number -= here;
+        return;
     }
 }
 
