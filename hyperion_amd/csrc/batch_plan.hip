@@ -9,10 +9,12 @@
 //
 // What bounds it: the latency of its steps (lengths, sums, table entries, slots), a few KB of
 // traffic. One workgroup keeps the sums in LDS and every thread finds its block's or row's
-// request there by bisection; rows past kRowsHere go to a second launch over all compute units,
-// which reads the finished tables.
+// request there by bisection. With more than kRowsHere rows the blocks and rows go to a second launch over
+// all compute units: 509 prompts (352000 rows, 12000 blocks) take 15.0 us, of which the launch of the sums is about 6.
+// 64 requests' decode step takes 7.9 us, 6400 rows of 64 requests 11.0 in one launch and 12.6 in two.
 #include "batch.h"
 #include "common.h"
+#include "wave.h"
 
 namespace hyperion::hip {
 namespace {
@@ -20,7 +22,7 @@ namespace {
 constexpr uint32_t kThreads = 1024;
 constexpr uint32_t kWaves = kThreads / 64u;
 constexpr uint32_t kPer = kMaxRequests / kThreads;   // consecutive requests of a thread
-constexpr uint32_t kRowsHere = 16384;
+constexpr uint32_t kRowsHere = 8192;
 constexpr uint32_t kRowThreads = 256;
 constexpr uint32_t kRowsEach = 4;
 
@@ -178,12 +180,12 @@ __global__ __launch_bounds__(kThreads) void batch_plan_kernel(PlanParams p) {
         *p.taken_out = c + fresh;
         *p.served = served;
     }
+    if (p.rows_here == 0u) return;
     for (uint32_t g = tid; g < fresh; g += kThreads) {
         const uint32_t r = owner(block_sum, served, g);
         const uint32_t entry = static_cast<uint32_t>(blocks_of(len_of[r])) + (g - block_sum[r]);
         b.tables[static_cast<size_t>(r) * b.max_blocks + entry] = p.free_blocks[c + g];
     }
-    if (p.rows_here == 0u) return;
     for (uint32_t t = tid; t < b.max_rows; t += kThreads) {
         uint32_t slot = HYP_SLOT_NONE;
         uint32_t pos = 0u;
@@ -202,23 +204,62 @@ __global__ __launch_bounds__(kThreads) void batch_plan_kernel(PlanParams p) {
     }
 }
 
-// The rows of a large step, from the finished tables: lens holds the lengths with this step's
-// rows, so row i of request b is token lens[b] - rows of b + i.
-__global__ __launch_bounds__(kRowThreads) void batch_rows_kernel(BatchView b) {
+// The new blocks and rows of a large step. lens holds the lengths with this step's rows, so row i of request b is
+// token lens[b] - rows of b + i, and a request's new blocks follow from the two: every workgroup forms their sums
+// for itself. A new block holds a new row, whose first one writes the table's entry.
+__global__ __launch_bounds__(kRowThreads) void batch_rows_kernel(PlanParams p) {
+    __shared__ uint32_t len_of[kMaxRequests];   // before the step
     __shared__ uint32_t row_sum[kMaxRequests + 1];
-    for (uint32_t r = threadIdx.x; r <= b.requests; r += kRowThreads) row_sum[r] = b.row_start[r];
+    __shared__ uint32_t block_sum[kMaxRequests];
+    __shared__ uint32_t wave_total[kRowThreads / 64u];
+    const BatchView& b = p.b;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t n = b.requests;
+    const uint32_t mask = (1u << b.shift) - 1u;
+    const uint32_t taken = *p.taken_out;
+    for (uint32_t r = tid; r <= n; r += kRowThreads) {
+        row_sum[r] = b.row_start[r];
+        if (r < n) len_of[r] = b.lens[r];
+    }
     __syncthreads();
-    const uint32_t total = row_sum[b.requests];
+    const uint32_t total = row_sum[n];
+    const uint32_t per = (n + kRowThreads - 1u) / kRowThreads;
+    const uint32_t begin = min(tid * per, n);
+    const uint32_t end = min(begin + per, n);
+    uint32_t sum = 0u;
+    for (uint32_t r = begin; r < end; ++r) {
+        const uint32_t after = len_of[r];
+        const uint32_t len = after - (row_sum[r + 1u] - row_sum[r]);
+        len_of[r] = len;
+        block_sum[r] = sum;
+        sum += ((after + mask) >> b.shift) - ((len + mask) >> b.shift);
+    }
+    const uint32_t incl = wave_incl(sum);
+    if ((tid & 63u) == 63u) wave_total[tid >> 6] = incl;
+    __syncthreads();
+    uint32_t before = incl - sum;
+    uint32_t fresh = 0u;
+    for (uint32_t w = 0; w < kRowThreads / 64u; ++w) {
+        if (w < tid >> 6) before += wave_total[w];
+        fresh += wave_total[w];
+    }
+    for (uint32_t r = begin; r < end; ++r) block_sum[r] += before;
+    __syncthreads();
+    const uint32_t c = taken - fresh;
 #pragma unroll
     for (uint32_t i = 0; i < kRowsEach; ++i) {
-        const uint32_t t = (blockIdx.x * kRowsEach + i) * kRowThreads + threadIdx.x;
+        const uint32_t t = (blockIdx.x * kRowsEach + i) * kRowThreads + tid;
         if (t >= b.max_rows) continue;
         uint32_t slot = HYP_SLOT_NONE;
         uint32_t pos = 0u;
         if (t < total) {
-            const uint32_t r = owner(row_sum, b.requests, t);
-            const uint32_t token = b.lens[r] - (row_sum[r + 1u] - t);
-            const uint32_t block = b.tables[static_cast<size_t>(r) * b.max_blocks + (token >> b.shift)];
+            const uint32_t r = owner(row_sum, n, t);
+            const uint32_t token = len_of[r] + (t - row_sum[r]);
+            const uint32_t entry = token >> b.shift;
+            const uint32_t have = (len_of[r] + mask) >> b.shift;
+            uint32_t* const at = b.tables + static_cast<size_t>(r) * b.max_blocks + entry;
+            const uint32_t block = entry < have ? *at : p.free_blocks[c + block_sum[r] + (entry - have)];
+            if ((token & mask) == 0u) *at = block;
             slot = slot_of(b, block, token);
             pos = b.prefix + token;
         }
@@ -238,7 +279,7 @@ void launch_batch_plan(const BatchView& b, const uint32_t* lens, const uint32_t*
     HYP_HIP_CHECK(hipGetLastError());
     if (here) return;
     const uint32_t per = kRowThreads * kRowsEach;
-    hipLaunchKernelGGL(batch_rows_kernel, dim3((b.max_rows + per - 1u) / per), dim3(kRowThreads), 0, stream, b);
+    hipLaunchKernelGGL(batch_rows_kernel, dim3((b.max_rows + per - 1u) / per), dim3(kRowThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
 }
 
