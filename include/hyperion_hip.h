@@ -156,7 +156,8 @@ HypStatus hyp_event_elapsed_ms(HypEvent start, HypEvent end, float* out_ms);
  * at mx::eval, forward.cc:171). Between begin and end, hyp_qmatmul, hyp_qmatmul_ex,
  * hyp_qmatmul_group, hyp_qmlp_gate_up_gelu and hyp_qmatmul_group_rmsnorm with m <= 4, hyp_rms_normalize, hyp_quantize_q4g64,
  * hyp_dequantize_q4g64, hyp_embed, hyp_sample_greedy, hyp_sample_greedy_topk, hyp_kv_cache_write,
- * hyp_attention, hyp_rope and the copies on `stream` are
+ * hyp_attention, hyp_rope, hyp_batch_plan, hyp_batch_prepare, hyp_batch_attention, hyp_sample_batch and
+ * the copies on `stream` are
  * recorded instead of run (they allocate nothing). Calls that may allocate or clear
  * memory - the matmul entries on their GEMM path (m > 4) and hyp_memset_device - check
  * the stream and return INVALID_ARGUMENT while it is capturing, before enqueueing
@@ -462,9 +463,10 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
  * sees the key positions p <= its own (with window > 0: p > its own - window) that are tokens of
  * the prefix or of the request. Grouped-query heads and layouts as hyp_attention: q, out
  * [max_rows][n_heads][head_dim], n_heads at most 1024, device bf16, 16-byte aligned; the scores are
- * scale * q.k (scale finite and positive). The rows' own K and V are read from the cache: call hyp_batch_prepare first. The
- * prefix's keys are read for all rows of the batch at once.
- * fp32 scores and softmax, probabilities in two bf16 terms, output rounded to bf16. A row that
+ * scale * q.k (scale finite and positive). The rows' own K and V are read from the cache: call
+ * hyp_batch_prepare first. The prefix's keys are read for all rows of the batch at once.
+ * fp32 scores and softmax, output rounded to bf16. Probabilities enter the products as one bf16 term
+ * where more than 16 rows of a kv head share keys, as two elsewhere. A row that
  * sees no key above -inf gives zeros; a NaN or +inf score that it sees gives NaN; keys that it does not see
  * change nothing, whatever they hold. Rows behind row_start[requests] are left as they are.
  * workspace: device memory of hyp_batch_attention_workspace's bytes, 16-byte aligned, whose
