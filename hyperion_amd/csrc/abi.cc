@@ -960,6 +960,13 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
         REQUIRE_ARG(std::isfinite(eps) && eps >= 0.0f, "eps must be finite and >= 0");
         REQUIRE_ARG(rotated_dims <= c.head_dim && rotated_dims % 2u == 0u, "rotated_dims must be even and <= head_dim");
         REQUIRE_ARG(std::isfinite(rope_base) && rope_base > 0.0f, "rope_base must be finite and positive");
+        const uint64_t row_bytes = static_cast<uint64_t>(b.max_rows) * c.head_dim * 2u;
+        const auto over_q_out = [&](const void* x, uint32_t heads) {
+            return x != nullptr && hyperion::hip::overlap(q_out, row_bytes * n_heads, x, row_bytes * heads);
+        };
+        REQUIRE_ARG(!over_q_out(k_raw, c.num_kv_heads) && !over_q_out(v_raw, c.num_kv_heads),
+                    "q_out must not overlap k_raw or v_raw");
+        REQUIRE_ARG(q_out == q || !over_q_out(q, n_heads), "q_out must be q or not overlap it");
         hyperion::hip::BatchPrepareArgs a{};
         a.q = static_cast<const uint16_t*>(q);
         a.k_raw = static_cast<const uint16_t*>(k_raw);
@@ -1030,6 +1037,10 @@ HypStatus hyp_sample_batch(const void* logits, uint32_t rows, uint32_t vocab, co
         REQUIRE_ARG(configs != nullptr && uniforms != nullptr && tokens != nullptr,
                     "configs, uniforms and tokens must be non-null device pointers");
         REQUIRE_ARG((reinterpret_cast<uintptr_t>(configs) & 7u) == 0u, "configs must be 8-byte aligned");
+        REQUIRE_ARG((reinterpret_cast<uintptr_t>(logits) & 1u) == 0u, "logits must be 2-byte aligned");
+        REQUIRE_ARG(((reinterpret_cast<uintptr_t>(uniforms) | reinterpret_cast<uintptr_t>(tokens) |
+                      reinterpret_cast<uintptr_t>(logprobs)) & 3u) == 0u,
+                    "uniforms, tokens and logprobs must be 4-byte aligned");
         const size_t need = hyperion::hip::sample_batch_workspace_bytes(rows, vocab);
         REQUIRE_ARG(workspace_bytes >= need && (need == 0 || workspace != nullptr), "batch sampling: workspace too small");
         REQUIRE_ARG(aligned16(workspace), "workspace must be 16-byte aligned");

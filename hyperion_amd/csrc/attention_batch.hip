@@ -1056,6 +1056,10 @@ void launch_batch_attention(const BatchView& b, const BatchAttentionArgs& a, hip
     const uint64_t keys = b.prefix + std::min<uint64_t>(static_cast<uint64_t>(b.max_blocks) << b.shift, 1u << 30);
     HYP_REQUIRE(keys < (1ull << 30) && tiles * a.n_kv_heads * (keys / kKeyBlock + 1u + kTileCost) < (1ull << 31),
                 HYP_STATUS_INVALID_ARGUMENT, "batch attention: too many rows for tables this long");
+    const uint64_t q_bytes = static_cast<uint64_t>(b.max_rows) * a.n_heads * a.head_dim * 2u;
+    HYP_REQUIRE(!overlap(a.out, q_bytes, a.q, q_bytes) && !overlap(a.workspace, l.bytes, a.q, q_bytes) &&
+                    !overlap(a.workspace, l.bytes, a.out, q_bytes),
+                HYP_STATUS_INVALID_ARGUMENT, "batch attention: q, out and workspace must not overlap");
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     BatchParams p{};
     p.b = b;

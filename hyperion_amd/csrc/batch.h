@@ -15,6 +15,12 @@ constexpr uint32_t kMaxRequests = 4096;            // their running sums fit one
 constexpr uint32_t kMaxBatchRows = 1u << 20;
 constexpr uint32_t kMaxPositions = 1u << 24;       // positions are exact in fp32 below
 
+// Whether two arrays of so many bytes share any.
+inline bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
 struct BatchView {
     uint32_t requests, shift, num_blocks, max_blocks, max_rows, prefix;   // block size 1 << shift
     const uint32_t* prefix_table;

@@ -446,7 +446,7 @@ HypStatus hyp_batch_plan(const HypBatch* batch, const uint32_t* lens, const uint
 /* hyp_attention_prepare for a batch's rows: row t of the step (t < row_start[requests]) at
  * positions[t], its K and V stored to slots[t] of the cache (HYP_SLOT_NONE or a slot outside the
  * cache: not stored),
- *   q_out[t][h]  <- rope(rms_norm(q[t][h], q_norm))            every head h (q_out may be q);
+ *   q_out[t][h]  <- rope(rms_norm(q[t][h], q_norm))            every head h (q_out may be q, not k_raw or v_raw);
  *   K[slot]      <- rope(rms_norm(k_raw[t][j], k_norm))        every kv head j;
  *   V[slot]      <- rms_norm(v_raw[t][j]) without a weight     (v_raw NULL reads k_raw).
  * q, q_out [max_rows][n_heads][head_dim], k_raw / v_raw [max_rows][num_kv_heads][head_dim],
@@ -464,7 +464,8 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
  * the prefix or of the request. Grouped-query heads and layouts as hyp_attention: q, out
  * [max_rows][n_heads][head_dim], n_heads at most 1024, device bf16, 16-byte aligned; the scores are
  * scale * q.k (scale finite and positive). The rows' own K and V are read from the cache: call
- * hyp_batch_prepare first. The prefix's keys are read for all rows of the batch at once.
+ * hyp_batch_prepare first. The prefix's keys are read for all rows of the batch at once. q, out and workspace
+ * do not overlap.
  * fp32 scores and softmax, output rounded to bf16. Probabilities enter the products as one bf16 term
  * where more than 16 rows of a kv head share keys, as two elsewhere. A row that
  * sees no key above -inf gives zeros; a NaN or +inf score that it sees gives NaN; keys that it does not see

@@ -208,3 +208,35 @@ def test_sample_reference_closed_forms():
     assert R.sample(x, 1.0, 0, 0.0, 0.3, 0.99)[0] == 3
     assert R.sample(np.array([-np.inf, np.nan]), 1.0, 0, 0.0, 0.0, 0.5) == (0, -np.inf)
     assert R.sample(np.array([3.0, np.inf, np.inf]), 1.0, 0, 0.0, 0.0, 0.7) == (2, pytest.approx(np.log(0.5)))
+
+
+AT = 0x10000000   # an address of its own
+Q_BYTES, KV_BYTES = 32 * 4 * 128 * 2, 32 * 2 * 128 * 2   # fields()' arrays
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(q=P, k=AT, v=2 * AT, out=AT), "k_raw or v_raw"),
+    (dict(q=P, k=AT, v=2 * AT, out=AT + KV_BYTES - 16), "k_raw or v_raw"),
+    (dict(q=P, k=AT, v=2 * AT, out=2 * AT - Q_BYTES + 16), "k_raw or v_raw"),
+    (dict(q=AT, k=2 * AT, v=None, out=AT + 16), "must be q or not overlap"),
+])
+def test_prepare_refuses_outputs_over_its_inputs(over, says):
+    refused("hyp_batch_prepare", *prepare_args(fields(), **over), says=says)
+
+
+@pytest.mark.parametrize("over", [
+    dict(q=AT, out=AT, work=2 * AT),
+    dict(q=AT, out=AT + Q_BYTES - 16, work=2 * AT),
+    dict(q=AT, out=2 * AT, work=AT + Q_BYTES - 16),
+    dict(q=AT, out=2 * AT, work=2 * AT - 16),
+])
+def test_attention_refuses_arrays_over_each_other(over):
+    refused("hyp_batch_attention", *attention_args(fields(), **over), says="must not overlap")
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(logits=AT + 1), "2-byte"), (dict(uniforms=AT + 2), "4-byte"), (dict(tokens=AT + 1), "4-byte"),
+    (dict(logprobs=AT + 2), "4-byte"),
+])
+def test_sample_refuses_odd_addresses(over, says):
+    refused("hyp_sample_batch", *sample_args(**over), says=says)
