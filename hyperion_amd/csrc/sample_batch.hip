@@ -25,6 +25,7 @@
 // counting). One row of 262144 takes 19.4 us, 64 rows 26.9, 200 rows of 50001 24.3.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -359,12 +360,12 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
             return bin <= kFine ? kLow + (kFine - bin) : (bin == kCentre ? bits_at(s.centre_lo) : 0x8000u | (kLow + (bin - kCentre - 1u)));
         };
         // The long way's windows that hold values, and its largest value.
-        bool slow = lead == kAbove || lead == kBelow || (s.count[kCentre] != 0u && s.centre_lo != s.centre_hi);
-        if (!slow && s.count[kBelow] != 0u)   // (2^23 times e^-80)
-            slow = !((value_of(fine_bits(lead)) + 128.0) * prm.by_t > 80.0);
+        bool windowed = lead == kAbove || lead == kBelow || (s.count[kCentre] != 0u && s.centre_lo != s.centre_hi);
+        if (!windowed && s.count[kBelow] != 0u)   // (2^23 times e^-80)
+            windowed = !((value_of(fine_bits(lead)) + 128.0) * prm.by_t > 80.0);
         double top = 0.0;
         uint32_t windows = 1u;
-        if (slow) {
+        if (windowed) {
             uint32_t best = 0xFFFFFFFFu;
             uint32_t held = 0u;
             for_tokens(row, 0u, vocab, tid, kThreads, [&](uint32_t, uint32_t b) {
@@ -381,155 +382,159 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         } else {
             top = value_of(fine_bits(lead));
         }
-        uint32_t window = 0u;   // the first place of the window in hand
-        const auto bits_of = [&](uint32_t bin) HYP_INLINE { return slow ? bits_at(window + bin) : fine_bits(bin); };
-        Before at{};
-        uint32_t here = 0u;     // this thread's tokens
-        const auto weigh = [&]() HYP_INLINE {
-            here = 0u;
-#pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) {
-                here += num[i];
-                weight[i] = 0.0;
-            }
-            double mass = 0.0;
-            if (here != 0u) {
+        const auto find = [&](auto by_windows) HYP_INLINE {
+            constexpr bool slow = decltype(by_windows)::value;
+            uint32_t window = 0u;   // the first place of the window in hand
+            const auto bits_of = [&](uint32_t bin) HYP_INLINE { return slow ? bits_at(window + bin) : fine_bits(bin); };
+            Before at{};
+            uint32_t here = 0u;     // this thread's tokens
+            const auto weigh = [&]() HYP_INLINE {
+                here = 0u;
 #pragma unroll
                 for (uint32_t i = 0; i < kPer; ++i) {
-                    const uint32_t bin = first + i;
-                    const double w = exp_below((value_of(bits_of(bin)) - top) * prm.by_t);
-                    if (num[i] != 0u && (slow || bin != kBelow)) weight[i] = w;
-                    mass += num[i] * weight[i];
+                    here += num[i];
+                    weight[i] = 0.0;
                 }
-            }
-            at = block_scan(mass, here, s.block);
-        };
-        if (!slow) weigh();
-        // f() with each window's counts and weights in hand, and what lies before this thread's bins.
-        const auto over_windows = [&](auto&& f) HYP_INLINE {
-            if (!slow) {
-                f(at.mass, at.count);
-                return;
-            }
-            double mass = 0.0;
-            uint32_t count = 0u;
-            for (uint32_t w = 0; w < kWindows; ++w) {
-                if (((windows >> w) & 1u) == 0u) continue;
-                __syncthreads();
-                for (uint32_t i = tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
-                __syncthreads();
-                window = w * kWindow;
-                for_tokens(row, 0u, vocab, tid, kThreads, [&](uint32_t, uint32_t b) {
-                    b = plain_bits(b);
-                    const uint32_t d = place_of(b) - window;
-                    if (finite_bits(b) && d < kWindow) atomicAdd(&s.count[d], 1u);
-                });
-                __syncthreads();
+                double mass = 0.0;
+                if (here != 0u) {
 #pragma unroll
-                for (uint32_t i = 0; i < kPer; ++i) num[i] = s.count[first + i];
-                weigh();
-                f(mass + at.mass, count + at.count);
-                mass += at.mass_all;
-                count += at.count_all;
-            }
-        };
-        // The mass up to and with this thread's bins.
-        const auto mass_with = [&](double mass) HYP_INLINE {
-#pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) mass += num[i] * weight[i];
-            return mass;
-        };
-        double total = 0.0;
-        uint32_t all = 0u;
-        if (slow) {
-            over_windows([&](double, uint32_t) HYP_INLINE {
-                total += at.mass_all;
-                all += at.count_all;
-            });
-        } else {
-            total = at.mass_all;
-            all = at.count_all;
-        }
-        uint32_t kept = all;
-        if (prm.top_k != 0u) kept = min(kept, prm.top_k);
-        if (prm.top_p != 0.0 || prm.min_p != 0.0) {
-            // A wave's first lane whose bins a filter does not keep whole goes through them.
-            const double enough = prm.top_p * total;
-            over_windows([&](double mass, uint32_t count) HYP_INLINE {
-                uint32_t keep = 0xFFFFFFFFu;
-                if (prm.top_p != 0.0) {
-                    const uint64_t past = __ballot(mass_with(mass) > enough);
-                    if (past != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(past))) {
-                        keep = count;
-                        double m = mass;
-#pragma unroll
-                        for (uint32_t i = 0; i < kPer; ++i) {
-                            const double room = enough - m;
-                            const double some = num[i] * weight[i];
-                            if (num[i] != 0u && room > 0.0)
-                                keep += room >= some ? num[i] : min(num[i], static_cast<uint32_t>(ceil(room / weight[i])));
-                            m += some;
-                        }
+                    for (uint32_t i = 0; i < kPer; ++i) {
+                        const uint32_t bin = first + i;
+                        const double w = exp_below((value_of(bits_of(bin)) - top) * prm.by_t);
+                        if (num[i] != 0u && (slow || bin != kBelow)) weight[i] = w;
+                        mass += num[i] * weight[i];
                     }
                 }
-                uint32_t light = 0u;   // before the first token that min-p drops
-                bool dropped = false;
+                at = block_scan(mass, here, s.block);
+            };
+            if (!slow) weigh();
+            // f() with each window's counts and weights in hand, and what lies before this thread's bins.
+            const auto over_windows = [&](auto&& f) HYP_INLINE {
+                if (!slow) {
+                    f(at.mass, at.count);
+                    return;
+                }
+                double mass = 0.0;
+                uint32_t count = 0u;
+                for (uint32_t w = 0; w < kWindows; ++w) {
+                    if (((windows >> w) & 1u) == 0u) continue;
+                    __syncthreads();
+                    for (uint32_t i = tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
+                    __syncthreads();
+                    window = w * kWindow;
+                    for_tokens(row, 0u, vocab, tid, kThreads, [&](uint32_t, uint32_t b) {
+                        b = plain_bits(b);
+                        const uint32_t d = place_of(b) - window;
+                        if (finite_bits(b) && d < kWindow) atomicAdd(&s.count[d], 1u);
+                    });
+                    __syncthreads();
+#pragma unroll
+                    for (uint32_t i = 0; i < kPer; ++i) num[i] = s.count[first + i];
+                    weigh();
+                    f(mass + at.mass, count + at.count);
+                    mass += at.mass_all;
+                    count += at.count_all;
+                }
+            };
+            // The mass up to and with this thread's bins.
+            const auto mass_with = [&](double mass) HYP_INLINE {
+#pragma unroll
+                for (uint32_t i = 0; i < kPer; ++i) mass += num[i] * weight[i];
+                return mass;
+            };
+            double total = 0.0;
+            uint32_t all = 0u;
+            if (slow) {
+                over_windows([&](double, uint32_t) HYP_INLINE {
+                    total += at.mass_all;
+                    all += at.count_all;
+                });
+            } else {
+                total = at.mass_all;
+                all = at.count_all;
+            }
+            uint32_t kept = all;
+            if (prm.top_k != 0u) kept = min(kept, prm.top_k);
+            if (prm.top_p != 0.0 || prm.min_p != 0.0) {
+                // A wave's first lane whose bins a filter does not keep whole goes through them.
+                const double enough = prm.top_p * total;
+                over_windows([&](double mass, uint32_t count) HYP_INLINE {
+                    uint32_t keep = 0xFFFFFFFFu;
+                    if (prm.top_p != 0.0) {
+                        const uint64_t past = __ballot(mass_with(mass) > enough);
+                        if (past != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(past))) {
+                            keep = count;
+                            double m = mass;
+#pragma unroll
+                            for (uint32_t i = 0; i < kPer; ++i) {
+                                const double room = enough - m;
+                                const double some = num[i] * weight[i];
+                                if (num[i] != 0u && room > 0.0)
+                                    keep += room >= some ? num[i] : min(num[i], static_cast<uint32_t>(ceil(room / weight[i])));
+                                m += some;
+                            }
+                        }
+                    }
+                    uint32_t light = 0u;   // before the first token that min-p drops
+                    bool dropped = false;
+#pragma unroll
+                    for (uint32_t i = 0; i < kPer; ++i) {
+                        dropped = dropped || (num[i] != 0u && weight[i] < prm.min_p);
+                        light += dropped ? 0u : num[i];
+                    }
+                    const uint64_t drops = __ballot(dropped);
+                    if (drops != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(drops))) keep = min(keep, count + light);
+                    if (keep != 0xFFFFFFFFu) atomicMin(&s.keep, keep);
+                });
+                __syncthreads();
+                kept = min(kept, s.keep);
+            }
+            kept = prm.greedy ? 1u : max(kept, 1u);
+            // The kept tokens' mass, the rank of the draw, its value.
+            over_windows([&](double mass, uint32_t count) HYP_INLINE {
+                if (kept - 1u - count >= here) return;
 #pragma unroll
                 for (uint32_t i = 0; i < kPer; ++i) {
-                    dropped = dropped || (num[i] != 0u && weight[i] < prm.min_p);
-                    light += dropped ? 0u : num[i];
+                    if (kept - 1u - count < num[i]) s.kept = mass + (kept - count) * weight[i];
+                    mass += num[i] * weight[i];
+                    count += num[i];
                 }
-                const uint64_t drops = __ballot(dropped);
-                if (drops != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(drops))) keep = min(keep, count + light);
-                if (keep != 0xFFFFFFFFu) atomicMin(&s.keep, keep);
             });
             __syncthreads();
-            kept = min(kept, s.keep);
-        }
-        kept = prm.greedy ? 1u : max(kept, 1u);
-        // The kept tokens' mass, the rank of the draw, its value.
-        over_windows([&](double mass, uint32_t count) HYP_INLINE {
-            if (kept - 1u - count >= here) return;
+            const double goal = prm.u * s.kept;
+            over_windows([&](double mass, uint32_t count) HYP_INLINE {
+                const uint64_t past = __ballot(mass_with(mass) > goal);
+                if (past == 0u || lane != static_cast<uint32_t>(__builtin_ctzll(past))) return;
+                uint32_t rank = 0xFFFFFFFFu;
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) {
-                if (kept - 1u - count < num[i]) s.kept = mass + (kept - count) * weight[i];
-                mass += num[i] * weight[i];
-                count += num[i];
-            }
-        });
-        __syncthreads();
-        const double goal = prm.u * s.kept;
-        over_windows([&](double mass, uint32_t count) HYP_INLINE {
-            const uint64_t past = __ballot(mass_with(mass) > goal);
-            if (past == 0u || lane != static_cast<uint32_t>(__builtin_ctzll(past))) return;
-            uint32_t rank = 0xFFFFFFFFu;
-#pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) {
-                if (rank == 0xFFFFFFFFu && num[i] != 0u && mass + num[i] * weight[i] > goal) {
-                    const double j = (goal - mass) / weight[i];
-                    rank = count + (j > 0.0 ? min(static_cast<uint32_t>(fmin(j, 4.0e9)), num[i] - 1u) : 0u);
+                for (uint32_t i = 0; i < kPer; ++i) {
+                    if (rank == 0xFFFFFFFFu && num[i] != 0u && mass + num[i] * weight[i] > goal) {
+                        const double j = (goal - mass) / weight[i];
+                        rank = count + (j > 0.0 ? min(static_cast<uint32_t>(fmin(j, 4.0e9)), num[i] - 1u) : 0u);
+                    }
+                    mass += num[i] * weight[i];
+                    count += num[i];
                 }
-                mass += num[i] * weight[i];
-                count += num[i];
-            }
-            atomicMin(&s.rank, rank);
-        });
-        __syncthreads();
-        const uint32_t rank = min(s.rank, kept - 1u);
-        over_windows([&](double, uint32_t count) HYP_INLINE {
-            if (rank - count >= here) return;
+                atomicMin(&s.rank, rank);
+            });
+            __syncthreads();
+            const uint32_t rank = min(s.rank, kept - 1u);
+            over_windows([&](double, uint32_t count) HYP_INLINE {
+                if (rank - count >= here) return;
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) {
-                if (rank - count < num[i]) {
-                    s.drawn = bits_of(first + i);
-                    s.number = rank - count;
-                    if (!slow) s.bin = first + i;
+                for (uint32_t i = 0; i < kPer; ++i) {
+                    if (rank - count < num[i]) {
+                        s.drawn = bits_of(first + i);
+                        s.number = rank - count;
+                        if (!slow) s.bin = first + i;
+                    }
+                    count += num[i];
                 }
-                count += num[i];
-            }
-        });
-        __syncthreads();
-        logprob = (value_of(s.drawn) - top) * prm.by_t - log(total);
+            });
+            __syncthreads();
+            logprob = (value_of(s.drawn) - top) * prm.by_t - log(total);
+        };
+        if (windowed) find(std::true_type{}); else find(std::false_type{});
     }
 
     // 3. The token, in the row or in the chunk that holds it: each wave marks the value's places in its stretch, 512
