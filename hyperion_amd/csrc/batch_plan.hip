@@ -10,8 +10,9 @@
 // What bounds it: the latency of its steps (lengths, sums, table entries, slots), a few KB of
 // traffic. One workgroup keeps the sums in LDS and every thread finds its block's or row's
 // request there by bisection. With more than kRowsHere rows the blocks and rows go to a second launch over
-// all compute units: 509 prompts (352000 rows, 12000 blocks) take 15.0 us, of which the launch of the sums is about 6.
-// 64 requests' decode step takes 7.9 us, 6400 rows of 64 requests 11.0 in one launch and 12.6 in two.
+// all compute units: 509 prompts (352000 rows, 12000 blocks) take 14.3 us, of which the launch of the sums is about 6.
+// 64 requests' decode step takes 7.1 us (7.9 with the waves' sums by LDS permutes), 6400 rows of 64 requests 10.3 in one
+// launch; in two they took 1.6 us more.
 #include "batch.h"
 #include "common.h"
 #include "wave.h"
@@ -45,15 +46,6 @@ __device__ __forceinline__ uint32_t owner(const uint32_t* sums, uint32_t n, uint
         if (sums[mid] <= at) lo = mid; else hi = mid;
     }
     return lo;
-}
-
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v, uint32_t lane) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const uint64_t y = __shfl_up(v, d, 64);
-        if (lane >= d) v += y;
-    }
-    return v;
 }
 
 __device__ __forceinline__ uint32_t slot_of(const BatchView& b, uint32_t block, uint32_t token) {
@@ -98,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void batch_plan_kernel(PlanParams p) {
     uint64_t before[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        const uint64_t incl = wave_scan(sum[k], lane);
+        const uint64_t incl = wave_incl64(sum[k]);
         before[k] = incl - sum[k];
         if (lane == 63u) wave_total[k][wave] = incl;
     }

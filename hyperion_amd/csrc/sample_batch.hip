@@ -126,7 +126,7 @@ struct Before {
 __device__ __forceinline__ Before block_scan(double mass, uint32_t count, Block& s) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = threadIdx.x >> 6;
-    const double m = wave_incl(mass);
+    const double m = wave_incl64(mass);
     const uint32_t c = wave_incl(count);
     if (lane == 63u) {
         s.d[wave] = m;

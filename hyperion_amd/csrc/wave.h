@@ -36,13 +36,15 @@ __device__ __forceinline__ int32_t wave_min(int32_t v) {
         return static_cast<uint32_t>(min(static_cast<int32_t>(a), static_cast<int32_t>(b)));
     }), 63u));
 }
-// Inclusive sums of doubles, in the same steps.
-__device__ __forceinline__ double wave_incl(double v) {
-    const auto step = [](double v, auto moved) __attribute__((always_inline)) {
+// Inclusive sums of 64-bit values, in the same steps.
+template <typename T>
+__device__ __forceinline__ T wave_incl64(T v) {
+    static_assert(sizeof(T) == 8u, "two registers");
+    const auto step = [](T v, auto moved) __attribute__((always_inline)) {
         const uint64_t b = __builtin_bit_cast(uint64_t, v);
         const uint64_t lo = static_cast<uint32_t>(moved(static_cast<int>(static_cast<uint32_t>(b))));
         const uint64_t hi = static_cast<uint32_t>(moved(static_cast<int>(static_cast<uint32_t>(b >> 32))));
-        return v + __builtin_bit_cast(double, lo | hi << 32);
+        return v + __builtin_bit_cast(T, lo | hi << 32);
     };
     v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false); });
     v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false); });
