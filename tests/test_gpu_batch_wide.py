@@ -1,5 +1,5 @@
 """hyp_batch_attention where many rows share keys, at the borders of its tiles, from several streams and far into a large
-cache; hyp_batch_plan's large steps. Bars as test_gpu_batch.py's."""
+cache; hyp_batch_plan's large steps; hyp_sample_batch over long rows and many. Bars as test_gpu_batch.py's."""
 import ctypes
 
 import numpy as np
@@ -8,7 +8,7 @@ import pytest
 import batch_ref as R
 import hyperion_amd as hy
 from hyperion_amd import synthetic as syn
-from test_gpu_batch import Plan, Scene, check_plan, dev, f64, plan_case, say, u32
+from test_gpu_batch import Plan, Scene, check_draw, check_plan, dev, draw, f64, mixed, plan_case, say, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,30 @@ def test_plan_of_many_rows(stream, n, block, hi, new_hi, done, spare, short_rows
     if not in_place:
         p.run()
         check_plan(p.results(), R.plan(*case))
+
+
+@pytest.mark.parametrize("vocab", [2**22 + 5, 2**23])
+def test_sample_rows_of_many_chunks(stream, vocab):
+    """More chunks than a wave has lanes; the drawn value stands in many of them."""
+    rng = np.random.default_rng(vocab)
+    bits = syn.bf16_bits((0.5 * np.round(2.0 * rng.standard_normal((2, vocab)))).astype(np.float32))
+    bits[1, ::5] = 0xFF80
+    configs = mixed(rng, 2, vocab)
+    configs["temperature"], configs["top_k"] = (1.0, 3.0), (0, 5000)
+    for uniforms in ([0.37, 0.9], [0.99999, 1e-6]):
+        check_draw(stream, bits, configs, np.array(uniforms, np.float32), f"vocab {vocab}")
+
+
+def test_sample_rows_alone_and_among_more_than_the_device_holds(stream):
+    """From 512 rows on a row is one workgroup's: the same tokens and bits of logprobs as a row alone."""
+    rng = np.random.default_rng(3)
+    rows, vocab = 530, 20001
+    bits = syn.bf16_bits((3.0 * rng.standard_normal((rows, vocab))).astype(np.float32))
+    bits[7, 100:400] = syn.bf16_bits(np.full(300, 200.0, np.float32))     # above the fine values
+    bits[8, ::2] = syn.bf16_bits(np.full(10001, -300.0, np.float32))      # and below
+    bits[9] = syn.bf16_bits((1e-9 * rng.standard_normal(vocab)).astype(np.float32))
+    configs, uniforms = mixed(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    tokens, logprobs = draw(stream, bits, configs, uniforms)
+    for r in (0, 7, 8, 9, 300, 529):
+        one, value = draw(stream, bits[r:r + 1], configs[r:r + 1], uniforms[r:r + 1])
+        assert one[0] == tokens[r] and value.view(np.uint32)[0] == logprobs.view(np.uint32)[r], r
