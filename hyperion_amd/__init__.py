@@ -801,7 +801,6 @@ class Batch:
         call("hyp_batch_prepare", self._ref, q.ptr, k_raw.ptr, None if v_raw is None else v_raw.ptr, n_heads,
              cache.handle, q_norm.ptr, k_norm.ptr, eps, rotated, base, q_out.ptr, stream.handle)
 
-
     def attention_workspace_bytes(self, n_heads: int, cache: KvCache) -> int:
         """Bytes of a workspace for attention() with this batch's sizes."""
         out = _SZ()

@@ -11,8 +11,9 @@
 // rounding.
 //
 // Steps, with one workgroup for 2 and 3 and, unless there are rows enough, several for 1:
-//  1. counts by value in LDS, each workgroup's for its chunk of the row; a second launch adds a row's chunks. A bin for each bf16 value of magnitude 2^-25 .. 2^7 (8192), one for
-//     what is nearer to 0, one for what is above and one for what is below;
+//  1. counts by value in LDS, each workgroup's for its chunk of the row; a second launch adds a row's chunks.
+//     A bin for each bf16 value of magnitude 2^-25 .. 2^7 (8192), one for what is nearer to 0, one for what
+//     is above and one for what is below;
 //  2. every thread takes 9 neighbouring bins, their weights, and scans of count and mass over the
 //     workgroup; then the kept count, the kept mass, the drawn rank, its bin and its number j there;
 //  3. the j-th token of that value: the chunk that holds it by the chunks' counts, then by counting along it.
@@ -422,7 +423,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         } else {
             top = value_of(fine_bits(lead));
         }
-        // (Written out for either way: one copy with a test at each step took 19.8 us for 19.3, one loop over steps 22.9.)
+        // (Written out for either way. For one row of 262144: 19.3 us so, 19.8 with one copy and a test at each step, 22.9
+        // with one loop over the steps.)
         const auto find = [&](auto by_windows) HYP_INLINE {
             constexpr bool slow = decltype(by_windows)::value;
             uint32_t window = 0u;   // the first place of the window in hand
