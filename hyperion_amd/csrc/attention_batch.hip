@@ -24,9 +24,10 @@
 // 777 tokens (8 of 128) 133 us, 4.5 TB/s; a copy reaches 5.0.
 //
 // Wide: four waves with 32 rows each on 32x32x16 products over K and V blocks that all of them read from LDS, and one
-// bf16 term of P (2^-8 of a weight at most; a second term would add half to the products, which bound it). 24 prompts of 9 to 250 rows behind 6000 tokens (16 heads on one of 512) take
-// 587 us with their merge, 770 TFLOP/s of 1270 that a large matrix product reaches; 50 decode rows behind
-// 16001 84 us, 331 TFLOP/s: there every workgroup has 8 blocks of one tile and writes a piece of 256 KB for them.
+// bf16 term of P (2^-8 of a weight at most; a second term would add half to the products, which bound it). 24
+// prompts of 9 to 250 rows behind 6000 tokens (16 heads on one of 512) take 587 us with their merge, 770 TFLOP/s of
+// 1270 that a large matrix product reaches; 50 decode rows behind 16001 84 us, 331 TFLOP/s: there a workgroup has some
+// 16 blocks of one tile (31 us), waits 11 us for the first and writes a piece of 256 KB for them (10 us).
 #include <algorithm>
 
 #include "attention.h"
