@@ -195,9 +195,12 @@ struct Walk {
         const uint32_t pre = apart ? p.b.prefix : 0u;
         return WideSpan(p.G, pre + s.hi, static_cast<int32_t>(pre) + s.pos, p.window);
     }
-    // Units of a request's wide tiles of one kv head.
+    // Units of a request's wide tiles of one kv head. A tile has a block at least: a request without keys has no
+    // tiles (the merge finds no pieces of its rows there).
     __device__ uint32_t wide_head(const BatchParams& p, const Source& s) const {
-        return kWide && s.rows != 0u && wide(p, s.rows) ? span(p, s).before(wide_tiles_of(s.rows, p.G)) : 0u;
+        if (!kWide || s.rows == 0u || !wide(p, s.rows)) return 0u;
+        const WideSpan keys = span(p, s);
+        return keys.all != 0u ? keys.before(wide_tiles_of(s.rows, p.G)) : 0u;
     }
     __device__ bool has_prefix() const { return prefix.blocks != 0u || wide_blocks != 0u; }
     // Units of the prefix's wide tiles of one kv head.
