@@ -380,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         uint32_t kept = infinite;
         if (prm.top_k != 0u) kept = min(kept, prm.top_k);
         if (prm.top_p != 0.0) kept = min(kept, static_cast<uint32_t>(ceil(prm.top_p * infinite)));
-        if (prm.greedy) kept = 1u;
+        if (prm.greedy || prm.min_p > 1.0) kept = 1u;
         if (tid == 0u) {
             s.drawn = 0x7F80u;
             s.number = static_cast<uint32_t>(fmin(prm.u * kept, static_cast<double>(kept - 1u)));

@@ -640,20 +640,23 @@ HypStatus hyp_decode_block_sampled(HypModel model, HypKvState kvstate, uint32_t 
 HypStatus hyp_sample_stochastic(const void* logits, uint32_t vocab, const HypSamplingConfig* config,
                                 uint64_t rng_state, HypTopKSample* out, HypStream stream);
 /* One token for each of `rows` rows of vocab bf16 logits (device, row-major), from a uniform and a
- * configuration of its own: configs [rows] (device; temperature, top_k, top_p, min_p as in
- * hyp_sample_stochastic, seed is not used), uniforms float [rows] (device) in [0, 1). tokens uint32
- * [rows] (device, as hyp_embed takes them), logprobs float [rows] (device) or NULL.
+ * configuration of its own: configs [rows] (device; temperature, top_k, top_p and min_p, seed is not
+ * used), uniforms float [rows] (device) in [0, 1). tokens uint32 [rows] (device, as hyp_embed takes
+ * them), logprobs float [rows] (device) or NULL. The host does not see the configurations: what
+ * hyp_sample_stochastic refuses in one (min_p of 1 and more, say) is not refused here but means what follows.
  * The order of a row is logit descending (-0 as +0), then index ascending, and
  * w = exp((logit - largest) / temperature) in fp64. Kept is the shortest of these prefixes of the
  * order: top_k tokens (<= 0 or above vocab: all); with top_p in (0, 1) the tokens before which the
- * running sum of w is below top_p times the total; with min_p > 0 those with w >= min_p; at least
- * one token. tokens[r] is the first token of the order whose running sum exceeds uniform times the
- * kept sum (a uniform below 0 or NaN draws as 0, one of 1 or more as the largest float below 1). A
- * temperature of 0, below 0 or NaN takes the first of the order. logprobs[r] = ln of the token's share of
- * the total of w before the filters, at temperature 1 where the row is greedy.
+ * running sum of w is below top_p times the total; with min_p > 0 those with w >= min_p (none
+ * where it is above 1: the first one's w is 1); at least one token. tokens[r] is the first token of
+ * the order whose running sum exceeds uniform times the kept sum (a uniform below 0 or NaN draws as
+ * 0, one of 1 or more as the largest float below 1). A temperature of 0, below 0 or NaN takes the
+ * first of the order. logprobs[r] = ln of the token's share of the total of w before the filters, at
+ * temperature 1 where the row is greedy.
  * NaN and -inf logits are never drawn; beside +inf logits finite ones weigh nothing; a row
  * with no logit above -inf gives token 0 and logprob -inf. hyp_sample_stochastic draws along the
- * index instead, so the two draw different tokens from one uniform, with the same probabilities.
+ * index instead, so the two draw different tokens from one uniform, with the same probabilities where
+ * no logit is NaN or +inf.
  * vocab is at most 2^23. The results do not depend on rows or on the order of execution.
  * workspace: device memory of hyp_sample_batch_workspace's bytes, 16-byte aligned (NULL where that
  * is 0), whose contents need not be kept between calls; calls that overlap need one each, and so do

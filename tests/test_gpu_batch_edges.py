@@ -1,7 +1,9 @@
 """Batched serving at the ends of what its calls define. Bars as test_gpu_batch.py's."""
+import numpy as np
 import pytest
 
-from test_gpu_batch import Scene, say
+from hyperion_amd import synthetic as syn
+from test_gpu_batch import CONFIG, Scene, check_draw, say
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +40,21 @@ def test_many_rows_behind_tables_without_entries(stream):
     s.lens[:] = 0
     s.run()
     s.check("no entries")
+
+
+@pytest.mark.parametrize("min_p", [1.0, 1.5, 2.0, 2.0**20, np.inf])
+@pytest.mark.parametrize("vocab", [5, 999, 70000])
+def test_sample_min_p_of_one_and_more(stream, vocab, min_p):
+    """A weight is at most 1: min_p above 1 leaves one token, min_p 1 the largest logit's; +inf logits weigh 1."""
+    rng = np.random.default_rng(vocab)
+    rows = 12
+    x = np.round(2.0 * rng.standard_normal((rows, vocab)))
+    x[:, 1::2] = np.max(x, axis=1, keepdims=True)        # many of the largest
+    x[::2, 3:] = np.where(rng.random((rows // 2, vocab - 3)) < 0.3, np.inf, x[::2, 3:])
+    x[::2, 4] = np.inf
+    x[::2, 3] = np.inf                                   # two at least
+    configs = np.zeros(rows, CONFIG)
+    configs["temperature"], configs["min_p"] = 0.8, min_p
+    configs["top_k"][4:8], configs["top_p"][6:10] = 2, 0.9
+    uniforms = np.resize(np.array([0.999, 0.5, 0.75], np.float32), rows)
+    check_draw(stream, syn.bf16_bits(x.astype(np.float32)), configs, uniforms, f"min_p {min_p}")
