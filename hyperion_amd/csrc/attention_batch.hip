@@ -94,7 +94,8 @@ __device__ __forceinline__ void row_alone(const BatchParams& p, uint32_t hk, con
         }
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) s += __shfl_xor(s, d);
-        if (seen) {
+        // (A score of -inf weighs nothing whatever the value is: 0 times one that is not finite would be NaN.)
+        if (seen && s * p.scale != -__builtin_huge_valf()) {
             const float w = __builtin_amdgcn_exp2f(fmaf(s, p.scale, -ref));
 #pragma unroll
             for (uint32_t c = 0; c < kC; ++c)

@@ -469,7 +469,7 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
  * fp32 scores and softmax, output rounded to bf16. Probabilities enter the products as one bf16 term
  * where more than 16 rows of a kv head share keys, as two elsewhere. A row that
  * sees no key above -inf gives zeros; a NaN or +inf score that it sees gives NaN; keys that it does not see
- * change nothing, whatever they hold. Rows behind row_start[requests] are left as they are.
+ * and those whose score is -inf change nothing, whatever they hold. Rows behind row_start[requests] are left as they are.
  * workspace: device memory of hyp_batch_attention_workspace's bytes, 16-byte aligned, whose
  * contents need not be kept between calls; calls that overlap need one each, and so do graphs
  * whose replays overlap. Row starts must not decrease. */

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from hyperion_amd import synthetic as syn
-from test_gpu_batch import CONFIG, Scene, check_draw, say
+from test_gpu_batch import CONFIG, Scene, check_draw, f64, say
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,38 @@ def test_sample_min_p_of_one_and_more(stream, vocab, min_p):
     configs["top_k"][4:8], configs["top_p"][6:10] = 2, 0.9
     uniforms = np.resize(np.array([0.999, 0.5, 0.75], np.float32), rows)
     check_draw(stream, syn.bf16_bits(x.astype(np.float32)), configs, uniforms, f"min_p {min_p}")
+
+
+UNWEIGHED = [
+    # rows of each request, H, KVH, D, prefix
+    (1, 2, 2, 64, 0),        # few rows, straight to the output
+    (3, 8, 2, 256, 0),
+    (1, 16, 1, 512, 20),     # and joined
+    (40, 4, 2, 128, 0),      # wide tiles, straight to the output
+    (40, 4, 2, 256, 0),
+    (20, 16, 1, 512, 20),
+]
+
+
+@pytest.mark.parametrize("rows,H,KVH,D,prefix", UNWEIGHED)
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_keys_with_a_score_of_minus_infinity_weigh_nothing(stream, rows, H, KVH, D, prefix, bad):
+    """Whatever their values are: a row whose every score is -inf gives zeros, one with others is their mean."""
+    say(f"scores of -inf: rows={rows} H={H} KVH={KVH} D={D} prefix={prefix} V={bad}")
+    s = Scene(D + rows, stream, [50, 90, 60], [rows] * 3, H, KVH, D, 16, prefix, 0)
+    low, worst = (syn.bf16_bits(np.array([v], np.float32))[0] for v in (-np.inf, bad))
+    one = syn.bf16_bits(np.ones(1, np.float32))[0]
+    s.q[:, :, 0] = one
+    at = np.arange(50)
+    own = s.tables[0, at // 16].astype(np.int64) * 16 + at % 16
+    s.ck[own, :, 0], s.cv[own] = low, worst                       # request 0: every own key
+    at = np.arange(3, 40)
+    own = s.tables[1, at // 16].astype(np.int64) * 16 + at % 16
+    s.ck[own, :, 0], s.cv[own, :, ::3] = low, worst               # request 1: some
+    if prefix:
+        at = s.prefix_table[np.arange(prefix) // 16].astype(np.int64) * 16 + np.arange(prefix) % 16
+        s.ck[at, :, 0], s.cv[at, :, 1] = low, worst               # the prefix
+    s.place()
+    s.run()
+    out = s.check("scores of -inf")
+    assert np.all(f64(out[:rows]) == 0.0)
