@@ -23,11 +23,12 @@
 // 1 to 1500 tokens without a prefix (8 kv heads of 256, window 1024) take 77 us, 4.7 TB/s; 96 rows of up to 3000 behind
 // 777 tokens (8 of 128) 133 us, 4.5 TB/s; a copy reaches 5.0.
 //
-// Wide: four waves with 32 rows each on 32x32x16 products over K and V blocks that all of them read from LDS, and one
-// bf16 term of P (2^-8 of a weight at most; a second term would add half to the products, which bound it). 24
-// prompts of 9 to 250 rows behind 6000 tokens (16 heads on one of 512) take 587 us with their merge, 770 TFLOP/s of
-// 1270 that a large matrix product reaches; 50 decode rows behind 16001 84 us, 331 TFLOP/s: there a workgroup has some
-// 16 blocks of one tile (31 us), waits 11 us for the first and writes a piece of 256 KB for them (10 us).
+// Wide: four waves with 32 rows each on 32x32x16 products over K and V blocks that all of them read from LDS, with the
+// same two terms of P: one alone halves what is spent on its product but leaves the output 2.4e-3 from the
+// 64-bit result in norm where its own rounding leaves 1.7e-3 (as two terms do), and a row would have fewer bits
+// where more than 16 share its keys. 24 prompts of 9 to 250 rows behind 6000 tokens (16 heads on one of 512) take
+// 720 us with their merge, 627 TFLOP/s of scores and values (940 with the second term) of 1270 that a large matrix
+// product reaches, with one term 590; 50 decode rows behind 16001 90 us, with one term 81.
 #include <algorithm>
 
 #include "attention.h"
@@ -41,7 +42,6 @@ namespace hyperion::hip {
 namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kMergeThreads = 256;
 constexpr uint32_t kMergeRows = 64;        // (row, head) pairs of a workgroup, at most
@@ -333,11 +333,8 @@ __device__ __forceinline__ void rows_segment(const BatchParams& p, const Source&
 // of one kv head, 32 a wave on 32x32x16 products, S^T = K Q^T and O^T = V^T P^T, K and V rows by loads
 // straight to two LDS stages - over paged keys. A lane looks up the slot of key lane % 32 of the block
 // after the next one, so its table entry has arrived a block before the rows are requested.
-// Probabilities enter as one bf16 term here, where the matrix products are what is waited for, and the
-// row's sum takes them as rounded: the output is then a weighted mean with slightly other weights, and a
-// row that one key dominates is exact however old its maximum is. (Two terms cost half as many
-// products again for an error of 1.7e-3 of the output's norm instead of 2.4e-3, most of both the
-// output's own rounding.)
+// Probabilities enter as two bf16 terms (2^-16 of a weight), as attention_chunk.hip's do where O is rescaled
+// lazily: a row's largest one need not be an exact 1.
 template <uint32_t D>
 struct TilesLds {
     static constexpr uint32_t kV = BlockLds<D>::kBytes;
@@ -594,17 +591,21 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
             float pr[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale, -ref));
-            // The sum takes them as rounded, two at a time.
-            uint32_t two[8];
+            // Two bf16 terms of each; the row's sum takes both, as the products do.
+            bf16x8_t pb[2], pl[2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                two[i] = cvt_pk_bf16(pr[2 * i], pr[2 * i + 1]);
-                l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two[i]), bf16x2_t{1.0f, 1.0f}, l, false);
+            for (int t = 0; t < 2; ++t) {
+                uint32_t two[4], rest[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = pr[8 * t + 2 * i], b = pr[8 * t + 2 * i + 1];
+                    two[i] = cvt_pk_bf16(a, b);
+                    rest[i] = cvt_pk_bf16(a - bf16_bits_to_f32(two[i] & 0xFFFFu), b - __uint_as_float(two[i] & 0xFFFF0000u));
+                    l += a + b;
+                }
+                pb[t] = __builtin_bit_cast(bf16x8_t, make_uint4(two[0], two[1], two[2], two[3]));
+                pl[t] = __builtin_bit_cast(bf16x8_t, make_uint4(rest[0], rest[1], rest[2], rest[3]));
             }
-            bf16x8_t pb[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                pb[t] = __builtin_bit_cast(bf16x8_t, make_uint4(two[4 * t], two[4 * t + 1], two[4 * t + 2], two[4 * t + 3]));
             if constexpr (D == 256u) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -614,6 +615,7 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
             for (uint32_t u = 0; u < kProducts; ++u) {
                 __builtin_amdgcn_sched_barrier(0);
                 o[u / 2u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u % kAhead], pb[u % 2u], o[u / 2u], 0, 0, 0);
+                o[u / 2u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u % kAhead], pl[u % 2u], o[u / 2u], 0, 0, 0);
                 if (u + kAhead < kProducts) vf[u % kAhead] = v_read(v_at, v_odd, u + kAhead);
             }
         }
@@ -1015,10 +1017,12 @@ void launch_walk(BatchParams p, hipStream_t stream) {
         }
     }
     p.groups = groups_of(D, kWide);
-    // Of two kinds of tile each gets a share of the workgroups. Measured with 1 to 12: 50 rows behind 16001 tokens at
-    // head_dim 512 took 83 us with 1.5, 95 with 2.5 and 112 with 4; 64 behind 2000 at 256 took 100 with 5.5, 106 with 4
-    // and 102 with 10; at 128 what was tried made a hundredth's difference.
-    p.wide_cost = D >= 512u ? 1.5f : (D == 256u ? 5.5f : 4.0f);
+    // Of two kinds of tile each gets a share of the workgroups. Measured with half of these up to three times as much
+    // (us, here first): head_dim 512, 50 rows behind 16001 tokens 92, 97 with 1, 100 with 3; 90 rows of up to 1500
+    // behind 700 57, 71 with 1, 53 with 3. 256 (window 1024), 64 rows of up to 1500 behind 2000 97, 105 with 4, 98 with
+    // 8. 128, 50 of up to 600 behind 16001 61, 56 with 3, 78 with 8; 96 of up to 3000 behind 777 132, 134, 134. 64, 48
+    // of up to 600 behind 12000 34, 34 with 2, 41 with 4; 64 of up to 1500 behind 2000 37, 40, 38.
+    p.wide_cost = D >= 512u ? 2.0f : (D == 256u ? 5.5f : (D == 128u ? 4.0f : 3.0f));
     const uint32_t scribes = (p.b.requests + 64u * kGroupWaves - 1u) / (64u * kGroupWaves);
     hipLaunchKernelGGL((attn_batch_kernel<D, kWide>), dim3(p.groups + scribes), dim3(kGroupThreads), lds, stream, p);
     HYP_HIP_CHECK(hipGetLastError());

@@ -466,10 +466,11 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
  * scale * q.k (scale finite and positive). The rows' own K and V are read from the cache: call
  * hyp_batch_prepare first. The prefix's keys are read for all rows of the batch at once. q, out and workspace
  * do not overlap.
- * fp32 scores and softmax, output rounded to bf16. Probabilities enter the products as one bf16 term
- * where more than 16 rows of a kv head share keys, as two elsewhere. A row that
- * sees no key above -inf gives zeros; a NaN or +inf score that it sees gives NaN; keys that it does not see
- * and those whose score is -inf change nothing, whatever they hold. Rows behind row_start[requests] are left as they are.
+ * fp32 scores and softmax, output rounded to bf16. Probabilities enter the products as two bf16 terms
+ * (2^-16 of a weight). The order in which a row's keys are summed, and so its last bits, depends on the
+ * step it is in; the same step gives the same bits. A row that sees no key above -inf gives zeros; a
+ * NaN or +inf score that it sees gives NaN; keys that it does not see and those whose score is -inf
+ * change nothing, whatever they hold. Rows behind row_start[requests] are left as they are.
  * workspace: device memory of hyp_batch_attention_workspace's bytes, 16-byte aligned, whose
  * contents need not be kept between calls; calls that overlap need one each, and so do graphs
  * whose replays overlap. Row starts must not decrease. */

@@ -93,3 +93,23 @@ def test_keys_with_a_score_of_minus_infinity_weigh_nothing(stream, rows, H, KVH,
     s.run()
     out = s.check("scores of -inf")
     assert np.all(f64(out[:rows]) == 0.0)
+
+
+@pytest.mark.parametrize("lens,rows,H,KVH,D,block,prefix,window,scale,spread", [
+    ([300], [1], 64, 1, 64, 16, 0, 0, None, 2.0),                          # one row of 64 heads
+    ([70, 300, 9], [60, 130, 9], 16, 8, 64, 16, 250, 0, None, 2.0),
+    ([70, 300, 9], [60, 130, 9], 16, 4, 128, 16, 250, 0, None, 2.0),
+    ([70, 300, 9], [60, 130, 9], 4, 2, 256, 16, 250, 100, 1.0, 2.0),
+    ([64, 300, 9], [60, 130, 9], 4, 2, 256, 16, 250, 0, 1.0, 8.0),         # scores far apart: maxima grow late
+    ([64, 300, 9], [60, 130, 9], 16, 1, 512, 16, 250, 0, 1.0, 8.0),
+    ([20] * 40, [1] * 40, 16, 1, 512, 16, 1500, 0, 1.0, 2.0),
+    ([20, 700], [20, 300], 16, 1, 512, 16, 70, 0, None, 0.5),              # many keys of like weight
+])
+def test_many_rows_weigh_in_two_terms(stream, lens, rows, H, KVH, D, block, prefix, window, scale, spread):
+    """Wide tiles round a probability by no more than tiles of few rows do (2^-16 of itself): the bound of
+    Scene.compare without its term for one rounding to bf16."""
+    say(f"two terms: {len(lens)} requests H={H} KVH={KVH} D={D} prefix={prefix} spread={spread}")
+    s = Scene(sum(lens) + D, stream, lens, rows, H, KVH, D, block, prefix, window, scale, spread=spread).place()
+    s.one_term = lambda: False
+    s.run()
+    s.check("two terms")
