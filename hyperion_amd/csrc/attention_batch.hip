@@ -43,6 +43,8 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+#define HYP_INLINE __attribute__((always_inline))
+
 constexpr uint32_t kMergeThreads = 256;
 constexpr uint32_t kMergeRows = 64;        // (row, head) pairs of a workgroup, at most
 constexpr uint32_t kMergeGroups = 2048;    // workgroups before one takes several
@@ -111,9 +113,6 @@ __device__ __forceinline__ void row_alone(const BatchParams& p, uint32_t hk, con
             o[c][e] += __shfl_xor(o[c][e], 32);
         }
 }
-
-// Where a segment's rows go: to the output (all their keys were in it), by output row, or to a piece.
-enum : uint32_t { kToOutput = 0u, kToRows = 1u, kToPiece = 2u };
 
 // Blocks [b0, b1) of tile `tile` of kv head hk of source s.
 template <uint32_t D>
@@ -351,15 +350,6 @@ constexpr float kRescaleLog2 = 8.0f;
 struct TileShared {
     int32_t range[kGroupWaves][2];   // the waves' first and last keys
     int32_t pos[kChunkRows];         // positions of a prefix tile's tokens
-};
-
-// The keys that a tile walks, positions 0 .. keys - 1: `pre` of the prefix's tokens, then own ones.
-struct Sequence {
-    const uint32_t* own;   // the request's row of tables
-    uint32_t pre, keys;
-    uint32_t row0, rows;   // query rows (tokens)
-    int32_t pos;           // the first one's position among the keys
-    bool by_request;       // rows of all requests: pos is their least position
 };
 
 template <uint32_t D>
@@ -714,95 +704,6 @@ __device__ __forceinline__ void tile_segment(const BatchParams& p, const Sequenc
     }
 }
 
-// A workgroup's units of wide tiles.
-template <uint32_t D>
-__device__ __forceinline__ void wide_units(const BatchParams& p, uint32_t worker, uint32_t begin, uint32_t end, uint32_t lds,
-                                           TileShared& shared) {
-    const uint32_t lane = threadIdx.x & 63u;
-    uint32_t u = begin;
-    while (u < end) {
-        // (Formed again for each tile rather than kept in registers beside the tile's.)
-        Walk<true> w;
-        if (!w.open(p, lane)) return;
-        Sequence s{nullptr, p.b.prefix, p.b.prefix, 0u, w.rows, w.first_pos, true};
-        const uint32_t hk = floor_div(u, w.wide_head_units);
-        const uint32_t in_head = u - hk * w.wide_head_units;
-        uint32_t tile, off, blocks, block0;   // off: units before u, with kTileCost before the blocks
-        if (in_head < w.prefix_units()) {
-            blocks = w.wide_blocks;
-            block0 = w.wide_lo;
-            tile = floor_div(in_head, blocks + kTileCost);
-            off = in_head - tile * (blocks + kTileCost);
-        } else {
-            Chunk<Walk<true>> c;
-            c.open(p, w, lane, true);
-            const uint32_t at = c.seek(p, w, in_head, lane);
-            if (at == 64u) return;   // (not with u below the total)
-            const Source src = source_of_lane(c.mine, at);
-            const uint32_t x = in_head - (c.before + from_lane(c.incl, at) - from_lane(c.own, at));
-            s.own = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
-            s.pre = w.apart ? p.b.prefix : 0u;
-            s.keys = s.pre + src.hi;
-            s.row0 = src.row0;
-            s.rows = src.rows;
-            s.pos = static_cast<int32_t>(s.pre) + src.pos;
-            s.by_request = false;
-            const WideSpan span = w.span(p, src);
-            uint32_t t0 = 0u, t1 = wide_tiles_of(src.rows, p.G);   // the last tile with before() <= x
-            while (t1 - t0 > 1u) {
-                const uint32_t mid = (t0 + t1) / 2u;
-                if (span.before(mid) <= x) t0 = mid; else t1 = mid;
-            }
-            tile = t0;
-            off = x - span.before(tile);
-            blocks = span.units(tile);
-            block0 = span.end(tile) - blocks;
-        }
-        const uint32_t take = min(blocks + kTileCost - off, end - u);
-        const bool complete = !s.by_request && !w.has_prefix();
-        const uint32_t to = take < blocks + kTileCost ? kToPiece : (complete ? kToOutput : kToRows);
-        const uint32_t piece = 2u * worker + (u == begin ? 0u : 1u);
-        const uint32_t b0 = max(off, kTileCost) - kTileCost;
-        const uint32_t b1 = max(off + take, kTileCost) - kTileCost;
-        if (b0 < b1) {
-            tile_segment<D>(p, s, scalar(hk), scalar(tile), scalar(block0 + b0), scalar(block0 + b1), to, piece, lds, shared);
-        } else if (threadIdx.x < kChunkRows) {   // a piece without blocks
-            p.wide_ml[static_cast<size_t>(piece) * kChunkRows + threadIdx.x] = make_float2(-__builtin_huge_valf(), 0.0f);
-        }
-        u = scalar(u + take);
-    }
-}
-
-// A wave's units of tiles of few rows.
-template <uint32_t D, typename W>
-__device__ __forceinline__ void few_units(const BatchParams& p, const W& w, uint32_t worker, uint32_t begin, uint32_t end,
-                                          uint32_t lds, uint32_t lane) {
-    Chunk<W> c;
-    c.open(p, w, lane, false);
-    uint32_t u = begin;
-    while (u < end) {
-        Source s = w.prefix;
-        const uint32_t* table = p.b.prefix_table;
-        uint32_t unit0 = 0u;
-        const bool is_prefix = u < w.prefix.units(p.KVH);
-        if (!is_prefix) {
-            const uint32_t at = c.seek(p, w, u, lane);
-            if (at == 64u) return;   // (not with u below the total)
-            s = source_of_lane(c.mine, at);
-            table = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
-            unit0 = c.before + from_lane(c.incl, at) - s.units(p.KVH);
-        }
-        const uint32_t g = floor_div(u - unit0, s.blocks);
-        const uint32_t b0 = u - unit0 - g * s.blocks;
-        const uint32_t b1 = min(s.blocks, b0 + (end - u));
-        const uint32_t hk = floor_div(g, s.tiles);
-        const uint32_t to = b1 - b0 < s.blocks ? kToPiece : (!is_prefix && !w.has_prefix() ? kToOutput : kToRows);
-        rows_segment<D>(p, s, table, is_prefix, scalar(hk), scalar(g - hk * s.tiles), scalar(b0), scalar(b1), to,
-                        2u * worker + (u == begin ? 0u : 1u), lds, lane);
-        u += b1 - b0;
-    }
-}
-
 // Workgroups: as many as the device holds at once.
 constexpr uint32_t groups_of(uint32_t D, bool wide) {
     return kComputeUnits * (D >= 512u ? 1u : (wide || D == 256u ? 2u : (D == 128u ? 3u : 4u)));
@@ -822,42 +723,23 @@ __global__ __launch_bounds__(kGroupThreads, groups_of(D, kWide) / kComputeUnits)
         scribe<kWide>(p, ((blockIdx.x - kGroups) * kGroupWaves + wave) * 64u, lane);
         return;
     }
-    Walk<kWide> w;
-    if (!w.open(p, lane)) return;
-    if (kWide && blockIdx.x < w.wide_groups) {
-        __shared__ TileShared shared;
-        const uint32_t worker = scalar(w.worker(blockIdx.x));
-        const uint32_t begin = worker * w.wide_per;
-        wide_units<D>(p, worker, begin, min(begin + w.wide_per, w.wide_units), lds, shared);
-    } else {
-        const uint32_t worker = (blockIdx.x - w.wide_groups) * kGroupWaves + wave;
-        const uint64_t begin = static_cast<uint64_t>(worker) * w.few_per;
-        if (begin >= w.units) return;   // (no barrier follows)
-        few_units<D>(p, w, worker, static_cast<uint32_t>(begin), min(static_cast<uint32_t>(begin) + w.few_per, w.units),
-                     lds + wave * BlockLds<D>::kBytes, lane);
-    }
+    worker_units<kWide>(
+        p, blockIdx.x, wave, lane,
+        [&](const Sequence& s, uint32_t hk, uint32_t tile, uint32_t b0, uint32_t b1, uint32_t to, uint32_t piece) HYP_INLINE {
+            if constexpr (kWide) {
+                __shared__ TileShared shared;
+                tile_segment<D>(p, s, hk, tile, b0, b1, to, piece, lds, shared);
+            }
+        },
+        [&](uint32_t piece) HYP_INLINE {
+            if (threadIdx.x < kChunkRows)
+                p.wide_ml[static_cast<size_t>(piece) * kChunkRows + threadIdx.x] = make_float2(-__builtin_huge_valf(), 0.0f);
+        },
+        [&](const Source& s, const uint32_t* table, bool is_prefix, uint32_t hk, uint32_t tile, uint32_t b0, uint32_t b1,
+            uint32_t to, uint32_t piece) HYP_INLINE {
+            rows_segment<D>(p, s, table, is_prefix, hk, tile, b0, b1, to, piece, lds + wave * BlockLds<D>::kBytes, lane);
+        });
 }
-
-// Where a row's pieces lie: of the prefix [0] and of its own tokens [1].
-struct Pieces {
-    uint32_t count;    // 0: no keys there
-    uint32_t place;    // the first worker's piece, then 2 (first + 1), 2 (first + 2), ...
-    uint32_t next;     // 2 (first + 1)
-    uint32_t at;       // the row's place in its tile
-    bool wide;
-
-    __device__ void set(uint32_t unit0, uint32_t blocks, uint32_t per, uint32_t row, bool wide_) {
-        const uint32_t tile_rows = wide_ ? kChunkRows : kTileRows;
-        at = row % tile_rows;
-        wide = wide_;
-        count = 0u;
-        if (blocks == 0u) return;
-        const uint32_t first = floor_div(unit0, per);
-        count = floor_div(unit0 + blocks - 1u, per) - first + 1u;
-        place = 2u * first + (first * per < unit0 ? 1u : 0u);
-        next = 2u * first + 2u;
-    }
-};
 
 // Joins the pieces of rows that one tile's walk did not finish. A workgroup takes `each` consecutive
 // (row, head) pairs: its first threads find their pieces, one pair a thread, then all of it joins the
@@ -878,33 +760,9 @@ __global__ __launch_bounds__(kMergeThreads) void attn_batch_merge_kernel(BatchPa
         const uint32_t h = pair - t * p.H;
         bool todo = threadIdx.x < each && t < min(p.b.row_start[p.b.requests], p.b.max_rows);
         if (todo) {
-            const Header head = *p.header;
-            const RowRecord row = p.row[t];
-            // (Row starts that skip a row leave its record unwritten.)
-            todo = head.few_per != 0u && row.request < p.b.requests && p.b.row_start[row.request] + row.row == t &&
-                   t < p.b.row_start[row.request + 1u];
+            Pieces a, b;
+            todo = row_pieces(p, t, h, a, b);
             if (todo) {
-                const Record own = p.request[row.request];
-                const uint32_t hk = p.by_G.of(h);
-                const uint32_t pr = t * p.G + (h - hk * p.G);           // its row among all rows of the kv head
-                const uint32_t orow = row.row * p.G + (h - hk * p.G);   // and among its request's
-                Pieces a, b;
-                if (head.wide_blocks != 0u) {
-                    const uint32_t cost = head.wide_blocks + kTileCost;
-                    a.set(hk * head.wide_head + pr / kChunkRows * cost, cost, head.wide_per, pr, true);
-                } else {
-                    a.set((hk * head.tiles + pr / kTileRows) * head.blocks, head.blocks, head.few_per, pr, false);
-                }
-                if (own.wide_units != 0u) {
-                    const Source src = request_source(p, row.request);
-                    const uint32_t pre = head.apart != 0u ? p.b.prefix : 0u;
-                    const WideSpan span(p.G, pre + src.hi, static_cast<int32_t>(pre) + src.pos, p.window);
-                    const uint32_t tile = orow / kChunkRows;
-                    b.set(hk * head.wide_head + own.wide_unit0 + span.before(tile), span.cost(tile), head.wide_per, orow, true);
-                } else {
-                    b.set(own.unit0 + (hk * own.tiles + orow / kTileRows) * own.blocks, own.blocks, head.few_per, orow, false);
-                }
-                todo = b.count != 1u || (head.apart == 0u && (head.blocks != 0u || head.wide_blocks != 0u));
                 found[threadIdx.x][0] = a;
                 found[threadIdx.x][1] = b;
             }

@@ -11,7 +11,6 @@
 
 #include "attention.h"
 #include "batch.h"
-#include "common.h"
 #include "wave.h"
 
 namespace hyperion::hip {
@@ -367,6 +366,181 @@ __device__ __forceinline__ void scribe(const BatchParams& p, uint32_t chunk, uin
         const uint32_t n = from_lane(s.rows, i);
         for (uint32_t t = lane; t < n; t += 64u) p.row[row0 + t] = RowRecord{chunk + i, t};
     }
+}
+
+// Where a segment's rows go: to the output (all their keys were in it), by output row, or to a piece.
+enum : uint32_t { kToOutput = 0u, kToRows = 1u, kToPiece = 2u };
+
+// The keys that a tile walks, positions 0 .. keys - 1: `pre` of the prefix's tokens, then own ones.
+struct Sequence {
+    const uint32_t* own;   // the request's row of tables
+    uint32_t pre, keys;
+    uint32_t row0, rows;   // query rows (tokens)
+    int32_t pos;           // the first one's position among the keys
+    bool by_request;       // rows of all requests: pos is their least position
+};
+
+// A workgroup's units of wide tiles: segment(sequence, kv head, tile, its blocks [b0, b1), where to, piece) of each
+// tile in turn, and nothing(piece) for a piece without blocks.
+template <typename Segment, typename Nothing>
+__device__ __forceinline__ void wide_units(const BatchParams& p, uint32_t worker, uint32_t begin, uint32_t end, uint32_t lane,
+                                           Segment&& segment, Nothing&& nothing) {
+    uint32_t u = begin;
+    while (u < end) {
+        // (Formed again for each tile rather than kept in registers beside the tile's.)
+        Walk<true> w;
+        if (!w.open(p, lane)) return;
+        Sequence s{nullptr, p.b.prefix, p.b.prefix, 0u, w.rows, w.first_pos, true};
+        const uint32_t hk = floor_div(u, w.wide_head_units);
+        const uint32_t in_head = u - hk * w.wide_head_units;
+        uint32_t tile, off, blocks, block0;   // off: units before u, with kTileCost before the blocks
+        if (in_head < w.prefix_units()) {
+            blocks = w.wide_blocks;
+            block0 = w.wide_lo;
+            tile = floor_div(in_head, blocks + kTileCost);
+            off = in_head - tile * (blocks + kTileCost);
+        } else {
+            Chunk<Walk<true>> c;
+            c.open(p, w, lane, true);
+            const uint32_t at = c.seek(p, w, in_head, lane);
+            if (at == 64u) return;   // (not with u below the total)
+            const Source src = source_of_lane(c.mine, at);
+            const uint32_t x = in_head - (c.before + from_lane(c.incl, at) - from_lane(c.own, at));
+            s.own = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
+            s.pre = w.apart ? p.b.prefix : 0u;
+            s.keys = s.pre + src.hi;
+            s.row0 = src.row0;
+            s.rows = src.rows;
+            s.pos = static_cast<int32_t>(s.pre) + src.pos;
+            s.by_request = false;
+            const WideSpan span = w.span(p, src);
+            uint32_t t0 = 0u, t1 = wide_tiles_of(src.rows, p.G);   // the last tile with before() <= x
+            while (t1 - t0 > 1u) {
+                const uint32_t mid = (t0 + t1) / 2u;
+                if (span.before(mid) <= x) t0 = mid; else t1 = mid;
+            }
+            tile = t0;
+            off = x - span.before(tile);
+            blocks = span.units(tile);
+            block0 = span.end(tile) - blocks;
+        }
+        const uint32_t take = min(blocks + kTileCost - off, end - u);
+        const bool complete = !s.by_request && !w.has_prefix();
+        const uint32_t to = take < blocks + kTileCost ? kToPiece : (complete ? kToOutput : kToRows);
+        const uint32_t piece = 2u * worker + (u == begin ? 0u : 1u);
+        const uint32_t b0 = max(off, kTileCost) - kTileCost;
+        const uint32_t b1 = max(off + take, kTileCost) - kTileCost;
+        if (b0 < b1) {
+            segment(s, scalar(hk), scalar(tile), scalar(block0 + b0), scalar(block0 + b1), to, piece);
+        } else {
+            nothing(piece);
+        }
+        u = scalar(u + take);
+    }
+}
+
+// A wave's units of tiles of few rows: segment(source, its table, whether that is the prefix, kv head, tile, its blocks
+// [b0, b1), where to, piece).
+template <typename W, typename Segment>
+__device__ __forceinline__ void few_units(const BatchParams& p, const W& w, uint32_t worker, uint32_t begin, uint32_t end,
+                                          uint32_t lane, Segment&& segment) {
+    Chunk<W> c;
+    c.open(p, w, lane, false);
+    uint32_t u = begin;
+    while (u < end) {
+        Source s = w.prefix;
+        const uint32_t* table = p.b.prefix_table;
+        uint32_t unit0 = 0u;
+        const bool is_prefix = u < w.prefix.units(p.KVH);
+        if (!is_prefix) {
+            const uint32_t at = c.seek(p, w, u, lane);
+            if (at == 64u) return;   // (not with u below the total)
+            s = source_of_lane(c.mine, at);
+            table = p.b.tables + static_cast<size_t>(c.base + at) * p.b.max_blocks;
+            unit0 = c.before + from_lane(c.incl, at) - s.units(p.KVH);
+        }
+        const uint32_t g = floor_div(u - unit0, s.blocks);
+        const uint32_t b0 = u - unit0 - g * s.blocks;
+        const uint32_t b1 = min(s.blocks, b0 + (end - u));
+        const uint32_t hk = floor_div(g, s.tiles);
+        const uint32_t to = b1 - b0 < s.blocks ? kToPiece : (!is_prefix && !w.has_prefix() ? kToOutput : kToRows);
+        segment(s, table, is_prefix, scalar(hk), scalar(g - hk * s.tiles), scalar(b0), scalar(b1), to,
+                2u * worker + (u == begin ? 0u : 1u));
+        u += b1 - b0;
+    }
+}
+
+// The units of wave `wave` of workgroup `group`. Every wave of a workgroup that takes wide tiles goes through all of
+// its units.
+template <bool kWide, typename Wide, typename Nothing, typename Few>
+__device__ __forceinline__ void worker_units(const BatchParams& p, uint32_t group, uint32_t wave, uint32_t lane, Wide&& wide,
+                                             Nothing&& nothing, Few&& few) {
+    Walk<kWide> w;
+    if (!w.open(p, lane)) return;
+    if (kWide && group < w.wide_groups) {
+        const uint32_t worker = scalar(w.worker(group));
+        const uint32_t begin = worker * w.wide_per;
+        wide_units(p, worker, begin, min(begin + w.wide_per, w.wide_units), lane, wide, nothing);
+    } else {
+        const uint32_t worker = (group - w.wide_groups) * kGroupWaves + wave;
+        const uint64_t begin = static_cast<uint64_t>(worker) * w.few_per;
+        if (begin >= w.units) return;   // (no barrier follows)
+        few_units(p, w, worker, static_cast<uint32_t>(begin), min(static_cast<uint32_t>(begin) + w.few_per, w.units), lane,
+                  few);
+    }
+}
+
+// Where a row's pieces lie, of the prefix or of its own tokens.
+struct Pieces {
+    uint32_t count;    // 0: no keys there
+    uint32_t place;    // the first worker's piece, then 2 (first + 1), 2 (first + 2), ...
+    uint32_t next;     // 2 (first + 1)
+    uint32_t at;       // the row's place in its tile
+    bool wide;
+
+    __device__ void set(uint32_t unit0, uint32_t blocks, uint32_t per, uint32_t row, bool wide_) {
+        const uint32_t tile_rows = wide_ ? kChunkRows : kTileRows;
+        at = row % tile_rows;
+        wide = wide_;
+        count = 0u;
+        if (blocks == 0u) return;
+        const uint32_t first = floor_div(unit0, per);
+        count = floor_div(unit0 + blocks - 1u, per) - first + 1u;
+        place = 2u * first + (first * per < unit0 ? 1u : 0u);
+        next = 2u * first + 2u;
+    }
+};
+
+// The pieces of head h of row t, of the prefix (a) and of its own tokens (b); false where the output has that row already,
+// or no request has it.
+__device__ __forceinline__ bool row_pieces(const BatchParams& p, uint32_t t, uint32_t h, Pieces& a, Pieces& b) {
+    const Header head = *p.header;
+    const RowRecord row = p.row[t];
+    // (Row starts that skip a row leave its record unwritten.)
+    if (head.few_per == 0u || row.request >= p.b.requests || p.b.row_start[row.request] + row.row != t ||
+        t >= p.b.row_start[row.request + 1u]) {
+        return false;
+    }
+    const Record own = p.request[row.request];
+    const uint32_t hk = p.by_G.of(h);
+    const uint32_t pr = t * p.G + (h - hk * p.G);           // its row among all rows of the kv head
+    const uint32_t orow = row.row * p.G + (h - hk * p.G);   // and among its request's
+    if (head.wide_blocks != 0u) {
+        const uint32_t cost = head.wide_blocks + kTileCost;
+        a.set(hk * head.wide_head + pr / kChunkRows * cost, cost, head.wide_per, pr, true);
+    } else {
+        a.set((hk * head.tiles + pr / kTileRows) * head.blocks, head.blocks, head.few_per, pr, false);
+    }
+    if (own.wide_units != 0u) {
+        const Source src = request_source(p, row.request);
+        const uint32_t pre = head.apart != 0u ? p.b.prefix : 0u;
+        const WideSpan span(p.G, pre + src.hi, static_cast<int32_t>(pre) + src.pos, p.window);
+        const uint32_t tile = orow / kChunkRows;
+        b.set(hk * head.wide_head + own.wide_unit0 + span.before(tile), span.cost(tile), head.wide_per, orow, true);
+    } else {
+        b.set(own.unit0 + (hk * own.tiles + orow / kTileRows) * own.blocks, own.blocks, head.few_per, orow, false);
+    }
+    return b.count != 1u || (head.apart == 0u && (head.blocks != 0u || head.wide_blocks != 0u));
 }
 
 }  // namespace hyperion::hip
