@@ -205,11 +205,9 @@ struct Walk {
     // Units of the prefix's wide tiles of one kv head.
     __device__ uint32_t prefix_units() const { return wide_blocks != 0u ? wide_tiles * (wide_blocks + kTileCost) : 0u; }
     // The worker for workgroup i. Workgroups go to the XCDs in turn, and each of those has a cache of its own:
-    // an XCD takes consecutive workers, whose tiles share keys. Not where the prefix's tiles are most of the work: then
-    // consecutive workers take a tile's keys in turn (200 rows behind 900 tokens at head_dim 256: 151 us so, 159 in
-    // that order; 24 prompts of 9 to 250 rows behind 6000 at 512: 625 us so, 591 in that order).
+    // an XCD takes consecutive workers, whose tiles share keys (24 prompts of 9 to 250 rows behind 6000 tokens, window 1024
+    // at head_dim 256: 159 us so, 171 with worker i; 478 and 490 at 128; 718 and 715 at 512).
     __device__ uint32_t worker(uint32_t i) const {
-        if (2u * prefix_units() >= wide_head_units) return i;
         const uint32_t n = wide_groups / kXcds, more = wide_groups % kXcds;
         const uint32_t x = i % kXcds;
         return x * n + min(x, more) + i / kXcds;
