@@ -24,11 +24,11 @@
 // 777 tokens (8 of 128) 133 us, 4.5 TB/s; a copy reaches 5.0.
 //
 // Wide: four waves with 32 rows each on 32x32x16 products over K and V blocks that all of them read from LDS, with the
-// same two terms of P: one alone halves what is spent on its product but leaves the output 2.4e-3 from the
+// same two terms of P: one alone halves the products with V but leaves the output 2.4e-3 from the
 // 64-bit result in norm where its own rounding leaves 1.7e-3 (as two terms do), and a row would have fewer bits
 // where more than 16 share its keys. 24 prompts of 9 to 250 rows behind 6000 tokens (16 heads on one of 512) take
-// 720 us with their merge, 627 TFLOP/s of scores and values (940 with the second term) of 1270 that a large matrix
-// product reaches, with one term 590; 50 decode rows behind 16001 90 us, with one term 81.
+// 718 us with their merge, 629 TFLOP/s of scores and values (943 with the second term) of 1270 that a large matrix
+// product reaches, with one term 590; 50 decode rows behind 16001 95 us, with one term 84.
 #include <algorithm>
 
 #include "attention.h"
@@ -710,7 +710,7 @@ constexpr uint32_t groups_of(uint32_t D, bool wide) {
 }
 
 // Without kWide every tile is of few rows (Walk). Both kinds go in one launch: two launches, one after the
-// other, took 124 us for one's 107 (64 rows behind 2000 tokens at head_dim 256, window 1024), 173 for 133 (96
+// other (wide tiles with one term of P), took 124 us for one's 107 (64 rows behind 2000 tokens at head_dim 256, window 1024), 173 for 133 (96
 // rows behind 777 at 128) and 115 for 111 (50 rows behind 16001 at 512).
 template <uint32_t D, bool kWide>
 __global__ __launch_bounds__(kGroupThreads, groups_of(D, kWide) / kComputeUnits) void attn_batch_kernel(BatchParams p) {

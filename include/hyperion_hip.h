@@ -389,9 +389,11 @@ HypStatus hyp_residual_rms_norm(const void* branch, void* residual, const void* 
  * What serving several sequences at once needs next to the calls above, whose caches hold
  * one sequence each; the reference has no counterpart (it decodes one sequence). A step is
  * hyp_batch_plan once, then per layer hyp_batch_prepare and hyp_batch_attention between the
- * projections (which take the step's rows as m), and hyp_batch_sample on the logits. No call
- * allocates or synchronises, so a step can be recorded into a graph; everything that changes
- * from step to step (lengths, blocks, rows) is device memory that the calls read there.
+ * projections (which take the step's rows as m), and hyp_sample_batch on the logits. None of these
+ * calls allocates or synchronises, so each can be recorded into a graph (the projections between them
+ * only while m <= 4, see hyp_graph_capture_begin: a larger step replays graphs of these calls and runs
+ * its projections between the replays); everything that changes from step to step (lengths,
+ * blocks, rows) is device memory that the calls read there.
  *
  * Token blocks: a HypKvCache of at least num_blocks * block_size slots is the pool, block i
  * being its slots [i * block_size, (i + 1) * block_size). Request r's own token j lies in
@@ -465,7 +467,9 @@ HypStatus hyp_batch_prepare(const HypBatch* batch, const void* q, const void* k_
  * [max_rows][n_heads][head_dim], n_heads at most 1024, device bf16, 16-byte aligned; the scores are
  * scale * q.k (scale finite and positive). The rows' own K and V are read from the cache: call
  * hyp_batch_prepare first. The prefix's keys are read for all rows of the batch at once. q, out and workspace
- * do not overlap.
+ * do not overlap. INVALID_ARGUMENT unless max_rows * n_heads * head_dim is below 2^31 and, K being the keys
+ * that a row could see (prefix_len + max_blocks * block_size), (max_rows * n_heads / (16 * num_kv_heads) +
+ * requests + 1) * num_kv_heads * (K / 32 + 5) is below 2^30.
  * fp32 scores and softmax, output rounded to bf16. Probabilities enter the products as two bf16 terms
  * (2^-16 of a weight). The order in which a row's keys are summed, and so its last bits, depends on the
  * step it is in; the same step gives the same bits. A row that sees no key above -inf gives zeros; a
@@ -478,7 +482,9 @@ HypStatus hyp_batch_attention(const HypBatch* batch, const void* q, uint32_t n_h
                               uint32_t window, float scale, void* out, void* workspace, size_t workspace_bytes,
                               HypStream stream);
 /* The workspace of hyp_batch_attention for batches of this size (requests, max_rows and whether there is a
- * prefix; host only). */
+ * prefix; host only). Most of it is the unfinished rows of all workgroups that the device holds at once, whatever
+ * the batch: 69 MB at head_dim 64, 119 at 128, 203 at 256 and 202 at 512. Beside that 4 * head_dim + 8 bytes for
+ * each row and head, twice with a prefix. One workspace serves all layers of a step in turn. */
 HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads, HypKvCache cache, size_t* out_bytes);
 
 /* ---- the model, its KV state and the step ABI (hyperion_mlx.h:50-248) -------------------
