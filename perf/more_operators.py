@@ -314,7 +314,7 @@ def _handles(case, st):
     st["dev"] = dev = {k: hy.DeviceView(v) for k, v in st.items() if isinstance(v, torch.Tensor)}
     need = 0
     if kind == "verify":
-        need = hy.verify_batch_workspace_bytes(st["logits"].shape[0], case["vocab"], case["drafter"])
+        need = hy.verify_batch_workspace_bytes(st["logits"].shape[0], case["vocab"], case["requests"], case["drafter"])
     elif kind == "copy":
         slots = st["num"] * case["block"]
         st["caches"] = []
