@@ -53,7 +53,8 @@ EXPORTED = [
     "hyp_kv_cache_create", "hyp_kv_cache_free", "hyp_kv_cache_buffers", "hyp_kv_cache_write", "hyp_attention",
     "hyp_attention_prepare", "hyp_residual_rms_norm",
     "hyp_batch_plan", "hyp_batch_prepare", "hyp_batch_attention", "hyp_batch_attention_workspace",
-    "hyp_sample_batch", "hyp_sample_batch_workspace",
+    "hyp_sample_batch", "hyp_sample_batch_workspace", "hyp_verify_batch", "hyp_verify_batch_workspace",
+    "hyp_batch_fork", "hyp_batch_rewind", "hyp_batch_compact", "hyp_batch_pages_workspace", "hyp_batch_copy",
     "hyp_model_create", "hyp_model_free", "hyp_model_load", "hyp_kvstate_create", "hyp_kvstate_free",
     "hyp_prefill_chunk", "hyp_decode_block", "hyp_prefill_chunk_sampled", "hyp_decode_block_sampled",
     "hyp_step_result_create", "hyp_step_result_free", "hyp_step_result_fields", "hyp_model_forward_hidden",
@@ -214,6 +215,7 @@ class BatchFields(ctypes.Structure):
 
 SLOT_NONE = 0xFFFFFFFF      # HYP_SLOT_NONE
 REQUEST_DONE = 0xFFFFFFFF   # HYP_REQUEST_DONE
+PARENT_NONE = 0xFFFFFFFF    # HYP_PARENT_NONE
 
 
 class StepResultFields(ctypes.Structure):
@@ -317,6 +319,13 @@ def load_library(path: str) -> ctypes.CDLL:
         "hyp_batch_attention_workspace": [_P, _U32, _P, ctypes.POINTER(_SZ)],
         "hyp_sample_batch": [_P, _U32, _U32, _P, _P, _P, _P, _P, _SZ, _P],
         "hyp_sample_batch_workspace": [_U32, _U32, ctypes.POINTER(_SZ)],
+        "hyp_verify_batch": [_P, _P, _U32, _U32, _P, _U32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+        "hyp_verify_batch_workspace": [_U32, _U32, _U32, ctypes.c_int, ctypes.POINTER(_SZ)],
+        "hyp_batch_fork": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+        "hyp_batch_rewind": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+        "hyp_batch_compact": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+        "hyp_batch_pages_workspace": [_P, ctypes.POINTER(_SZ)],
+        "hyp_batch_copy": [_P, _P, _U32, _P, _U32, _P, _P],
         "hyp_model_create": [_PP],
         "hyp_model_free": [_PP],
         "hyp_model_load": [_P, ctypes.POINTER(GeometryParams), ctypes.c_char_p],
@@ -813,6 +822,40 @@ class Batch:
         call("hyp_batch_attention", self._ref, q.ptr, n_heads, cache.handle, window, scale, out.ptr, workspace.ptr,
              workspace.nbytes, stream.handle)
 
+    def fork(self, lens: "DeviceArray", parents: "DeviceArray", free_blocks: "DeviceArray", taken: "DeviceArray",
+             taken_out: "DeviceArray", served: "DeviceArray", copies: "DeviceArray", n_copies: "DeviceArray",
+             stream: "Stream") -> None:
+        """hyp_batch_fork: requests become copies of their parents (PARENT_NONE: none); copies [requests, 3]
+        lists the blocks that copy() then copies."""
+        call("hyp_batch_fork", self._ref, lens.ptr, parents.ptr, free_blocks.ptr, taken.ptr, taken_out.ptr, served.ptr,
+             copies.ptr, n_copies.ptr, stream.handle)
+
+    def pages_workspace_bytes(self) -> int:
+        """Bytes of a workspace for rewind() and compact()."""
+        out = _SZ()
+        call("hyp_batch_pages_workspace", self._ref, ctypes.byref(out))
+        return int(out.value)
+
+    def rewind(self, lens: "DeviceArray", drop: "DeviceArray", free_blocks: "DeviceArray", taken: "DeviceArray",
+               taken_out: "DeviceArray", copies: "DeviceArray", n_copies: "DeviceArray", workspace: "DeviceArray",
+               stream: "Stream") -> None:
+        """hyp_batch_rewind: requests lose their last drop tokens (REQUEST_DONE: all); blocks that nobody holds
+        go back. copies [requests, 3]."""
+        call("hyp_batch_rewind", self._ref, lens.ptr, drop.ptr, free_blocks.ptr, taken.ptr, taken_out.ptr, copies.ptr,
+             n_copies.ptr, workspace.ptr, workspace.nbytes, stream.handle)
+
+    def compact(self, tables_out: "DeviceArray", prefix_out: Optional["DeviceArray"], free_blocks: "DeviceArray",
+                taken_out: "DeviceArray", copies: "DeviceArray", n_copies: "DeviceArray", workspace: "DeviceArray",
+                stream: "Stream") -> None:
+        """hyp_batch_compact: the blocks in use get the lowest ids. copies [num_blocks // 2, 3]."""
+        call("hyp_batch_compact", self._ref, tables_out.ptr, None if prefix_out is None else prefix_out.ptr,
+             free_blocks.ptr, taken_out.ptr, copies.ptr, n_copies.ptr, workspace.ptr, workspace.nbytes, stream.handle)
+
+    def copy(self, caches, copies: "DeviceArray", n_copies: "DeviceArray", stream: "Stream") -> None:
+        """hyp_batch_copy: the listed blocks [.., 3] of (from, to, tokens) in every cache."""
+        handles = (ctypes.c_void_p * len(caches))(*[c.handle.value for c in caches])
+        call("hyp_batch_copy", self._ref, handles, len(caches), copies.ptr, copies.shape[0], n_copies.ptr, stream.handle)
+
 
 def residual_rms_norm(branch: "DeviceArray", residual: "DeviceArray", post_w: "DeviceArray",
                       scalar: Optional["DeviceArray"], next_w: Optional["DeviceArray"], nxt: Optional["DeviceArray"],
@@ -1013,6 +1056,25 @@ def sample_batch(logits: DeviceArray, rows: int, vocab: int, configs: DeviceArra
     call("hyp_sample_batch", logits.ptr, rows, vocab, configs.ptr, uniforms.ptr, tokens.ptr,
          None if logprobs is None else logprobs.ptr, None if workspace is None else workspace.ptr,
          0 if workspace is None else workspace.nbytes, stream.handle)
+
+
+def verify_batch_workspace_bytes(rows: int, vocab: int, requests: int, drafted: bool) -> int:
+    """Bytes of a workspace for verify_batch() of these sizes, with (drafted) or without draft logits."""
+    out = _SZ()
+    call("hyp_verify_batch_workspace", rows, vocab, requests, int(drafted), ctypes.byref(out))
+    return int(out.value)
+
+
+def verify_batch(logits: DeviceArray, draft_logits: Optional[DeviceArray], rows: int, vocab: int, row_start: DeviceArray,
+                 requests: int, ids: DeviceArray, configs: DeviceArray, draft_configs: Optional[DeviceArray],
+                 uniforms: DeviceArray, accepted: DeviceArray, rejected: DeviceArray, tokens: DeviceArray,
+                 logprobs: Optional[DeviceArray], workspace: DeviceArray, stream: Stream) -> None:
+    """hyp_verify_batch: how many of each request's drafts (ids behind its first row) stand against the
+    target's logits, and the token that follows them."""
+    opt = lambda a: None if a is None else a.ptr  # noqa: E731
+    call("hyp_verify_batch", logits.ptr, opt(draft_logits), rows, vocab, row_start.ptr, requests, ids.ptr, configs.ptr,
+         opt(draft_configs), uniforms.ptr, accepted.ptr, rejected.ptr, tokens.ptr, opt(logprobs), workspace.ptr,
+         workspace.nbytes, stream.handle)
 
 
 def topk_samples(out: DeviceArray, rows: int, stream: Stream):

@@ -7,12 +7,15 @@
 #include <cstdio>
 #include <cstring>
 #include <filesystem>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <new>
 #include <string>
+#include <vector>
 
 #include "batch.h"
+#include "batch_pages.h"
 #include "hyperion_hip.h"
 #include "kernels.h"
 #include "decoder.h"
@@ -20,6 +23,7 @@
 #include "sample_batch.h"
 #include "sampling.h"
 #include "step_program_host.h"
+#include "verify_batch.h"
 
 using hyperion::hip::Epilogue;
 using hyperion::hip::NativeError;
@@ -913,10 +917,15 @@ hyperion::hip::BatchView batch_ref(const HypBatch* b) {
             b->tables,   b->lens,   b->row_start,  b->slots,      b->positions};
 }
 
-HypKvCacheOpaque& batch_cache(const HypBatch& b, HypKvCache cache, uint32_t n_heads) {
+HypKvCacheOpaque& batch_cache(const HypBatch& b, HypKvCache cache) {
     HypKvCacheOpaque& c = kv_ref(cache);
     REQUIRE_ARG(static_cast<uint64_t>(b.num_blocks) * b.block_size <= c.capacity,
                 "the cache must hold num_blocks * block_size tokens");
+    return c;
+}
+
+HypKvCacheOpaque& batch_cache(const HypBatch& b, HypKvCache cache, uint32_t n_heads) {
+    HypKvCacheOpaque& c = batch_cache(b, cache);
     REQUIRE_ARG(n_heads > 0 && n_heads % c.num_kv_heads == 0, "n_heads must be a multiple of the cache's num_kv_heads");
     REQUIRE_ARG(n_heads <= 1024u, "n_heads must be at most 1024");
     REQUIRE_ARG(static_cast<uint64_t>(b.max_rows) * n_heads * c.head_dim < (1ull << 31), "q too large");
@@ -1055,6 +1064,198 @@ HypStatus hyp_sample_batch_workspace(uint32_t rows, uint32_t vocab, size_t* out_
         REQUIRE_ARG(vocab <= hyperion::hip::sample_batch_max_vocab(), "vocab must be at most 2^23");
         REQUIRE_ARG(rows <= hyperion::hip::kMaxBatchRows, "a call has at most 2^20 rows");
         *out_bytes = hyperion::hip::sample_batch_workspace_bytes(rows, vocab);
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+// Device memory of a call, for the refusal of outputs that lie over other arrays.
+struct Span {
+    const void* at;
+    uint64_t bytes;
+};
+void require_apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span* w = written.begin(); w != written.end(); ++w) {
+        const auto over = [&](const Span& x) {
+            return w->at != nullptr && x.at != nullptr && w->bytes != 0 && x.bytes != 0 &&
+                   hyperion::hip::overlap(w->at, w->bytes, x.at, x.bytes);
+        };
+        for (const Span* x = w + 1; x != written.end(); ++x) REQUIRE_ARG(!over(*x), "outputs must not overlap each other");
+        for (const Span& x : read) REQUIRE_ARG(!over(x), "outputs must not overlap inputs");
+    }
+}
+bool aligned4(std::initializer_list<const void*> all) {
+    for (const void* p : all)
+        if ((reinterpret_cast<uintptr_t>(p) & 3u) != 0u) return false;
+    return true;
+}
+// What may be the array `out` itself, as an input of its own otherwise.
+Span unless_same(const void* in, const void* out, uint64_t bytes) { return in == out ? Span{nullptr, 0} : Span{in, bytes}; }
+
+uint64_t table_bytes(const hyperion::hip::BatchView& b) { return uint64_t{4} * b.requests * b.max_blocks; }
+
+}  // namespace
+
+extern "C" {
+
+HypStatus hyp_batch_fork(const HypBatch* batch, const uint32_t* lens, const uint32_t* parents,
+                         const uint32_t* free_blocks, const uint32_t* taken, uint32_t* taken_out, uint32_t* served,
+                         HypBlockCopy* copies, uint32_t* n_copies, HypStream stream) {
+    return abi_call("hyp_batch_fork", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        REQUIRE_ARG(b.requests == 0 || (lens != nullptr && parents != nullptr && copies != nullptr),
+                    "lens, parents and copies must be non-null device pointers");
+        REQUIRE_ARG(free_blocks != nullptr && taken != nullptr && taken_out != nullptr && served != nullptr &&
+                        n_copies != nullptr,
+                    "free_blocks, taken, taken_out, served and n_copies must be non-null device pointers");
+        REQUIRE_ARG(aligned4({b.tables, b.lens, lens, parents, free_blocks, taken, taken_out, served, copies, n_copies}),
+                    "arrays must be 4-byte aligned");
+        const uint64_t n = uint64_t{4} * b.requests;
+        require_apart({{b.lens, n}, {b.tables, table_bytes(b)}, {taken_out, 4}, {served, 4}, {copies, 3 * n}, {n_copies, 4}},
+                      {unless_same(lens, b.lens, n), {parents, n}, {free_blocks, uint64_t{4} * b.num_blocks},
+                       unless_same(taken, taken_out, 4)});
+        hyperion::hip::launch_batch_fork(b, lens, parents, free_blocks, taken, taken_out, served, copies, n_copies, s);
+    });
+}
+
+HypStatus hyp_batch_rewind(const HypBatch* batch, const uint32_t* lens, const uint32_t* drop, uint32_t* free_blocks,
+                           const uint32_t* taken, uint32_t* taken_out, HypBlockCopy* copies, uint32_t* n_copies,
+                           void* workspace, size_t workspace_bytes, HypStream stream) {
+    return abi_call("hyp_batch_rewind", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        REQUIRE_ARG(b.requests == 0 || (lens != nullptr && drop != nullptr && copies != nullptr),
+                    "lens, drop and copies must be non-null device pointers");
+        REQUIRE_ARG(free_blocks != nullptr && taken != nullptr && taken_out != nullptr && n_copies != nullptr,
+                    "free_blocks, taken, taken_out and n_copies must be non-null device pointers");
+        REQUIRE_ARG(aligned4({b.tables, b.lens, lens, drop, free_blocks, taken, taken_out, copies, n_copies}),
+                    "arrays must be 4-byte aligned");
+        const size_t need = hyperion::hip::batch_pages_workspace_bytes(b);
+        REQUIRE_ARG(workspace != nullptr && workspace_bytes >= need, "batch rewind: workspace too small");
+        REQUIRE_ARG(aligned16(workspace), "workspace must be 16-byte aligned");
+        const uint64_t n = uint64_t{4} * b.requests;
+        require_apart({{b.lens, n}, {b.tables, table_bytes(b)}, {free_blocks, uint64_t{4} * b.num_blocks}, {taken_out, 4},
+                       {copies, 3 * n}, {n_copies, 4}, {workspace, need}},
+                      {unless_same(lens, b.lens, n), {drop, n}, unless_same(taken, taken_out, 4)});
+        hyperion::hip::launch_batch_rewind(b, lens, drop, free_blocks, taken, taken_out, copies, n_copies, workspace, s);
+    });
+}
+
+HypStatus hyp_batch_compact(const HypBatch* batch, uint32_t* tables_out, uint32_t* prefix_out, uint32_t* free_blocks,
+                            uint32_t* taken_out, HypBlockCopy* copies, uint32_t* n_copies, void* workspace,
+                            size_t workspace_bytes, HypStream stream) {
+    return abi_call("hyp_batch_compact", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        REQUIRE_ARG(b.requests == 0 || b.max_blocks == 0 || tables_out != nullptr,
+                    "tables_out must be a non-null device pointer");
+        REQUIRE_ARG(b.prefix == 0 || (b.prefix_table != nullptr && prefix_out != nullptr),
+                    "a prefix needs its prefix_table and prefix_out");
+        REQUIRE_ARG(free_blocks != nullptr && taken_out != nullptr && n_copies != nullptr,
+                    "free_blocks, taken_out and n_copies must be non-null device pointers");
+        REQUIRE_ARG(b.num_blocks < 2 || copies != nullptr, "copies must be a non-null device pointer");
+        REQUIRE_ARG(aligned4({b.tables, b.lens, b.prefix_table, tables_out, prefix_out, free_blocks, taken_out, copies,
+                              n_copies}),
+                    "arrays must be 4-byte aligned");
+        const size_t need = hyperion::hip::batch_pages_workspace_bytes(b);
+        REQUIRE_ARG(workspace != nullptr && workspace_bytes >= need, "batch compact: workspace too small");
+        REQUIRE_ARG(aligned16(workspace), "workspace must be 16-byte aligned");
+        const uint64_t prefix_bytes = b.prefix == 0 ? 0 : ((uint64_t{b.prefix} + (1u << b.shift) - 1u) >> b.shift) * 4u;
+        require_apart({{tables_out, table_bytes(b)}, {prefix_out, prefix_bytes}, {free_blocks, uint64_t{4} * b.num_blocks},
+                       {taken_out, 4}, {copies, uint64_t{12} * (b.num_blocks / 2)}, {n_copies, 4}, {workspace, need}},
+                      {{b.lens, uint64_t{4} * b.requests}, unless_same(b.tables, tables_out, table_bytes(b)),
+                       unless_same(b.prefix_table, prefix_out, prefix_bytes)});
+        hyperion::hip::launch_batch_compact(b, tables_out, prefix_out, free_blocks, taken_out, copies, n_copies, workspace, s);
+    });
+}
+
+HypStatus hyp_batch_pages_workspace(const HypBatch* batch, size_t* out_bytes) {
+    return abi_call("hyp_batch_pages_workspace", [&] {
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        REQUIRE_ARG(out_bytes != nullptr, "out_bytes must be non-null");
+        *out_bytes = hyperion::hip::batch_pages_workspace_bytes(b);
+    });
+}
+
+HypStatus hyp_batch_copy(const HypBatch* batch, const HypKvCache* caches, uint32_t n_caches, const HypBlockCopy* copies,
+                         uint32_t max_copies, const uint32_t* n_copies, HypStream stream) {
+    return abi_call("hyp_batch_copy", [&] {
+        hipStream_t s = stream_of(stream);
+        const hyperion::hip::BatchView b = batch_ref(batch);
+        if (n_caches == 0 || max_copies == 0) return;
+        REQUIRE_ARG(caches != nullptr, "caches must be non-null");
+        REQUIRE_ARG(copies != nullptr && n_copies != nullptr, "copies and n_copies must be non-null device pointers");
+        REQUIRE_ARG(aligned4({copies, n_copies}), "arrays must be 4-byte aligned");
+        std::vector<hyperion::hip::CopyCache> all(n_caches);
+        for (uint32_t i = 0; i < n_caches; ++i) {
+            HypKvCacheOpaque& c = batch_cache(*batch, caches[i]);
+            all[i] = {static_cast<uint8_t*>(c.k.data()), static_cast<uint8_t*>(c.v.data()), 2u * c.num_kv_heads * c.head_dim};
+        }
+        hyperion::hip::launch_batch_copy(b, all.data(), n_caches, copies, max_copies, n_copies, s);
+    });
+}
+
+HypStatus hyp_verify_batch(const void* logits, const void* draft_logits, uint32_t rows, uint32_t vocab,
+                           const uint32_t* row_start, uint32_t requests, const uint32_t* ids,
+                           const HypSamplingConfig* configs, const HypSamplingConfig* draft_configs, const float* uniforms,
+                           uint32_t* accepted, uint32_t* rejected, uint32_t* tokens, float* logprobs, void* workspace,
+                           size_t workspace_bytes, HypStream stream) {
+    return abi_call("hyp_verify_batch", [&] {
+        hipStream_t s = stream_of(stream);
+        REQUIRE_ARG(vocab <= hyperion::hip::sample_batch_max_vocab(), "vocab must be at most 2^23");
+        REQUIRE_ARG(rows <= hyperion::hip::kMaxBatchRows, "a call has at most 2^20 rows");
+        REQUIRE_ARG(requests <= hyperion::hip::kMaxRequests, "a call has at most 4096 requests");
+        if (requests == 0) return;
+        REQUIRE_ARG(rows == 0 || vocab == 0 || logits != nullptr, "logits must be a non-null device pointer");
+        REQUIRE_ARG(row_start != nullptr && configs != nullptr, "row_start and configs must be non-null device pointers");
+        REQUIRE_ARG(rows == 0 || (ids != nullptr && uniforms != nullptr), "ids and uniforms must be non-null device pointers");
+        REQUIRE_ARG(accepted != nullptr && rejected != nullptr && tokens != nullptr,
+                    "accepted, rejected and tokens must be non-null device pointers");
+        REQUIRE_ARG(((reinterpret_cast<uintptr_t>(configs) | reinterpret_cast<uintptr_t>(draft_configs)) & 7u) == 0u,
+                    "configs and draft_configs must be 8-byte aligned");
+        REQUIRE_ARG(((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_logits)) & 1u) == 0u,
+                    "logits and draft_logits must be 2-byte aligned");
+        REQUIRE_ARG(aligned4({row_start, ids, uniforms, accepted, rejected, tokens, logprobs}),
+                    "arrays must be 4-byte aligned");
+        const size_t need = hyperion::hip::verify_batch_workspace_bytes(rows, vocab, requests, draft_logits != nullptr);
+        REQUIRE_ARG(workspace_bytes >= need && (need == 0 || workspace != nullptr), "batch verification: workspace too small");
+        REQUIRE_ARG(aligned16(workspace), "workspace must be 16-byte aligned");
+        const uint64_t logit_bytes = uint64_t{2} * rows * vocab, config_bytes = uint64_t{sizeof(HypSamplingConfig)} * requests;
+        const uint64_t of_rows = uint64_t{4} * rows, of_requests = uint64_t{4} * requests;
+        require_apart({{accepted, of_requests}, {rejected, of_requests}, {tokens, of_requests}, {logprobs, of_rows},
+                       {workspace, need}},
+                      {{logits, logit_bytes}, {draft_logits, logit_bytes}, {row_start, of_requests + 4}, {ids, of_rows},
+                       {configs, config_bytes}, {draft_configs, config_bytes}, {uniforms, of_rows}});
+        hyperion::hip::VerifyArgs a{};
+        a.logits = static_cast<const uint16_t*>(logits);
+        a.draft_logits = static_cast<const uint16_t*>(draft_logits);
+        a.rows = rows;
+        a.vocab = vocab;
+        a.requests = requests;
+        a.row_start = row_start;
+        a.ids = ids;
+        a.configs = configs;
+        a.draft_configs = draft_configs != nullptr ? draft_configs : configs;
+        a.uniforms = uniforms;
+        a.accepted = accepted;
+        a.rejected = rejected;
+        a.tokens = tokens;
+        a.logprobs = logprobs;
+        a.workspace = workspace;
+        hyperion::hip::launch_verify_batch(a, s);
+    });
+}
+
+HypStatus hyp_verify_batch_workspace(uint32_t rows, uint32_t vocab, uint32_t requests, int drafted, size_t* out_bytes) {
+    return abi_call("hyp_verify_batch_workspace", [&] {
+        REQUIRE_ARG(out_bytes != nullptr, "out_bytes must be non-null");
+        REQUIRE_ARG(vocab <= hyperion::hip::sample_batch_max_vocab(), "vocab must be at most 2^23");
+        REQUIRE_ARG(rows <= hyperion::hip::kMaxBatchRows, "a call has at most 2^20 rows");
+        REQUIRE_ARG(requests <= hyperion::hip::kMaxRequests, "a call has at most 4096 requests");
+        *out_bytes = hyperion::hip::verify_batch_workspace_bytes(rows, vocab, requests, drafted != 0);
     });
 }
 

@@ -156,8 +156,8 @@ HypStatus hyp_event_elapsed_ms(HypEvent start, HypEvent end, float* out_ms);
  * at mx::eval, forward.cc:171). Between begin and end, hyp_qmatmul, hyp_qmatmul_ex,
  * hyp_qmatmul_group, hyp_qmlp_gate_up_gelu and hyp_qmatmul_group_rmsnorm with m <= 4, hyp_rms_normalize, hyp_quantize_q4g64,
  * hyp_dequantize_q4g64, hyp_embed, hyp_sample_greedy, hyp_sample_greedy_topk, hyp_kv_cache_write,
- * hyp_attention, hyp_rope, hyp_batch_plan, hyp_batch_prepare, hyp_batch_attention, hyp_sample_batch and
- * the copies on `stream` are
+ * hyp_attention, hyp_rope, hyp_batch_plan, hyp_batch_prepare, hyp_batch_attention, hyp_sample_batch,
+ * hyp_batch_fork, hyp_batch_rewind, hyp_batch_compact, hyp_batch_copy, hyp_verify_batch and the copies on `stream` are
  * recorded instead of run (they allocate nothing). Calls that may allocate or clear
  * memory - the matmul entries on their GEMM path (m > 4) and hyp_memset_device - check
  * the stream and return INVALID_ARGUMENT while it is capturing, before enqueueing
@@ -487,6 +487,77 @@ HypStatus hyp_batch_attention(const HypBatch* batch, const void* q, uint32_t n_h
  * each row and head, twice with a prefix. One workspace serves all layers of a step in turn. */
 HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads, HypKvCache cache, size_t* out_bytes);
 
+/* ---- forked requests and blocks given back ----------------------------------------------
+ * Operations on a batch's tables between its steps; like the calls above they neither allocate nor
+ * synchronise, and record into graphs. Requests may hold blocks in common: hyp_batch_fork makes a request a
+ * copy of another without moving its tokens. A block that a request fills only in part, so that its next tokens
+ * go there, is its own: fork and rewind keep that, by listing blocks to copy, which hyp_batch_copy does in the caches
+ * of all layers. Who holds a block follows from tables and lengths alone. Which requests share one matters to
+ * the end of a request: hyp_batch_plan's HYP_REQUEST_DONE returns a request's blocks without asking who else
+ * holds them, so a request that was forked, or is a fork, ends by hyp_batch_rewind. A request's row of
+ * tables holds a block once. Arrays that a call writes do not overlap each other or any that it reads, but
+ * where it says that they may be the same (INVALID_ARGUMENT). */
+
+/* The first `tokens` tokens of block `from` to block `to`. */
+typedef struct HypBlockCopy {
+    uint32_t from;
+    uint32_t to;
+    uint32_t tokens;
+} HypBlockCopy;
+
+#define HYP_PARENT_NONE 0xFFFFFFFFu
+
+/* Requests become copies of others. parents [requests]: HYP_PARENT_NONE, or the request that r becomes a copy of, a
+ * request whose own entry is HYP_PARENT_NONE; any other value counts as HYP_PARENT_NONE. r holds no blocks before (what its
+ * row of tables says is forgotten, not given back). lens [requests] are the lengths before (may be batch->lens itself).
+ *  - The copies are served in order. r gets its parent's length and whole blocks, in common with it; where
+ *    the parent's last block is filled in part, the next free block free_blocks[taken ..] instead of it, and an entry
+ *    of copies [requests] in that order. taken and taken_out are one uint32 each (may be the same).
+ *  - served (one uint32) is the first copy for which no block is free, or requests. It and all copies behind it
+ *    stay as they are.
+ *  - batch->lens: the lengths of all requests; n_copies (one uint32): entries written to copies.
+ * Row starts, slots and positions are not touched. */
+HypStatus hyp_batch_fork(const HypBatch* batch, const uint32_t* lens, const uint32_t* parents,
+                         const uint32_t* free_blocks, const uint32_t* taken, uint32_t* taken_out, uint32_t* served,
+                         HypBlockCopy* copies, uint32_t* n_copies, HypStream stream);
+
+/* Requests lose their last tokens: drop [requests] of them, all where drop is lens or more (HYP_REQUEST_DONE, say:
+ * the request ends, as by hyp_batch_plan). lens [requests] are the lengths before (may be batch->lens itself).
+ *  - Blocks that no request holds any longer go back to the stack, in the order of requests and of their tables (one
+ *    that several give up where the first of them does), as entries [taken - returned, taken) of free_blocks.
+ *  - A request that is shortened into a block which others hold too gets a free block of its own instead, in order of
+ *    requests, from the stack's entry taken - returned upwards, and an entry of copies [requests] (where all
+ *    holders of a block are shortened into it, the last of them keeps it). Where none is free it loses that
+ *    block's tokens as well: batch->lens says so.
+ *  - batch->lens: the lengths after; n_copies (one uint32): entries written to copies. taken and taken_out are one uint32
+ *    each (may be the same). The rest of a request's row of tables stays as it is.
+ * After hyp_verify_batch, its `rejected` is the drop. Ids of blocks >= num_blocks are not given back. workspace: device
+ * memory of hyp_batch_pages_workspace's bytes, 16-byte aligned, whose contents need not be kept between calls;
+ * calls that overlap need one each, and so do graphs whose replays overlap. */
+HypStatus hyp_batch_rewind(const HypBatch* batch, const uint32_t* lens, const uint32_t* drop, uint32_t* free_blocks,
+                           const uint32_t* taken, uint32_t* taken_out, HypBlockCopy* copies, uint32_t* n_copies,
+                           void* workspace, size_t workspace_bytes, HypStream stream);
+
+/* The blocks in use - all that a request holds by tables and lens, and the prefix's - move to the ids below their
+ * number L: the i-th of those with an id of L or more, ascending, to the i-th id below L that is not in use.
+ *  - tables_out [requests][max_blocks] (may be batch->tables) and prefix_out (may be the prefix's table; NULL without
+ *    a prefix): the tables with the new ids; entries that no request holds as they are.
+ *  - copies [num_blocks / 2], n_copies (one uint32): the moves, whole blocks.
+ *  - free_blocks: entry i is i, from L on; taken_out (one uint32): L. What else was taken from the stack is free now.
+ * Workspace as hyp_batch_rewind. */
+HypStatus hyp_batch_compact(const HypBatch* batch, uint32_t* tables_out, uint32_t* prefix_out, uint32_t* free_blocks,
+                            uint32_t* taken_out, HypBlockCopy* copies, uint32_t* n_copies, void* workspace,
+                            size_t workspace_bytes, HypStream stream);
+/* The workspace of hyp_batch_rewind and hyp_batch_compact (host only; a device need not be there). */
+HypStatus hyp_batch_pages_workspace(const HypBatch* batch, size_t* out_bytes);
+
+/* Carry out min(n_copies[0], max_copies) entries of copies (device) in the K and V of n_caches caches (host array of
+ * handles; the layers of one batch, of any shapes): at most block_size tokens each. Entries with an id >= num_blocks, or of
+ * a block to itself, do nothing. No block is the `to` of one entry and the `from` or `to` of another (as the calls above
+ * list them): entries run in no order. Call it before the next hyp_batch_prepare. */
+HypStatus hyp_batch_copy(const HypBatch* batch, const HypKvCache* caches, uint32_t n_caches, const HypBlockCopy* copies,
+                         uint32_t max_copies, const uint32_t* n_copies, HypStream stream);
+
 /* ---- the model, its KV state and the step ABI (hyperion_mlx.h:50-248) -------------------
  * The reference's model-level entry points over this library's kernels: hyp_model_load
  * makes the projections, norm vectors and layer scalars resident; hyp_prefill_chunk and
@@ -673,6 +744,37 @@ HypStatus hyp_sample_batch(const void* logits, uint32_t rows, uint32_t vocab, co
                            size_t workspace_bytes, HypStream stream);
 /* The workspace of hyp_sample_batch for this many rows (host only; a device need not be there). */
 HypStatus hyp_sample_batch_workspace(uint32_t rows, uint32_t vocab, size_t* out_bytes);
+
+/* Drafted tokens against the target's probabilities (speculative decoding): how many of each request's drafts stand, and
+ * the token that follows them, drawn so that all are distributed as tokens drawn from the target one by one. Request r's
+ * rows are row_start[r] .. row_start[r + 1] - 1 of `rows` (row_start [requests + 1], device, not decreasing; a step's, say;
+ * cut off at rows): ids [rows] (device) are the tokens that the target read there, the first one known, the others
+ * drafted. So row t's logits [vocab] (bf16, device, row-major) judge ids[t + 1], but behind the last row nothing was drafted.
+ *  - p of row t: the distribution that hyp_sample_batch draws from with configs[r] (device; one for each request): w
+ *    of the kept tokens over their sum, in fp64. A greedy request's first token has 1. A row with no logit above
+ *    -inf has p = 0 everywhere.
+ *  - q of row t: the same of draft_logits [rows][vocab], with draft_configs[r] (NULL: configs); a
+ *    request's last row of draft_logits is not read. draft_logits NULL: the drafts have no distribution (found by lookup
+ *    or greedily), q is 1 at the draft.
+ *  - A draft x is accepted iff uniforms[t] * q(x) < p(x); one of vocab or more is not. accepted[r]: the drafts before
+ *    the first that is not; rejected[r]: the others (hyp_batch_rewind's drop).
+ *  - tokens[r], as hyp_embed takes them: drawn from p behind the last draft, otherwise from max(0, p - q) of the first
+ *    row whose draft fell (from p should that be 0 everywhere): the first token along the index whose running
+ *    sum exceeds the whole times the uniform of the request's last row, which no draft uses. p = 0 everywhere gives token 0.
+ *  - logprobs [rows] (device) or NULL: ln of the share of the token that follows row t, before the filters, as
+ *    hyp_sample_batch gives it, for the accepted drafts and the drawn token; rows behind stay as they are.
+ * A uniform below 0 or NaN counts as 0, one of 1 or more as the largest float below 1. A request without rows has accepted and
+ * rejected 0, its token stays as it is. vocab is at most 2^23, rows at most 2^20, requests at most 4096. The results do not depend on
+ * the rest of the batch or on the order of execution. Arrays that the call writes do not overlap each other or
+ * any that it reads. workspace: device memory of hyp_verify_batch_workspace's bytes, 16-byte aligned,
+ * whose contents need not be kept between calls; calls that overlap need one each, and so do graphs whose replays overlap. */
+HypStatus hyp_verify_batch(const void* logits, const void* draft_logits, uint32_t rows, uint32_t vocab,
+                           const uint32_t* row_start, uint32_t requests, const uint32_t* ids,
+                           const HypSamplingConfig* configs, const HypSamplingConfig* draft_configs, const float* uniforms,
+                           uint32_t* accepted, uint32_t* rejected, uint32_t* tokens, float* logprobs, void* workspace,
+                           size_t workspace_bytes, HypStream stream);
+/* The workspace of hyp_verify_batch; drafted: 1 with draft_logits, 0 without (host only; a device need not be there). */
+HypStatus hyp_verify_batch_workspace(uint32_t rows, uint32_t vocab, uint32_t requests, int drafted, size_t* out_bytes);
 
 HypStatus hyp_step_result_create(HypStepResult* out_result);
 HypStatus hyp_step_result_free(HypStepResult* result);
