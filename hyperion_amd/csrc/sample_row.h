@@ -160,7 +160,8 @@ struct alignas(16) RowLds {
     double top, total, kept;       // the largest value, the tokens' mass, the kept tokens'
     uint32_t keep, rank;           // how many tokens the filters keep, the drawn one's rank
     uint32_t lead[kWaves];         // a wave's first bin with a token
-    uint32_t whole;                // find_cut: every token of the cut's value is kept
+    uint32_t whole;                // without a draw: every token of the last kept value is kept
+    uint32_t redo;                 // and: by windows after all
 };
 
 // s.count, s.infinite, s.centre_lo and s.centre_hi of the tokens [begin, end) of a row. (A call has a barrier at its end.)
@@ -356,7 +357,8 @@ __device__ __forceinline__ bool find_row(const uint16_t* row, uint32_t vocab, co
             return bin <= kFine ? kLow + (kFine - bin) : (bin == kCentre ? bits_at(s.centre_lo) : 0x8000u | (kLow + (bin - kCentre - 1u)));
         };
         // The long way's windows that hold values, and its largest value.
-        bool windowed = lead == kAbove || lead == kBelow || (s.count[kCentreAt] != 0u && s.centre_lo != s.centre_hi);
+        const bool centres = s.count[kCentreAt] != 0u && s.centre_lo != s.centre_hi;
+        bool windowed = lead == kAbove || lead == kBelow || (centres && (kDraw || lead == kCentre));
         if (!windowed && s.count[kBelowAt] != 0u)   // (2^23 times e^-80)
             windowed = !((value_of(fine_bits(lead)) + 128.0) * prm.by_t > 80.0);
         double top = 0.0;
@@ -378,7 +380,8 @@ __device__ __forceinline__ bool find_row(const uint16_t* row, uint32_t vocab, co
         };
         // (Written out for either way. For one row of 262144: 19.3 us so, 19.8 with one copy and a test at each step, 22.9
         // with one loop over the steps.)
-        // False where the cut is among the values below -2^7, so that one bin cannot tell where (e^-80 is above 2^-116).
+        // False where one bin cannot tell: the cut is among the values below -2^7 (e^-80 is above 2^-116) or next to 0, or
+        // several values next to 0, less than 2^-24 apart, weigh enough for that to matter to an fp64 sum.
         const auto find = [&](auto by_windows) HYP_INLINE {
             constexpr bool slow = decltype(by_windows)::value;
             uint32_t window = 0u;   // the first place of the window in hand
@@ -491,6 +494,17 @@ __device__ __forceinline__ bool find_row(const uint16_t* row, uint32_t vocab, co
                 const uint32_t below = s.count[kBelowAt];
                 if (below != 0u && ((kept > all - below && kept != all) || (prm.min_p != 0.0 && prm.min_p < 0x1p-110)))
                     return false;
+                if (centres) {
+                    uint32_t count = at.count;
+#pragma unroll
+                    for (uint32_t i = 0; i < kPer; ++i) {
+                        if (first + i == kCentre)
+                            s.redo = kept - 1u - count < num[i] || num[i] * weight[i] * prm.by_t > 0x1p-30 * total;
+                        count += num[i];
+                    }
+                    __syncthreads();
+                    if (s.redo != 0u) return false;
+                }
             }
             // The kept tokens' mass, the rank of the draw, its value.
             over_windows([&](double mass, uint32_t count) HYP_INLINE {
