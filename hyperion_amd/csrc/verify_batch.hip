@@ -6,14 +6,21 @@
 // first token along the index whose running sum exceeds u times the whole. So the accepted tokens and the drawn one are
 // distributed as tokens drawn from p one by one.
 //
-// Steps:
-//  1, 2. of every row of both models, what hyp_sample_batch counts and filters (sample_row.h), up to the last token that
-//     is kept: a row is then its largest logit, the kept and the whole mass, the last kept value and the last kept
-//     token of that value. With that any token's p follows from its logit alone;
-//  3. each request's stop row, by every workgroup for itself (a few loads), and the sums of max(0, p - q) over tiles of
-//     the vocabulary;
+// Steps, a launch each:
+//  1. every row of both models counted by value, in chunks (sample_row.h): the one pass over all logits;
+//  2. a workgroup a row: 32 neighbouring values to a thread, their weights, scans of mass and count, what the filters
+//     keep. A row is then its largest logit, the kept and the whole mass, the last kept value and the last kept token of
+//     that value: a token's p follows from its logit alone. And the probability of the row's draft;
+//  3. each request's stop row, by those probabilities, and the sums of max(0, p - q) over tiles of that row;
 //  4. a workgroup a request: the tile, then the token in it.
 // All weights and sums are fp64; tokens that p does not keep have no weight, so their exponentials are not formed.
+//
+// A row takes windows of 8192 values instead of its counts (step 2 over each, counting the row again) where the
+// counts' bins of more than one value matter: a value above 2^7; values next to 0 that hold the cut, or weigh enough that
+// their differences of less than 2^-24 do; values below -2^7 that are not negligible, or hold the cut.
+//
+// Steps 2 to 4 are bound by the instructions that all waves of a workgroup issue alike (scans, parameters, borders): with 16 waves
+// each is 16 cycles, so they have four, and loops over a thread's values are kept rolled.
 #include <algorithm>
 #include <cstdint>
 
@@ -21,18 +28,24 @@
 #include "common.h"
 #include "sample_row.h"
 #include "verify_batch.h"
+#include "wave.h"
 
 namespace hyperion::hip {
 namespace {
 
+#define HYP_INLINE __attribute__((always_inline))
+
 using namespace sampling;
 
-constexpr uint32_t kDrawThreads = 256;
-constexpr uint32_t kDrawWaves = kDrawThreads / 64u;
-constexpr uint32_t kTile = 8u * kDrawThreads;   // eight consecutive tokens a thread
-constexpr uint32_t kNoToken = 0xFFFFFFFFu;
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+constexpr uint32_t kFew = 256;              // threads of steps 2 to 4
+constexpr uint32_t kFewWaves = kFew / 64u;
+constexpr uint32_t kTile = 8u * kFew;       // eight consecutive tokens a thread
+constexpr uint32_t kLongest = 65024;         // tokens of a chunk: its counts are 16 bits
+static_assert((kMaxVocab + kLongest - 1u) / kLongest <= kFew, "a chunk to a thread");
 
-enum RowKind : uint32_t { kEmpty = 0, kFinite = 1, kInfinite = 2 };   // nothing above -inf; ...; +inf among the logits
+// Nothing above -inf; by the counts; by windows; +inf among the logits.
+enum RowKind : uint32_t { kEmpty = 0, kCounted = 1, kWindowed = 2, kInfinite = 3 };
 
 // A row and its filters.
 struct alignas(16) RowStat {
@@ -44,10 +57,14 @@ struct alignas(16) RowStat {
 struct VerifyParams {
     VerifyArgs a;
     Chunks chunks;
-    RowStat* stats;        // [rows], then those of the drafting model
-    double2* sums;         // [requests][tiles]: of max(0, p - q), of p
-    ChunkCounts* counts;   // [rows, then the drafting model's][chunks.n]
-    uint32_t tiles;
+    uint32_t tiles, groups;   // tiles of a row, workgroups of a request in step 3
+    // [rows], then those of the drafting model:
+    RowStat* stats;
+    double* chances;          // the draft's probability
+    float* shares;            // ln of its share before the filters
+    uint32_t* requests;       // whose row it is, kNone: of no use
+    ChunkCounts* counts;      // [chunks.n] each
+    double2* sums;            // [requests][tiles]: of max(0, p - q), of p
 };
 
 // The request whose rows hold row t < row_start[n]: the last r < n with row_start[r] <= t, by every wave for itself.
@@ -65,75 +82,49 @@ __device__ __forceinline__ uint32_t request_of(const uint32_t* row_start, uint32
     return lo;
 }
 
-// The row that a workgroup of the first two launches has, if it has one: nothing follows a request's last row, whose
-// drafting model's logits do not matter.
-struct Source {
-    const uint16_t* logits;
-    uint32_t request;
-    bool live, draft;
-};
-__device__ __forceinline__ Source source_of(const VerifyArgs& a, uint32_t index) {
-    Source s{nullptr, 0u, false, index >= a.rows};
-    const uint32_t row = s.draft ? index - a.rows : index;
-    if (row >= a.row_start[a.requests]) return s;
-    s.request = request_of(a.row_start, a.requests, row);
-    s.live = !s.draft || row + 1u < a.row_start[s.request + 1u];
-    s.logits = (s.draft ? a.draft_logits : a.logits) + static_cast<size_t>(row) * a.vocab;
-    return s;
+__device__ __forceinline__ const uint16_t* logits_of(const VerifyArgs& a, uint32_t index) {
+    return index < a.rows ? a.logits + static_cast<size_t>(index) * a.vocab
+                          : a.draft_logits + static_cast<size_t>(index - a.rows) * a.vocab;
 }
+
+// ---- 1. counts ----------------------------------------------------------------------------------
 
 __global__ __launch_bounds__(kThreads) void verify_count_kernel(VerifyParams p) {
     __shared__ RowLds s;
+    const VerifyArgs& a = p.a;
     const uint32_t index = blockIdx.x / p.chunks.n;
-    const Source src = source_of(p.a, index);
-    if (!src.live) return;
-    const uint32_t begin = min(p.a.vocab, (blockIdx.x - index * p.chunks.n) * p.chunks.tokens);
-    count_values(src.logits, begin, min(p.a.vocab, begin + p.chunks.tokens), s);
+    const uint32_t chunk = blockIdx.x - index * p.chunks.n;
+    // Rows of no request, and the drafting model's behind which nothing was drafted, are of no use.
+    const bool draft = index >= a.rows;
+    const uint32_t row = draft ? index - a.rows : index;
+    uint32_t request = kNone;
+    if (row < a.row_start[a.requests]) {
+        request = request_of(a.row_start, a.requests, row);
+        if (draft && row + 1u >= a.row_start[request + 1u]) request = kNone;
+    }
+    if (chunk == 0u && threadIdx.x == 0u) p.requests[index] = request;
+    if (request == kNone) return;
+    const uint32_t begin = min(a.vocab, chunk * p.chunks.tokens);
+    count_values(logits_of(a, index), begin, min(a.vocab, begin + p.chunks.tokens), s);
     store_counts(s, p.counts[blockIdx.x]);
 }
 
-template <bool kSplit>
-__global__ __launch_bounds__(kThreads) void verify_filter_kernel(VerifyParams p) {
-    __shared__ RowLds s;
-    const uint32_t index = blockIdx.x;
-    const Source src = source_of(p.a, index);
-    if (!src.live) return;
-    const RowParams prm = row_params((src.draft ? p.a.draft_configs : p.a.configs)[src.request], 0.0f);
-    const ChunkCounts* const counts = kSplit ? p.counts + static_cast<size_t>(index) * p.chunks.n : nullptr;
-    if constexpr (kSplit) {
-        sum_counts(counts, p.chunks.n, s);
-    } else {
-        count_values(src.logits, 0u, p.a.vocab, s);
-    }
-    const bool any = find_row<false>(src.logits, p.a.vocab, prm, s);
-    RowStat* const out = p.stats + index;
-    const auto leave = [&](uint32_t last) {
-        RowStat r{};
-        r.top = s.top;
-        r.by_t = prm.by_t;
-        r.by_kept = 1.0 / s.kept;
-        r.total = s.total;
-        r.cut = place_of(s.drawn);
-        r.last = last;
-        r.kind = s.infinite != 0u ? kInfinite : kFinite;
-        *out = r;
-    };
-    if (!any) {
-        if (threadIdx.x == 0u) *out = RowStat{};
-    } else if (s.whole != 0u) {
-        if (threadIdx.x == 0u) leave(p.a.vocab);
-    } else {
-        find_token<kSplit>(src.logits, p.a.vocab, p.chunks, counts, s, leave);
-    }
+// ---- 2. filters ---------------------------------------------------------------------------------
+
+// A value that all lanes have, in scalar registers.
+__device__ __forceinline__ double scalar(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = from_lane(static_cast<uint32_t>(b), 0u), hi = from_lane(static_cast<uint32_t>(b >> 32), 0u);
+    return __builtin_bit_cast(double, lo | hi << 32);
 }
 
 // The probability of a token from its logit.
 __device__ __forceinline__ double probability(const RowStat& r, uint32_t bits, uint32_t token) {
     bits = plain_bits(bits);
-    if (r.kind != kFinite) return r.kind == kInfinite && bits == 0x7F80u && token <= r.last ? r.by_kept : 0.0;
     const uint32_t place = place_of(bits);
-    if (!finite_bits(bits) || place > r.cut || (place == r.cut && token > r.last)) return 0.0;
-    return exp_below((value_of(bits) - r.top) * r.by_t) * r.by_kept;
+    if (r.kind == kEmpty || place > r.cut || (place == r.cut && token > r.last)) return 0.0;
+    if (r.kind == kInfinite) return bits == 0x7F80u ? r.by_kept : 0.0;
+    return finite_bits(bits) ? exp_below((value_of(bits) - r.top) * r.by_t) * r.by_kept : 0.0;
 }
 
 // ln of a token's share of the mass before the filters.
@@ -143,52 +134,555 @@ __device__ __forceinline__ float log_share(const RowStat& r, uint32_t bits) {
     return static_cast<float>(gap - log(r.total));
 }
 
+// Inclusive sums in thread order and the whole. (Every wave has left `waves`; a call has a barrier at its end.)
+template <typename T>
+struct Scan {
+    T incl, all;
+};
+template <typename T>
+__device__ __forceinline__ Scan<T> few_scan(T v, T* waves) {
+    const uint32_t wave = threadIdx.x >> 6;
+    T incl;
+    if constexpr (sizeof(T) == 8u) incl = wave_incl64(v); else incl = wave_incl(v);
+    if ((threadIdx.x & 63u) == 63u) waves[wave] = incl;
+    __syncthreads();
+    T before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kFewWaves; ++w) {
+        if (w == wave) before = all;
+        all += waves[w];
+    }
+    __syncthreads();
+    return {before + incl, all};
+}
+__device__ __forceinline__ uint32_t few_min(uint32_t v, uint32_t* waves) {
+    v = from_lane(wave_scan(v, kNone, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);
+    if ((threadIdx.x & 63u) == 0u) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kFewWaves; ++w) v = min(v, waves[w]);
+    __syncthreads();
+    return v;
+}
+
+// The 32 bins of a thread, neighbours in one binade and so equally far apart, in an order that gives the threads' in
+// descending order of values.
+constexpr uint32_t kBinsEach = kWindow / kFew;
+__device__ __forceinline__ uint32_t bin_of(uint32_t tid, uint32_t i) {
+    return tid < kFew / 2u ? kFine - 1u - (kBinsEach * tid + i) : kBinsEach * tid + i;
+}
+__device__ __forceinline__ uint32_t bits_of_bin(uint32_t tid, uint32_t i) {
+    const uint32_t at = bin_of(tid, i);
+    return (at & 0xFFFu) + kLow + ((at & 0x1000u) << 3);
+}
+static_assert(2u * kFine == kWindow && kFine == 0x1000u && 128u % kBinsEach == 0u, "a thread's fine values");
+
+// e^((x - top) by_t) of those: the first one's, and from one to the next a factor, so that each is right to a few fp64
+// roundings. (An exponential for each took five times as long.) The largest value's is 1 exactly, as min-p may be; those
+// above it mean nothing.
+struct Weights {
+    double w, step;
+    uint32_t at_top;   // which of them is the largest value
+    __device__ __forceinline__ Weights(uint32_t tid, double top, double by_t) : w(0.0), step(0.0) {
+        const double x = value_of(bits_of_bin(tid, 0u));
+        const double apart = x - value_of(bits_of_bin(tid, 1u));
+        const double which = (x - top) / apart;
+        at_top = which >= 0.0 && which < kBinsEach ? static_cast<uint32_t>(which) : kBinsEach;
+#pragma unroll 1
+        for (uint32_t k = 0; k < 2u; ++k) {   // (the code of one exponential)
+            const double v = exp_below((k == 0u ? x - top : -apart) * by_t);
+            if (k == 0u) w = v; else step = v;
+        }
+        if (at_top == 0u) w = 1.0;
+    }
+    __device__ __forceinline__ void next(uint32_t i) { w = i + 1u == at_top ? 1.0 : w * step; }   // from i to the one after
+};
+
+constexpr uint32_t kSlots = 1u + kBinsEach;   // values of a thread: those next to 0 (thread 128's), its bins
+constexpr uint32_t kCentreThread = kFew / 2u;
+constexpr uint32_t kRow = kFew + 1u;            // (four lanes that store slots of one thread do not meet in a bank)
+
+struct FilterLds {
+    double mass[kFewWaves], kept;        // ..., mass of the kept tokens
+    uint32_t word[kFewWaves];
+    uint32_t count[kSlots * kRow];       // of slot i of thread t at i * kRow + t; by value, of a window
+    uint32_t infinite, centre_lo, centre_hi, centre, above, below;
+    uint32_t lead;                       // kBinsEach * thread + i of the first bin with a token
+    uint32_t keep, redo;
+    uint32_t cut, number, whole;         // bits of the last kept value, the last kept token's number there, are all kept
+    uint32_t last;
+};
+
+// The filters of a row from its counts in s: leaves s.kept, s.cut, s.number, s.whole and the mass of all tokens. False: the
+// row takes windows. (A call has a barrier at its end.)
+__device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, FilterLds& s, double& total) {
+    const uint32_t tid = threadIdx.x;
+    const uint32_t lane = tid & 63u;
+    const uint32_t centre = s.count[tid];
+    double centre_weight = 0.0, sum = 0.0;
+    uint32_t here = centre;
+    bool light = false;   // min-p drops some
+    if (centre != 0u) {
+        centre_weight = exp_below((value_of(bits_at(s.centre_lo)) - top) * prm.by_t);
+        sum = centre * centre_weight;
+        light = centre_weight < prm.min_p;
+    }
+    {
+        Weights e(tid, top, prm.by_t);
+#pragma unroll 1
+        for (uint32_t base = 0; base < kBinsEach; base += 8u) {
+            uint32_t n[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) n[i] = s.count[(base + i + 1u) * kRow + tid];
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+                sum += n[i] * e.w;
+                here += n[i];
+                light = light || (n[i] != 0u && e.w < prm.min_p);
+                e.next(base + i);
+            }
+        }
+    }
+    const Scan<double> mass_at = few_scan(sum, s.mass);
+    const Scan<uint32_t> count_at = few_scan(here, s.word);
+    const double mass_before = mass_at.incl - sum;
+    const uint32_t count_before = count_at.incl - here;
+    total = scalar(mass_at.all);
+    const uint32_t all = count_at.all + s.below;   // (those weigh nothing)
+    uint32_t kept = all;
+    if (prm.top_k != 0u) kept = min(kept, prm.top_k);
+    // The values of the thread of lane `from`, a slot to a lane: tokens, weight, and what comes before.
+    struct One {
+        uint32_t n, before, bits;
+        double w, mass;   // (mass: before)
+    };
+    const auto spread = [&](uint32_t from) HYP_INLINE {
+        One o{0u, 0u, 0u, 0.0, 0.0};
+        const uint32_t thread = (tid & ~63u) + from;
+        if (lane < kSlots) {
+            o.n = s.count[lane * kRow + thread];
+            o.bits = lane == 0u ? bits_at(s.centre_lo & 0xFFFFu) : bits_of_bin(thread, lane - 1u);
+            if (o.n != 0u) o.w = exp_below((value_of(o.bits) - top) * prm.by_t);
+        }
+        const double m = o.n * o.w;
+        const uint64_t before = __builtin_bit_cast(uint64_t, mass_before);
+        const uint64_t lo = from_lane(static_cast<uint32_t>(before), from), hi = from_lane(static_cast<uint32_t>(before >> 32), from);
+        o.mass = __builtin_bit_cast(double, lo | hi << 32) + (wave_incl64(m) - m);
+        o.before = from_lane(count_before, from) + (wave_incl(o.n) - o.n);
+        return o;
+    };
+    if (prm.top_p != 0.0 || prm.min_p != 0.0) {
+        // Of each wave the first lane whose values a filter does not keep whole.
+        const double enough = prm.top_p * total;
+        const uint64_t past = __ballot((prm.top_p != 0.0 && mass_at.incl > enough) || light);
+        if (past != 0u) {
+            const One o = spread(static_cast<uint32_t>(__builtin_ctzll(past)));
+            const bool dropped = o.n != 0u && o.w < prm.min_p;
+            const bool full = o.n != 0u && prm.top_p != 0.0 && o.n * o.w > enough - o.mass;
+            uint32_t some = 0u;   // (kept are the tokens before which the running sum is below)
+            if (!dropped && full && enough > o.mass) some = min(o.n, static_cast<uint32_t>(ceil((enough - o.mass) / o.w)));
+            const uint64_t ends = __ballot(dropped || full);
+            if (ends != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(ends))) atomicMin(&s.keep, o.before + some);
+        }
+        __syncthreads();
+        kept = min(kept, s.keep);
+    }
+    if (s.below != 0u) {
+        // Nothing there weighs enough for top-p; min-p drops it unless it is tiny: e^-80 is above 2^-116.
+        if (prm.min_p != 0.0) kept = min(kept, count_at.all);
+        if ((kept > count_at.all && kept != all) || (prm.min_p != 0.0 && prm.min_p < 0x1p-110)) return false;
+    }
+    kept = prm.greedy ? 1u : max(kept, 1u);
+    if (centre != 0u && s.centre_lo != s.centre_hi)   // several values next to 0
+        s.redo = kept - 1u - count_before < centre || centre * centre_weight * prm.by_t > 0x1p-30 * total;
+    const uint64_t holds = __ballot(kept - 1u - count_before < here);
+    if (holds != 0u) {
+        const One o = spread(static_cast<uint32_t>(__builtin_ctzll(holds)));
+        if (kept - 1u - o.before < o.n) {
+            s.kept = o.mass + (kept - o.before) * o.w;
+            s.cut = o.bits;
+            s.number = kept - 1u - o.before;
+            s.whole = kept - o.before == o.n;
+        }
+    }
+    if (kept == all && s.below != 0u && tid == 0u) {   // everything
+        s.kept = total;
+        s.cut = 0xFF7Fu;
+        s.number = 0u;
+        s.whole = 1u;
+    }
+    __syncthreads();
+    return s.redo == 0u;
+}
+
+// The same for a row by windows. (A call has a barrier at its end.)
+__device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t vocab, const RowParams& prm, RowStat& r, FilterLds& s) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t best = kNone, held = 0u, windows = 0u;
+    for_tokens(row, 0u, vocab, tid, kFew, [&](uint32_t, uint32_t b) HYP_INLINE {
+        b = plain_bits(b);
+        if (!finite_bits(b)) return;
+        best = min(best, place_of(b));
+        held |= 1u << (place_of(b) / kWindow);
+    });
+    best = few_min(best, s.word);
+    for (uint32_t w = 0; w < kWindows; ++w)
+        if (few_min((held >> w) & 1u ? 0u : 1u, s.word) == 0u) windows |= 1u << w;
+    r.top = scalar(value_of(bits_at(best)));
+    uint32_t kept = kNone;
+    // Step 0: the mass and number of all tokens; 1: what top-p and min-p keep; 2: the last kept one.
+#pragma unroll 1
+    for (uint32_t step = 0; step < 3u; ++step) {
+        double mass_all = 0.0;
+        uint32_t count_all = 0u;
+#pragma unroll 1
+        for (uint32_t k = 0; k < kWindows; ++k) {
+            if (((windows >> k) & 1u) == 0u) continue;
+            const uint32_t window = k * kWindow;
+            __syncthreads();
+            for (uint32_t i = tid; i < kWindow; i += kFew) s.count[i] = 0u;
+            __syncthreads();
+            for_tokens(row, 0u, vocab, tid, kFew, [&](uint32_t, uint32_t b) HYP_INLINE {
+                b = plain_bits(b);
+                const uint32_t d = place_of(b) - window;
+                if (finite_bits(b) && d < kWindow) atomicAdd(&s.count[d], 1u);
+            });
+            __syncthreads();
+            const auto weight = [&](uint32_t i) HYP_INLINE {
+                return exp_below((value_of(bits_at(window + kBinsEach * tid + i)) - r.top) * r.by_t);
+            };
+            double sum = 0.0;
+            uint32_t here = 0u;
+#pragma unroll 1
+            for (uint32_t i = 0; i < kBinsEach; ++i) {
+                const uint32_t n = s.count[kBinsEach * tid + i];
+                if (n != 0u) sum += n * weight(i);
+                here += n;
+            }
+            const Scan<double> mass_at = few_scan(sum, s.mass);
+            const Scan<uint32_t> count_at = few_scan(here, s.word);
+            double mass = mass_all + (mass_at.incl - sum);
+            uint32_t count = count_all + (count_at.incl - here);
+            if (step == 1u && here != 0u) {
+                const double enough = prm.top_p * r.total;
+                bool open = true;
+#pragma unroll 1
+                for (uint32_t i = 0; i < kBinsEach && open; ++i) {
+                    const uint32_t n = s.count[kBinsEach * tid + i];
+                    if (n == 0u) continue;
+                    const double w = weight(i);
+                    const bool dropped = w < prm.min_p;
+                    const bool full = prm.top_p != 0.0 && n * w > enough - mass;
+                    open = !dropped && !full;
+                    if (open) count += n;
+                    else if (!dropped && enough > mass) count += min(n, static_cast<uint32_t>(ceil((enough - mass) / w)));
+                    mass += n * w;
+                }
+                if (!open) atomicMin(&s.keep, count);
+            }
+            if (step == 2u && kept - 1u - count < here) {
+#pragma unroll 1
+                for (uint32_t i = 0; i < kBinsEach; ++i) {
+                    const uint32_t n = s.count[kBinsEach * tid + i];
+                    const double w = n != 0u ? weight(i) : 0.0;
+                    if (kept - 1u - count < n) {
+                        s.kept = mass + (kept - count) * w;
+                        s.cut = bits_at(window + kBinsEach * tid + i);
+                        s.number = kept - 1u - count;
+                        s.whole = kept - count == n;
+                    }
+                    mass += n * w;
+                    count += n;
+                }
+            }
+            mass_all += mass_at.all;
+            count_all += count_at.all;
+        }
+        __syncthreads();
+        if (step == 0u) {
+            r.total = scalar(mass_all);
+            kept = count_all;
+            if (prm.top_k != 0u) kept = min(kept, prm.top_k);
+            if (tid == 0u) s.keep = kNone;
+        } else if (step == 1u) {
+            kept = min(kept, s.keep);
+            kept = prm.greedy ? 1u : max(kept, 1u);
+        }
+        __syncthreads();
+    }
+}
+
+// The index of the number-th token of value `bits` among the tokens [begin, end) of a row, in s.last. Each wave marks the value's
+// places in its stretch, 512 tokens a step. (A call has a barrier at its end.)
+__device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, uint32_t end, uint32_t bits, uint32_t number,
+                                          FilterLds& s) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = threadIdx.x >> 6;
+    constexpr uint32_t kStep = 512u, kSteps = 16u;
+#pragma unroll 1
+    for (uint32_t base = begin; base < end; base += kFewWaves * kSteps * kStep) {
+        const uint32_t stop = min(end, base + kFewWaves * kSteps * kStep);
+        const uint32_t steps = (stop - base + kFewWaves * kStep - 1u) / (kFewWaves * kStep);
+        const uint32_t first = base + wave * steps * kStep + 8u * lane;   // the lane's, of the first step
+        uint32_t hits[kSteps / 4u] = {};   // a byte a step
+        uint32_t mine = 0u;
+#pragma unroll
+        for (uint32_t q = 0; q < kSteps / 4u; ++q) {
+            if (4u * q >= steps) continue;
+            Eight e[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint32_t from = first + (4u * q + k) * kStep;
+                if (from + 8u <= stop) __builtin_memcpy(&e[k], row + from, 16);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint32_t from = first + (4u * q + k) * kStep;
+                uint32_t hit = 0u;
+                if (4u * q + k < steps && from + 8u <= stop) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) hit |= plain_bits(e[k].v[i]) == bits ? 1u << i : 0u;
+                } else if (4u * q + k < steps && from < stop) {
+#pragma unroll 1
+                    for (uint32_t i = 0; from + i < stop; ++i) hit |= plain_bits(row[from + i]) == bits ? 1u << i : 0u;
+                }
+                hits[q] |= hit << (8u * k);
+            }
+            mine += static_cast<uint32_t>(__popc(hits[q]));
+        }
+        const uint32_t wave_all = wave_sum(mine);
+        if (lane == 0u) s.word[wave] = wave_all;
+        __syncthreads();
+        uint32_t before = 0u, all = 0u;
+#pragma unroll
+        for (uint32_t w = 0; w < kFewWaves; ++w) {
+            if (w == wave) before = all;
+            all += s.word[w];
+        }
+        __syncthreads();
+        if (number >= all) {
+            number -= all;
+            continue;
+        }
+        uint32_t left = number - before;   // (wraps past the holder)
+        if (left < wave_all) {
+#pragma unroll 1
+            for (uint32_t k = 0; k < steps; ++k) {
+                uint32_t hit = hits[0];
+#pragma unroll
+                for (uint32_t q = 1; q < kSteps / 4u; ++q) hit = k / 4u == q ? hits[q] : hit;
+                hit = (hit >> (8u * (k % 4u))) & 0xFFu;
+                const uint32_t n = static_cast<uint32_t>(__popc(hit));
+                const uint32_t incl = wave_incl(n);
+                const uint32_t step = from_lane(incl, 63u);
+                if (left < step) {
+                    if (left - (incl - n) < n) {
+                        for (uint32_t i = left - (incl - n); i != 0u; --i) hit &= hit - 1u;
+                        s.last = first + k * kStep + static_cast<uint32_t>(__builtin_ctz(hit));
+                    }
+                    break;
+                }
+                left -= step;
+            }
+        }
+        break;
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
+    __shared__ FilterLds s;
+    const VerifyArgs& a = p.a;
+    const uint32_t index = blockIdx.x;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t lane = tid & 63u;
+    const uint32_t row_at = index < a.rows ? index : index - a.rows;
+    const uint16_t* const row = logits_of(a, index);
+    const ChunkCounts* const counts = p.counts + static_cast<size_t>(index) * p.chunks.n;
+    const uint32_t request = p.requests[index];
+    const uint32_t x = row_at + 1u < a.rows ? a.ids[row_at + 1u] : kNone;   // the row's draft
+    if (tid == 0u) {
+        s.infinite = s.centre_hi = s.centre = s.above = s.below = s.redo = 0u;
+        s.centre_lo = s.lead = s.keep = kNone;
+    }
+    __syncthreads();
+    // The row's counts from its chunks', the other bins a chunk to a thread.
+    {
+        uint32_t more[6] = {0u, kNone, 0u, 0u, 0u, 0u};
+        if (tid < p.chunks.n) {
+            const ChunkCounts& c = counts[tid];
+            more[0] = c.infinite;
+            more[1] = c.centre_lo;
+            more[2] = c.centre_hi;
+            more[3] = c.count[kCentreAt];
+            more[4] = c.count[kAboveAt];
+            more[5] = c.count[kBelowAt];
+        }
+        // Eight bins in each quarter of them to a thread, which then go to the threads that have them.
+        uint32_t n[kBinsEach] = {};
+#pragma unroll 1
+        for (uint32_t c = 0; c < p.chunks.n; c += 4u) {
+            uint4 v[4][kBinsEach / 8u];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint4* const from = reinterpret_cast<const uint4*>(counts[c + k].count) + tid;
+#pragma unroll
+                for (uint32_t q = 0; q < kBinsEach / 8u; ++q) {
+                    v[k][q] = make_uint4(0u, 0u, 0u, 0u);
+                    if (c + k < p.chunks.n) v[k][q] = from[kFew * q];
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);   // (all of them on their way before the first is waited for)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+#pragma unroll
+                for (uint32_t q = 0; q < kBinsEach / 8u; ++q) {
+                    const uint32_t word[4] = {v[k][q].x, v[k][q].y, v[k][q].z, v[k][q].w};
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) {
+                        n[8u * q + 2u * j] += word[j] & 0xFFFFu;
+                        n[8u * q + 2u * j + 1u] += word[j] >> 16;
+                    }
+                }
+            }
+        }
+        uint32_t first = kNone;
+#pragma unroll
+        for (uint32_t q = 0; q < kBinsEach / 8u; ++q) {
+            const uint32_t bin = 8u * (kFew * q + tid);
+            // (its place in descending order: positive values are stored ascending)
+            const uint32_t place = bin < kFine ? kFine - 1u - bin : bin;
+            const uint32_t thread = place / kBinsEach, slot = 1u + place % kBinsEach;
+            uint32_t* const to = &s.count[slot * kRow + thread];
+            uint32_t lead = kNone;
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+                to[static_cast<int>(q < kBinsEach / 16u ? -static_cast<int>(i) : static_cast<int>(i)) * static_cast<int>(kRow)] = n[8u * q + i];
+                if (n[8u * q + i] != 0u && (lead == kNone || q < kBinsEach / 16u))
+                    lead = q < kBinsEach / 16u ? place - i : place + i;
+            }
+            first = min(first, lead);
+        }
+        first = from_lane(wave_scan(first, kNone, [](uint32_t x_, uint32_t y_) { return min(x_, y_); }), 63u);
+        if (lane == 0u) atomicMin(&s.lead, first);
+        if (tid < p.chunks.n) {
+            if (more[0] != 0u) atomicAdd(&s.infinite, more[0]);
+            atomicMin(&s.centre_lo, more[1]);
+            atomicMax(&s.centre_hi, more[2]);
+            atomicAdd(&s.centre, more[3]);
+            atomicAdd(&s.above, more[4]);
+            atomicAdd(&s.below, more[5]);
+        }
+    }
+    if (request == kNone) return;
+    RowParams prm = row_params((index < a.rows ? a.configs : a.draft_configs)[request], 0.0f);
+    prm.by_t = scalar(prm.by_t);
+    prm.top_p = scalar(prm.top_p);
+    prm.min_p = scalar(prm.min_p);
+    __syncthreads();
+    s.count[tid] = tid == kCentreThread ? s.centre : 0u;   // (this thread's alone)
+    RowStat r{};
+    r.by_t = prm.by_t;
+    if (s.infinite != 0u) {
+        // Weight 1 for each, 0 for everything else.
+        const uint32_t infinite = s.infinite;
+        uint32_t kept = infinite;
+        if (prm.top_k != 0u) kept = min(kept, prm.top_k);
+        if (prm.top_p != 0.0) kept = min(kept, static_cast<uint32_t>(ceil(prm.top_p * infinite)));
+        if (prm.greedy || prm.min_p > 1.0) kept = 1u;
+        if (tid == 0u) {
+            s.kept = kept;
+            s.cut = 0x7F80u;
+            s.number = kept - 1u;
+            s.whole = kept == infinite;
+        }
+        r.kind = kInfinite;
+        r.total = infinite;
+        __syncthreads();
+    } else if (s.lead != kNone || s.centre != 0u || s.above != 0u || s.below != 0u) {
+        const uint32_t lead = s.lead;
+        const bool next_to_0 = s.centre != 0u && lead >= kFine;   // the largest
+        bool counted = s.above == 0u && (next_to_0 ? s.centre_lo == s.centre_hi : lead != kNone);
+        r.top = scalar(value_of(next_to_0 ? bits_at(s.centre_lo) : bits_of_bin((lead / kBinsEach) % kFew, lead % kBinsEach)));
+        if (counted && s.below != 0u) counted = (r.top + 128.0) * prm.by_t > 80.0;   // (2^23 times e^-80)
+        if (counted) counted = filter_counts(prm, r.top, s, r.total);
+        r.kind = counted ? kCounted : kWindowed;
+        if (!counted) filter_windows(row, a.vocab, prm, r, s);
+    }
+    if (r.kind != kEmpty) {
+        r.by_kept = 1.0 / s.kept;
+        r.cut = place_of(s.cut);
+        r.last = a.vocab;
+        if (s.whole == 0u) {   // some of the last kept value's tokens are dropped
+            uint32_t number = s.number, begin = 0u, end = a.vocab;
+            if (r.kind == kCounted) {
+                const uint32_t t = s.cut - kLow;   // (the place of its count, as count_values has it)
+                const uint32_t at = (t & 0x7000u) == 0u ? (t & 0xFFFu) | ((t >> 3) & 0x1000u) : kCentreAt;
+                begin = min(a.vocab, find_chunk(counts, p.chunks.n, at, number) * p.chunks.tokens);
+                end = min(a.vocab, begin + p.chunks.tokens);
+            }
+            find_last(row, begin, end, s.cut, number, s);
+            r.last = s.last;
+        }
+    }
+    // The draft of a target's row follows every row but a request's last (whose next row is another request's).
+    if (tid == 0u) {
+        p.stats[index] = r;
+        const bool there = x < a.vocab;
+        const uint32_t bits = there ? row[x] : 0u;
+        p.chances[index] = there ? probability(r, bits, x) : 0.0;
+        if (index < a.rows) p.shares[index] = there ? log_share(r, bits) : 0.0f;
+    }
+}
+
+// ---- 3, 4. the stop row and its draw ------------------------------------------------------------
+
 __device__ __forceinline__ double uniform_of(float u) {   // as a draw takes it
     return u > 0.0f ? static_cast<double>(fminf(u, 0x1.fffffep-1f)) : 0.0;
 }
 
-// Where a request stops.
+// Where a request stops: the first row whose draft is not accepted, or the last.
 struct Stop {
     uint32_t first, rows, accepted;
     [[nodiscard]] __device__ uint32_t row() const { return first + accepted; }
     [[nodiscard]] __device__ bool rejects() const { return accepted + 1u < rows; }
 };
 
-// By a whole workgroup; `least` is a word of its LDS. (A call has a barrier at its end.)
-__device__ __forceinline__ Stop find_stop(const VerifyParams& p, uint32_t request, uint32_t& least) {
+// By every wave for itself.
+__device__ __forceinline__ Stop find_stop(const VerifyParams& p, uint32_t request) {
     const VerifyArgs& a = p.a;
+    const uint32_t lane = threadIdx.x & 63u;
     const uint32_t first = min(a.row_start[request], a.rows);
     const uint32_t end = min(a.row_start[request + 1u], a.rows);
     const uint32_t rows = end > first ? end - first : 0u;
-    if (threadIdx.x == 0u) least = rows != 0u ? rows - 1u : 0u;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i + 1u < rows; i += kDrawThreads) {
-        const uint32_t row = first + i;
-        const uint32_t x = a.ids[row + 1u];
-        bool taken = false;
-        if (x < a.vocab) {
-            const size_t at = static_cast<size_t>(row) * a.vocab + x;
-            const double q = a.draft_logits != nullptr ? probability(p.stats[a.rows + row], a.draft_logits[at], x) : 1.0;
-            taken = uniform_of(a.uniforms[row]) * q < probability(p.stats[row], a.logits[at], x);
+    uint32_t accepted = rows != 0u ? rows - 1u : 0u;
+#pragma unroll 1
+    for (uint32_t base = 0; base + 1u < rows; base += 64u) {
+        const uint32_t i = base + lane;
+        bool falls = false;
+        if (i + 1u < rows) {
+            const uint32_t row = first + i;
+            const double q = a.draft_logits != nullptr ? p.chances[a.rows + row] : 1.0;
+            falls = !(uniform_of(a.uniforms[row]) * q < p.chances[row]);   // (a draft outside the vocabulary: 0 < 0)
         }
-        if (!taken) {
-            atomicMin(&least, i);
+        const uint64_t fallen = __ballot(falls);
+        if (fallen != 0u) {
+            accepted = base + static_cast<uint32_t>(__builtin_ctzll(fallen));
             break;
         }
     }
-    __syncthreads();
-    return {first, rows, least};
+    return {first, rows, accepted};
 }
 
-// max(0, p - q) and p of a tile's eight tokens of this thread, at the stop row.
+// max(0, p - q) and p of tokens of the stop row.
 struct Rest {
     const uint16_t* logits;
     const uint16_t* draft_logits;   // null: q is 1 at `without` and 0 elsewhere
     RowStat p, q;
     uint32_t without, vocab;
-    __device__ Rest(const VerifyParams& v, const Stop& stop)
+    __device__ __forceinline__ Rest(const VerifyParams& v, const Stop& stop)
         : logits(v.a.logits + static_cast<size_t>(stop.row()) * v.a.vocab), draft_logits(nullptr), p(v.stats[stop.row()]), q{},
-          without(kNoToken), vocab(v.a.vocab) {
+          without(kNone), vocab(v.a.vocab) {
         if (!stop.rejects()) return;
         if (v.a.draft_logits != nullptr) {
             draft_logits = v.a.draft_logits + static_cast<size_t>(stop.row()) * vocab;
@@ -197,7 +691,7 @@ struct Rest {
             without = v.a.ids[stop.row() + 1u];
         }
     }
-    // f(k, max(0, p - q), p) for the tokens begin + k, k < 8, that there are.
+    // f(k, max(0, p - q), p) for the tokens begin + k, k < 8, that p keeps.
     template <typename F>
     __device__ __forceinline__ void each(uint32_t begin, F&& f) const {
         Eight x, y;
@@ -214,93 +708,89 @@ struct Rest {
 #pragma unroll
         for (uint32_t k = 0; k < 8u; ++k) {
             const double here = probability(p, x.v[k], begin + k);
+            if (!(here > 0.0)) continue;
             double rest = here;
-            if (here > 0.0) {
-                if (draft_logits != nullptr) rest = fmax(0.0, here - probability(q, y.v[k], begin + k));
-                if (begin + k == without) rest = 0.0;
-            }
+            if (draft_logits != nullptr) rest = fmax(0.0, here - probability(q, y.v[k], begin + k));
+            if (begin + k == without) rest = 0.0;
             f(k, rest, here);
         }
     }
 };
 
-// Exclusive sums in thread order and the whole, by a workgroup of kDrawThreads. (Every wave has left `waves`.)
-struct DrawScan {
-    double incl, all;
-};
-__device__ __forceinline__ DrawScan draw_scan(double v, double* waves) {
-    const uint32_t wave = threadIdx.x >> 6;
-    double incl = wave_incl64(v);
-    if ((threadIdx.x & 63u) == 63u) waves[wave] = incl;
-    __syncthreads();
-    double all = 0.0;
-    for (uint32_t w = 0; w < kDrawWaves; ++w) {
-        if (w == wave) incl += all;
-        all += waves[w];
-    }
-    __syncthreads();
-    return {incl, all};
-}
-
-__global__ __launch_bounds__(kDrawThreads) void verify_sum_kernel(VerifyParams p, uint32_t groups) {
-    __shared__ uint32_t least;
-    __shared__ double waves[kDrawWaves];
-    const uint32_t request = blockIdx.x / groups;
-    const Stop stop = find_stop(p, request, least);
+// The sums of max(0, p - q) and of p over the tiles of each request's stop row: `groups` workgroups to each.
+__global__ __launch_bounds__(kFew) void verify_sum_kernel(VerifyParams p) {
+    __shared__ double waves[2][kFewWaves];
+    const uint32_t tid = threadIdx.x;
+    const uint32_t request = blockIdx.x / p.groups;
+    const Stop stop = find_stop(p, request);
     if (stop.rows == 0u) return;
     const Rest rest(p, stop);
-    for (uint32_t tile = blockIdx.x - request * groups; tile < p.tiles; tile += groups) {
+#pragma unroll 1
+    for (uint32_t tile = blockIdx.x - request * p.groups; tile < p.tiles; tile += p.groups) {
         double r_sum = 0.0, p_sum = 0.0;
-        rest.each(tile * kTile + 8u * threadIdx.x, [&](uint32_t, double r, double here) {
+        rest.each(tile * kTile + 8u * tid, [&](uint32_t, double r, double here) HYP_INLINE {
             r_sum += r;
             p_sum += here;
         });
-        const double r_all = draw_scan(r_sum, waves).all;
-        const double p_all = draw_scan(p_sum, waves).all;
-        if (threadIdx.x == 0u) p.sums[static_cast<size_t>(request) * p.tiles + tile] = make_double2(r_all, p_all);
+        const bool some = __ballot(p_sum != 0.0) != 0u;
+        if (some) {
+            r_sum = wave_incl64(r_sum);
+            p_sum = wave_incl64(p_sum);
+        }
+        __syncthreads();
+        if ((tid & 63u) == 63u) {
+            waves[0][tid >> 6] = r_sum;
+            waves[1][tid >> 6] = p_sum;
+        }
+        __syncthreads();
+        if (tid == 0u) {
+            double2 sum = make_double2(0.0, 0.0);
+#pragma unroll
+            for (uint32_t w = 0; w < kFewWaves; ++w) {
+                sum.x += waves[0][w];
+                sum.y += waves[1][w];
+            }
+            p.sums[static_cast<size_t>(request) * p.tiles + tile] = sum;
+        }
     }
 }
 
+struct DrawLds {
+    double mass[kFewWaves];
+    double base;
+    uint32_t pick[2], tile;
+};
+
 // The first thread with v > 0 whose inclusive sum exceeds the goal, or the last with v > 0 (rounding can leave none
-// above); kDrawThreads where no v is above 0. pick[0] and pick[1] are words of LDS.
-__device__ __forceinline__ uint32_t draw_thread(double v, double incl, double goal, uint32_t* pick) {
-    const uint32_t tid = threadIdx.x;
-    if (tid == 0u) {
-        pick[0] = kDrawThreads;
-        pick[1] = 0u;
+// above); kNone where no v is above 0. (A call has a barrier at its end.)
+__device__ __forceinline__ uint32_t draw_thread(double v, double incl, double goal, DrawLds& s) {
+    if (threadIdx.x == 0u) {
+        s.pick[0] = kNone;
+        s.pick[1] = 0u;
     }
     __syncthreads();
-    if (v > 0.0) {
-        if (incl > goal) atomicMin(&pick[0], tid);
-        atomicMax(&pick[1], tid + 1u);
+    const uint64_t some = __ballot(v > 0.0);
+    const uint64_t past = __ballot(v > 0.0 && incl > goal);
+    const uint32_t first = threadIdx.x & ~63u;
+    if ((threadIdx.x & 63u) == 0u) {
+        if (past != 0u) atomicMin(&s.pick[0], first + static_cast<uint32_t>(__builtin_ctzll(past)));
+        if (some != 0u) atomicMax(&s.pick[1], first + 64u - static_cast<uint32_t>(__builtin_clzll(some)));
     }
     __syncthreads();
-    const uint32_t got = pick[0] != kDrawThreads ? pick[0] : (pick[1] != 0u ? pick[1] - 1u : kDrawThreads);
+    const uint32_t got = s.pick[0] != kNone ? s.pick[0] : (s.pick[1] != 0u ? s.pick[1] - 1u : kNone);
     __syncthreads();
     return got;
 }
 
-__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams p) {
-    __shared__ uint32_t least, pick[2], tile_at;
-    __shared__ double waves[kDrawWaves], before_tile;
+// A workgroup a request: accepted, rejected, the logprobs, and the token.
+__global__ __launch_bounds__(kFew) void verify_draw_kernel(VerifyParams p) {
+    __shared__ DrawLds s;
+    const VerifyArgs& a = p.a;
     const uint32_t tid = threadIdx.x;
     const uint32_t request = blockIdx.x;
-    const VerifyArgs& a = p.a;
-    const Stop stop = find_stop(p, request, least);
-    if (tid == 0u) {
-        a.accepted[request] = stop.accepted;
-        a.rejected[request] = stop.rejects() ? stop.rows - 1u - stop.accepted : 0u;
-    }
-    if (stop.rows == 0u) return;
-    if (a.logprobs != nullptr) {
-        for (uint32_t i = tid; i < stop.accepted; i += kDrawThreads) {
-            const uint32_t row = stop.first + i;
-            a.logprobs[row] = log_share(p.stats[row], a.logits[static_cast<size_t>(row) * a.vocab + a.ids[row + 1u]]);
-        }
-    }
-    // The tile: consecutive ones to a thread.
+    // The sums of the request's tiles: consecutive ones to a thread.
     const double2* const sums = p.sums + static_cast<size_t>(request) * p.tiles;
-    const uint32_t per = (p.tiles + kDrawThreads - 1u) / kDrawThreads;
+    const uint32_t per = (p.tiles + kFew - 1u) / kFew;
     const uint32_t begin = min(tid * per, p.tiles);
     const uint32_t end = min(begin + per, p.tiles);
     double r_sum = 0.0, p_sum = 0.0;
@@ -308,14 +798,26 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
         r_sum += sums[t].x;
         p_sum += sums[t].y;
     }
-    const DrawScan r_scan = draw_scan(r_sum, waves);
-    const DrawScan p_scan = draw_scan(p_sum, waves);
-    const bool by_rest = r_scan.all > 0.0;
-    const double mine = by_rest ? r_sum : p_sum;
-    const DrawScan scan = by_rest ? r_scan : p_scan;
-    const double goal = uniform_of(a.uniforms[stop.first + stop.rows - 1u]) * scan.all;
-    const uint32_t holder = draw_thread(mine, scan.incl, goal, pick);
-    if (holder == kDrawThreads) {   // nothing above -inf
+    const Stop stop = find_stop(p, request);
+    if (tid == 0u) {
+        a.accepted[request] = stop.accepted;
+        a.rejected[request] = stop.rejects() ? stop.rows - 1u - stop.accepted : 0u;
+    }
+    if (stop.rows == 0u) return;
+    if (a.logprobs != nullptr)
+        for (uint32_t i = tid; i < stop.accepted; i += kFew) a.logprobs[stop.first + i] = p.shares[stop.first + i];
+    const double u = uniform_of(a.uniforms[stop.first + stop.rows - 1u]);
+    const Rest rest(p, stop);
+    Scan<double> scan = few_scan(r_sum, s.mass);
+    const bool by_rest = scan.all > 0.0;
+    double mine = r_sum;
+    if (!by_rest) {
+        scan = few_scan(p_sum, s.mass);
+        mine = p_sum;
+    }
+    const double goal = u * scan.all;
+    const uint32_t holder = draw_thread(mine, scan.incl, goal, s);
+    if (holder == kNone) {   // nothing above -inf
         if (tid == 0u) {
             a.tokens[request] = 0u;
             if (a.logprobs != nullptr) a.logprobs[stop.row()] = -__builtin_huge_valf();
@@ -335,20 +837,20 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
             }
             sum += v;
         }
-        tile_at = at;
-        before_tile = before;
+        s.tile = at;
+        s.base = before;
     }
     __syncthreads();
-    const Rest rest(p, stop);
-    const uint32_t from = tile_at * kTile + 8u * tid;
-    double v[8], sum = 0.0;
-    rest.each(from, [&](uint32_t k, double r, double here) {
+    const uint32_t from = s.tile * kTile + 8u * tid;
+    const double base = s.base;
+    double v[8] = {}, sum = 0.0;
+    rest.each(from, [&](uint32_t k, double r, double here) HYP_INLINE {
         v[k] = by_rest ? r : here;
         sum += v[k];
     });
-    const DrawScan in_tile = draw_scan(sum, waves);
-    if (tid != draw_thread(sum, before_tile + in_tile.incl, goal, pick)) return;
-    double running = before_tile + (in_tile.incl - sum);
+    const Scan<double> in_tile = few_scan(sum, s.mass);
+    if (tid != draw_thread(sum, base + in_tile.incl, goal, s)) return;
+    double running = base + (in_tile.incl - sum);
     uint32_t token = from;
     bool found = false;
 #pragma unroll
@@ -363,21 +865,40 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyParams 
     if (a.logprobs != nullptr) a.logprobs[stop.row()] = log_share(rest.p, rest.logits[token]);
 }
 
-// Workgroups that the sums of all requests are given: eight are on a compute unit.
-constexpr uint32_t kSumGroups = 2048;
+// A row's chunks: enough workgroups to fill the device, but no more of them than the filters read in little time.
+constexpr uint32_t kFill = 512;
+constexpr uint32_t kMinChunk = 8192;
+constexpr uint32_t kMostChunks = 16;
+Chunks chunks_of(uint32_t rows, uint32_t vocab) {
+    if (rows == 0u || vocab == 0u) return {1u, vocab};
+    uint32_t n = std::min((kFill + rows - 1u) / rows, std::min(vocab / kMinChunk + 1u, kMostChunks));
+    n = std::max(n, (vocab + kLongest - 1u) / kLongest);
+    const uint32_t tokens = std::min(((vocab + n - 1u) / n + 511u) & ~511u, kLongest);
+    return {(vocab + tokens - 1u) / tokens, tokens};
+}
 
-uint32_t tiles_of(uint32_t vocab) { return (vocab + kTile - 1u) / kTile; }
+// Workgroups that the sums of all requests are given.
+constexpr uint32_t kSumGroups = 2048;
 
 struct Layout {
     Chunks chunks;
-    size_t stats, sums, counts, bytes;   // offsets, the whole
+    uint32_t tiles;
+    size_t stats, sums, counts, chances, shares, requests, bytes;   // offsets, the whole
 };
 Layout layout_of(uint32_t rows, uint32_t vocab, uint32_t requests, bool drafted) {
-    const uint32_t all = rows * (drafted ? 2u : 1u);
-    Layout l{chunks_of(all, vocab), 0u, 0u, 0u, 0u};
-    l.sums = l.stats + static_cast<size_t>(all) * sizeof(RowStat);
-    l.counts = l.sums + static_cast<size_t>(requests) * tiles_of(vocab) * sizeof(double2);
-    l.bytes = l.counts + (l.chunks.n > 1u ? static_cast<size_t>(all) * l.chunks.n * sizeof(ChunkCounts) : 0u);
+    const size_t all = static_cast<size_t>(rows) * (drafted ? 2u : 1u);
+    Layout l{chunks_of(static_cast<uint32_t>(all), vocab), (vocab + kTile - 1u) / kTile, 0, 0, 0, 0, 0, 0, 0};
+    const auto add = [&](size_t bytes) {
+        const size_t at = l.bytes;
+        l.bytes += (bytes + 15u) & ~size_t{15u};
+        return at;
+    };
+    l.stats = add(all * sizeof(RowStat));
+    l.sums = add(static_cast<size_t>(requests) * l.tiles * sizeof(double2));
+    l.counts = add(all * l.chunks.n * sizeof(ChunkCounts));
+    l.chances = add(all * sizeof(double));
+    l.shares = add(all * sizeof(float));
+    l.requests = add(all * sizeof(uint32_t));
     return l;
 }
 
@@ -392,22 +913,26 @@ void launch_verify_batch(const VerifyArgs& a, hipStream_t stream) {
     const uint32_t all = a.rows * (drafted ? 2u : 1u);
     const Layout l = layout_of(a.rows, a.vocab, a.requests, drafted);
     char* const w = static_cast<char*>(a.workspace);
-    const VerifyParams p{a, l.chunks, reinterpret_cast<RowStat*>(w + l.stats), reinterpret_cast<double2*>(w + l.sums),
-                         reinterpret_cast<ChunkCounts*>(w + l.counts), tiles_of(a.vocab)};
-    if (all == 0u) {
-        // (no row of any request)
-    } else if (l.chunks.n > 1u) {
+    VerifyParams p{};
+    p.a = a;
+    p.chunks = l.chunks;
+    p.tiles = l.tiles;
+    p.groups = std::max(1u, std::min(l.tiles, kSumGroups / a.requests));
+    p.stats = reinterpret_cast<RowStat*>(w + l.stats);
+    p.sums = reinterpret_cast<double2*>(w + l.sums);
+    p.counts = reinterpret_cast<ChunkCounts*>(w + l.counts);
+    p.chances = reinterpret_cast<double*>(w + l.chances);
+    p.shares = reinterpret_cast<float*>(w + l.shares);
+    p.requests = reinterpret_cast<uint32_t*>(w + l.requests);
+    if (all != 0u) {
         hipLaunchKernelGGL(verify_count_kernel, dim3(all * l.chunks.n), dim3(kThreads), 0, stream, p);
         HYP_HIP_CHECK(hipGetLastError());
-        hipLaunchKernelGGL(verify_filter_kernel<true>, dim3(all), dim3(kThreads), 0, stream, p);
-    } else {
-        hipLaunchKernelGGL(verify_filter_kernel<false>, dim3(all), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL(verify_filter_kernel, dim3(all), dim3(kFew), 0, stream, p);
+        HYP_HIP_CHECK(hipGetLastError());
+        hipLaunchKernelGGL(verify_sum_kernel, dim3(a.requests * p.groups), dim3(kFew), 0, stream, p);
+        HYP_HIP_CHECK(hipGetLastError());
     }
-    HYP_HIP_CHECK(hipGetLastError());
-    const uint32_t groups = std::max(1u, std::min(p.tiles, kSumGroups / a.requests));
-    hipLaunchKernelGGL(verify_sum_kernel, dim3(a.requests * groups), dim3(kDrawThreads), 0, stream, p, groups);
-    HYP_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(verify_draw_kernel, dim3(a.requests), dim3(kDrawThreads), 0, stream, p);
+    hipLaunchKernelGGL(verify_draw_kernel, dim3(a.requests), dim3(kFew), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
 }
 
