@@ -412,43 +412,49 @@ __device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t voc
     }
 }
 
-// The index of the number-th token of value `bits` among the tokens [begin, end) of a row, in s.last. Each wave marks the value's
-// places in its stretch, 512 tokens a step. (A call has a barrier at its end.)
+// The index of the number-th token of value `bits` among the tokens [begin, end) of a row, in s.last. Each wave counts the
+// value's places in its stretch, 512 tokens a step, two to an instruction. (A call has a barrier at its end.)
 __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, uint32_t end, uint32_t bits, uint32_t number,
                                           FilterLds& s) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = threadIdx.x >> 6;
     constexpr uint32_t kStep = 512u, kSteps = 16u;
+    const uint32_t pattern = bits | bits << 16;
+    const uint32_t mask = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu;   // (-0 is +0)
 #pragma unroll 1
     for (uint32_t base = begin; base < end; base += kFewWaves * kSteps * kStep) {
         const uint32_t stop = min(end, base + kFewWaves * kSteps * kStep);
         const uint32_t steps = (stop - base + kFewWaves * kStep - 1u) / (kFewWaves * kStep);
         const uint32_t first = base + wave * steps * kStep + 8u * lane;   // the lane's, of the first step
-        uint32_t hits[kSteps / 4u] = {};   // a byte a step
+        uint64_t found = 0u;   // the lane's of each step, four bits to one
         uint32_t mine = 0u;
-#pragma unroll
-        for (uint32_t q = 0; q < kSteps / 4u; ++q) {
-            if (4u * q >= steps) continue;
-            Eight e[4];
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                const uint32_t from = first + (4u * q + k) * kStep;
-                if (from + 8u <= stop) __builtin_memcpy(&e[k], row + from, 16);
-            }
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                const uint32_t from = first + (4u * q + k) * kStep;
-                uint32_t hit = 0u;
-                if (4u * q + k < steps && from + 8u <= stop) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) hit |= plain_bits(e[k].v[i]) == bits ? 1u << i : 0u;
-                } else if (4u * q + k < steps && from < stop) {
 #pragma unroll 1
-                    for (uint32_t i = 0; from + i < stop; ++i) hit |= plain_bits(row[from + i]) == bits ? 1u << i : 0u;
+        for (uint32_t k = 0; k < steps; k += 4u) {
+            uint32_t w[4][4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) {
+                const uint32_t from = first + (k + j) * kStep;
+                if (k + j < steps && from + 8u <= stop) {
+                    __builtin_memcpy(w[j], row + from, 16);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; ++i) w[j][i] = ~pattern;
                 }
-                hits[q] |= hit << (8u * k);
             }
-            mine += static_cast<uint32_t>(__popc(hits[q]));
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) {
+                u16x2_t apart = {0, 0};
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; ++i)
+                    apart += __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, (w[j][i] ^ pattern) & mask), u16x2_t{1, 1});
+                uint32_t n = 8u - apart.x - apart.y;
+                const uint32_t from = first + (k + j) * kStep;
+                if (k + j < steps && from < stop && from + 8u > stop)
+                    for (uint32_t i = from; i < stop; ++i) n += plain_bits(row[i]) == bits ? 1u : 0u;
+                found |= static_cast<uint64_t>(n) << (4u * (k + j));
+                mine += n;
+            }
         }
         const uint32_t wave_all = wave_sum(mine);
         if (lane == 0u) s.word[wave] = wave_all;
@@ -468,17 +474,18 @@ __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, u
         if (left < wave_all) {
 #pragma unroll 1
             for (uint32_t k = 0; k < steps; ++k) {
-                uint32_t hit = hits[0];
-#pragma unroll
-                for (uint32_t q = 1; q < kSteps / 4u; ++q) hit = k / 4u == q ? hits[q] : hit;
-                hit = (hit >> (8u * (k % 4u))) & 0xFFu;
-                const uint32_t n = static_cast<uint32_t>(__popc(hit));
+                const uint32_t n = static_cast<uint32_t>(found >> (4u * k)) & 15u;
                 const uint32_t incl = wave_incl(n);
                 const uint32_t step = from_lane(incl, 63u);
                 if (left < step) {
                     if (left - (incl - n) < n) {
-                        for (uint32_t i = left - (incl - n); i != 0u; --i) hit &= hit - 1u;
-                        s.last = first + k * kStep + static_cast<uint32_t>(__builtin_ctz(hit));
+                        uint32_t i = first + k * kStep;
+                        for (uint32_t skip = left - (incl - n);; ++i) {
+                            if (plain_bits(row[i]) != bits) continue;
+                            if (skip == 0u) break;
+                            --skip;
+                        }
+                        s.last = i;
                     }
                     break;
                 }
@@ -868,7 +875,7 @@ __global__ __launch_bounds__(kFew) void verify_draw_kernel(VerifyParams p) {
 // A row's chunks: enough workgroups to fill the device, but no more of them than the filters read in little time.
 constexpr uint32_t kFill = 512;
 constexpr uint32_t kMinChunk = 8192;
-constexpr uint32_t kMostChunks = 16;
+constexpr uint32_t kMostChunks = 8;
 Chunks chunks_of(uint32_t rows, uint32_t vocab) {
     if (rows == 0u || vocab == 0u) return {1u, vocab};
     uint32_t n = std::min((kFill + rows - 1u) / rows, std::min(vocab / kMinChunk + 1u, kMostChunks));
