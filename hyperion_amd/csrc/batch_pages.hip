@@ -151,10 +151,13 @@ __global__ __launch_bounds__(kEntryThreads) void fork_rows_kernel(ForkParams p) 
 
 // ---- rewind -----------------------------------------------------------------------------------
 
-// Workspace: for each block who still holds it (0: nobody; r + 1: request r, which was shortened into it, the
-// largest such; kFirmly: a request that was not) and the first request that gives it up.
+// Workspace: for each block a word, the largest of: kFirmly where a request still holds it; 1 << 31 | r + 1 where request r was
+// shortened into it; 1 << 30 | 4095 - r where request r gives it up. So a block that nobody holds names the first request that
+// gave it up, and one that all its holders were shortened into the last of those.
 constexpr uint32_t kFirmly = 0xFFFFFFFFu;
 constexpr uint32_t kNobody = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t cut_by(uint32_t request) { return 0x80000000u | (request + 1u); }
+__device__ __forceinline__ uint32_t left_by(uint32_t request) { return 0x40000000u | (kMaxRequests - 1u - request); }
 
 struct RewindParams {
     BatchView b;
@@ -165,21 +168,18 @@ struct RewindParams {
     uint32_t* taken_out;
     HypBlockCopy* copies;
     uint32_t* n_copies;
-    uint32_t* holds;    // [num_blocks]
-    uint32_t* leaves;   // [num_blocks]
+    uint32_t* state;    // [num_blocks]
 };
 
 __global__ __launch_bounds__(kEntryThreads) void rewind_clear_kernel(RewindParams p) {
     const uint32_t i = blockIdx.x * kEntryThreads + threadIdx.x;
-    if (i >= p.b.num_blocks) return;
-    p.holds[i] = 0u;
-    p.leaves[i] = kNobody;
+    if (i < p.b.num_blocks) p.state[i] = 0u;
 }
 
 struct Shortened {
     uint32_t len, keep;
     uint32_t had, has;   // blocks
-    uint32_t part;       // the block that it was shortened into and fills partly, kNobody if none
+    uint32_t part;       // the entry of the block that it was shortened into and fills partly, kNobody if none
 };
 __device__ __forceinline__ Shortened shortened(const RewindParams& p, uint32_t request) {
     const BatchView& b = p.b;
@@ -200,15 +200,13 @@ __global__ __launch_bounds__(kEntryThreads) void rewind_mark_kernel(RewindParams
     const uint32_t* const table = table_of(b, r);
     for (uint32_t e = blockIdx.y * kEntryThreads + threadIdx.x; e < s.had; e += gridDim.y * kEntryThreads) {
         const uint32_t block = table[e];
-        if (block >= b.num_blocks) continue;
-        if (e >= s.has) {
-            atomicMin(&p.leaves[block], r);
-        } else {
-            atomicMax(&p.holds[block], e == s.part ? r + 1u : kFirmly);
-        }
+        if (block < b.num_blocks) atomicMax(&p.state[block], e >= s.has ? left_by(r) : (e == s.part ? cut_by(r) : kFirmly));
     }
 }
 
+// The entries given up, from the last to the first: so a block that goes back has its place in the stack, from the top down,
+// without their number. Eight consecutive ones to a thread, with their loads on the way together.
+constexpr uint32_t kGoneEach = 8;
 __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
     __shared__ uint32_t gone_sum[kMaxRequests + 1];   // entries given up by the requests before
     __shared__ uint32_t first_gone[kMaxRequests];     // a request's first of them
@@ -242,23 +240,35 @@ __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
         if (tid == 0u) gone_sum[n] = sum.all;
     }
     __syncthreads();
-    // The blocks that go back, in order: how many, then where each goes.
-    const auto back = [&](uint32_t g, uint32_t& block) {
-        if (g >= sum.all) return false;
-        const uint32_t r = owner(gone_sum, n, g);
-        block = table_of(b, r)[first_gone[r] + (g - gone_sum[r])];
-        return block < b.num_blocks && p.holds[block] == 0u && p.leaves[block] == r;
-    };
-    uint32_t mine = 0u, block = 0u;
-    for (uint32_t g = tid; g < sum.all; g += kThreads) mine += back(g, block) ? 1u : 0u;
-    const uint32_t returned = min(block_sum(mine, waves).all, taken);
-    const uint32_t c = taken - returned;
-    for (uint32_t base = 0u, before = 0u; base < sum.all && before < returned; base += kThreads) {
-        const bool goes = back(base + tid, block);
-        const Sum here = block_sum(goes ? 1u : 0u, waves);
-        if (goes && before + here.before < returned) p.free_blocks[c + before + here.before] = block;
-        before += here.all;
+    uint32_t returned = 0u;
+    for (uint32_t base = 0u; base < sum.all && returned < taken; base += kThreads * kGoneEach) {
+        uint32_t block[kGoneEach], by[kGoneEach], goes = 0u;
+        const uint32_t at = base + tid * kGoneEach;   // from the end
+        uint32_t r = at < sum.all ? owner(gone_sum, n, sum.all - 1u - at) : 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < kGoneEach; ++i) {
+            block[i] = kNobody;
+            if (at + i >= sum.all) continue;
+            const uint32_t g = sum.all - 1u - (at + i);
+            while (g < gone_sum[r]) --r;
+            by[i] = r;
+            block[i] = table_of(b, r)[first_gone[r] + (g - gone_sum[r])];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kGoneEach; ++i)
+            if (block[i] < b.num_blocks && p.state[block[i]] == left_by(by[i])) goes |= 1u << i;
+        const Sum here = block_sum(static_cast<uint32_t>(__popc(goes)), waves);
+        uint32_t rank = returned + here.before;
+#pragma unroll
+        for (uint32_t i = 0; i < kGoneEach; ++i)
+            if ((goes >> i) & 1u) {
+                if (rank < taken) p.free_blocks[taken - 1u - rank] = block[i];
+                ++rank;
+            }
+        returned += here.all;
     }
+    returned = min(returned, taken);
+    const uint32_t c = taken - returned;
     __syncthreads();
     // Blocks that were shared and are now filled partly.
     uint32_t need = 0u, held[kPer];
@@ -268,7 +278,7 @@ __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
         held[i] = kNobody;
         if (i >= per || r >= n || s[i].part == kNobody) continue;
         const uint32_t at = table_of(b, r)[s[i].part];
-        if (at >= b.num_blocks || p.holds[at] == r + 1u) continue;
+        if (at >= b.num_blocks || p.state[at] == cut_by(r)) continue;
         held[i] = at;
         ++need;
     }
@@ -300,6 +310,7 @@ __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
 
 // ---- compact ----------------------------------------------------------------------------------
 
+// Workspace: for each block its number among those that move, then a byte each that says whether it is in use.
 struct CompactParams {
     BatchView b;
     uint32_t* tables_out;
@@ -308,14 +319,14 @@ struct CompactParams {
     uint32_t* taken_out;
     HypBlockCopy* copies;
     uint32_t* n_copies;
-    uint32_t* to;      // [num_blocks]: where a block goes, of those that move
-    uint32_t* live;    // [num_blocks]: 1 for blocks in use
+    uint32_t* move;    // [num_blocks]
+    uint4* live;       // [num_blocks] bytes, 16 to one
     uint32_t prefix_blocks;
 };
 
 __global__ __launch_bounds__(kEntryThreads) void compact_clear_kernel(CompactParams p) {
     const uint32_t i = blockIdx.x * kEntryThreads + threadIdx.x;
-    if (i < p.b.num_blocks) p.live[i] = 0u;
+    if (16u * i < p.b.num_blocks) p.live[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // A row of blocks: a request's, or behind those the prefix's.
@@ -330,42 +341,66 @@ __device__ __forceinline__ const uint32_t* row_of(const CompactParams& p, uint32
 }
 
 __global__ __launch_bounds__(kEntryThreads) void compact_mark_kernel(CompactParams p) {
+    uint8_t* const live = reinterpret_cast<uint8_t*>(p.live);
     uint32_t held, width;
     const uint32_t* const row = row_of(p, blockIdx.x, held, width);
     for (uint32_t e = blockIdx.y * kEntryThreads + threadIdx.x; e < held; e += gridDim.y * kEntryThreads) {
         const uint32_t block = row[e];
-        if (block < p.b.num_blocks) p.live[block] = 1u;
+        if (block < p.b.num_blocks) live[block] = 1u;
     }
 }
 
-// The moves: with L blocks in use, the i-th of those from L upwards goes to the i-th free one below L.
-__global__ __launch_bounds__(kThreads) void compact_kernel(CompactParams p) {
+// Which of 16 blocks are in use, as bits (bytes of 0 or 1).
+__device__ __forceinline__ uint32_t bits_of(uint4 v) {
+    const auto four = [](uint32_t w) { return (w * 0x01020408u) >> 24; };   // bit i from byte i, and nothing carried over
+    return four(v.x) | four(v.y) << 4 | four(v.z) << 8 | four(v.w) << 12;
+}
+
+// The moves: with L blocks in use, the i-th of those from L upwards goes to the i-th free one below L. How many in use are
+// before a block gives its number: before block j < L are j less that many free ones. Every workgroup forms L and what comes
+// before its own words for itself, from all of them: a byte for each block, where one workgroup alone for all took 42 us at
+// 78000 blocks.
+constexpr uint32_t kMoveGroups = 64;
+__global__ __launch_bounds__(kThreads) void compact_moves_kernel(CompactParams p) {
     __shared__ uint32_t waves[kWaves];
     const uint32_t tid = threadIdx.x;
-    const uint32_t num = p.b.num_blocks;
-    uint32_t mine = 0u;
-    for (uint32_t i = tid; i < num; i += kThreads) mine += p.live[i];
-    const uint32_t count = block_sum(mine, waves).all;
-    uint32_t movers = 0u, holes = 0u;
-    for (uint32_t base = 0u; base < num; base += kThreads) {
-        const uint32_t i = base + tid;
-        const bool live = i < num && p.live[i] != 0u;
-        const bool mover = live && i >= count;
-        const bool hole = !live && i < count;
-        const Sum m = block_sum(mover ? 1u : 0u, waves);
-        const Sum h = block_sum(hole ? 1u : 0u, waves);
-        if (mover) {
-            p.copies[movers + m.before].from = i;
-            p.copies[movers + m.before].tokens = 1u << p.b.shift;
-        }
-        if (hole) p.copies[holes + h.before].to = i;
-        movers += m.all;
-        holes += h.all;
+    const uint32_t words = (p.b.num_blocks + 15u) / 16u;
+    const uint32_t each = (words + gridDim.x - 1u) / gridDim.x;
+    const uint32_t begin = min(blockIdx.x * each, words);
+    const uint32_t end = min(begin + each, words);
+    uint32_t mine = 0u, before = 0u;
+#pragma unroll 4
+    for (uint32_t i = tid; i < words; i += kThreads) {
+        const uint32_t n = static_cast<uint32_t>(__popc(bits_of(p.live[i])));
+        mine += n;
+        before += i < begin ? n : 0u;
     }
-    __syncthreads();
-    for (uint32_t i = tid; i < movers; i += kThreads) p.to[p.copies[i].from] = p.copies[i].to;
-    if (tid == 0u) {
-        *p.n_copies = movers;
+    const uint32_t count = block_sum(mine, waves).all;
+    before = block_sum(before, waves).all;
+    mine = 0u;   // in use below L
+#pragma unroll 4
+    for (uint32_t i = tid; i <= count / 16u && i < words; i += kThreads) {
+        const uint32_t used = bits_of(p.live[i]);
+        mine += static_cast<uint32_t>(__popc(i < count / 16u ? used : used & ((1u << (count % 16u)) - 1u)));
+    }
+    const uint32_t low = block_sum(mine, waves).all;
+    // A block to a thread.
+    for (uint32_t base = 16u * begin; base < 16u * end; base += kThreads) {
+        const uint32_t block = base + tid;
+        const bool live = block < 16u * end && reinterpret_cast<const uint8_t*>(p.live)[block] != 0u;
+        const Sum here = block_sum(live ? 1u : 0u, waves);
+        const uint32_t number = before + here.before;   // in use before it
+        if (live && block >= count) {
+            p.copies[number - low].from = block;
+            p.copies[number - low].tokens = 1u << p.b.shift;
+            p.move[block] = number - low;
+        } else if (!live && block < count && block < 16u * end) {
+            p.copies[block - number].to = block;
+        }
+        before += here.all;
+    }
+    if (blockIdx.x == 0u && tid == 0u) {
+        *p.n_copies = count - low;
         *p.taken_out = count;
     }
 }
@@ -386,7 +421,7 @@ __global__ __launch_bounds__(kEntryThreads) void compact_tables_kernel(CompactPa
     uint32_t* const out = row_at == p.b.requests ? p.prefix_out : p.tables_out + static_cast<size_t>(row_at) * width;
     for (uint32_t e = begin; e < width; e += stride) {
         const uint32_t block = row[e];
-        out[e] = e < held && block >= count && block < num ? p.to[block] : block;
+        out[e] = e < held && block >= count && block < num ? p.copies[p.move[block]].to : block;
     }
 }
 
@@ -434,13 +469,16 @@ void launch_batch_fork(const BatchView& b, const uint32_t* lens, const uint32_t*
     HYP_HIP_CHECK(hipGetLastError());
 }
 
-size_t batch_pages_workspace_bytes(const BatchView& b) { return 2u * sizeof(uint32_t) * static_cast<size_t>(b.num_blocks); }
+size_t batch_pages_workspace_bytes(const BatchView& b) {
+    const size_t blocks = (static_cast<size_t>(b.num_blocks) + 15u) & ~size_t{15u};
+    return 5u * blocks;   // a word and a byte each
+}
 
 void launch_batch_rewind(const BatchView& b, const uint32_t* lens, const uint32_t* drop, uint32_t* free_blocks,
                          const uint32_t* taken, uint32_t* taken_out, HypBlockCopy* copies, uint32_t* n_copies,
                          void* workspace, hipStream_t stream) {
     uint32_t* const w = static_cast<uint32_t*>(workspace);
-    const RewindParams p{b, lens, drop, free_blocks, taken, taken_out, copies, n_copies, w, w + b.num_blocks};
+    const RewindParams p{b, lens, drop, free_blocks, taken, taken_out, copies, n_copies, w};
     if (b.requests != 0u && b.max_blocks != 0u) {
         hipLaunchKernelGGL(rewind_clear_kernel, dim3((b.num_blocks + kEntryThreads - 1u) / kEntryThreads),
                            dim3(kEntryThreads), 0, stream, p);
@@ -457,15 +495,16 @@ void launch_batch_compact(const BatchView& b, uint32_t* tables_out, uint32_t* pr
                           hipStream_t stream) {
     uint32_t* const w = static_cast<uint32_t*>(workspace);
     const uint32_t prefix_blocks = static_cast<uint32_t>((static_cast<uint64_t>(b.prefix) + (1u << b.shift) - 1u) >> b.shift);
-    const CompactParams p{b,      tables_out, prefix_out,         free_blocks, taken_out, copies,
-                          n_copies, w,        w + b.num_blocks, prefix_blocks};
+    uint4* const live = reinterpret_cast<uint4*>(w + ((b.num_blocks + 15u) & ~15u));
+    const CompactParams p{b, tables_out, prefix_out, free_blocks, taken_out, copies, n_copies, w, live, prefix_blocks};
     const uint32_t pieces = pieces_of(std::max(b.max_blocks, prefix_blocks));
-    hipLaunchKernelGGL(compact_clear_kernel, dim3((b.num_blocks + kEntryThreads - 1u) / kEntryThreads), dim3(kEntryThreads),
-                       0, stream, p);
+    const uint32_t clear = (b.num_blocks + 16u * kEntryThreads - 1u) / (16u * kEntryThreads);
+    hipLaunchKernelGGL(compact_clear_kernel, dim3(clear), dim3(kEntryThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL(compact_mark_kernel, dim3(b.requests + 1u, pieces), dim3(kEntryThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kThreads), 0, stream, p);
+    const uint32_t groups = std::min(kMoveGroups, (b.num_blocks + kThreads - 1u) / kThreads);
+    hipLaunchKernelGGL(compact_moves_kernel, dim3(groups), dim3(kThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
     const uint32_t wide = std::max(pieces, pieces_of(b.num_blocks));
     hipLaunchKernelGGL(compact_tables_kernel, dim3(b.requests + 2u, wide), dim3(kEntryThreads), 0, stream, p);

@@ -45,7 +45,7 @@ def rewind(lens, drop, tables, free, taken, block):
         for b in held(tables[r], n, block)[blocks(k, block):]:
             if b < num and b not in holders and b not in back:
                 back.append(b)
-    back = back[:int(taken)]
+    back = back[max(0, len(back) - int(taken)):]   # (a stack holds no more than was taken from it)
     top = int(taken) - len(back)
     free[top:int(taken)] = back
     cut = {}   # block -> the requests that were shortened into it

@@ -89,7 +89,7 @@ def test_fork_refusals(over, says):
 @pytest.mark.parametrize("over,says", [
     (dict(lens=None), "null"), (dict(drop=None), "null"), (dict(free=None), "null"), (dict(taken=None), "null"),
     (dict(taken_out=None), "null"), (dict(copies=None), "null"), (dict(n=None), "null"), (dict(stream=None), "null"),
-    (dict(drop=ODD), "aligned"), (dict(work=None), "workspace too small"), (dict(bytes=8 * 64 - 1), "workspace too small"),
+    (dict(drop=ODD), "aligned"), (dict(work=None), "workspace too small"), (dict(bytes=5 * 64 - 1), "workspace too small"),
     (dict(work=ptr(0x900004)), "aligned"), (dict(work=ptr(A[2].value + 16)), "overlap"), (dict(drop=A[11]), "overlap"),
     (dict(drop=A[2]), "overlap"), (dict(copies=A[4]), "overlap"), (dict(taken=A[7]), "overlap")])
 def test_rewind_refusals(over, says):
@@ -143,7 +143,7 @@ def test_verify_of_no_requests():
 def test_workspaces():
     out = ctypes.c_size_t()
     assert hy.lib().hyp_batch_pages_workspace(ctypes.byref(batch()), ctypes.byref(out)) == 0
-    assert out.value == 8 * 64
+    assert out.value == 5 * 64
     refused("hyp_batch_pages_workspace", ctypes.byref(batch()), None, says="out_bytes")
     refused("hyp_verify_batch_workspace", 6, 1000, 2, 1, None, says="out_bytes")
     for args, says in (((6, (1 << 23) + 1, 2, 1), "2^23"), (((1 << 20) + 1, 5, 2, 1), "2^20"), ((6, 5, 4097, 1), "4096")):
