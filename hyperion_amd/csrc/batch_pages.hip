@@ -56,6 +56,35 @@ __device__ __forceinline__ Sum block_sum(uint32_t v, uint32_t* waves) {
     return s;
 }
 
+// Small tables are gone through by the one workgroup that has the rest to do, all entries of all rows in a line: a launch
+// takes longer than 32 entries a thread.
+constexpr uint32_t kSmallTable = 32u * kThreads;   // entries
+constexpr uint32_t kSmallRequests = kThreads;
+constexpr uint32_t kSmallPool = 32u * kThreads;    // blocks
+bool small_table(const BatchView& b) {
+    return b.requests <= kSmallRequests && static_cast<uint64_t>(b.requests) * b.max_blocks <= kSmallTable;
+}
+// f(request, entry, where it is) of each, four to a thread on their way together (of load(...), then use(..., loaded)).
+template <typename Load, typename Use>
+__device__ __forceinline__ void for_entries(const BatchView& b, Load&& load, Use&& use) {
+    const uint32_t all = b.requests * b.max_blocks;
+    const float by_width = 1.0f / static_cast<float>(b.max_blocks);   // (exact below 2^21 entries)
+#pragma unroll 1
+    for (uint32_t base = threadIdx.x; base < all; base += 4u * kThreads) {
+        uint32_t r[4], e[4], v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t at = base + i * kThreads;
+            r[i] = at < all ? static_cast<uint32_t>((static_cast<float>(at) + 0.5f) * by_width) : 0u;
+            e[i] = at - r[i] * b.max_blocks;
+            v[i] = at < all ? load(r[i], e[i], at) : 0u;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i)
+            if (base + i * kThreads < all) use(r[i], e[i], base + i * kThreads, v[i]);
+    }
+}
+
 // ---- fork -------------------------------------------------------------------------------------
 
 struct ForkParams {
@@ -77,9 +106,12 @@ __device__ __forceinline__ uint32_t parent_of(const ForkParams& p, uint32_t requ
     return parent;
 }
 
-// Lengths, the blocks of their own that copies get, and how far the free ones go.
+// Lengths, the blocks of their own that copies get, and how far the free ones go; the entries of whole blocks too where the
+// table is small.
+template <bool kSmall>
 __global__ __launch_bounds__(kThreads) void fork_kernel(ForkParams p) {
     __shared__ uint32_t waves[kWaves];
+    __shared__ uint32_t parent_at[kSmall ? kSmallRequests : 1u], whole_of[kSmall ? kSmallRequests : 1u];
     __shared__ uint32_t served_at;
     const BatchView& b = p.b;
     const uint32_t tid = threadIdx.x;
@@ -127,12 +159,24 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(ForkParams p) {
         }
         if (needs(i)) ++rank;
         b.lens[r] = parent[i] == HYP_PARENT_NONE || in ? len[i] : p.lens[r];
+        if constexpr (kSmall) {
+            parent_at[r] = parent[i];
+            whole_of[r] = in ? min(len[i] >> b.shift, b.max_blocks) : 0u;
+        }
     }
     if (tid == 0u) {
         const uint32_t copied = min(sum.all, free_left);
         *p.n_copies = copied;
         *p.taken_out = taken + copied;
         *p.served = served;
+    }
+    if constexpr (kSmall) {
+        __syncthreads();
+        for_entries(
+            b, [&](uint32_t r, uint32_t e, uint32_t) { return e < whole_of[r] ? table_of(b, parent_at[r])[e] : 0u; },
+            [&](uint32_t r, uint32_t e, uint32_t at, uint32_t v) {
+                if (e < whole_of[r]) b.tables[at] = v;
+            });
     }
 }
 
@@ -205,18 +249,63 @@ __global__ __launch_bounds__(kEntryThreads) void rewind_mark_kernel(RewindParams
 }
 
 // The entries given up, from the last to the first: so a block that goes back has its place in the stack, from the top down,
-// without their number. Eight consecutive ones to a thread, with their loads on the way together.
-constexpr uint32_t kGoneEach = 8;
+// without their number. kEach consecutive ones to a thread, with their loads on the way together. How many went back.
+// (One to a thread while that does: 64 requests' drafts 4.2 us so, 6.8 with four; 10000 blocks of 71 requests that end 14.8 with
+// four, 22.2 with one, 16.4 with eight.)
+template <uint32_t kEach>
+__device__ __forceinline__ uint32_t give_back(const RewindParams& p, const uint32_t* state, const uint32_t* gone_sum,
+                                              const uint32_t* first_gone, uint32_t all, uint32_t taken, uint32_t* waves) {
+    const BatchView& b = p.b;
+    const uint32_t n = b.requests;
+    uint32_t returned = 0u;
+    for (uint32_t base = 0u; base < all && returned < taken; base += kThreads * kEach) {
+        uint32_t block[kEach], by[kEach], goes = 0u;
+        const uint32_t at = base + threadIdx.x * kEach;   // from the end
+        uint32_t r = at < all ? owner(gone_sum, n, all - 1u - at) : 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            block[i] = kNobody;
+            by[i] = 0u;
+            if (at + i >= all) continue;
+            const uint32_t g = all - 1u - (at + i);
+            while (g < gone_sum[r]) --r;
+            by[i] = r;
+            block[i] = table_of(b, r)[first_gone[r] + (g - gone_sum[r])];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i)
+            if (block[i] < b.num_blocks && state[block[i]] == left_by(by[i])) goes |= 1u << i;
+        const Sum here = block_sum(static_cast<uint32_t>(__popc(goes)), waves);
+        uint32_t rank = returned + here.before;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i)
+            if ((goes >> i) & 1u) {
+                if (rank < taken) p.free_blocks[taken - 1u - rank] = block[i];
+                ++rank;
+            }
+        returned += here.all;
+    }
+    return min(returned, taken);
+}
+
+// kSmall: the marks are this workgroup's own, in LDS.
+template <bool kSmall>
 __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
-    __shared__ uint32_t gone_sum[kMaxRequests + 1];   // entries given up by the requests before
-    __shared__ uint32_t first_gone[kMaxRequests];     // a request's first of them
+    constexpr uint32_t kRequests = kSmall ? kSmallRequests : kMaxRequests;
+    __shared__ uint32_t gone_sum[kRequests + 1];   // entries given up by the requests before
+    __shared__ uint32_t first_gone[kRequests];     // a request's first of them
+    __shared__ uint32_t had[kSmall ? kRequests : 1u], part[kSmall ? kRequests : 1u];
+    __shared__ uint32_t marks[kSmall ? kSmallPool : 1u];
     __shared__ uint32_t waves[kWaves];
+    uint32_t* const state = kSmall ? marks : p.state;
     const BatchView& b = p.b;
     const uint32_t tid = threadIdx.x;
     const uint32_t n = b.requests;
     const uint32_t per = (n + kThreads - 1u) / kThreads;
     const uint32_t first = tid * per;
     const uint32_t taken = min(*p.taken, b.num_blocks);
+    if constexpr (kSmall)
+        for (uint32_t i = tid; i < b.num_blocks; i += kThreads) marks[i] = 0u;
     Shortened s[kPer];
     uint32_t gone = 0u;
 #pragma unroll
@@ -236,38 +325,25 @@ __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
             gone_sum[r] = at;
             first_gone[r] = s[i].has;
             at += s[i].had - s[i].has;
+            if constexpr (kSmall) {
+                had[r] = s[i].had;
+                part[r] = s[i].part;
+            }
         }
         if (tid == 0u) gone_sum[n] = sum.all;
     }
     __syncthreads();
-    uint32_t returned = 0u;
-    for (uint32_t base = 0u; base < sum.all && returned < taken; base += kThreads * kGoneEach) {
-        uint32_t block[kGoneEach], by[kGoneEach], goes = 0u;
-        const uint32_t at = base + tid * kGoneEach;   // from the end
-        uint32_t r = at < sum.all ? owner(gone_sum, n, sum.all - 1u - at) : 0u;
-#pragma unroll
-        for (uint32_t i = 0; i < kGoneEach; ++i) {
-            block[i] = kNobody;
-            if (at + i >= sum.all) continue;
-            const uint32_t g = sum.all - 1u - (at + i);
-            while (g < gone_sum[r]) --r;
-            by[i] = r;
-            block[i] = table_of(b, r)[first_gone[r] + (g - gone_sum[r])];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kGoneEach; ++i)
-            if (block[i] < b.num_blocks && p.state[block[i]] == left_by(by[i])) goes |= 1u << i;
-        const Sum here = block_sum(static_cast<uint32_t>(__popc(goes)), waves);
-        uint32_t rank = returned + here.before;
-#pragma unroll
-        for (uint32_t i = 0; i < kGoneEach; ++i)
-            if ((goes >> i) & 1u) {
-                if (rank < taken) p.free_blocks[taken - 1u - rank] = block[i];
-                ++rank;
-            }
-        returned += here.all;
+    if constexpr (kSmall) {
+        for_entries(
+            b, [&](uint32_t r, uint32_t e, uint32_t at) { return e < had[r] ? b.tables[at] : kNobody; },
+            [&](uint32_t r, uint32_t e, uint32_t, uint32_t block) {
+                if (block < b.num_blocks)
+                    atomicMax(&marks[block], e >= first_gone[r] ? left_by(r) : (e == part[r] ? cut_by(r) : kFirmly));
+            });
+        __syncthreads();
     }
-    returned = min(returned, taken);
+    const uint32_t returned = sum.all <= kThreads ? give_back<1>(p, state, gone_sum, first_gone, sum.all, taken, waves)
+                                                  : give_back<4>(p, state, gone_sum, first_gone, sum.all, taken, waves);
     const uint32_t c = taken - returned;
     __syncthreads();
     // Blocks that were shared and are now filled partly.
@@ -278,7 +354,7 @@ __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
         held[i] = kNobody;
         if (i >= per || r >= n || s[i].part == kNobody) continue;
         const uint32_t at = table_of(b, r)[s[i].part];
-        if (at >= b.num_blocks || p.state[at] == cut_by(r)) continue;
+        if (at >= b.num_blocks || state[at] == cut_by(r)) continue;
         held[i] = at;
         ++need;
     }
@@ -405,6 +481,72 @@ __global__ __launch_bounds__(kThreads) void compact_moves_kernel(CompactParams p
     }
 }
 
+// All of it for a small table and pool, by one workgroup: 32 blocks to a thread, their marks a bit each.
+__global__ __launch_bounds__(kThreads) void compact_small_kernel(CompactParams p) {
+    static_assert(kSmallPool == 32u * kThreads, "a word to a thread");
+    __shared__ uint32_t marks[kThreads], before[kThreads];   // blocks in use, how many before a word's
+    __shared__ uint32_t held[kSmallRequests];
+    __shared__ uint16_t holes[kSmallPool / 2u];
+    __shared__ uint32_t waves[kWaves];
+    __shared__ uint32_t below;   // blocks in use below L
+    const BatchView& b = p.b;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t num = b.num_blocks;
+    marks[tid] = 0u;
+    if (tid < b.requests) held[tid] = blocks_of(b, b.lens[tid]);
+    __syncthreads();
+    const auto mark = [&](uint32_t block) {
+        if (block < num) atomicOr(&marks[block / 32u], 1u << (block % 32u));
+    };
+    for (uint32_t i = tid; i < p.prefix_blocks; i += kThreads) mark(b.prefix_table[i]);
+    for_entries(
+        b, [&](uint32_t r, uint32_t e, uint32_t at) { return e < held[r] ? b.tables[at] : HYP_PARENT_NONE; },
+        [&](uint32_t, uint32_t, uint32_t, uint32_t block) { mark(block); });
+    __syncthreads();
+    const uint32_t used = marks[tid];
+    const Sum in_use = block_sum(static_cast<uint32_t>(__popc(used)), waves);
+    const uint32_t count = in_use.all;   // L
+    before[tid] = in_use.before;
+    if (tid == min(count / 32u, kThreads - 1u))   // (at kSmallPool, all)
+        below = count == kSmallPool ? count
+                                    : in_use.before + static_cast<uint32_t>(__popc(used & ((1u << (count % 32u)) - 1u)));
+    __syncthreads();
+    const uint32_t low = below;
+    // Of this thread's blocks, those that move and the free ones below L.
+    const auto up_to = [&](uint32_t first) {   // bits of the blocks below `first`
+        return first <= 32u * tid ? 0u : (first >= 32u * tid + 32u ? 0xFFFFFFFFu : (1u << (first - 32u * tid)) - 1u);
+    };
+    for (uint32_t bits = used & ~up_to(count); bits != 0u; bits &= bits - 1u) {
+        const uint32_t j = static_cast<uint32_t>(__builtin_ctz(bits));
+        const uint32_t number = in_use.before + static_cast<uint32_t>(__popc(used & ((1u << j) - 1u))) - low;
+        p.copies[number].from = 32u * tid + j;
+        p.copies[number].tokens = 1u << b.shift;
+    }
+    for (uint32_t bits = ~used & up_to(count); bits != 0u; bits &= bits - 1u) {
+        const uint32_t j = static_cast<uint32_t>(__builtin_ctz(bits));
+        const uint32_t block = 32u * tid + j;
+        const uint32_t number = block - (in_use.before + static_cast<uint32_t>(__popc(used & ((1u << j) - 1u))));
+        p.copies[number].to = block;
+        holes[number] = static_cast<uint16_t>(block);
+    }
+    __syncthreads();
+    const auto moved = [&](uint32_t block) {
+        if (block < count || block >= num) return block;
+        const uint32_t word = marks[block / 32u];
+        return static_cast<uint32_t>(
+            holes[before[block / 32u] + static_cast<uint32_t>(__popc(word & ((1u << (block % 32u)) - 1u))) - low]);
+    };
+    for_entries(
+        b, [&](uint32_t, uint32_t, uint32_t at) { return b.tables[at]; },
+        [&](uint32_t r, uint32_t e, uint32_t at, uint32_t block) { p.tables_out[at] = e < held[r] ? moved(block) : block; });
+    for (uint32_t i = tid; i < p.prefix_blocks; i += kThreads) p.prefix_out[i] = moved(b.prefix_table[i]);
+    for (uint32_t i = count + tid; i < num; i += kThreads) p.free_blocks[i] = i;
+    if (tid == 0u) {
+        *p.n_copies = count - low;
+        *p.taken_out = count;
+    }
+}
+
 __global__ __launch_bounds__(kEntryThreads) void compact_tables_kernel(CompactParams p) {
     const uint32_t count = *p.taken_out;
     const uint32_t num = p.b.num_blocks;
@@ -462,9 +604,13 @@ void launch_batch_fork(const BatchView& b, const uint32_t* lens, const uint32_t*
                        const uint32_t* taken, uint32_t* taken_out, uint32_t* served, HypBlockCopy* copies,
                        uint32_t* n_copies, hipStream_t stream) {
     const ForkParams p{b, lens, parents, free_blocks, taken, taken_out, served, copies, n_copies};
-    hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(kThreads), 0, stream, p);
+    if (small_table(b)) {
+        hipLaunchKernelGGL(fork_kernel<true>, dim3(1), dim3(kThreads), 0, stream, p);
+        HYP_HIP_CHECK(hipGetLastError());
+        return;
+    }
+    hipLaunchKernelGGL(fork_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
-    if (b.requests == 0u || b.max_blocks == 0u) return;
     hipLaunchKernelGGL(fork_rows_kernel, dim3(b.requests, pieces_of(b.max_blocks)), dim3(kEntryThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
 }
@@ -479,6 +625,11 @@ void launch_batch_rewind(const BatchView& b, const uint32_t* lens, const uint32_
                          void* workspace, hipStream_t stream) {
     uint32_t* const w = static_cast<uint32_t*>(workspace);
     const RewindParams p{b, lens, drop, free_blocks, taken, taken_out, copies, n_copies, w};
+    if (small_table(b) && b.num_blocks <= kSmallPool) {
+        hipLaunchKernelGGL(rewind_kernel<true>, dim3(1), dim3(kThreads), 0, stream, p);
+        HYP_HIP_CHECK(hipGetLastError());
+        return;
+    }
     if (b.requests != 0u && b.max_blocks != 0u) {
         hipLaunchKernelGGL(rewind_clear_kernel, dim3((b.num_blocks + kEntryThreads - 1u) / kEntryThreads),
                            dim3(kEntryThreads), 0, stream, p);
@@ -486,7 +637,7 @@ void launch_batch_rewind(const BatchView& b, const uint32_t* lens, const uint32_
         hipLaunchKernelGGL(rewind_mark_kernel, dim3(b.requests, pieces_of(b.max_blocks)), dim3(kEntryThreads), 0, stream, p);
         HYP_HIP_CHECK(hipGetLastError());
     }
-    hipLaunchKernelGGL(rewind_kernel, dim3(1), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(rewind_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
 }
 
@@ -497,6 +648,11 @@ void launch_batch_compact(const BatchView& b, uint32_t* tables_out, uint32_t* pr
     const uint32_t prefix_blocks = static_cast<uint32_t>((static_cast<uint64_t>(b.prefix) + (1u << b.shift) - 1u) >> b.shift);
     uint4* const live = reinterpret_cast<uint4*>(w + ((b.num_blocks + 15u) & ~15u));
     const CompactParams p{b, tables_out, prefix_out, free_blocks, taken_out, copies, n_copies, w, live, prefix_blocks};
+    if (small_table(b) && b.num_blocks <= kSmallPool && prefix_blocks <= kSmallTable) {
+        hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kThreads), 0, stream, p);
+        HYP_HIP_CHECK(hipGetLastError());
+        return;
+    }
     const uint32_t pieces = pieces_of(std::max(b.max_blocks, prefix_blocks));
     const uint32_t clear = (b.num_blocks + 16u * kEntryThreads - 1u) / (16u * kEntryThreads);
     hipLaunchKernelGGL(compact_clear_kernel, dim3(clear), dim3(kEntryThreads), 0, stream, p);
