@@ -50,7 +50,8 @@ enum RowKind : uint32_t { kEmpty = 0, kCounted = 1, kWindowed = 2, kInfinite = 3
 // A row and its filters.
 struct alignas(16) RowStat {
     double top, by_t, by_kept, total;   // largest logit, 1 / temperature, 1 / kept mass, mass of all tokens
-    uint32_t cut, last;                 // place of the last value that is kept, the last kept token of that value
+    float cut;                          // the last value that is kept (NaN: none)
+    uint32_t last;                      // the last kept token of that value
     uint32_t kind, unused;
 };
 
@@ -118,13 +119,16 @@ __device__ __forceinline__ double scalar(double v) {
     return __builtin_bit_cast(double, lo | hi << 32);
 }
 
+__device__ __forceinline__ float logit_of(uint32_t bits) { return __uint_as_float(bits << 16); }
+// Whether the filters keep a token (a NaN is above nothing, -inf above no cut).
+__device__ __forceinline__ bool keeps(const RowStat& r, float x, uint32_t token) {
+    return x > r.cut || (x == r.cut && token <= r.last);
+}
 // The probability of a token from its logit.
 __device__ __forceinline__ double probability(const RowStat& r, uint32_t bits, uint32_t token) {
-    bits = plain_bits(bits);
-    const uint32_t place = place_of(bits);
-    if (r.kind == kEmpty || place > r.cut || (place == r.cut && token > r.last)) return 0.0;
-    if (r.kind == kInfinite) return bits == 0x7F80u ? r.by_kept : 0.0;
-    return finite_bits(bits) ? exp_below((value_of(bits) - r.top) * r.by_t) * r.by_kept : 0.0;
+    const float x = logit_of(bits);
+    if (!keeps(r, x, token)) return 0.0;
+    return r.kind == kInfinite ? r.by_kept : exp_below((static_cast<double>(x) - r.top) * r.by_t) * r.by_kept;
 }
 
 // ln of a token's share of the mass before the filters.
@@ -590,6 +594,7 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
     s.count[tid] = tid == kCentreThread ? s.centre : 0u;   // (this thread's alone)
     RowStat r{};
     r.by_t = prm.by_t;
+    r.cut = __builtin_nanf("");
     if (s.infinite != 0u) {
         // Weight 1 for each, 0 for everything else.
         const uint32_t infinite = s.infinite;
@@ -618,7 +623,7 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
     }
     if (r.kind != kEmpty) {
         r.by_kept = 1.0 / s.kept;
-        r.cut = place_of(s.cut);
+        r.cut = logit_of(s.cut);
         r.last = a.vocab;
         if (s.whole == 0u) {   // some of the last kept value's tokens are dropped
             uint32_t number = s.number, begin = 0u, end = a.vocab;
@@ -681,6 +686,29 @@ __device__ __forceinline__ Stop find_stop(const VerifyParams& p, uint32_t reques
     return {first, rows, accepted};
 }
 
+// e^x of many x <= 0: 2^(n / 64) e^r with |r| <= ln 2 / 128, the first by a table, the series to r^5 (the rest is below 2^-54).
+// (15 instructions where exp_below takes 25: a request's whole vocabulary goes through it, without filters.)
+constexpr uint32_t kPowers = 64;
+struct Powers {
+    double p[kPowers];   // 2^(j / 64) / 2
+    __device__ __forceinline__ void fill() {   // (before a barrier)
+        const uint32_t j = threadIdx.x;
+        if (j < kPowers) p[j] = exp_below(-0x1.62e42fefa39efp-7 * static_cast<double>(kPowers - j));
+    }
+    __device__ __forceinline__ double exp(double x) const {
+        x = fmax(x, -1100.0);
+        const double n = __builtin_rint(x * 0x1.71547652b82fep+6);
+        const double r = __builtin_fma(n, -0x1.abc9e3b39803fp-62, __builtin_fma(n, -0x1.62e42fefa39efp-7, x));
+        const int k = static_cast<int>(n);
+        double y = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
+        y = __builtin_fma(y, r, 1.0 / 6.0);
+        y = __builtin_fma(y, r, 0.5);
+        y = __builtin_fma(y, r, 1.0);
+        y = __builtin_fma(y, r, 1.0);
+        return __builtin_amdgcn_ldexp(y * p[k & 63], (k >> 6) + 1);
+    }
+};
+
 // max(0, p - q) and p of tokens of the stop row.
 struct Rest {
     const uint16_t* logits;
@@ -698,9 +726,12 @@ struct Rest {
             without = v.a.ids[stop.row() + 1u];
         }
     }
+    static __device__ __forceinline__ double chance(const RowStat& r, const Powers& powers, float x) {   // of a token that r keeps
+        return r.kind == kInfinite ? r.by_kept : powers.exp((static_cast<double>(x) - r.top) * r.by_t) * r.by_kept;
+    }
     // f(k, max(0, p - q), p) for the tokens begin + k, k < 8, that p keeps.
     template <typename F>
-    __device__ __forceinline__ void each(uint32_t begin, F&& f) const {
+    __device__ __forceinline__ void each(const Powers& powers, uint32_t begin, F&& f) const {
         Eight x, y;
         if (begin + 8u <= vocab) {
             __builtin_memcpy(&x, logits + begin, 16);
@@ -714,10 +745,14 @@ struct Rest {
         }
 #pragma unroll
         for (uint32_t k = 0; k < 8u; ++k) {
-            const double here = probability(p, x.v[k], begin + k);
-            if (!(here > 0.0)) continue;
+            const float l = logit_of(x.v[k]);
+            if (!keeps(p, l, begin + k)) continue;
+            const double here = chance(p, powers, l);
             double rest = here;
-            if (draft_logits != nullptr) rest = fmax(0.0, here - probability(q, y.v[k], begin + k));
+            if (draft_logits != nullptr) {
+                const float d = logit_of(y.v[k]);
+                if (keeps(q, d, begin + k)) rest = fmax(0.0, here - chance(q, powers, d));
+            }
             if (begin + k == without) rest = 0.0;
             f(k, rest, here);
         }
@@ -727,15 +762,18 @@ struct Rest {
 // The sums of max(0, p - q) and of p over the tiles of each request's stop row: `groups` workgroups to each.
 __global__ __launch_bounds__(kFew) void verify_sum_kernel(VerifyParams p) {
     __shared__ double waves[2][kFewWaves];
+    __shared__ Powers powers;
     const uint32_t tid = threadIdx.x;
     const uint32_t request = blockIdx.x / p.groups;
+    powers.fill();
     const Stop stop = find_stop(p, request);
     if (stop.rows == 0u) return;
     const Rest rest(p, stop);
+    __syncthreads();
 #pragma unroll 1
     for (uint32_t tile = blockIdx.x - request * p.groups; tile < p.tiles; tile += p.groups) {
         double r_sum = 0.0, p_sum = 0.0;
-        rest.each(tile * kTile + 8u * tid, [&](uint32_t, double r, double here) HYP_INLINE {
+        rest.each(powers, tile * kTile + 8u * tid, [&](uint32_t, double r, double here) HYP_INLINE {
             r_sum += r;
             p_sum += here;
         });
@@ -763,6 +801,7 @@ __global__ __launch_bounds__(kFew) void verify_sum_kernel(VerifyParams p) {
 }
 
 struct DrawLds {
+    Powers powers;
     double mass[kFewWaves];
     double base;
     uint32_t pick[2], tile;
@@ -795,6 +834,7 @@ __global__ __launch_bounds__(kFew) void verify_draw_kernel(VerifyParams p) {
     const VerifyArgs& a = p.a;
     const uint32_t tid = threadIdx.x;
     const uint32_t request = blockIdx.x;
+    s.powers.fill();
     // The sums of the request's tiles: consecutive ones to a thread.
     const double2* const sums = p.sums + static_cast<size_t>(request) * p.tiles;
     const uint32_t per = (p.tiles + kFew - 1u) / kFew;
@@ -851,7 +891,7 @@ __global__ __launch_bounds__(kFew) void verify_draw_kernel(VerifyParams p) {
     const uint32_t from = s.tile * kTile + 8u * tid;
     const double base = s.base;
     double v[8] = {}, sum = 0.0;
-    rest.each(from, [&](uint32_t k, double r, double here) HYP_INLINE {
+    rest.each(s.powers, from, [&](uint32_t k, double r, double here) HYP_INLINE {
         v[k] = by_rest ? r : here;
         sum += v[k];
     });
