@@ -42,6 +42,48 @@ namespace {
 
 using namespace sampling;
 
+__device__ __forceinline__ uint32_t block_min(uint32_t v, Block& s) {
+    v = from_lane(wave_scan(v, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0u) s.u[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint32_t r = 0xFFFFFFFFu;
+    for (uint32_t w = 0; w < kWaves; ++w) r = min(r, s.u[w]);
+    return r;
+}
+
+// Mass and count before this thread's bins, and the totals: added in the same order for every thread.
+struct Before {
+    double mass, mass_all;
+    uint32_t count, count_all;
+};
+
+// (Every wave has left the block's words.)
+__device__ __forceinline__ Before block_scan(double mass, uint32_t count, Block& s) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = threadIdx.x >> 6;
+    const double m = wave_incl64(mass);
+    const uint32_t c = wave_incl(count);
+    if (lane == 63u) {
+        s.d[wave] = m;
+        s.u[wave] = c;
+    }
+    __syncthreads();
+    Before b{0.0, 0.0, 0u, 0u};
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        if (w == wave) {
+            b.mass = b.mass_all;
+            b.count = b.count_all;
+        }
+        b.mass_all += s.d[w];
+        b.count_all += s.u[w];
+    }
+    const double mx = __shfl_up(m, 1u, 64);
+    if (lane != 0u) b.mass += mx;
+    b.count += c - count;
+    return b;
+}
+
 __global__ __launch_bounds__(kThreads) void sample_count_kernel(const uint16_t* __restrict__ logits, uint32_t vocab,
                                                                 Chunks chunks, ChunkCounts* __restrict__ counts) {
     __shared__ RowLds s;
@@ -353,17 +395,84 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         if (windowed) find(std::true_type{}); else find(std::false_type{});
     }
 
-    // 3. The token, in the row or in the chunk that holds it.
+    // 3. The token, in the row or in the chunk that holds it: each wave marks the value's places in its stretch, 512
+    // tokens a step.
+    const uint32_t drawn = s.drawn;
     uint32_t number = s.number;
     uint32_t from_token = 0u, to_token = vocab;
     if (kSplit && s.bin != kBins) {
-        from_token = min(vocab, find_chunk(counts, chunks.n, count_at(s.bin), number) * chunks.tokens);
+        const uint32_t at = count_at(s.bin);
+        uint32_t chunk = 0u;
+        for (uint32_t base = 0; base < chunks.n; base += 64u) {   // (every wave for itself)
+            const uint32_t n = base + lane < chunks.n ? counts[base + lane].count[at] : 0u;
+            const uint32_t incl = wave_incl(n);
+            const uint64_t past = __ballot(incl > number);
+            if (past != 0u) {
+                const uint32_t holder = static_cast<uint32_t>(__builtin_ctzll(past));
+                chunk = base + holder;
+                number -= from_lane(incl - n, holder);
+                break;
+            }
+            number -= from_lane(incl, 63u);
+        }
+        from_token = min(vocab, chunk * chunks.tokens);
         to_token = min(vocab, from_token + chunks.tokens);
     }
-    find_token<8>(row, from_token, to_token, s.drawn, number, s.block.u, [&](uint32_t token) {
-        tokens[row_at] = token;
-        if (logprobs != nullptr) logprobs[row_at] = static_cast<float>(logprob);
-    });
+    constexpr uint32_t kStep = 512u, kSteps = 8u;
+    for (uint32_t base = from_token; base < to_token; base += kWaves * kSteps * kStep) {
+        const uint32_t end = min(to_token, base + kWaves * kSteps * kStep);
+        const uint32_t steps = (end - base + kWaves * kStep - 1u) / (kWaves * kStep);
+        const uint32_t begin = base + wave * steps * kStep + 8u * lane;   // the lane's, of the first step
+        Eight e[kSteps];
+#pragma unroll
+        for (uint32_t k = 0; k < kSteps; ++k)
+            if (k < steps && begin + k * kStep + 8u <= end) __builtin_memcpy(&e[k], row + begin + k * kStep, 16);
+        uint64_t hits = 0u;   // a byte a step
+#pragma unroll
+        for (uint32_t k = 0; k < kSteps; ++k) {
+            const uint32_t from = begin + k * kStep;
+            if (k >= steps || from >= end) continue;
+            uint32_t bits = 0u;
+            if (from + 8u <= end) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) bits |= plain_bits(e[k].v[i]) == drawn ? 1u << i : 0u;
+            } else {
+                for (uint32_t i = 0; from + i < end; ++i) bits |= plain_bits(row[from + i]) == drawn ? 1u << i : 0u;
+            }
+            hits |= static_cast<uint64_t>(bits) << (8u * k);
+        }
+        const uint32_t mine = wave_sum(static_cast<uint32_t>(__popcll(hits)));
+        __syncthreads();
+        if (lane == 0u) s.block.u[wave] = mine;
+        __syncthreads();
+        uint32_t before = 0u, all = 0u;
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            if (w == wave) before = all;
+            all += s.block.u[w];
+        }
+        if (number >= all) {
+            number -= all;
+            continue;
+        }
+        uint32_t left = number - before;   // (wraps past the holder)
+        if (left >= mine) return;
+        for (uint32_t k = 0; k < steps; ++k) {
+            uint32_t bits = static_cast<uint32_t>(hits >> (8u * k)) & 0xFFu;
+            const uint32_t n = static_cast<uint32_t>(__popc(bits));
+            const uint32_t incl = wave_incl(n);
+            const uint32_t step = from_lane(incl, 63u);
+            if (left < step) {
+                if (left - (incl - n) < n) {
+                    for (uint32_t i = left - (incl - n); i != 0u; --i) bits &= bits - 1u;
+                    tokens[row_at] = begin + k * kStep + static_cast<uint32_t>(__builtin_ctz(bits));
+                    if (logprobs != nullptr) logprobs[row_at] = static_cast<float>(logprob);
+                }
+                return;
+            }
+            left -= step;
+        }
+        return;
+    }
 }
 
 // A row's chunks: enough workgroups for the device (two are on a compute unit), but no more than the second launch

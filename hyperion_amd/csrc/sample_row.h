@@ -43,7 +43,8 @@ struct RowParams {
     bool greedy;
 };
 
-__device__ __forceinline__ RowParams row_params(const HypSamplingConfig& c, float u) {
+__device__ __forceinline__ RowParams row_params(const HypSamplingConfig& config, float u) {
+    const HypSamplingConfig c = config;   // (one load)
     RowParams r;
     r.greedy = !(c.temperature > 0.0f);
     r.by_t = r.greedy ? 1.0 : 1.0 / static_cast<double>(c.temperature);
@@ -88,48 +89,6 @@ struct Block {
     double d[kWaves];
     uint32_t u[kWaves];
 };
-
-__device__ __forceinline__ uint32_t block_min(uint32_t v, Block& s) {
-    v = from_lane(wave_scan(v, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0u) s.u[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint32_t r = 0xFFFFFFFFu;
-    for (uint32_t w = 0; w < kWaves; ++w) r = min(r, s.u[w]);
-    return r;
-}
-
-// Mass and count before this thread's bins, and the totals: added in the same order for every thread.
-struct Before {
-    double mass, mass_all;
-    uint32_t count, count_all;
-};
-
-// (Every wave has left the block's words.)
-__device__ __forceinline__ Before block_scan(double mass, uint32_t count, Block& s) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t wave = threadIdx.x >> 6;
-    const double m = wave_incl64(mass);
-    const uint32_t c = wave_incl(count);
-    if (lane == 63u) {
-        s.d[wave] = m;
-        s.u[wave] = c;
-    }
-    __syncthreads();
-    Before b{0.0, 0.0, 0u, 0u};
-    for (uint32_t w = 0; w < kWaves; ++w) {
-        if (w == wave) {
-            b.mass = b.mass_all;
-            b.count = b.count_all;
-        }
-        b.mass_all += s.d[w];
-        b.count_all += s.u[w];
-    }
-    const double mx = __shfl_up(m, 1u, 64);
-    if (lane != 0u) b.mass += mx;
-    b.count += c - count;
-    return b;
-}
 
 // e^x of an x <= 0: 2^n e^r with r = x - n ln 2 in [-ln 2 / 2, ln 2 / 2], the series to r^13 (the rest is below 2^-57).
 // Without the library's branches nine of them run side by side.
@@ -218,7 +177,7 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
     __syncthreads();
 }
 
-// A chunk's counts between the two launches (a chunk has at most kMaxChunk tokens: 16 bits do).
+// A chunk's counts between two launches (a chunk has fewer than 65536 tokens: 16 bits do).
 constexpr uint32_t kStoredBins = (kBins + 7u) & ~7u;
 constexpr uint32_t kMaxChunk = 32768;
 struct alignas(16) ChunkCounts {
@@ -260,70 +219,6 @@ __device__ __forceinline__ uint32_t find_chunk(const ChunkCounts* counts, uint32
         number -= from_lane(incl, 63u);
     }
     return 0u;
-}
-
-// f(index) by the lane that holds it, of the number-th token of the value `drawn` among the tokens [begin, end) of a row, by a
-// workgroup with a word a wave in LDS. Each wave marks the value's places in its stretch, 512 tokens a step, kSteps at once.
-template <uint32_t kSteps, typename F>
-__device__ __forceinline__ void find_token(const uint16_t* row, uint32_t from_token, uint32_t to_token, uint32_t drawn,
-                                           uint32_t number, uint32_t* waves, F&& f) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t wave = threadIdx.x >> 6;
-    static_assert(kSteps <= 8u, "a byte a step");
-    constexpr uint32_t kStep = 512u;
-    for (uint32_t base = from_token; base < to_token; base += kWaves * kSteps * kStep) {
-        const uint32_t end = min(to_token, base + kWaves * kSteps * kStep);
-        const uint32_t steps = (end - base + kWaves * kStep - 1u) / (kWaves * kStep);
-        const uint32_t begin = base + wave * steps * kStep + 8u * lane;   // the lane's, of the first step
-        Eight e[kSteps];
-#pragma unroll
-        for (uint32_t k = 0; k < kSteps; ++k)
-            if (k < steps && begin + k * kStep + 8u <= end) __builtin_memcpy(&e[k], row + begin + k * kStep, 16);
-        uint64_t hits = 0u;   // a byte a step
-#pragma unroll
-        for (uint32_t k = 0; k < kSteps; ++k) {
-            const uint32_t from = begin + k * kStep;
-            if (k >= steps || from >= end) continue;
-            uint32_t bits = 0u;
-            if (from + 8u <= end) {
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) bits |= plain_bits(e[k].v[i]) == drawn ? 1u << i : 0u;
-            } else {
-                for (uint32_t i = 0; from + i < end; ++i) bits |= plain_bits(row[from + i]) == drawn ? 1u << i : 0u;
-            }
-            hits |= static_cast<uint64_t>(bits) << (8u * k);
-        }
-        const uint32_t mine = wave_sum(static_cast<uint32_t>(__popcll(hits)));
-        __syncthreads();
-        if (lane == 0u) waves[wave] = mine;
-        __syncthreads();
-        uint32_t before = 0u, all = 0u;
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            if (w == wave) before = all;
-            all += waves[w];
-        }
-        if (number >= all) {
-            number -= all;
-            continue;
-        }
-        uint32_t left = number - before;   // (wraps past the holder)
-        if (left >= mine) return;
-        for (uint32_t k = 0; k < steps; ++k) {
-            uint32_t bits = static_cast<uint32_t>(hits >> (8u * k)) & 0xFFu;
-            const uint32_t n = static_cast<uint32_t>(__popc(bits));
-            const uint32_t incl = wave_incl(n);
-            const uint32_t step = from_lane(incl, 63u);
-            if (left < step) {
-                if (left - (incl - n) < n) {
-                    for (uint32_t i = left - (incl - n); i != 0u; --i) bits &= bits - 1u;
-                    f(begin + k * kStep + static_cast<uint32_t>(__builtin_ctz(bits)));
-                }
-                return;
-            }
-            left -= step;
-        }
-        return;
-    }
 }
 
 #undef HYP_INLINE
