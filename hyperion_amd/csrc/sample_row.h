@@ -110,6 +110,7 @@ struct alignas(16) RowLds {
     Block block;
     uint32_t infinite;             // +inf tokens
     uint32_t centre_lo, centre_hi; // least and largest place of the values next to 0
+    uint32_t below;                // bits of the largest value below the fine ones (their least)
     uint32_t drawn, number;        // the drawn value's bits, the token's number among those
     uint32_t bin;                  // and its bin, kBins where that is none of the first way
     double kept;                   // the kept tokens' mass
@@ -117,7 +118,8 @@ struct alignas(16) RowLds {
     uint32_t lead[kWaves];         // a wave's first bin with a token
 };
 
-// s.count, s.infinite, s.centre_lo and s.centre_hi of the tokens [begin, end) of a row. (A call has a barrier at its end.)
+// s.count, s.infinite, s.centre_lo, s.centre_hi and s.below of the tokens [begin, end) of a row. (A call has a barrier at its
+// end.)
 __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin, uint32_t end, RowLds& s) {
     const uint32_t tid = threadIdx.x;
     for (uint32_t i = tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
@@ -125,8 +127,12 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
         s.infinite = 0u;
         s.centre_lo = 0xFFFFFFFFu;
         s.centre_hi = 0u;
+        s.below = 0xFFFFFFFFu;
     }
     __syncthreads();
+    // Masked tokens, most of a row maybe, are counted in registers (through LDS 60 % of 640 rows of 262144 at the type's lowest
+    // value took 320 us).
+    uint32_t below = 0u, below_bits = 0xFFFFFFFFu;
     // The bits less kLow, in 16 bits: a fine value has 0 in bits 12 to 14, its sign in bit 15.
     const auto one = [&](uint32_t b) HYP_INLINE {
         const uint32_t t = b - kLow;
@@ -134,6 +140,10 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
             atomicAdd(&s.count[(t & 0xFFFu) | ((t >> 3) & 0x1000u)], 1u);
             return;
         }
+        const bool low = b - 0xC300u < 0xFF80u - 0xC300u;   // -2^7 to the lowest
+        below += low ? 1u : 0u;
+        below_bits = min(below_bits, low ? b : 0xFFFFFFFFu);
+        if (low || b == 0xFF80u) return;
         b = plain_bits(b);
         if (!finite_bits(b)) {
             if (b == 0x7F80u) atomicAdd(&s.infinite, 1u);
@@ -142,7 +152,7 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
             atomicMax(&s.centre_hi, place_of(b));
             atomicAdd(&s.count[kCentreAt], 1u);
         } else {
-            atomicAdd(&s.count[(b & 0x8000u) != 0u ? kBelowAt : kAboveAt], 1u);
+            atomicAdd(&s.count[kAboveAt], 1u);
         }
     };
     // Eight tokens at once, two in a register, unless one of them is no fine value (the counting of 64 rows of
@@ -174,6 +184,14 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
         }
     }
     for (uint32_t k = i; k < end && k < i + 8u; ++k) one(row[k]);
+    if (__ballot(below != 0u) != 0u) {
+        below = wave_sum(below);
+        below_bits = from_lane(wave_scan(below_bits, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);
+        if ((tid & 63u) == 0u) {
+            atomicAdd(&s.count[kBelowAt], below);
+            atomicMin(&s.below, below_bits);
+        }
+    }
     __syncthreads();
 }
 
@@ -182,7 +200,7 @@ constexpr uint32_t kStoredBins = (kBins + 7u) & ~7u;
 constexpr uint32_t kMaxChunk = 32768;
 struct alignas(16) ChunkCounts {
     uint16_t count[kStoredBins];
-    uint32_t infinite, centre_lo, centre_hi, unused;
+    uint32_t infinite, centre_lo, centre_hi, below;
 };
 static_assert(kStoredBins <= kThreads * kPer && kMaxChunk < 65536u, "a chunk's counts");
 
@@ -200,6 +218,7 @@ __device__ __forceinline__ void store_counts(const RowLds& s, ChunkCounts& c) {
         c.infinite = s.infinite;
         c.centre_lo = s.centre_lo;
         c.centre_hi = s.centre_hi;
+        c.below = s.below;
     }
 }
 

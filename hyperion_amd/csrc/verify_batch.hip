@@ -17,7 +17,8 @@
 //
 // A row takes windows of 8192 values instead of its counts (step 2 over each, counting the row again) where the
 // counts' bins of more than one value matter: a value above 2^7; values next to 0 that hold the cut, or weigh enough that
-// their differences of less than 2^-24 do; values below -2^7 that are not negligible, or hold the cut.
+// their differences of less than 2^-24 do; values below -2^7 that are not negligible, or hold the cut. (Rows with 60 % of the
+// type's lowest value took windows at temperatures of 1.9 and more, 64 requests of 5 of 262144 so 3.0 ms.)
 //
 // Steps 2 to 4 are bound by the instructions that all waves of a workgroup issue alike (scans, parameters, borders): with 16 waves
 // each is 16 cycles, so they have four, and loops over a thread's values are kept rolled.
@@ -210,7 +211,7 @@ struct FilterLds {
     double mass[kFewWaves], kept;        // ..., mass of the kept tokens
     uint32_t word[kFewWaves];
     uint32_t count[kSlots * kRow];       // of slot i of thread t at i * kRow + t; by value, of a window
-    uint32_t infinite, centre_lo, centre_hi, centre, above, below;
+    uint32_t infinite, centre_lo, centre_hi, centre, above, below, below_bits;
     uint32_t lead;                       // kBinsEach * thread + i of the first bin with a token
     uint32_t keep, redo;
     uint32_t cut, number, whole;         // bits of the last kept value, the last kept token's number there, are all kept
@@ -252,7 +253,10 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
     const double mass_before = mass_at.incl - sum;
     const uint32_t count_before = count_at.incl - here;
     total = scalar(mass_at.all);
-    const uint32_t all = count_at.all + s.below;   // (those weigh nothing)
+    // Tokens below -2^7 weigh next to nothing; masked ones nothing at all, so that it is the same whether they are kept.
+    const bool masked = s.below != 0u && (top - value_of(s.below_bits)) * prm.by_t > 750.0;   // (e^-750 is 0)
+    const uint32_t below = masked ? 0u : s.below;
+    const uint32_t all = count_at.all + below;
     uint32_t kept = all;
     if (prm.top_k != 0u) kept = min(kept, prm.top_k);
     // The values of the thread of lane `from`, a slot to a lane: tokens, weight, and what comes before.
@@ -291,7 +295,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
         __syncthreads();
         kept = min(kept, s.keep);
     }
-    if (s.below != 0u) {
+    if (below != 0u) {
         // Nothing there weighs enough for top-p; min-p drops it unless it is tiny: e^-80 is above 2^-116.
         if (prm.min_p != 0.0) kept = min(kept, count_at.all);
         if ((kept > count_at.all && kept != all) || (prm.min_p != 0.0 && prm.min_p < 0x1p-110)) return false;
@@ -309,7 +313,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
             s.whole = kept - o.before == o.n;
         }
     }
-    if (kept == all && s.below != 0u && tid == 0u) {   // everything
+    if (kept == all && below != 0u && tid == 0u) {   // everything
         s.kept = total;
         s.cut = 0xFF7Fu;
         s.number = 0u;
@@ -514,12 +518,12 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
     const uint32_t x = row_at + 1u < a.rows ? a.ids[row_at + 1u] : kNone;   // the row's draft
     if (tid == 0u) {
         s.infinite = s.centre_hi = s.centre = s.above = s.below = s.redo = 0u;
-        s.centre_lo = s.lead = s.keep = kNone;
+        s.centre_lo = s.lead = s.keep = s.below_bits = kNone;
     }
     __syncthreads();
     // The row's counts from its chunks', the other bins a chunk to a thread.
     {
-        uint32_t more[6] = {0u, kNone, 0u, 0u, 0u, 0u};
+        uint32_t more[7] = {0u, kNone, 0u, 0u, 0u, 0u, kNone};
         if (tid < p.chunks.n) {
             const ChunkCounts& c = counts[tid];
             more[0] = c.infinite;
@@ -528,6 +532,7 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
             more[3] = c.count[kCentreAt];
             more[4] = c.count[kAboveAt];
             more[5] = c.count[kBelowAt];
+            more[6] = c.below;
         }
         // Eight bins in each quarter of them to a thread, which then go to the threads that have them.
         uint32_t n[kBinsEach] = {};
@@ -583,6 +588,7 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
             atomicAdd(&s.centre, more[3]);
             atomicAdd(&s.above, more[4]);
             atomicAdd(&s.below, more[5]);
+            atomicMin(&s.below_bits, more[6]);
         }
     }
     if (request == kNone) return;
@@ -616,7 +622,7 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
         const bool next_to_0 = s.centre != 0u && lead >= kFine;   // the largest
         bool counted = s.above == 0u && (next_to_0 ? s.centre_lo == s.centre_hi : lead != kNone);
         r.top = scalar(value_of(next_to_0 ? bits_at(s.centre_lo) : bits_of_bin((lead / kBinsEach) % kFew, lead % kBinsEach)));
-        if (counted && s.below != 0u) counted = (r.top + 128.0) * prm.by_t > 80.0;   // (2^23 times e^-80)
+        if (counted && s.below != 0u) counted = (r.top - value_of(s.below_bits)) * prm.by_t > 80.0;   // (2^23 times e^-80)
         if (counted) counted = filter_counts(prm, r.top, s, r.total);
         r.kind = counted ? kCounted : kWindowed;
         if (!counted) filter_windows(row, a.vocab, prm, r, s);

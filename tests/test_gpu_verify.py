@@ -1,7 +1,7 @@
 """GPU parity of hyp_verify_batch against pages_ref.py's 64-bit reference.
 
 Bars: accepted, rejected and tokens equal. A logprob is one rounding to fp32 of an fp64 value: 2^-24 of itself, plus
-1e-12 for the fp64 sums of up to 262144 weights.
+1e-12 for the fp64 sums (some hundred roundings each: weights are counted by value, and 2^23 tokens are 128 chunks).
 """
 import numpy as np
 import pytest
@@ -251,6 +251,70 @@ def test_cut_among_values_far_below(stream, top_k):
                np.zeros(40))
     v.run()
     v.check(("cut", top_k))
+
+
+LOWEST = -3.3895314e38
+
+
+@pytest.mark.parametrize("fill", [-127.5, -128.0, -129.0, -400.0, -2000.0, LOWEST, -np.inf])
+@pytest.mark.parametrize("allowed", [1, 5, 300])
+def test_masked_tokens(stream, allowed, fill):
+    """Masks of any value under any temperature, with fewer tokens left than top-k keeps; drafts that are masked among them."""
+    say(f"verify: {allowed} tokens left of a mask of {fill}")
+    rng = np.random.default_rng(allowed)
+    vocab, n = 3000, 60
+    x = 4.0 * rng.standard_normal((3 * n, vocab))
+    at = np.argsort(rng.random((n, vocab)), -1)[:, allowed:].repeat(3, 0)
+    y = x + rng.standard_normal(x.shape)
+    np.put_along_axis(x, at, fill, -1)
+    np.put_along_axis(y[::2], at[::2], fill, -1)   # (of some rows the target alone is masked)
+    bits = [syn.bf16_bits(a.astype(np.float32)).reshape(a.shape) for a in (x, y)]
+    some = config([(rng.choice([0.0, 0.3, 1.0, 1.9, 2.5, 60.0, 1e30]), rng.choice([0, 2, 64, 2000]), rng.choice([0.0, 0.95]),
+                    rng.choice([0.0, 0.0, 0.02])) for _ in range(n)])
+    u = np.where(rng.random(3 * n) < 0.2, 0.0, rng.random(3 * n))
+    for draft in (bits[1], None):
+        v = Verify(stream, [3] * n, bits[0], draft, drafts(rng, bits[1], None), some, None, u)
+        v.run()
+        v.check((allowed, fill, draft is None))
+
+
+def test_largest_vocabulary(stream):
+    say("verify: 2^23 tokens")
+    vocab, keep = 1 << 23, 6000001
+    flat = np.full((3, vocab), 0x3F80, np.uint16)
+    v = Verify(stream, [3], flat, None, [0, keep - 1, keep], config([(1.0, keep, 0.0, 0.0)]), None, [0.0, 0.0, 0.7])
+    v.run()
+    got = v.check("flat")
+    assert (got["accepted"][0], got["rejected"][0]) == (1, 1)
+    v = scene(stream, 5, "usual", [2], vocab - 1, True)
+    v.run()
+    v.check("usual")
+
+
+def test_rows_past_2_to_the_32_bytes(stream):
+    """The last rows of 300 of 2^23 tokens, 5 GB: the same as those alone."""
+    say("verify: rows far behind the first")
+    vocab, rows, skip = 1 << 23, 300, 297
+    rng = np.random.default_rng(8)
+    x = syn.bf16_bits((2.5 * rng.standard_normal((3, vocab), np.float32))).reshape(3, vocab)
+    ids = np.concatenate(([0], np.argmax(syn.bf16_to_f32(x[:2]).reshape(2, vocab), -1)))
+    u, c = [0.0, 0.0, 0.6], config([(0.9, 0, 0.99, 0.0)])
+    alone = Verify(stream, [3], x, None, ids, c, None, u)
+    alone.run()
+    want = alone.check("alone")
+    logits = hy.DeviceArray((rows, vocab), np.uint16)
+    hy.call("hyp_memcpy_htod", hy.ctypes.c_void_p(logits.ptr.value + skip * vocab * 2), x.ctypes.data_as(hy.ctypes.c_void_p),
+            x.nbytes, stream.handle)
+    pad = lambda a, t: dev(np.concatenate((np.zeros(skip, t), np.asarray(a, t))), stream)  # noqa: E731
+    out = [dev(np.zeros(1, np.uint32), stream) for _ in range(3)]
+    logprobs = dev(np.full(rows, 77.0, np.float32), stream)
+    work = hy.DeviceArray((hy.verify_batch_workspace_bytes(rows, vocab, 1, False),), np.uint8)
+    hy.verify_batch(logits, None, rows, vocab, dev(np.array([skip, rows], np.uint32), stream), 1, pad(ids, np.uint32), alone.d["configs"],
+                    None, pad(u, np.float32), *out, logprobs, work, stream)
+    got = [o.to_host(stream)[0] for o in out]
+    assert got == [want[k][0] for k in ("accepted", "rejected", "tokens")]
+    got = logprobs.to_host(stream)
+    assert np.array_equal(got[skip:], want["logprobs"]) and np.all(got[:skip] == 77.0)
 
 
 @pytest.mark.parametrize("vocab", [70, 5000, 262144])
