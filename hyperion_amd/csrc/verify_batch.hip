@@ -207,12 +207,19 @@ constexpr uint32_t kSlots = 1u + kBinsEach;   // values of a thread: those next 
 constexpr uint32_t kCentreThread = kFew / 2u;
 constexpr uint32_t kRow = kFew + 1u;            // (four lanes that store slots of one thread do not meet in a bank)
 
-struct FilterLds {
+// What a row has beside its fine values.
+struct Others {
+    uint32_t infinite, centre, above, below;   // tokens
+    uint32_t centre_lo, centre_hi;             // least and largest place of the values next to 0
+    uint32_t below_bits;                       // of the largest below
+    uint32_t lead;                             // kBinsEach * thread + i of the first bin with a token, kNone: none
+};
+
+struct alignas(16) FilterLds {
     double mass[kFewWaves], kept;        // ..., mass of the kept tokens
     uint32_t word[kFewWaves];
     uint32_t count[kSlots * kRow];       // of slot i of thread t at i * kRow + t; by value, of a window
-    uint32_t infinite, centre_lo, centre_hi, centre, above, below, below_bits;
-    uint32_t lead;                       // kBinsEach * thread + i of the first bin with a token
+    alignas(16) uint32_t others[kFewWaves][8];   // a wave's
     uint32_t keep, redo;
     uint32_t cut, number, whole;         // bits of the last kept value, the last kept token's number there, are all kept
     uint32_t last;
@@ -220,7 +227,8 @@ struct FilterLds {
 
 // The filters of a row from its counts in s: leaves s.kept, s.cut, s.number, s.whole and the mass of all tokens. False: the
 // row takes windows. (A call has a barrier at its end.)
-__device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, FilterLds& s, double& total) {
+__device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, const Others& others, FilterLds& s,
+                                              double& total) {
     const uint32_t tid = threadIdx.x;
     const uint32_t lane = tid & 63u;
     const uint32_t centre = s.count[tid];
@@ -228,7 +236,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
     uint32_t here = centre;
     bool light = false;   // min-p drops some
     if (centre != 0u) {
-        centre_weight = exp_below((value_of(bits_at(s.centre_lo)) - top) * prm.by_t);
+        centre_weight = exp_below((value_of(bits_at(others.centre_lo)) - top) * prm.by_t);
         sum = centre * centre_weight;
         light = centre_weight < prm.min_p;
     }
@@ -254,8 +262,8 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
     const uint32_t count_before = count_at.incl - here;
     total = scalar(mass_at.all);
     // Tokens below -2^7 weigh next to nothing; masked ones nothing at all, so that it is the same whether they are kept.
-    const bool masked = s.below != 0u && (top - value_of(s.below_bits)) * prm.by_t > 750.0;   // (e^-750 is 0)
-    const uint32_t below = masked ? 0u : s.below;
+    const bool masked = others.below != 0u && (top - value_of(others.below_bits)) * prm.by_t > 750.0;   // (e^-750 is 0)
+    const uint32_t below = masked ? 0u : others.below;
     const uint32_t all = count_at.all + below;
     uint32_t kept = all;
     if (prm.top_k != 0u) kept = min(kept, prm.top_k);
@@ -269,7 +277,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
         const uint32_t thread = (tid & ~63u) + from;
         if (lane < kSlots) {
             o.n = s.count[lane * kRow + thread];
-            o.bits = lane == 0u ? bits_at(s.centre_lo & 0xFFFFu) : bits_of_bin(thread, lane - 1u);
+            o.bits = lane == 0u ? bits_at(others.centre_lo & 0xFFFFu) : bits_of_bin(thread, lane - 1u);
             if (o.n != 0u) o.w = exp_below((value_of(o.bits) - top) * prm.by_t);
         }
         const double m = o.n * o.w;
@@ -301,7 +309,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
         if ((kept > count_at.all && kept != all) || (prm.min_p != 0.0 && prm.min_p < 0x1p-110)) return false;
     }
     kept = prm.greedy ? 1u : max(kept, 1u);
-    if (centre != 0u && s.centre_lo != s.centre_hi)   // several values next to 0
+    if (centre != 0u && others.centre_lo != others.centre_hi)   // several values next to 0
         s.redo = kept - 1u - count_before < centre || centre * centre_weight * prm.by_t > 0x1p-30 * total;
     const uint64_t holds = __ballot(kept - 1u - count_before < here);
     if (holds != 0u) {
@@ -435,6 +443,8 @@ __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, u
         const uint32_t stop = min(end, base + kFewWaves * kSteps * kStep);
         const uint32_t steps = (stop - base + kFewWaves * kStep - 1u) / (kFewWaves * kStep);
         const uint32_t first = base + wave * steps * kStep + 8u * lane;   // the lane's, of the first step
+        const uint32_t room = first < stop ? stop - first : 0u;
+        const uint32_t whole = room < 8u ? 0u : min(steps, (room - 8u) / kStep + 1u);   // steps with all eight tokens
         uint64_t found = 0u;   // the lane's of each step, four bits to one
         uint32_t mine = 0u;
 #pragma unroll 1
@@ -442,27 +452,31 @@ __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, u
             uint32_t w[4][4];
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j) {
-                const uint32_t from = first + (k + j) * kStep;
-                if (k + j < steps && from + 8u <= stop) {
-                    __builtin_memcpy(w[j], row + from, 16);
+                if (k + j < whole) {
+                    __builtin_memcpy(w[j], row + first + (k + j) * kStep, 16);
                 } else {
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; ++i) w[j][i] = ~pattern;
                 }
             }
+            uint32_t four = 0u;
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j) {
-                u16x2_t apart = {0, 0};
+                u16x2_t same = {0, 0};
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i)
-                    apart += __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, (w[j][i] ^ pattern) & mask), u16x2_t{1, 1});
-                uint32_t n = 8u - apart.x - apart.y;
-                const uint32_t from = first + (k + j) * kStep;
-                if (k + j < steps && from < stop && from + 8u > stop)
-                    for (uint32_t i = from; i < stop; ++i) n += plain_bits(row[i]) == bits ? 1u : 0u;
-                found |= static_cast<uint64_t>(n) << (4u * (k + j));
+                    same += __builtin_elementwise_sub_sat(u16x2_t{1, 1}, __builtin_bit_cast(u16x2_t, (w[j][i] ^ pattern) & mask));
+                const uint32_t n = static_cast<uint32_t>(same.x) + same.y;
+                four |= n << (4u * j);
                 mine += n;
             }
+            found |= static_cast<uint64_t>(four) << (4u * k);
+        }
+        if (whole < steps && whole * kStep < room) {   // the row's last tokens
+            uint32_t n = 0u;
+            for (uint32_t i = first + whole * kStep; i < stop; ++i) n += plain_bits(row[i]) == bits ? 1u : 0u;
+            found |= static_cast<uint64_t>(n) << (4u * whole);
+            mine += n;
         }
         const uint32_t wave_all = wave_sum(mine);
         if (lane == 0u) s.word[wave] = wave_all;
@@ -483,17 +497,19 @@ __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, u
 #pragma unroll 1
             for (uint32_t k = 0; k < steps; ++k) {
                 const uint32_t n = static_cast<uint32_t>(found >> (4u * k)) & 15u;
+                if (__ballot(n != 0u) == 0u) continue;
                 const uint32_t incl = wave_incl(n);
                 const uint32_t step = from_lane(incl, 63u);
                 if (left < step) {
                     if (left - (incl - n) < n) {
-                        uint32_t i = first + k * kStep;
-                        for (uint32_t skip = left - (incl - n);; ++i) {
-                            if (plain_bits(row[i]) != bits) continue;
-                            if (skip == 0u) break;
-                            --skip;
-                        }
-                        s.last = i;
+                        const uint32_t from = first + k * kStep;
+                        uint32_t b[8], places = 0u;
+#pragma unroll
+                        for (uint32_t i = 0; i < 8u; ++i) b[i] = row[min(from + i, stop - 1u)];   // (the last one's copies: behind it)
+#pragma unroll
+                        for (uint32_t i = 0; i < 8u; ++i) places |= plain_bits(b[i]) == bits ? 1u << i : 0u;
+                        for (uint32_t skip = left - (incl - n); skip != 0u; --skip) places &= places - 1u;
+                        s.last = from + static_cast<uint32_t>(__builtin_ctz(places));
                     }
                     break;
                 }
@@ -517,22 +533,22 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
     const uint32_t request = p.requests[index];
     const uint32_t x = row_at + 1u < a.rows ? a.ids[row_at + 1u] : kNone;   // the row's draft
     if (tid == 0u) {
-        s.infinite = s.centre_hi = s.centre = s.above = s.below = s.redo = 0u;
-        s.centre_lo = s.lead = s.keep = s.below_bits = kNone;
+        s.redo = 0u;
+        s.keep = kNone;
     }
     __syncthreads();
     // The row's counts from its chunks', the other bins a chunk to a thread.
     {
-        uint32_t more[7] = {0u, kNone, 0u, 0u, 0u, 0u, kNone};
+        uint32_t sum[4] = {}, least[4] = {kNone, kNone, kNone, kNone};
         if (tid < p.chunks.n) {
             const ChunkCounts& c = counts[tid];
-            more[0] = c.infinite;
-            more[1] = c.centre_lo;
-            more[2] = c.centre_hi;
-            more[3] = c.count[kCentreAt];
-            more[4] = c.count[kAboveAt];
-            more[5] = c.count[kBelowAt];
-            more[6] = c.below;
+            sum[0] = c.infinite;
+            sum[1] = c.count[kCentreAt];
+            sum[2] = c.count[kAboveAt];
+            sum[3] = c.count[kBelowAt];
+            least[0] = c.centre_lo;
+            least[1] = ~c.centre_hi;
+            least[2] = c.below;
         }
         // Eight bins in each quarter of them to a thread, which then go to the threads that have them.
         uint32_t n[kBinsEach] = {};
@@ -549,6 +565,10 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
                 }
             }
             __builtin_amdgcn_sched_barrier(0);   // (all of them on their way before the first is waited for)
+            if (c == 0u) {   // (and those above with them, not where they are used)
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; ++i) asm volatile("" : "+v"(sum[i]), "+v"(least[i]));
+            }
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k) {
 #pragma unroll
@@ -562,7 +582,6 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
                 }
             }
         }
-        uint32_t first = kNone;
 #pragma unroll
         for (uint32_t q = 0; q < kBinsEach / 8u; ++q) {
             const uint32_t bin = 8u * (kFew * q + tid);
@@ -577,18 +596,18 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
                 if (n[8u * q + i] != 0u && (lead == kNone || q < kBinsEach / 16u))
                     lead = q < kBinsEach / 16u ? place - i : place + i;
             }
-            first = min(first, lead);
+            least[3] = min(least[3], lead);
         }
-        first = from_lane(wave_scan(first, kNone, [](uint32_t x_, uint32_t y_) { return min(x_, y_); }), 63u);
-        if (lane == 0u) atomicMin(&s.lead, first);
-        if (tid < p.chunks.n) {
-            if (more[0] != 0u) atomicAdd(&s.infinite, more[0]);
-            atomicMin(&s.centre_lo, more[1]);
-            atomicMax(&s.centre_hi, more[2]);
-            atomicAdd(&s.centre, more[3]);
-            atomicAdd(&s.above, more[4]);
-            atomicAdd(&s.below, more[5]);
-            atomicMin(&s.below_bits, more[6]);
+        // (By the wave: with additions to one word in LDS by several lanes this took 4000 cycles.)
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            sum[i] = wave_sum(sum[i]);
+            least[i] = from_lane(wave_scan(least[i], kNone, [](uint32_t x_, uint32_t y_) { return min(x_, y_); }), 63u);
+        }
+        if (lane == 0u) {
+            uint4* const to = reinterpret_cast<uint4*>(s.others[tid >> 6]);
+            to[0] = make_uint4(sum[0], sum[1], sum[2], sum[3]);
+            to[1] = make_uint4(least[0], least[1], least[2], least[3]);
         }
     }
     if (request == kNone) return;
@@ -597,13 +616,26 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
     prm.top_p = scalar(prm.top_p);
     prm.min_p = scalar(prm.min_p);
     __syncthreads();
-    s.count[tid] = tid == kCentreThread ? s.centre : 0u;   // (this thread's alone)
+    Others others;
+    {
+        uint32_t sum[4] = {}, least[4] = {kNone, kNone, kNone, kNone};
+#pragma unroll
+        for (uint32_t w = 0; w < kFewWaves; ++w)
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                sum[i] += s.others[w][i];
+                least[i] = min(least[i], s.others[w][4u + i]);
+            }
+        others = {from_lane(sum[0], 0u),   from_lane(sum[1], 0u),    from_lane(sum[2], 0u),   from_lane(sum[3], 0u),
+                  from_lane(least[0], 0u), ~from_lane(least[1], 0u), from_lane(least[2], 0u), from_lane(least[3], 0u)};
+    }
+    s.count[tid] = tid == kCentreThread ? others.centre : 0u;   // (this thread's alone)
     RowStat r{};
     r.by_t = prm.by_t;
     r.cut = __builtin_nanf("");
-    if (s.infinite != 0u) {
+    if (others.infinite != 0u) {
         // Weight 1 for each, 0 for everything else.
-        const uint32_t infinite = s.infinite;
+        const uint32_t infinite = others.infinite;
         uint32_t kept = infinite;
         if (prm.top_k != 0u) kept = min(kept, prm.top_k);
         if (prm.top_p != 0.0) kept = min(kept, static_cast<uint32_t>(ceil(prm.top_p * infinite)));
@@ -617,13 +649,13 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
         r.kind = kInfinite;
         r.total = infinite;
         __syncthreads();
-    } else if (s.lead != kNone || s.centre != 0u || s.above != 0u || s.below != 0u) {
-        const uint32_t lead = s.lead;
-        const bool next_to_0 = s.centre != 0u && lead >= kFine;   // the largest
-        bool counted = s.above == 0u && (next_to_0 ? s.centre_lo == s.centre_hi : lead != kNone);
-        r.top = scalar(value_of(next_to_0 ? bits_at(s.centre_lo) : bits_of_bin((lead / kBinsEach) % kFew, lead % kBinsEach)));
-        if (counted && s.below != 0u) counted = (r.top - value_of(s.below_bits)) * prm.by_t > 80.0;   // (2^23 times e^-80)
-        if (counted) counted = filter_counts(prm, r.top, s, r.total);
+    } else if (others.lead != kNone || others.centre != 0u || others.above != 0u || others.below != 0u) {
+        const uint32_t lead = others.lead;
+        const bool next_to_0 = others.centre != 0u && lead >= kFine;   // the largest
+        bool counted = others.above == 0u && (next_to_0 ? others.centre_lo == others.centre_hi : lead != kNone);
+        r.top = scalar(value_of(next_to_0 ? bits_at(others.centre_lo) : bits_of_bin((lead / kBinsEach) % kFew, lead % kBinsEach)));
+        if (counted && others.below != 0u) counted = (r.top - value_of(others.below_bits)) * prm.by_t > 80.0;   // (2^23 times e^-80)
+        if (counted) counted = filter_counts(prm, r.top, others, s, r.total);
         r.kind = counted ? kCounted : kWindowed;
         if (!counted) filter_windows(row, a.vocab, prm, r, s);
     }
