@@ -223,6 +223,10 @@ struct alignas(16) FilterLds {
     uint32_t keep, redo;
     uint32_t cut, number, whole;         // bits of the last kept value, the last kept token's number there, are all kept
     uint32_t last;
+    // Of a row by windows: each one's.
+    double window_mass[kWindows];
+    uint32_t window_count[kWindows];
+    uint32_t window_light;   // a bit each: min-p drops some
 };
 
 // The filters of a row from its counts in s: leaves s.kept, s.cut, s.number, s.whole and the mass of all tokens. False: the
@@ -345,7 +349,10 @@ __device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t voc
     for (uint32_t w = 0; w < kWindows; ++w)
         if (few_min((held >> w) & 1u ? 0u : 1u, s.word) == 0u) windows |= 1u << w;
     r.top = scalar(value_of(bits_at(best)));
-    uint32_t kept = kNone;
+    for (uint32_t k = best / kWindow + 1u; k < kWindows; ++k)   // (e^-750 is 0: the same whether they are kept)
+        if ((value_of(bits_at(k * kWindow)) - r.top) * prm.by_t < -750.0) windows &= ~(1u << k);
+    if (tid == 0u) s.window_light = 0u;
+    uint32_t kept = kNone, counted = kNone;
     // Step 0: the mass and number of all tokens; 1: what top-p and min-p keep; 2: the last kept one.
 #pragma unroll 1
     for (uint32_t step = 0; step < 3u; ++step) {
@@ -355,32 +362,53 @@ __device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t voc
         for (uint32_t k = 0; k < kWindows; ++k) {
             if (((windows >> k) & 1u) == 0u) continue;
             const uint32_t window = k * kWindow;
+            const double enough = prm.top_p * r.total;
+            // Those that a filter ends in or that hold the last kept token are looked into, the others have their sums.
+            if ((step == 1u && !(prm.top_p != 0.0 && mass_all + s.window_mass[k] > enough) && ((s.window_light >> k) & 1u) == 0u) ||
+                (step == 2u && kept - 1u - count_all >= s.window_count[k])) {
+                mass_all += s.window_mass[k];
+                count_all += s.window_count[k];
+                continue;
+            }
             __syncthreads();
-            for (uint32_t i = tid; i < kWindow; i += kFew) s.count[i] = 0u;
-            __syncthreads();
-            for_tokens(row, 0u, vocab, tid, kFew, [&](uint32_t, uint32_t b) HYP_INLINE {
-                b = plain_bits(b);
-                const uint32_t d = place_of(b) - window;
-                if (finite_bits(b) && d < kWindow) atomicAdd(&s.count[d], 1u);
-            });
-            __syncthreads();
+            if (counted != k) {
+                for (uint32_t i = tid; i < kWindow; i += kFew) s.count[i] = 0u;
+                __syncthreads();
+                for_tokens(row, 0u, vocab, tid, kFew, [&](uint32_t, uint32_t b) HYP_INLINE {
+                    b = plain_bits(b);
+                    const uint32_t d = place_of(b) - window;
+                    if (finite_bits(b) && d < kWindow) atomicAdd(&s.count[d], 1u);
+                });
+                __syncthreads();
+                counted = k;
+            }
             const auto weight = [&](uint32_t i) HYP_INLINE {
                 return exp_below((value_of(bits_at(window + kBinsEach * tid + i)) - r.top) * r.by_t);
             };
             double sum = 0.0;
             uint32_t here = 0u;
+            bool light = false;
 #pragma unroll 1
             for (uint32_t i = 0; i < kBinsEach; ++i) {
                 const uint32_t n = s.count[kBinsEach * tid + i];
-                if (n != 0u) sum += n * weight(i);
+                if (n == 0u) continue;
+                const double w = weight(i);
+                sum += n * w;
+                light = light || w < prm.min_p;
                 here += n;
             }
             const Scan<double> mass_at = few_scan(sum, s.mass);
             const Scan<uint32_t> count_at = few_scan(here, s.word);
             double mass = mass_all + (mass_at.incl - sum);
             uint32_t count = count_all + (count_at.incl - here);
+            if (step == 0u) {
+                if (light) atomicOr(&s.window_light, 1u << k);
+                if (tid == 0u) {
+                    s.window_mass[k] = mass_at.all;
+                    s.window_count[k] = count_at.all;
+                }
+            }
             if (step == 1u && here != 0u) {
-                const double enough = prm.top_p * r.total;
                 bool open = true;
 #pragma unroll 1
                 for (uint32_t i = 0; i < kBinsEach && open; ++i) {
@@ -413,6 +441,11 @@ __device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t voc
             }
             mass_all += mass_at.all;
             count_all += count_at.all;
+            if (step == 2u) break;
+            if (step == 1u) {
+                __syncthreads();
+                if (s.keep != kNone) break;
+            }
         }
         __syncthreads();
         if (step == 0u) {

@@ -253,6 +253,28 @@ def test_cut_among_values_far_below(stream, top_k):
     v.check(("cut", top_k))
 
 
+@pytest.mark.parametrize("vocab", [700, 20001])
+def test_filters_end_anywhere_in_the_order(stream, vocab):
+    """Logits on both sides of 2^7 and of 0, at temperatures under which all of them weigh something: the filters end among the
+    large, the small, the negative or the far negative ones."""
+    say(f"verify: a wide order of {vocab}")
+    rng = np.random.default_rng(vocab)
+    n = 96
+    x = rng.uniform(-400.0, 300.0, (2 * n, vocab))
+    x[:, ::9] = 1e-9 * x[:, ::9]
+    x[::3] = np.where(x[::3] > 0.0, x[::3] * 1e-3, x[::3])     # (and some whose largest is small)
+    bits = syn.bf16_bits(x.astype(np.float32)).reshape(x.shape)
+    some = config([(rng.choice([20.0, 100.0, 400.0, 3000.0]), rng.choice([0, 0, vocab // 3, vocab - vocab // 9]),
+                    rng.choice([0.0, 0.2, 0.6, 0.97, 0.99999]), rng.choice([0.0, 0.0, 0.9, 0.5, 0.02, 1e-5])) for _ in range(n)])
+    v = Verify(stream, [2] * n, bits, None, rng.integers(0, vocab, 2 * n), some, None,
+               np.where(rng.random(2 * n) < 0.3, 0.0, rng.random(2 * n)))
+    v.run()
+    v.check("wide")
+    v = Verify(stream, [2] * n, bits, np.roll(bits, 1, 0), rng.integers(0, vocab, 2 * n), some, some[::-1].copy(), rng.random(2 * n))
+    v.run()
+    v.check("wide, drafted")
+
+
 LOWEST = -3.3895314e38
 
 
