@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(const uint16_t* 
     __shared__ RowLds s;
     const uint32_t row = blockIdx.x / chunks.n;
     const uint32_t begin = min(vocab, (blockIdx.x - row * chunks.n) * chunks.tokens);
-    count_values(logits + static_cast<size_t>(row) * vocab, begin, min(vocab, begin + chunks.tokens), s);
+    count_values<0u>(logits + static_cast<size_t>(row) * vocab, begin, min(vocab, begin + chunks.tokens), s);
     store_counts(s, counts[blockIdx.x]);
 }
 
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const uint16_t* _
         counts += static_cast<size_t>(row_at) * chunks.n;
         sum_counts(counts, chunks.n, s);
     } else {
-        count_values(row, 0u, vocab, s);
+        count_values<0u>(row, 0u, vocab, s);
     }
 
     // 2. The drawn value and the token's number among those of that value.

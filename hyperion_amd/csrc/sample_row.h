@@ -119,9 +119,19 @@ struct alignas(16) RowLds {
 };
 
 // s.count, s.infinite, s.centre_lo, s.centre_hi and s.below of the tokens [begin, end) of a row. (A call has a barrier at its
-// end.)
+// end.) kAhead > 0: the 16-byte loads of a thread, at most so many for all of [begin, end), are all on their way before the
+// counts are cleared.
+template <uint32_t kAhead>
 __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin, uint32_t end, RowLds& s) {
     const uint32_t tid = threadIdx.x;
+    uint32_t i = begin + 8u * tid;
+    uint32_t ahead[kAhead != 0u ? kAhead : 1u][4];
+    if constexpr (kAhead != 0u) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k)
+            if (i + k * 8u * kThreads + 8u <= end) __builtin_memcpy(ahead[k], row + i + k * 8u * kThreads, 16);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     for (uint32_t i = tid; i < kThreads * kPer; i += kThreads) s.count[i] = 0u;
     if (tid == 0u) {
         s.infinite = 0u;
@@ -158,11 +168,8 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
     // Eight tokens at once, two in a register, unless one of them is no fine value (the counting of 64 rows of
     // 262144 took 12.2 us one by one and takes 9.5).
     typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-    uint32_t i = begin + 8u * tid;
-#pragma unroll 4
-    for (; i + 8u <= end; i += 8u * kThreads) {
-        uint32_t w[4], at[4], odd = 0u;
-        __builtin_memcpy(w, row + i, 16);
+    const auto eight = [&](const uint32_t (&w)[4]) HYP_INLINE {
+        uint32_t at[4], odd = 0u;
 #pragma unroll
         for (uint32_t k = 0; k < 4u; ++k) {
             const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2_t, w[k]) - u16x2_t{kLow, kLow});
@@ -181,6 +188,21 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
                 one(w[k] & 0xFFFFu);
                 one(w[k] >> 16);
             }
+        }
+    };
+    if constexpr (kAhead != 0u) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k)
+            if (i + 8u <= end) {
+                eight(ahead[k]);
+                i += 8u * kThreads;
+            }
+    } else {
+#pragma unroll 4
+        for (; i + 8u <= end; i += 8u * kThreads) {
+            uint32_t w[4];
+            __builtin_memcpy(w, row + i, 16);
+            eight(w);
         }
     }
     for (uint32_t k = i; k < end && k < i + 8u; ++k) one(row[k]);
