@@ -1094,6 +1094,13 @@ bool aligned4(std::initializer_list<const void*> all) {
 // What may be the array `out` itself, as an input of its own otherwise.
 Span unless_same(const void* in, const void* out, uint64_t bytes) { return in == out ? Span{nullptr, 0} : Span{in, bytes}; }
 
+// The batch of a call on its tables' entries, which the kernels number with 32 bits.
+hyperion::hip::BatchView pages_ref(const HypBatch* batch) {
+    const hyperion::hip::BatchView b = batch_ref(batch);
+    REQUIRE_ARG(uint64_t{b.requests} * b.max_blocks < (1ull << 31), "requests * max_blocks must be below 2^31");
+    return b;
+}
+
 uint64_t table_bytes(const hyperion::hip::BatchView& b) { return uint64_t{4} * b.requests * b.max_blocks; }
 
 }  // namespace
@@ -1105,7 +1112,7 @@ HypStatus hyp_batch_fork(const HypBatch* batch, const uint32_t* lens, const uint
                          HypBlockCopy* copies, uint32_t* n_copies, HypStream stream) {
     return abi_call("hyp_batch_fork", [&] {
         hipStream_t s = stream_of(stream);
-        const hyperion::hip::BatchView b = batch_ref(batch);
+        const hyperion::hip::BatchView b = pages_ref(batch);
         REQUIRE_ARG(b.requests == 0 || (lens != nullptr && parents != nullptr && copies != nullptr),
                     "lens, parents and copies must be non-null device pointers");
         REQUIRE_ARG(free_blocks != nullptr && taken != nullptr && taken_out != nullptr && served != nullptr &&
@@ -1126,7 +1133,7 @@ HypStatus hyp_batch_rewind(const HypBatch* batch, const uint32_t* lens, const ui
                            void* workspace, size_t workspace_bytes, HypStream stream) {
     return abi_call("hyp_batch_rewind", [&] {
         hipStream_t s = stream_of(stream);
-        const hyperion::hip::BatchView b = batch_ref(batch);
+        const hyperion::hip::BatchView b = pages_ref(batch);
         REQUIRE_ARG(b.requests == 0 || (lens != nullptr && drop != nullptr && copies != nullptr),
                     "lens, drop and copies must be non-null device pointers");
         REQUIRE_ARG(free_blocks != nullptr && taken != nullptr && taken_out != nullptr && n_copies != nullptr,
@@ -1149,7 +1156,7 @@ HypStatus hyp_batch_compact(const HypBatch* batch, uint32_t* tables_out, uint32_
                             size_t workspace_bytes, HypStream stream) {
     return abi_call("hyp_batch_compact", [&] {
         hipStream_t s = stream_of(stream);
-        const hyperion::hip::BatchView b = batch_ref(batch);
+        const hyperion::hip::BatchView b = pages_ref(batch);
         REQUIRE_ARG(b.requests == 0 || b.max_blocks == 0 || tables_out != nullptr,
                     "tables_out must be a non-null device pointer");
         REQUIRE_ARG(b.prefix == 0 || (b.prefix_table != nullptr && prefix_out != nullptr),
@@ -1192,7 +1199,8 @@ HypStatus hyp_batch_copy(const HypBatch* batch, const HypKvCache* caches, uint32
         std::vector<hyperion::hip::CopyCache> all(n_caches);
         for (uint32_t i = 0; i < n_caches; ++i) {
             HypKvCacheOpaque& c = batch_cache(*batch, caches[i]);
-            all[i] = {static_cast<uint8_t*>(c.k.data()), static_cast<uint8_t*>(c.v.data()), 2u * c.num_kv_heads * c.head_dim};
+            all[i] = {static_cast<uint8_t*>(c.k.data()), static_cast<uint8_t*>(c.v.data()),
+                      uint64_t{2} * c.num_kv_heads * c.head_dim};
         }
         hyperion::hip::launch_batch_copy(b, all.data(), n_caches, copies, max_copies, n_copies, s);
     });

@@ -28,7 +28,7 @@ void launch_batch_compact(const BatchView& b, uint32_t* tables_out, uint32_t* pr
 struct CopyCache {
     uint8_t* k;
     uint8_t* v;
-    uint32_t token_bytes;
+    uint64_t token_bytes;
 };
 constexpr uint32_t kCopyCaches = 128;   // of one launch: they travel as its arguments
 void launch_batch_copy(const BatchView& b, const CopyCache* caches, uint32_t n_caches, const HypBlockCopy* copies,

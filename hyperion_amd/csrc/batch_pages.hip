@@ -592,11 +592,11 @@ __global__ __launch_bounds__(kEntryThreads) void copy_kernel(CopyParams p) {
         if (c.from >= p.b.num_blocks || c.to >= p.b.num_blocks || c.from == c.to) continue;
         const CopyCache& cache = p.caches[which / 2u];
         uint8_t* const base = which % 2u != 0u ? cache.v : cache.k;
-        const size_t block_bytes = static_cast<size_t>(cache.token_bytes) << p.b.shift;
+        const size_t block_bytes = cache.token_bytes << p.b.shift;
         const uint4* const from = reinterpret_cast<const uint4*>(base + c.from * block_bytes);
         uint4* const to = reinterpret_cast<uint4*>(base + c.to * block_bytes);
-        const uint32_t words = min(c.tokens, 1u << p.b.shift) * (cache.token_bytes / 16u);
-        for (uint32_t i = threadIdx.x; i < words; i += kEntryThreads) to[i] = from[i];
+        const size_t words = min(c.tokens, 1u << p.b.shift) * (cache.token_bytes / 16u);
+        for (size_t i = threadIdx.x; i < words; i += kEntryThreads) to[i] = from[i];
     }
 }
 

@@ -412,7 +412,7 @@ typedef struct HypBatch {
     uint32_t max_blocks;            /* entries of a request's row of tables */
     uint32_t max_rows;              /* rows of the step's arrays, at most 2^20 */
     uint32_t prefix_len;            /* tokens of the shared prefix (0: none), at most 2^24 */
-    const uint32_t* prefix_table;   /* [ceil(prefix_len / block_size)]; only hyp_batch_attention reads it */
+    const uint32_t* prefix_table;   /* [ceil(prefix_len / block_size)]; hyp_batch_attention and hyp_batch_compact read it */
     uint32_t* tables;               /* [requests][max_blocks] */
     uint32_t* lens;                 /* [requests]: own tokens, this step's among them */
     uint32_t* row_start;            /* [requests + 1]: request r's rows are row_start[r] .. row_start[r + 1] - 1 */
@@ -495,8 +495,8 @@ HypStatus hyp_batch_attention_workspace(const HypBatch* batch, uint32_t n_heads,
  * of all layers. Who holds a block follows from tables and lengths alone. Which requests share one matters to
  * the end of a request: hyp_batch_plan's HYP_REQUEST_DONE returns a request's blocks without asking who else
  * holds them, so a request that was forked, or is a fork, ends by hyp_batch_rewind. A request's row of
- * tables holds a block once. Arrays that a call writes do not overlap each other or any that it reads, but
- * where it says that they may be the same (INVALID_ARGUMENT). */
+ * tables holds a block once, requests * max_blocks is below 2^31. Arrays that a call writes do not overlap each
+ * other or any that it reads, but where it says that they may be the same (INVALID_ARGUMENT). */
 
 /* The first `tokens` tokens of block `from` to block `to`. */
 typedef struct HypBlockCopy {

@@ -68,6 +68,13 @@ def test_bad_batches_are_refused(over, says):
     refused("hyp_batch_pages_workspace", ctypes.byref(b), ctypes.byref(ctypes.c_size_t()), says=says)
 
 
+def test_tables_of_too_many_entries_are_refused():
+    for b in (batch(requests=4096, max_blocks=1 << 19), batch(requests=1, max_blocks=1 << 31)):
+        refused("hyp_batch_fork", *fork_args(b), says="2^31")
+        refused("hyp_batch_rewind", *rewind_args(b), says="2^31")
+        refused("hyp_batch_compact", *compact_args(b), says="2^31")
+
+
 ODD = ptr(0x100002)
 
 
