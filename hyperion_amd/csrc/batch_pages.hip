@@ -3,10 +3,11 @@
 // Requests may hold a block in common (forked ones do). How many hold one is nowhere stored: rewind and compact mark the
 // blocks in use from the tables and lengths, so there is no count that could go wrong between calls.
 //
-// What bounds the first three: the latency of launches and of dependent trips to memory within them; their data are a few KB to
-// 1 MB. 12 requests forked 4.5 us a call, 480 7.9; 64 requests' drafts given back 8.3, 500 requests of which 71 end 23 (clear 4.0,
-// mark 5.6, rewind 15: one workgroup takes 10000 blocks' marks, a line of memory each); 16 requests compacted 5.5, 400 in a pool of
-// 78000 blocks 15. Copies are bound by memory: 1.05 GB in 213 us, 4.9 TB/s, the rate of a large copy; 29 MB in 8.3.
+// What bounds the first three: the latency of launches and of dependent trips to memory within them; their data are a few
+// KB to 1 MB. 12 requests forked take 4.5 us a call, 480 7.9; 64 requests' drafts given back 8.3, 500 requests of which 71
+// end 23 (clear 4.0, mark 5.6, rewind 15: one workgroup takes 10000 blocks' marks, a line of memory each); 16 requests
+// compacted 5.5, 400 in a pool of 78000 blocks 15. Copies are bound by memory: 1.05 GB in 213 us, 4.9 TB/s, the rate of a
+// large copy; 29 MB in 8.3.
 #include <algorithm>
 #include <cstdint>
 
@@ -60,8 +61,8 @@ __device__ __forceinline__ Sum block_sum(uint32_t v, uint32_t* waves) {
 }
 
 // Small tables are gone through by the one workgroup that has the rest to do, all entries of all rows in a line: a launch
-// takes longer than 32 entries a thread. (64 requests of up to 250 blocks: rewind 8 us so, 12 with clearing and marking by the whole
-// device; 16 compacted 5 and 15; 12 forked 3 and 7. The marks of 32768 blocks fill LDS.)
+// takes longer than 32 entries a thread. (64 requests of up to 250 blocks: rewind 8 us so, 12 with clearing and marking by
+// the whole device; 16 compacted 5 and 15; 12 forked 3 and 7. The marks of 32768 blocks fill LDS.)
 constexpr uint32_t kSmallTable = 32u * kThreads;   // entries
 constexpr uint32_t kSmallRequests = kThreads;
 constexpr uint32_t kSmallPool = 32u * kThreads;    // blocks
@@ -581,8 +582,8 @@ struct CopyParams {
     CopyCache caches[kCopyCaches];
 };
 
-// A workgroup to a block of one cache's K or V at a time. (Blocks in pieces, with four loads of a thread at once: 20 us for the 29
-// MB of a fork instead of 7.5, 217 instead of 213 for 1.05 GB.)
+// A workgroup to a block of one cache's K or V at a time. (Blocks in pieces, with four loads of a thread at once: 20 us
+// for the 29 MB of a fork instead of 7.5, 217 instead of 213 for 1.05 GB.)
 __global__ __launch_bounds__(kEntryThreads) void copy_kernel(CopyParams p) {
     const uint32_t count = min(*p.n_copies, p.max_copies);
     const uint64_t units = static_cast<uint64_t>(count) * p.n_caches * 2u;

@@ -15,16 +15,18 @@
 //  4. a workgroup a request: the tile, then the token in it.
 // All weights and sums are fp64; tokens that p does not keep have no weight, so their exponentials are not formed.
 //
-// A row takes windows of 8192 values instead of its counts (step 2 over each, counting the row again) where the
-// counts' bins of more than one value matter: a value above 2^7; values next to 0 that hold the cut, or weigh enough that
-// their differences of less than 2^-24 do; values below -2^7 that are not negligible, or hold the cut. (Rows with 60 % of the
-// type's lowest value took windows at temperatures of 1.9 and more, 64 requests of 5 of 262144 so 3.0 ms.)
+// A row takes windows of 8192 values instead of its counts (step 2 counts the row again for each, and again for those that a
+// filter ends in) where the counts' bins of more than one value matter: a value above 2^7; values next to 0 that hold the
+// cut, or weigh enough that their differences of less than 2^-24 do; values below -2^7 that are not negligible, or hold the
+// cut. One request of 5 rows past 2^7 takes 180 to 540 us so. Masks go by their own size: 60 % of 576 rows of 262144 at the
+// type's lowest value take 139 us, 3.0 ms at temperatures of 1.9 and more when all below -2^7 counted as -2^7.
 //
-// What bounds it: with many rows the one pass over the logits (64 requests of 1 to 8 rows of 262144, 268 MB: 60 us of 109, 4.5
-// TB/s), then the exponentials of the requests that keep most tokens (17). With few, latency: one request of 5 rows takes 22.6 us,
-// count 5.7, filters 8.8, sums 3.8, draw 4.5, where its 4.7 MB are 1 us. Steps 2 to 4 issue instructions that all waves of a workgroup
-// issue alike (scans, parameters, borders): with 16 waves each is 16 cycles, so they have four (48 requests
-// without a drafting model 72 us with 16, 52 with four), and as the code itself comes from memory in a short kernel, loops over a thread's values are kept rolled.
+// What bounds it: with many rows the one pass over the logits (64 requests of 1 to 8 rows of 262144, 268 MB: 60 us of 108,
+// 4.5 TB/s), then the exponentials of the requests that keep most tokens (17). With few, latency: one request of 5 rows
+// takes 22.6 us, count 5.7, filters 8.8, sums 3.8, draw 4.5, where its 4.7 MB are 1 us. The instructions of steps 2 to 4 are
+// mostly such that all waves of a workgroup issue alike (scans, parameters, borders): with 16 waves each is 16 cycles, so
+// they have four (48 requests without a drafting model 72 us with 16, 52 with four). And as the code itself comes from
+// memory in a short kernel, loops over a thread's values are kept rolled.
 #include <algorithm>
 #include <cstdint>
 
@@ -95,8 +97,8 @@ __device__ __forceinline__ const uint16_t* logits_of(const VerifyArgs& a, uint32
 // ---- 1. counts ----------------------------------------------------------------------------------
 
 // Rows of more bytes than the caches hold are waited for from memory: with all of a chunk's loads on their way at once 64
-// requests' 268 MB take 60 us instead of 68 when no cache has them (50 instead of 55 when some does). What a cache holds is counted
-// faster while the next comes in: 126 MB 24.7 us so, 26.9 with all loads first; 60 MB 18.2 and 19.5.
+// requests' 268 MB take 60 us instead of 68 when no cache has them (50 instead of 55 when some does). What a cache holds
+// is counted faster while the next comes in: 126 MB 24.7 us so, 26.9 with all loads first; 60 MB 18.2 and 19.5.
 constexpr uint64_t kCached = 1ull << 27;   // bytes
 constexpr uint32_t kChunkLoads = 8;
 static_assert(kLongest <= kChunkLoads * 8u * kThreads, "a chunk's loads");
@@ -296,7 +298,8 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
         }
         const double m = o.n * o.w;
         const uint64_t before = __builtin_bit_cast(uint64_t, mass_before);
-        const uint64_t lo = from_lane(static_cast<uint32_t>(before), from), hi = from_lane(static_cast<uint32_t>(before >> 32), from);
+        const uint64_t lo = from_lane(static_cast<uint32_t>(before), from);
+        const uint64_t hi = from_lane(static_cast<uint32_t>(before >> 32), from);
         o.mass = __builtin_bit_cast(double, lo | hi << 32) + (wave_incl64(m) - m);
         o.before = from_lane(count_before, from) + (wave_incl(o.n) - o.n);
         return o;
@@ -346,7 +349,8 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
 }
 
 // The same for a row by windows. (A call has a barrier at its end.)
-__device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t vocab, const RowParams& prm, RowStat& r, FilterLds& s) {
+__device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t vocab, const RowParams& prm, RowStat& r,
+                                               FilterLds& s) {
     const uint32_t tid = threadIdx.x;
     uint32_t best = kNone, held = 0u, windows = 0u;
     for_tokens(row, 0u, vocab, tid, kFew, [&](uint32_t, uint32_t b) HYP_INLINE {
@@ -374,8 +378,8 @@ __device__ __forceinline__ void filter_windows(const uint16_t* row, uint32_t voc
             const uint32_t window = k * kWindow;
             const double enough = prm.top_p * r.total;
             // Those that a filter ends in or that hold the last kept token are looked into, the others have their sums.
-            if ((step == 1u && !(prm.top_p != 0.0 && mass_all + s.window_mass[k] > enough) && ((s.window_light >> k) & 1u) == 0u) ||
-                (step == 2u && kept - 1u - count_all >= s.window_count[k])) {
+            const bool ends = (prm.top_p != 0.0 && mass_all + s.window_mass[k] > enough) || ((s.window_light >> k) & 1u) != 0u;
+            if ((step == 1u && !ends) || (step == 2u && kept - 1u - count_all >= s.window_count[k])) {
                 mass_all += s.window_mass[k];
                 count_all += s.window_count[k];
                 continue;
@@ -508,7 +512,8 @@ __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, u
                 u16x2_t same = {0, 0};
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i)
-                    same += __builtin_elementwise_sub_sat(u16x2_t{1, 1}, __builtin_bit_cast(u16x2_t, (w[j][i] ^ pattern) & mask));
+                    same += __builtin_elementwise_sub_sat(u16x2_t{1, 1},
+                                                          __builtin_bit_cast(u16x2_t, (w[j][i] ^ pattern) & mask));
                 const uint32_t n = static_cast<uint32_t>(same.x) + same.y;
                 four |= n << (4u * j);
                 mine += n;
@@ -548,7 +553,7 @@ __device__ __forceinline__ void find_last(const uint16_t* row, uint32_t begin, u
                         const uint32_t from = first + k * kStep;
                         uint32_t b[8], places = 0u;
 #pragma unroll
-                        for (uint32_t i = 0; i < 8u; ++i) b[i] = row[min(from + i, stop - 1u)];   // (the last one's copies: behind it)
+                        for (uint32_t i = 0; i < 8u; ++i) b[i] = row[min(from + i, stop - 1u)];   // (copies: behind it)
 #pragma unroll
                         for (uint32_t i = 0; i < 8u; ++i) places |= plain_bits(b[i]) == bits ? 1u << i : 0u;
                         for (uint32_t skip = left - (incl - n); skip != 0u; --skip) places &= places - 1u;
@@ -635,7 +640,7 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
             uint32_t lead = kNone;
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) {
-                to[static_cast<int>(q < kBinsEach / 16u ? -static_cast<int>(i) : static_cast<int>(i)) * static_cast<int>(kRow)] = n[8u * q + i];
+                to[(q < kBinsEach / 16u ? -static_cast<int>(i) : static_cast<int>(i)) * static_cast<int>(kRow)] = n[8u * q + i];
                 if (n[8u * q + i] != 0u && (lead == kNone || q < kBinsEach / 16u))
                     lead = q < kBinsEach / 16u ? place - i : place + i;
             }
@@ -696,8 +701,10 @@ __global__ __launch_bounds__(kFew) void verify_filter_kernel(VerifyParams p) {
         const uint32_t lead = others.lead;
         const bool next_to_0 = others.centre != 0u && lead >= kFine;   // the largest
         bool counted = others.above == 0u && (next_to_0 ? others.centre_lo == others.centre_hi : lead != kNone);
-        r.top = scalar(value_of(next_to_0 ? bits_at(others.centre_lo) : bits_of_bin((lead / kBinsEach) % kFew, lead % kBinsEach)));
-        if (counted && others.below != 0u) counted = (r.top - value_of(others.below_bits)) * prm.by_t > 80.0;   // (2^23 times e^-80)
+        r.top = scalar(value_of(next_to_0 ? bits_at(others.centre_lo)
+                                          : bits_of_bin((lead / kBinsEach) % kFew, lead % kBinsEach)));
+        // (2^23 times e^-80 is below a rounding.)
+        if (counted && others.below != 0u) counted = (r.top - value_of(others.below_bits)) * prm.by_t > 80.0;
         if (counted) counted = filter_counts(prm, r.top, others, s, r.total);
         r.kind = counted ? kCounted : kWindowed;
         if (!counted) filter_windows(row, a.vocab, prm, r, s);
@@ -767,8 +774,8 @@ __device__ __forceinline__ Stop find_stop(const VerifyParams& p, uint32_t reques
     return {first, rows, accepted};
 }
 
-// e^x of many x <= 0: 2^(n / 64) e^r with |r| <= ln 2 / 128, the first by a table, the series to r^5 (the rest is below 2^-54).
-// (15 instructions where exp_below takes 25: a request's whole vocabulary goes through it, without filters.)
+// e^x of many x <= 0: 2^(n / 64) e^r with |r| <= ln 2 / 128, the first by a table, the series to r^5 (the rest is below
+// 2^-54). (15 instructions where exp_below takes 25: a request's whole vocabulary goes through it, without filters.)
 constexpr uint32_t kPowers = 64;
 struct Powers {
     double p[kPowers];   // 2^(j / 64) / 2
@@ -993,10 +1000,9 @@ __global__ __launch_bounds__(kFew) void verify_draw_kernel(VerifyParams p) {
     if (a.logprobs != nullptr) a.logprobs[stop.row()] = log_share(rest.p, rest.logits[token]);
 }
 
-// A row's chunks: enough workgroups to fill the device, but no more of them than the filters read in little time. With 1024 or
-// 2048 workgroups instead of 512, 100 requests of 50001 tokens take 18.6 + 11.9 us or 21.6 + 13.2 (counts and filters) instead of
-// 17.1 + 10.6; with up to 16 chunks a row instead of 8, one request of 5 rows 5.0 + 14.0 instead of 5.6 + 10.2, with 4 as long as
-// with 8.
+// A row's chunks: enough workgroups to fill the device, but no more of them than the filters read in little time. Counts and
+// filters of 100 requests of 50001 tokens take 18.0 + 10.5 us with 512 workgroups, 19.0 + 12.0 with 1024, 22.2 + 13.0 with
+// 2048; those of one request of 5 rows 5.7 + 8.8 with 8 chunks a row, 6.8 + 8.4 with 4, 5.2 + 11.7 with 16.
 constexpr uint32_t kFill = 512;
 constexpr uint32_t kMinChunk = 8192;
 constexpr uint32_t kMostChunks = 8;
