@@ -20,7 +20,7 @@
 // Rows whose other three bins matter to the result (a value above 2^7; several values nearer to 0 than
 // 2^-25; values below -2^7 that would not be negligible at this temperature were they -2^7) take the same steps over
 // windows of 8192 values of the whole order, counting the row again for each: one row of 262144 with half of it at
-// bf16's lowest value 21 us at temperature 0.8, 1125 in windows at 2; with values past 2^7 566.
+// bf16's lowest value 20 us at temperature 0.8, 1125 in windows at 2; with values past 2^7 566.
 //
 // What bounds it: the steps' latency (the second launch takes 13 to 16 us whatever the rows: 3 for the counts, 3.5 for the
 // weights, 3 for the filters and the draw, 3 for the token) and the LDS additions (64 rows of 262144: 9.5 us of

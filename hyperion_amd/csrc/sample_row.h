@@ -144,16 +144,16 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
     // value took 320 us).
     uint32_t below = 0u, below_bits = 0xFFFFFFFFu;
     // The bits less kLow, in 16 bits: a fine value has 0 in bits 12 to 14, its sign in bit 15.
-    const auto one = [&](uint32_t b) HYP_INLINE {
+    const auto usual = [&](uint32_t b) HYP_INLINE {   // a fine value, one of -2^7 to the lowest, -inf; false: another
         const uint32_t t = b - kLow;
-        if ((t & 0x7000u) == 0u) {
-            atomicAdd(&s.count[(t & 0xFFFu) | ((t >> 3) & 0x1000u)], 1u);
-            return;
-        }
-        const bool low = b - 0xC300u < 0xFF80u - 0xC300u;   // -2^7 to the lowest
+        const bool fine = (t & 0x7000u) == 0u;
+        if (fine) atomicAdd(&s.count[(t & 0xFFFu) | ((t >> 3) & 0x1000u)], 1u);
+        const bool low = b - 0xC300u < 0xFF80u - 0xC300u;
         below += low ? 1u : 0u;
         below_bits = min(below_bits, low ? b : 0xFFFFFFFFu);
-        if (low || b == 0xFF80u) return;
+        return fine || b - 0xC300u <= 0xFF80u - 0xC300u;
+    };
+    const auto other = [&](uint32_t b) HYP_INLINE {
         b = plain_bits(b);
         if (!finite_bits(b)) {
             if (b == 0x7F80u) atomicAdd(&s.infinite, 1u);
@@ -183,10 +183,18 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
                 atomicAdd(&s.count[at[k] >> 18], 1u);
             }
         } else {
+            uint32_t others = 0u;
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k) {
-                one(w[k] & 0xFFFFu);
-                one(w[k] >> 16);
+                others |= usual(w[k] & 0xFFFFu) ? 0u : 1u << (2u * k);
+                others |= usual(w[k] >> 16) ? 0u : 2u << (2u * k);
+            }
+            if (others != 0u) {
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) {
+                    if (((others >> (2u * k)) & 1u) != 0u) other(w[k] & 0xFFFFu);
+                    if (((others >> (2u * k)) & 2u) != 0u) other(w[k] >> 16);
+                }
             }
         }
     };
@@ -205,7 +213,8 @@ __device__ __forceinline__ void count_values(const uint16_t* row, uint32_t begin
             eight(w);
         }
     }
-    for (uint32_t k = i; k < end && k < i + 8u; ++k) one(row[k]);
+    for (uint32_t k = i; k < end && k < i + 8u; ++k)
+        if (!usual(row[k])) other(row[k]);
     if (__ballot(below != 0u) != 0u) {
         below = wave_sum(below);
         below_bits = from_lane(wave_scan(below_bits, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return min(a, b); }), 63u);

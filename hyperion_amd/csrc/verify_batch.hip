@@ -19,7 +19,7 @@
 // filter ends in) where the counts' bins of more than one value matter: a value above 2^7; values next to 0 that hold the
 // cut, or weigh enough that their differences of less than 2^-24 do; values below -2^7 that are not negligible, or hold the
 // cut. One request of 5 rows past 2^7 takes 180 to 540 us so. Masks go by their own size: 60 % of 576 rows of 262144 at the
-// type's lowest value take 139 us, 3.0 ms at temperatures of 1.9 and more when all below -2^7 counted as -2^7.
+// type's lowest value take 123 us, 3.0 ms at temperatures of 1.9 and more when all below -2^7 counted as -2^7.
 //
 // What bounds it: with many rows the one pass over the logits (64 requests of 1 to 8 rows of 262144, 268 MB: 60 us of 108,
 // 4.5 TB/s), then the exponentials of the requests that keep most tokens (17). With few, latency: one request of 5 rows
