@@ -278,7 +278,7 @@ def test_filters_end_anywhere_in_the_order(stream, vocab):
 LOWEST = -3.3895314e38
 
 
-@pytest.mark.parametrize("fill", [-127.5, -128.0, -129.0, -400.0, -2000.0, LOWEST, -np.inf])
+@pytest.mark.parametrize("fill", [-127.5, -128.0, -129.0, -400.0, -2000.0, LOWEST, -np.inf, 0.0, 1e-9, np.inf, np.nan])
 @pytest.mark.parametrize("allowed", [1, 5, 300])
 def test_masked_tokens(stream, allowed, fill):
     """Masks of any value under any temperature, with fewer tokens left than top-k keeps; drafts that are masked among them."""
