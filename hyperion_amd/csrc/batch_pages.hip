@@ -5,7 +5,7 @@
 //
 // What bounds the first three: the latency of launches and of dependent trips to memory within them; their data are a few
 // KB to 1 MB. 12 requests forked take 4.5 us a call, 480 7.9; 64 requests' drafts given back 8.3, 500 requests of which 71
-// end 23 (clear 4.0, mark 5.6, rewind 15: one workgroup takes 10000 blocks' marks, a line of memory each); 16 requests
+// end 20 (clear 3.9, mark 5.7, rewind 12.4: one workgroup goes through 10000 blocks that may go back); 16 requests
 // compacted 5.5, 400 in a pool of 78000 blocks 15. Copies are bound by memory: 1.05 GB in 213 us, 4.9 TB/s, the rate of a
 // large copy; 29 MB in 8.3.
 #include <algorithm>
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kEntryThreads) void rewind_mark_kernel(RewindParams
 // The entries given up, from the last to the first: so a block that goes back has its place in the stack, from the top down,
 // without their number. kEach consecutive ones to a thread, with their loads on the way together. How many went back.
 // (One to a thread while that does: 64 requests' drafts 4.2 us so, 6.8 with four; 10000 blocks of 71 requests that end 14.8 with
-// four, 22.2 with one, 16.4 with eight.)
+// four, 22.2 with one, 16.4 with eight, each mark from memory.)
 template <uint32_t kEach>
 __device__ __forceinline__ uint32_t give_back(const RewindParams& p, const uint32_t* state, const uint32_t* gone_sum,
                                               const uint32_t* first_gone, uint32_t all, uint32_t taken, uint32_t* waves) {
@@ -293,16 +293,19 @@ __device__ __forceinline__ uint32_t give_back(const RewindParams& p, const uint3
     return min(returned, taken);
 }
 
-// kSmall: the marks are this workgroup's own, in LDS.
-template <bool kSmall>
+// kSmall: the marks are this workgroup's own. kMarks: they are in LDS, read at once where others made them (500 requests of
+// which 71 end, 20000 blocks: 12.4 us, 15.2 with each mark from memory).
+constexpr uint32_t kMarkPool = 28u * kThreads;   // blocks whose marks fit LDS beside 4096 requests
+template <bool kSmall, bool kMarks>
 __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
+    static_assert(kMarks || !kSmall, "the workgroup's own marks");
     constexpr uint32_t kRequests = kSmall ? kSmallRequests : kMaxRequests;
     __shared__ uint32_t gone_sum[kRequests + 1];   // entries given up by the requests before
     __shared__ uint32_t first_gone[kRequests];     // a request's first of them
     __shared__ uint32_t had[kSmall ? kRequests : 1u], part[kSmall ? kRequests : 1u];
-    __shared__ uint32_t marks[kSmall ? kSmallPool : 1u];
+    alignas(16) __shared__ uint32_t marks[kSmall ? kSmallPool : (kMarks ? kMarkPool : 1u)];
     __shared__ uint32_t waves[kWaves];
-    uint32_t* const state = kSmall ? marks : p.state;
+    uint32_t* const state = kMarks ? marks : p.state;
     const BatchView& b = p.b;
     const uint32_t tid = threadIdx.x;
     const uint32_t n = b.requests;
@@ -311,6 +314,13 @@ __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
     const uint32_t taken = min(*p.taken, b.num_blocks);
     if constexpr (kSmall)
         for (uint32_t i = tid; i < b.num_blocks; i += kThreads) marks[i] = 0u;
+    if constexpr (kMarks && !kSmall) {   // (a workspace has whole words of 16 bytes)
+#pragma unroll
+        for (uint32_t k = 0; k < kMarkPool / (4u * kThreads); ++k) {
+            const uint32_t i = k * kThreads + tid;
+            if (4u * i < b.num_blocks) reinterpret_cast<uint4*>(marks)[i] = reinterpret_cast<const uint4*>(p.state)[i];
+        }
+    }
     Shortened s[kPer];
     uint32_t gone = 0u;
 #pragma unroll
@@ -632,7 +642,7 @@ void launch_batch_rewind(const BatchView& b, const uint32_t* lens, const uint32_
     uint32_t* const w = static_cast<uint32_t*>(workspace);
     const RewindParams p{b, lens, drop, free_blocks, taken, taken_out, copies, n_copies, w};
     if (small_table(b) && b.num_blocks <= kSmallPool) {
-        hipLaunchKernelGGL(rewind_kernel<true>, dim3(1), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL((rewind_kernel<true, true>), dim3(1), dim3(kThreads), 0, stream, p);
         HYP_HIP_CHECK(hipGetLastError());
         return;
     }
@@ -643,7 +653,8 @@ void launch_batch_rewind(const BatchView& b, const uint32_t* lens, const uint32_
         hipLaunchKernelGGL(rewind_mark_kernel, dim3(b.requests, pieces_of(b.max_blocks)), dim3(kEntryThreads), 0, stream, p);
         HYP_HIP_CHECK(hipGetLastError());
     }
-    hipLaunchKernelGGL(rewind_kernel<false>, dim3(1), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((b.num_blocks <= kMarkPool ? rewind_kernel<false, true> : rewind_kernel<false, false>), dim3(1),
+                       dim3(kThreads), 0, stream, p);
     HYP_HIP_CHECK(hipGetLastError());
 }
 

@@ -141,6 +141,9 @@ POOLS = [
     (4096, 16, 60, 700, 3, 500),  # the most requests
     (3, 65536, 200000, 4, 2, 0),
     (20, 16, 40000, 9, 2, 4),     # long tables
+    (40, 16, 300, 33000, 2, 6),   # small tables, a pool beyond LDS
+    (250, 16, 6000, 40, 3, 30),   # tables beyond one workgroup, marks that fit LDS or not
+    (400, 8, 9000, 5000, 3, 20),
 ]
 
 
