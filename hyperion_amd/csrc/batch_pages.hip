@@ -6,8 +6,8 @@
 // What bounds the first three: the latency of launches and of dependent trips to memory within them; their data are a few
 // KB to 1 MB. 12 requests forked take 4.5 us a call, 480 7.9; 64 requests' drafts given back 8.3, 500 requests of which 71
 // end 20 (clear 3.9, mark 5.7, rewind 12.4: one workgroup goes through 10000 blocks that may go back); 16 requests
-// compacted 5.5, 400 in a pool of 78000 blocks 15. Copies are bound by memory: 1.05 GB in 213 us, 4.9 TB/s, the rate of a
-// large copy; 29 MB in 8.3.
+// compacted 5.5, 400 in a pool of 78000 blocks 15. Copies are bound by memory: 1.05 GB in 210 us, 5.0 TB/s, the rate of a
+// large copy; 29 MB in 7.2.
 #include <algorithm>
 #include <cstdint>
 
@@ -589,25 +589,43 @@ struct CopyParams {
     const HypBlockCopy* copies;
     const uint32_t* n_copies;
     uint32_t max_copies, n_caches;
+    uint32_t pieces;   // of a block, at most
     CopyCache caches[kCopyCaches];
 };
 
-// A workgroup to a block of one cache's K or V at a time. (Blocks in pieces, with four loads of a thread at once: 20 us
-// for the 29 MB of a fork instead of 7.5, 217 instead of 213 for 1.05 GB.)
+// A workgroup to a piece of a block of one cache's K or V at a time, four 16-byte loads of a thread on their way together. (One
+// block of 4096 tokens in 16 layers of 8 heads of 128, 537 MB moved: 99 us, 5.4 TB/s; 930 with whole blocks and a load at
+// a time. The 29 MB of a fork 6.5 and 7.3.)
+constexpr uint32_t kCopyGroups = 16384;
+constexpr uint32_t kPiece = 4u * 4u * kEntryThreads;   // words of 16 bytes
 __global__ __launch_bounds__(kEntryThreads) void copy_kernel(CopyParams p) {
+    typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
     const uint32_t count = min(*p.n_copies, p.max_copies);
-    const uint64_t units = static_cast<uint64_t>(count) * p.n_caches * 2u;
-    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const uint32_t which = static_cast<uint32_t>(u % (2u * p.n_caches));
-        const HypBlockCopy c = p.copies[u / (2u * p.n_caches)];
+    const uint32_t which = blockIdx.x / p.pieces;
+    const CopyCache& cache = p.caches[which / 2u];
+    uint8_t* const base = which % 2u != 0u ? cache.v : cache.k;
+    const uint64_t token_words = cache.token_bytes / 16u;
+    const uint64_t begin = static_cast<uint64_t>(blockIdx.x - which * p.pieces) * kPiece;
+    const uint64_t step = static_cast<uint64_t>(p.pieces) * kPiece;
+    for (uint32_t at = blockIdx.y; at < count; at += gridDim.y) {
+        const HypBlockCopy c = p.copies[at];
         if (c.from >= p.b.num_blocks || c.to >= p.b.num_blocks || c.from == c.to) continue;
-        const CopyCache& cache = p.caches[which / 2u];
-        uint8_t* const base = which % 2u != 0u ? cache.v : cache.k;
-        const size_t block_bytes = cache.token_bytes << p.b.shift;
-        const uint4* const from = reinterpret_cast<const uint4*>(base + c.from * block_bytes);
-        uint4* const to = reinterpret_cast<uint4*>(base + c.to * block_bytes);
-        const size_t words = min(c.tokens, 1u << p.b.shift) * (cache.token_bytes / 16u);
-        for (size_t i = threadIdx.x; i < words; i += kEntryThreads) to[i] = from[i];
+        const uint64_t words = min(c.tokens, 1u << p.b.shift) * token_words;
+        const u32x4_t* const from = reinterpret_cast<const u32x4_t*>(base) + ((c.from * token_words) << p.b.shift);
+        u32x4_t* const to = reinterpret_cast<u32x4_t*>(base) + ((c.to * token_words) << p.b.shift);
+        for (uint64_t piece = begin; piece < words; piece += step) {
+            const uint64_t end = min(words, piece + kPiece);
+            uint64_t i = piece + threadIdx.x;
+            for (; i + 3u * kEntryThreads < end; i += 4u * kEntryThreads) {
+                u32x4_t v[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) v[k] = from[i + k * kEntryThreads];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) to[i + k * kEntryThreads] = v[k];
+            }
+            for (; i < end; i += kEntryThreads) to[i] = from[i];
+        }
     }
 }
 
@@ -687,11 +705,14 @@ void launch_batch_compact(const BatchView& b, uint32_t* tables_out, uint32_t* pr
 void launch_batch_copy(const BatchView& b, const CopyCache* caches, uint32_t n_caches, const HypBlockCopy* copies,
                        uint32_t max_copies, const uint32_t* n_copies, hipStream_t stream) {
     for (uint32_t at = 0u; at < n_caches; at += kCopyCaches) {
-        CopyParams p{b, copies, n_copies, max_copies, std::min(kCopyCaches, n_caches - at), {}};
+        CopyParams p{b, copies, n_copies, max_copies, std::min(kCopyCaches, n_caches - at), 1u, {}};
         std::copy(caches + at, caches + at + p.n_caches, p.caches);
-        const uint64_t units = static_cast<uint64_t>(max_copies) * p.n_caches * 2u;
-        const uint32_t groups = static_cast<uint32_t>(std::min<uint64_t>(units, 4096u));
-        hipLaunchKernelGGL(copy_kernel, dim3(groups), dim3(kEntryThreads), 0, stream, p);
+        uint64_t longest = 0;
+        for (uint32_t i = 0; i < p.n_caches; ++i) longest = std::max(longest, (p.caches[i].token_bytes / 16u) << b.shift);
+        const uint32_t sides = 2u * p.n_caches;
+        p.pieces = static_cast<uint32_t>(std::min<uint64_t>((longest + kPiece - 1u) / kPiece, std::max(1u, kCopyGroups / sides)));
+        const uint32_t along = std::min(max_copies, std::max(1u, kCopyGroups / (sides * p.pieces)));
+        hipLaunchKernelGGL(copy_kernel, dim3(sides * p.pieces, along), dim3(kEntryThreads), 0, stream, p);
         HYP_HIP_CHECK(hipGetLastError());
     }
 }

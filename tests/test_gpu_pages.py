@@ -365,6 +365,26 @@ def test_copy(stream, shapes, block, num, count):
     compare()
 
 
+@pytest.mark.parametrize("tokens", [65536, 40001, 16385, 1])
+def test_copy_of_the_longest_blocks_in_many_caches(stream, tokens):
+    """More pieces than a launch has workgroups: blocks of 65536 tokens, 128 caches (two, listed over and over)."""
+    say(f"copy: {tokens} of 65536 tokens, 128 caches")
+    rng = np.random.default_rng(tokens)
+    block, num, kvh, d = 65536, 2, 1, 64
+    caches, host = [hy.KvCache(num * block, kvh, d) for _ in range(2)], []
+    for c in caches:
+        host.append([rng.integers(0, 1 << 16, (num * block, kvh, d), dtype=np.uint16) for _ in range(2)])
+        fill_cache(c, *host[-1], stream)
+    one = dev(np.zeros(1, np.uint32), stream)
+    batch = hy.Batch(block, num, dev(np.zeros((1, 1), np.uint32), stream), one, dev(u32(0, 0), stream), one, one)
+    batch.copy(caches * 64, dev(np.array([[1, 0, tokens]], np.uint32), stream), dev(u32(1), stream), stream)
+    for c, kv in zip(caches, host):
+        for got, was in zip(read_cache(c, (num * block, kvh, d), stream), kv):
+            was[:tokens] = was[block:block + tokens]
+            assert np.array_equal(got, was)
+        c.close()
+
+
 def test_copy_past_2_to_the_32_bytes(stream):
     """A cache of more than 2^32 bytes: offsets need 64 bits."""
     say("copy: a large cache")
