@@ -98,9 +98,9 @@ __device__ __forceinline__ const uint16_t* logits_of(const VerifyArgs& a, uint32
 
 // Rows of more bytes than the caches hold are waited for from memory: with all of a chunk's loads on their way at once 64
 // requests' 268 MB take 60 us instead of 68 read again and again, 69 instead of 76 just written. What a cache holds is
-// counted faster while the next comes in: 60 MB 18.2 us so, 19.5 with all loads first (just written 18.9 and 20.3); 126 MB
-// 24.7 and 26.9 (27.4 and 27.6; 32 and 29 with other inputs in between).
-constexpr uint64_t kCached = 1ull << 27;   // bytes
+// counted faster while the next comes in: 60 MB 18.2 us so, 19.5 with all loads first (just written 18.9 and 20.3). Between
+// them 126 MB take 24.7 and 26.9 read again and again, 27.4 and 27.6 just written, 32 and 29 with other inputs in between.
+constexpr uint64_t kCached = 1ull << 26;   // bytes
 constexpr uint32_t kChunkLoads = 8;
 static_assert(kLongest <= kChunkLoads * 8u * kThreads, "a chunk's loads");
 template <uint32_t kAhead>
