@@ -34,6 +34,7 @@
 #include "common.h"
 #include "sample_row.h"
 #include "verify_batch.h"
+#include "verify_border.h"
 #include "wave.h"
 
 namespace hyperion::hip {
@@ -251,11 +252,11 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
     const uint32_t centre = s.count[tid];
     double centre_weight = 0.0, sum = 0.0;
     uint32_t here = centre;
-    bool light = false;   // min-p drops some
+    bool light = false;   // min-p may drop some
     if (centre != 0u) {
         centre_weight = exp_below((value_of(bits_at(others.centre_lo)) - top) * prm.by_t);
         sum = centre * centre_weight;
-        light = centre_weight < prm.min_p;
+        light = may_be_light(centre_weight, prm.min_p);
     }
     {
         Weights e(tid, top, prm.by_t);
@@ -268,7 +269,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
             for (uint32_t i = 0; i < 8u; ++i) {
                 sum += n[i] * e.w;
                 here += n[i];
-                light = light || (n[i] != 0u && e.w < prm.min_p);
+                light = light || (n[i] != 0u && may_be_light(e.w, prm.min_p));
                 e.next(base + i);
             }
         }
@@ -284,13 +285,9 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
     const uint32_t all = count_at.all + below;
     uint32_t kept = all;
     if (prm.top_k != 0u) kept = min(kept, prm.top_k);
-    // The values of the thread of lane `from`, a slot to a lane: tokens, weight, and what comes before.
-    struct One {
-        uint32_t n, before, bits;
-        double w, mass;   // (mass: before)
-    };
+    // The values of the thread of lane `from`, a slot to a lane.
     const auto spread = [&](uint32_t from) HYP_INLINE {
-        One o{0u, 0u, 0u, 0.0, 0.0};
+        OneValue o{0u, 0u, 0u, 0.0, 0.0};
         const uint32_t thread = (tid & ~63u) + from;
         if (lane < kSlots) {
             o.n = s.count[lane * kRow + thread];
@@ -306,18 +303,11 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
         return o;
     };
     if (prm.top_p != 0.0 || prm.min_p != 0.0) {
-        // Of each wave the first lane whose values a filter does not keep whole.
         const double enough = prm.top_p * total;
-        const uint64_t past = __ballot((prm.top_p != 0.0 && mass_at.incl > enough) || light);
-        if (past != 0u) {
-            const One o = spread(static_cast<uint32_t>(__builtin_ctzll(past)));
-            const bool dropped = o.n != 0u && o.w < prm.min_p;
-            const bool full = o.n != 0u && prm.top_p != 0.0 && o.n * o.w > enough - o.mass;
-            uint32_t some = 0u;   // (kept are the tokens before which the running sum is below)
-            if (!dropped && full && enough > o.mass) some = min(o.n, static_cast<uint32_t>(ceil((enough - o.mass) / o.w)));
-            const uint64_t ends = __ballot(dropped || full);
-            if (ends != 0u && lane == static_cast<uint32_t>(__builtin_ctzll(ends))) atomicMin(&s.keep, o.before + some);
-        }
+        const bool by_mass = prm.top_p != 0.0;
+        const uint64_t maybe = __ballot(here != 0u && (light || (by_mass && may_be_past(mass_at.incl, enough))));
+        const uint32_t border = wave_border(maybe, by_mass, enough, prm.min_p, spread);
+        if (lane == 0u && border != kNone) atomicMin(&s.keep, border);
         __syncthreads();
         kept = min(kept, s.keep);
     }
@@ -331,7 +321,7 @@ __device__ __forceinline__ bool filter_counts(const RowParams& prm, double top, 
         s.redo = kept - 1u - count_before < centre || centre * centre_weight * prm.by_t > 0x1p-30 * total;
     const uint64_t holds = __ballot(kept - 1u - count_before < here);
     if (holds != 0u) {
-        const One o = spread(static_cast<uint32_t>(__builtin_ctzll(holds)));
+        const OneValue o = spread(static_cast<uint32_t>(__builtin_ctzll(holds)));
         if (kept - 1u - o.before < o.n) {
             s.kept = o.mass + (kept - o.before) * o.w;
             s.cut = o.bits;

@@ -751,8 +751,9 @@ HypStatus hyp_sample_batch_workspace(uint32_t rows, uint32_t vocab, size_t* out_
  * cut off at rows): ids [rows] (device) are the tokens that the target read there, the first one known, the others
  * drafted. So row t's logits [vocab] (bf16, device, row-major) judge ids[t + 1], but behind the last row nothing was drafted.
  *  - p of row t: the distribution that hyp_sample_batch draws from with configs[r] (device; one for each request): w
- *    of the kept tokens over their sum, in fp64. A greedy request's first token has 1. A row with no logit above
- *    -inf has p = 0 everywhere.
+ *    of the kept tokens over their sum, in fp64 (a running sum within its roundings of top-p's border may end the kept
+ *    ones a token apart in the two). A greedy request's first token has 1. A row with no logit above -inf has p = 0
+ *    everywhere.
  *  - q of row t: the same of draft_logits [rows][vocab], with draft_configs[r] (NULL: configs); a
  *    request's last row of draft_logits is not read. draft_logits NULL: the drafts have no distribution (found by lookup
  *    or greedily), q is 1 at the draft.
