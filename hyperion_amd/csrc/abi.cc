@@ -1199,6 +1199,8 @@ HypStatus hyp_batch_copy(const HypBatch* batch, const HypKvCache* caches, uint32
         std::vector<hyperion::hip::CopyCache> all(n_caches);
         for (uint32_t i = 0; i < n_caches; ++i) {
             HypKvCacheOpaque& c = batch_cache(*batch, caches[i]);
+            for (const auto* side : {&c.k, &c.v})
+                require_apart({{side->data(), side->bytes()}}, {{copies, uint64_t{12} * max_copies}, {n_copies, 4}});
             all[i] = {static_cast<uint8_t*>(c.k.data()), static_cast<uint8_t*>(c.v.data()),
                       uint64_t{2} * c.num_kv_heads * c.head_dim};
         }

@@ -552,9 +552,10 @@ HypStatus hyp_batch_compact(const HypBatch* batch, uint32_t* tables_out, uint32_
 HypStatus hyp_batch_pages_workspace(const HypBatch* batch, size_t* out_bytes);
 
 /* Carry out min(n_copies[0], max_copies) entries of copies (device) in the K and V of n_caches caches (host array of
- * handles; the layers of one batch, of any shapes): at most block_size tokens each. Entries with an id >= num_blocks, or of
- * a block to itself, do nothing. No block is the `to` of one entry and the `from` or `to` of another (as the calls above
- * list them): entries run in no order. Call it before the next hyp_batch_prepare. */
+ * handles; the layers of one batch, of any shapes; one may be listed more than once): at most block_size tokens each.
+ * Entries with an id >= num_blocks, or of a block to itself, do nothing. No block is the `to` of one entry and the `from`
+ * or `to` of another (as the calls above list them): entries run in no order. copies and n_copies lie outside the caches'
+ * memory (INVALID_ARGUMENT). Call it before the next hyp_batch_prepare. */
 HypStatus hyp_batch_copy(const HypBatch* batch, const HypKvCache* caches, uint32_t n_caches, const HypBlockCopy* copies,
                          uint32_t max_copies, const uint32_t* n_copies, HypStream stream);
 
