@@ -4,10 +4,10 @@
 // blocks in use from the tables and lengths, so there is no count that could go wrong between calls.
 //
 // What bounds the first three: the latency of launches and of dependent trips to memory within them; their data are a few
-// KB to 1 MB. 12 requests forked take 4.5 us a call, 480 7.9; 64 requests' drafts given back 8.3, 500 requests of which 71
-// end 20 (clear 3.9, mark 5.7, rewind 12.4: one workgroup goes through 10000 blocks that may go back); 16 requests
-// compacted 5.5, 400 in a pool of 78000 blocks 15. Copies are bound by memory: 1.05 GB in 210 us, 5.0 TB/s, the rate of a
-// large copy; 29 MB in 7.2.
+// KB to 1 MB. A call in a stream of calls takes: 12 requests forked 4.1 to 4.7 us, 480 8.0; 64 requests' drafts given back
+// 8.3, 500 requests of which 71 end 20 (12.4 of a traced call's 22 are one workgroup that goes through 10000 blocks that
+// may go back); 16 requests compacted 5.7, 400 in a pool of 78000 blocks 14.3. Copies are bound by memory: 1.05 GB in
+// 210 us, 5.0 TB/s, the rate of a large copy; 29 MB in 7.2.
 #include <algorithm>
 #include <cstdint>
 
@@ -61,8 +61,8 @@ __device__ __forceinline__ Sum block_sum(uint32_t v, uint32_t* waves) {
 }
 
 // Small tables are gone through by the one workgroup that has the rest to do, all entries of all rows in a line: a launch
-// takes longer than 32 entries a thread. (64 requests of up to 250 blocks: rewind 8 us so, 12 with clearing and marking by
-// the whole device; 16 compacted 5 and 15; 12 forked 3 and 7. The marks of 32768 blocks fill LDS.)
+// takes longer than 32 entries a thread. (A call on 64 requests of up to 250 blocks: rewind 8.4 us so, 11.4 with clearing and
+// marking by the whole device; 16 compacted 5.7 and 11.3; 12 forked 4.7 and 6.5. The marks of 32768 blocks fill LDS.)
 constexpr uint32_t kSmallTable = 32u * kThreads;   // entries
 constexpr uint32_t kSmallRequests = kThreads;
 constexpr uint32_t kSmallPool = 32u * kThreads;    // blocks
@@ -255,8 +255,8 @@ __global__ __launch_bounds__(kEntryThreads) void rewind_mark_kernel(RewindParams
 
 // The entries given up, from the last to the first: so a block that goes back has its place in the stack, from the top down,
 // without their number. kEach consecutive ones to a thread, with their loads on the way together. How many went back.
-// (One to a thread while that does: 64 requests' drafts 4.2 us so, 6.8 with four; 10000 blocks of 71 requests that end 14.8 with
-// four, 22.2 with one, 16.4 with eight, each mark from memory.)
+// (One to a thread while that does: the kernel takes 8.1 us for 64 requests' drafts so, 9.8 with four; for 10000 blocks of 71
+// requests that end 12.5 with four, 19.6 with one, 13.4 with eight.)
 template <uint32_t kEach>
 __device__ __forceinline__ uint32_t give_back(const RewindParams& p, const uint32_t* state, const uint32_t* gone_sum,
                                               const uint32_t* first_gone, uint32_t all, uint32_t taken, uint32_t* waves) {
@@ -294,7 +294,7 @@ __device__ __forceinline__ uint32_t give_back(const RewindParams& p, const uint3
 }
 
 // kSmall: the marks are this workgroup's own. kMarks: they are in LDS, read at once where others made them (500 requests of
-// which 71 end, 20000 blocks: 12.4 us, 15.2 with each mark from memory).
+// which 71 end, 20000 blocks: the kernel takes 12.5 us, 15.2 with each mark from memory).
 constexpr uint32_t kMarkPool = 28u * kThreads;   // blocks whose marks fit LDS beside 4096 requests
 template <bool kSmall, bool kMarks>
 __global__ __launch_bounds__(kThreads) void rewind_kernel(RewindParams p) {
@@ -595,7 +595,7 @@ struct CopyParams {
 
 // A workgroup to a piece of a block of one cache's K or V at a time, four 16-byte loads of a thread on their way together. (One
 // block of 4096 tokens in 16 layers of 8 heads of 128, 537 MB moved: 99 us, 5.4 TB/s; 930 with whole blocks and a load at
-// a time. The 29 MB of a fork 6.5 and 7.3.)
+// a time. A call on the 29 MB of a fork 7.2 and 8.3.)
 constexpr uint32_t kCopyGroups = 16384;
 constexpr uint32_t kPiece = 4u * 4u * kEntryThreads;   // words of 16 bytes
 __global__ __launch_bounds__(kEntryThreads) void copy_kernel(CopyParams p) {

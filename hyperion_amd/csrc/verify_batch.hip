@@ -21,9 +21,10 @@
 // cut. One request of 5 rows past 2^7 takes 180 to 540 us so. Masks go by their own size: 60 % of 576 rows of 262144 at the
 // type's lowest value take 123 us, 3.0 ms at temperatures of 1.9 and more when all below -2^7 counted as -2^7.
 //
-// What bounds it: with many rows the one pass over the logits (64 requests of 1 to 8 rows of 262144, 268 MB: 60 us of 108,
-// 4.5 TB/s), then the exponentials of the requests that keep most tokens (17). With few, latency: one request of 5 rows
-// takes 22.6 us, count 5.7, filters 8.8, sums 3.8, draw 4.5, where its 4.7 MB are 1 us. The instructions of steps 2 to 4 are
+// What bounds it: with many rows the one pass over the logits (64 requests of 1 to 8 rows of 262144, 268 MB: a call 108 us;
+// its kernels 60, which is 4.5 TB/s, 23, 17 and 7.4), then the exponentials of the requests that keep most tokens. With few,
+// latency: one request of 5 rows takes 22.6 us a call, its kernels 5.8, 8.9, 3.9 and 4.4, where its 4.7 MB are 1 us. (A call's
+// time is that of one in a stream of calls, a kernel's that of a traced dispatch.) The instructions of steps 2 to 4 are
 // mostly such that all waves of a workgroup issue alike (scans, parameters, borders): with 16 waves each is 16 cycles, so
 // they have four (48 requests without a drafting model 72 us with 16, 52 with four). And as the code itself comes from
 // memory in a short kernel, loops over a thread's values are kept rolled.
@@ -97,10 +98,11 @@ __device__ __forceinline__ const uint16_t* logits_of(const VerifyArgs& a, uint32
 
 // ---- 1. counts ----------------------------------------------------------------------------------
 
-// Rows of more bytes than the caches hold are waited for from memory: with all of a chunk's loads on their way at once 64
-// requests' 268 MB take 60 us instead of 68 read again and again, 69 instead of 76 just written. What a cache holds is
-// counted faster while the next comes in: 60 MB 18.2 us so, 19.5 with all loads first (just written 18.9 and 20.3). Between
-// them 126 MB take 24.7 and 26.9 read again and again, 27.4 and 27.6 just written, 32 and 29 with other inputs in between.
+// Rows that come from memory are waited for: with all of a chunk's loads on their way at once the counts of 64 requests'
+// 268 MB take 60 us, 68 otherwise. What a cache holds is counted faster while the next comes in. A whole call in turn over
+// 1, 3 and 8 sets of inputs, without and with all loads first: 42 MB 38.3, 39.3, 43.6 and 38.6, 39.1, 42.9 us; 63 MB 46.3,
+// 46.9, 55.0 and 47.5, 48.1, 53.4; 70 MB 47.7, 48.4, 56.0 and 49.3, 49.6, 54.8; 125 MB 49.2, 58.3, 61.4 and 51.3, 55.0, 57.8.
+// A step's logits are just written, and the rest of the step lies between two calls.
 constexpr uint64_t kCached = 1ull << 26;   // bytes
 constexpr uint32_t kChunkLoads = 8;
 static_assert(kLongest <= kChunkLoads * 8u * kThreads, "a chunk's loads");
@@ -1006,8 +1008,8 @@ Chunks chunks_of(uint32_t rows, uint32_t vocab) {
 }
 
 // Workgroups that the sums of all requests are given: twice what the device runs at once, so that requests without filters,
-// whose exponentials take their time, do not end alone. (With half as many 64 mixed requests 22.7 us, now 19.9, 100 of 50001
-// tokens without filters 16.2, now 14.0; 48 with filters and no drafting model 9.1, now 9.8.)
+// whose exponentials take their time, do not end alone. (With half as many the sums of 64 mixed requests take 17.8 us, so 17.0,
+// of 100 of 50001 tokens without filters 16.2 and 13.9; of 48 with filters and no drafting model 9.0 and 9.8.)
 constexpr uint32_t kSumGroups = 4096;
 
 struct Layout {
