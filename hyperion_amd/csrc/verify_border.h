@@ -28,7 +28,8 @@ struct OneValue {
 // How many tokens of the row the filters keep, if they end in the values of a lane in `maybe`, 0xFFFFFFFF otherwise:
 // the tokens before which the running sum is below `enough` (by_mass), of weights not below min_p. spread(lane): that
 // lane's values, one to a lane, in order. (By all lanes of a wave. Lanes without tokens are not in `maybe`: a wave behind
-// the border would ask them all.)
+// the border would ask them all. Nearly always the first lane asked has the end; where all weights are within 2^-40 of
+// min_p, at a temperature of 1e30 and a min_p of 1, every lane is: one request of 5 rows 41.6 us instead of 22.7.)
 template <typename Spread>
 __device__ __forceinline__ uint32_t wave_border(uint64_t maybe, bool by_mass, double enough, double min_p, Spread&& spread) {
 #pragma unroll 1
